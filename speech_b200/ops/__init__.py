@@ -162,6 +162,41 @@ def mha_attention(q, k, v, mask=None, dropout_p: float = 0.0, training: bool = F
     return reference.mha_attention(q, k, v, mask, dropout_p, training, scale)
 
 
+def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: Optional[float] = None):
+    """Attention of a decoder over an encoder's states, without the score matrix in memory: ``[B, Tq, H * D]``.
+
+    ``q [B, Tq, H, D]``; ``k``, ``v [M, Tk, Hk, D]`` (any strides, e.g. slices of one fused projection).  ``B`` is a multiple of
+    ``M``: query row ``b`` reads memory ``b // (B / M)``, so beams or sampled answers of one utterance share its states without
+    copies; ``H`` is a multiple of ``Hk`` and head ``h`` reads key head ``h // (H / Hk)``.  Gradients of shared keys and values are
+    summed over everything that read them.  ``key_lengths [M]`` (integers) hides the keys from a length on, ``key_mask [M, Tk]``
+    (bool, True = hidden) single keys; both may be given.  A hidden place has no influence whatever it holds, and a query that sees
+    no key gets zeros.  ``scale`` defaults to ``1 / sqrt(D)``.  No dropout on the weights: :func:`mha_attention` has it.
+
+    On GPUs bf16 and fp16 with ``D`` a multiple of 8 up to 128 run as fused kernels, one for a few query rows per key head (decoding
+    steps) and one for many; anything else runs the plain form.  First derivatives only."""
+    reference.check_cross_attention(q, k, v, key_lengths, key_mask)
+    if _use_native(q) and q.dtype in (torch.bfloat16, torch.float16):
+        return _nat().cross_attention(q, k, v, key_lengths, key_mask, scale)
+    return reference.cross_attention(q, k, v, key_lengths, key_mask, scale)
+
+
+def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths=None, scale: Optional[float] = None):
+    """Decoding-step attention of a batch in which groups of rows share a prompt: ``[B, Tq, H * D]``.
+
+    ``q [B, Tq, H, D]`` holds the newest ``Tq`` tokens of every row (their keys are in the cache already); ``k_prefix``,
+    ``v_prefix [P, S, Hk, D]`` the prompts, row ``b`` continuing prompt ``b // (B / P)``, of which the first ``prefix_lengths [P]``
+    positions count (default: all); ``k``, ``v [B, Smax, Hk, D]`` the rows' own caches, in which row ``b`` holds ``lengths[b]``
+    positions, the new tokens included.  Token ``t`` sees its prompt and its row's positions up to its own, ``lengths[b] - Tq + t``;
+    one that sees nothing gets zeros.  Lengths beyond a cache count as its size.  The prompt's keys and values are read once for the
+    whole group.  Caches may have any strides (``[B, Hk, Smax, D]`` caches are passed as ``cache.transpose(1, 2)``).
+
+    For inference: on GPUs there is no backward pass, and inputs that need gradients are refused."""
+    reference.check_shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths)
+    if _use_native(q) and q.dtype in (torch.bfloat16, torch.float16):
+        return _nat().shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths, scale)
+    return reference.shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths, scale)
+
+
 def conv_module_core(g, dw_weight, dw_bias, norm_type, norm_weight, norm_bias, running_mean, running_var,
                      pad_mask=None, training=False, momentum=0.1, eps=1e-5, left_pad=4, right_pad=4, cache=None,
                      cache_drop_size=0, bn_stats_reduce=None):
@@ -210,6 +245,49 @@ def ctc_loss(log_probs, targets, input_lengths, target_lengths, blank, zero_infi
     if _use_native(log_probs) and hasattr(_nat(), "ctc_loss"):
         return _nat().ctc_loss(log_probs, targets, input_lengths, target_lengths, blank)
     return reference.ctc_loss(log_probs, targets, input_lengths, target_lengths, blank, zero_infinity)
+
+
+def policy_loss(logits, targets, mask, old_logp, advantages, ref_logp=None, clip: float = 0.2, clip_high: Optional[float] = None,
+                kl_beta: float = 0.0):
+    """Clipped policy loss with a KL term, straight from logits: ``(loss, logp)``.
+
+    ``logits [N, T, V]`` or ``[N, T, C, V]`` (C codebooks), ``targets`` the sampled tokens ``[N, T(, C)]``, ``mask [N, T]`` non-zero at
+    positions that count (None: all), ``old_logp`` the log-probabilities under the policy that sampled, ``ref_logp`` those under the
+    frozen policy (with ``kl_beta`` > 0), both of the targets' shape, ``advantages [N]``.  With ``r = exp(logp - old_logp)`` a position's
+    term is ``-min(r A, clip(r, 1 - clip, 1 + clip_high) A) + kl_beta (exp(d) - d - 1)``, ``d = ref_logp - logp``; the loss is the mean
+    over all counted positions (0 when there are none).  ``logp`` (fp32, detached, 0 where masked) is the next ``old_logp``.  Gradients
+    go to ``logits`` only.  Masked positions are not read, whatever they hold.  On GPUs a counted target outside the vocabulary makes
+    the loss NaN (the CPU raises), and a forward pass that needs gradients holds the logits' gradient until backward."""
+    reference.check_sequence_loss("policy_loss", logits, targets, mask, (("old_logp", old_logp), ("ref_logp", ref_logp)),
+                                  (("advantages", advantages, logits.shape[0]),))
+    if kl_beta != 0.0 and ref_logp is None:
+        raise ValueError("a KL term (kl_beta != 0) needs ref_logp")
+    if clip < 0 or (clip_high is not None and clip_high < 0):
+        raise ValueError(f"clip ranges must not be negative, got {clip}, {clip_high}")
+    if _use_native(logits) and logits.dtype in (torch.bfloat16, torch.float16, torch.float32) and targets.numel() > 0:
+        return _nat().policy_loss(logits, targets, mask, old_logp, advantages, ref_logp, clip, clip_high, kl_beta)
+    return reference.policy_loss(logits, targets, mask, old_logp, advantages, ref_logp, clip, clip_high, kl_beta)
+
+
+def preference_loss(logits, targets, mask, ref_logp, beta: float = 0.1, loss_type: str = "dpo", reward_gap=None):
+    """Paired preference loss straight from logits: ``(loss, rewards)``.
+
+    The first half of the ``2 N`` sequences holds the chosen answers, the second half the rejected ones in the same order; ``logits``,
+    ``targets``, ``mask`` and ``ref_logp`` as in :func:`policy_loss`.  With ``ratio`` the sum of ``logp - ref_logp`` over a sequence's
+    counted positions and ``margin = ratio_chosen - ratio_rejected``, a pair's loss is ``-log sigmoid(beta margin)`` (``dpo``),
+    ``(margin - 1 / (2 beta))^2`` (``ipo``) or ``(beta margin - reward_gap)^2`` (``rpo_sq``, ``reward_gap [N]``); the loss is their mean.
+    ``rewards [2 N]`` = ``beta * ratio`` (fp32, detached)."""
+    N = logits.shape[0] if logits.dim() > 0 else 0
+    reference.check_sequence_loss("preference_loss", logits, targets, mask, (("ref_logp", ref_logp),), (("reward_gap", reward_gap, N // 2),))
+    if N == 0 or N % 2:
+        raise ValueError(f"preference_loss takes pairs: chosen answers, then as many rejected ones; got {N} sequences")
+    if loss_type not in ("dpo", "ipo", "rpo_sq"):
+        raise NotImplementedError(f"loss type {loss_type} is not implemented")
+    if loss_type == "rpo_sq" and reward_gap is None:
+        raise ValueError("rpo_sq needs the reward gap of every pair")
+    if _use_native(logits) and logits.dtype in (torch.bfloat16, torch.float16, torch.float32) and targets.numel() > 0:
+        return _nat().preference_loss(logits, targets, mask, ref_logp, beta, loss_type, reward_gap)
+    return reference.preference_loss(logits, targets, mask, ref_logp, beta, loss_type, reward_gap)
 
 
 # ----------------------------------------------------------------------------- front-end

@@ -1,0 +1,555 @@
+// Losses of preference / policy optimisation straight from logits: clipped policy loss with a KL term, paired preference loss.
+//
+// For a row x (one position, V logits) with target y:   logp = x_y - m - log s,   m = max x,  s = sum exp(x - m)
+//   policy      r = exp(logp - old),  term = -min(r A, clip(r) A) + beta (exp(d) - d - 1),  d = ref - logp
+//               loss = sum_counted term / count,   slope = dloss/dlogp = (-r A [r A <= clip(r) A] + beta (1 - exp(d))) / count
+//   preference  ratio_i = sum_counted (logp - ref) of sequence i,  margin = ratio_chosen - ratio_rejected, a scalar loss of the
+//               margin per pair; slope of every counted position of a sequence = +-(dloss/dmargin) / pairs
+//   gradient    dx_v = slope (1[v = y] - exp(x_v - m) / s)
+//
+// What bounds them: bytes.  The policy loss knows a row's slope as soon as it knows the row's logp, so the forward pass writes the
+// gradient (for an upstream gradient of 1) while the row is still on the chip: logits are read from memory once.  A preference
+// slope needs both sequences of the pair, so the rows are read a second time; the gradient kernel walks them backwards, and what
+// the forward pass read last is then still in the L2.
+//
+// Rounding: exponentials and sums over a thread's share of a row are fp32, shares are joined in fp64, and logarithm, ratio,
+// clip decision and the sums over rows are fp64: a policy at its reference has log ratios near zero, and in fp32 the rounding of
+// a logp of -8 (5e-7) would be all that is left after a few thousand positions are summed.  The gradient is rounded once.
+// Every sum has a fixed order (no floating-point atomics).
+#include "common.cuh"
+#include <cuda_fp16.h>
+
+namespace {
+
+template <typename T> struct Vec;   // 16-byte groups of the logits' type
+template <> struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* f) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f[2 * u] = __uint_as_float(w[u] << 16);
+      f[2 * u + 1] = __uint_as_float(w[u] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    __align__(16) __nv_bfloat162 o[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) o[u] = __floats2bfloat162_rn(f[2 * u], f[2 * u + 1]);
+    return *reinterpret_cast<uint4*>(o);
+  }
+  static __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
+  static __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16(v); }
+};
+template <> struct Vec<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* f) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float2 v = __half22float2(h[u]);
+      f[2 * u] = v.x;
+      f[2 * u + 1] = v.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    __align__(16) __half2 o[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) o[u] = __floats2half2_rn(f[2 * u], f[2 * u + 1]);
+    return *reinterpret_cast<uint4*>(o);
+  }
+  static __device__ __forceinline__ float up(__half v) { return __half2float(v); }
+  static __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+};
+template <> struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& r, float* f) {
+    f[0] = __uint_as_float(r.x); f[1] = __uint_as_float(r.y); f[2] = __uint_as_float(r.z); f[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  static __device__ __forceinline__ float up(float v) { return v; }
+  static __device__ __forceinline__ float down(float v) { return v; }
+};
+
+struct RowArgs {
+  const void* logits;               // row (n, t, c) starts at element n * sn + t * st + c * sc
+  long long sn, st, sc;
+  const long long* targets;         // [rows]
+  const uint8_t* mask;              // [N * T], null = every position counts
+  const float* ref;                 // [rows] or null
+  const float* old;                 // [rows] or null
+  const float* adv;                 // [N]
+  long long rows;
+  int T, C, V;
+  float clip_lo, clip_hi, kl_beta;
+};
+
+struct Row { long long n, nt; long long off; };
+__device__ __forceinline__ Row locate(const RowArgs& a, long long row) {
+  Row r;
+  r.nt = row / a.C;
+  const long long c = row - r.nt * a.C;
+  r.n = r.nt / a.T;
+  const long long t = r.nt - r.n * a.T;
+  r.off = r.n * a.sn + t * a.st + c * a.sc;
+  return r;
+}
+
+// The 16-byte groups of a row start at its first aligned element: `head` elements before it and `tail` after the last whole group
+// are handled one by one (a row of an odd number of 16-bit logits starts at any even address).
+struct Span { int head, nv, tail; };
+template <typename T> __device__ __forceinline__ Span span_of(const T* p, int V) {
+  Span s;
+  s.head = (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T));
+  if (s.head > V) s.head = V;
+  s.nv = (V - s.head) / Vec<T>::N;
+  s.tail = V - s.head - s.nv * Vec<T>::N;
+  return s;
+}
+
+// (max, sum) pairs with sum taken relative to max; an empty share is (-inf, 0)
+__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
+
+// TPR threads work on a row: one warp (TPR = 32) or a whole block.  NV > 0: the row stays in registers, NV 16-byte groups per
+// thread; NV = 0: rows of any length, read again (from the L2: 148 rows of 300 KB in flight are a third of it) for the gradient.
+template <int TPR> __device__ __forceinline__ float group_max(float v, float* red) {
+  v = warp_max(v);
+  if (TPR == 32) return v;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float r = red[0];
+#pragma unroll
+  for (int i = 1; i < TPR / 32; ++i) r = fmaxf(r, red[i]);
+  return r;
+}
+template <int TPR> __device__ __forceinline__ double group_sum(double v, double* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if (TPR == 32) return v;
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double r = red[0];
+#pragma unroll
+  for (int i = 1; i < TPR / 32; ++i) r += red[i];
+  return r;
+}
+
+template <typename T> __device__ __forceinline__ T* out_row(void* d, long long row, int V) { return reinterpret_cast<T*>(d) + row * V; }
+
+template <typename T, int TPR> __device__ __forceinline__ void write_zeros(T* o, int V, int lane) {
+  const Span s = span_of(o, V);
+  if (lane < s.head) o[lane] = Vec<T>::down(0.f);
+  uint4* ov = reinterpret_cast<uint4*>(o + s.head);
+  for (int i = lane; i < s.nv; i += TPR) ov[i] = make_uint4(0, 0, 0, 0);
+  if (lane < s.tail) o[s.head + s.nv * Vec<T>::N + lane] = Vec<T>::down(0.f);
+}
+
+// Gradient of a row read again from memory: slope * (1[v = y] - exp(x - shift) * inv).  Input and output may be aligned differently
+// (logits that are a slice of a longer tensor): groups are formed on the output where the input allows it, else one by one.
+template <typename T, int TPR>
+__device__ __forceinline__ void grad_from_memory(const T* x, T* o, int V, int lane, int y, float slope, float shift, float inv) {
+  const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
+  auto one = [&](int v) {
+    const float p = __expf(Vec<T>::up(x[v]) - shift) * inv;
+    o[v] = Vec<T>::down(slope * ((v == y ? 1.f : 0.f) - p));
+  };
+  if (!same) {
+    for (int v = lane; v < V; v += TPR) one(v);
+    return;
+  }
+  constexpr int E = Vec<T>::N;
+  const Span s = span_of(x, V);
+  if (lane < s.head) one(lane);
+  const uint4* xv = reinterpret_cast<const uint4*>(x + s.head);
+  uint4* ov = reinterpret_cast<uint4*>(o + s.head);
+  for (int i = lane; i < s.nv; i += TPR) {
+    float f[E];
+    Vec<T>::unpack(xv[i], f);
+    const int v0 = s.head + i * E;
+#pragma unroll
+    for (int u = 0; u < E; ++u) f[u] = slope * ((v0 + u == y ? 1.f : 0.f) - __expf(f[u] - shift) * inv);
+    ov[i] = Vec<T>::pack(f);
+  }
+  if (lane < s.tail) one(s.head + s.nv * E + lane);
+}
+
+enum { LOSS_POLICY = 0, LOSS_PREFERENCE = 1 };
+
+// Forward pass over all rows.  lse / logp / slope: fp32 [rows]; dlogits: contiguous [rows, V] or null (no gradient wanted now);
+// partial: fp64, per block the sum of its policy terms; ratio: fp64 [rows], preference only.
+template <typename T, int MODE, int TPR, int NV, int THREADS>
+__global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, const int* __restrict__ count_p, float* __restrict__ logp_out, float* __restrict__ lse_out,
+                                                               float* __restrict__ slope_out, void* __restrict__ dlogits, double* __restrict__ partial,
+                                                               double* __restrict__ ratio) {
+  constexpr int E = Vec<T>::N, GROUPS = THREADS / TPR;
+  __shared__ float redf[32];
+  __shared__ double redd[32];
+  const int lane = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
+  const int group = TPR == 32 ? (threadIdx.x >> 5) : 0;
+  const double inv_count = MODE == LOSS_POLICY ? 1.0 / (double)max(1, *count_p) : 0.0;
+  double mine = 0.0;                                     // same value in every thread of the group
+  for (long long row = (long long)blockIdx.x * GROUPS + group; row < a.rows; row += (long long)gridDim.x * GROUPS) {
+    const Row r = locate(a, row);
+    T* o = dlogits ? out_row<T>(dlogits, row, a.V) : nullptr;
+    if (a.mask && !a.mask[r.nt]) {                       // hidden position: its logits are not read
+      if (lane == 0) {
+        lse_out[row] = 0.f;
+        if (MODE == LOSS_POLICY) logp_out[row] = slope_out[row] = 0.f;
+        else ratio[row] = 0.0;
+      }
+      if (o) write_zeros<T, TPR>(o, a.V, lane);
+      continue;
+    }
+    const T* x = reinterpret_cast<const T*>(a.logits) + r.off;
+    const long long y64 = a.targets[row];
+    const bool known = y64 >= 0 && y64 < a.V;            // a target outside the vocabulary makes the row's results NaN
+    const int y = known ? (int)y64 : -1;
+    const float xy = known ? Vec<T>::up(x[y]) : NAN;
+    const Span s = span_of(x, a.V);
+    const uint4* xv = reinterpret_cast<const uint4*>(x + s.head);
+    const int vt = s.head + s.nv * E;
+    float hx = lane < s.head ? Vec<T>::up(x[lane]) : -INFINITY;
+    float tx = lane < s.tail ? Vec<T>::up(x[vt + lane]) : -INFINITY;
+    float m, share;
+    float e[NV > 0 ? NV : 1][E];
+    if (NV > 0) {
+      uint4 raw[NV > 0 ? NV : 1];
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (lane + k * TPR < s.nv) raw[k] = xv[lane + k * TPR];
+      m = fmaxf(hx, tx);
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        if (lane + k * TPR < s.nv) Vec<T>::unpack(raw[k], e[k]);
+        else {
+#pragma unroll
+          for (int u = 0; u < E; ++u) e[k][u] = -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < E; ++u) m = fmaxf(m, e[k][u]);
+      }
+      m = finite_or_zero(group_max<TPR>(m, redf));
+      hx = __expf(hx - m);
+      tx = __expf(tx - m);
+      share = hx + tx;
+#pragma unroll
+      for (int k = 0; k < NV; ++k) {
+        float part = 0.f;
+#pragma unroll
+        for (int u = 0; u < E; ++u) {
+          e[k][u] = __expf(e[k][u] - m);
+          part += e[k][u];
+        }
+        share += part;
+      }
+    } else {
+      float tm = fmaxf(hx, tx), ts = 0.f;
+      ts = __expf(hx - finite_or_zero(tm)) + __expf(tx - finite_or_zero(tm));
+#pragma unroll 4
+      for (int i = lane; i < s.nv; i += TPR) {
+        float f[E];
+        Vec<T>::unpack(xv[i], f);
+        float nm = tm;
+#pragma unroll
+        for (int u = 0; u < E; ++u) nm = fmaxf(nm, f[u]);
+        const float ref_m = finite_or_zero(nm);
+        float part = 0.f;
+#pragma unroll
+        for (int u = 0; u < E; ++u) part += __expf(f[u] - ref_m);
+        ts = ts * __expf(finite_or_zero(tm) - ref_m) + part;
+        tm = nm;
+      }
+      m = finite_or_zero(group_max<TPR>(tm, redf));
+      share = ts * __expf(finite_or_zero(tm) - m);
+    }
+    const double sum = group_sum<TPR>((double)share, redd);
+    const double log_sum = log(sum);
+    const double logp = (double)xy - (double)m - log_sum;
+    float slope = 0.f;
+    if (MODE == LOSS_POLICY) {
+      const double rt = exp(logp - (double)a.old[row]), A = (double)a.adv[r.n];
+      const double lo = 1.0 - (double)a.clip_lo, hi = 1.0 + (double)a.clip_hi;
+      const double plain = rt * A, clipped = (rt < lo ? lo : (rt > hi ? hi : rt)) * A;
+      const bool inside = plain <= clipped;
+      double term = -(inside || plain != plain ? plain : clipped), sl = inside || plain != plain ? -plain : 0.0;
+      if (a.ref && a.kl_beta != 0.f) {
+        const double d = (double)a.ref[row] - logp, ed = exp(d);
+        term += (double)a.kl_beta * (ed - d - 1.0);
+        sl += (double)a.kl_beta * (1.0 - ed);
+      }
+      mine += term;
+      slope = (float)(sl * inv_count);
+    }
+    if (lane == 0) {
+      lse_out[row] = (float)((double)m + log_sum);
+      if (MODE == LOSS_POLICY) {
+        logp_out[row] = (float)logp;
+        slope_out[row] = slope;
+      } else {
+        ratio[row] = logp - (double)a.ref[row];
+      }
+    }
+    if (MODE == LOSS_POLICY && o) {
+      if (slope == 0.f) {
+        write_zeros<T, TPR>(o, a.V, lane);
+        continue;
+      }
+      const float inv = (float)(1.0 / sum);
+      if (NV > 0 && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
+        const float si = slope * inv;
+        uint4* ov = reinterpret_cast<uint4*>(o + s.head);
+        if (lane < s.head) o[lane] = Vec<T>::down((lane == y ? slope : 0.f) - hx * si);
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+          if (lane + k * TPR < s.nv) {
+            const int v0 = s.head + (lane + k * TPR) * E;
+            float f[E];
+#pragma unroll
+            for (int u = 0; u < E; ++u) f[u] = (v0 + u == y ? slope : 0.f) - e[k][u] * si;
+            ov[lane + k * TPR] = Vec<T>::pack(f);
+          }
+        if (lane < s.tail) o[vt + lane] = Vec<T>::down((vt + lane == y ? slope : 0.f) - tx * si);
+      } else {
+        grad_from_memory<T, TPR>(x, o, a.V, lane, y, slope, m, inv);
+      }
+    }
+  }
+  if (MODE == LOSS_POLICY) {
+    // fixed order: groups of the block in turn, blocks in turn (policy_finish_kernel)
+    __syncthreads();
+    if (TPR == 32) {
+      if (lane == 0) redd[group] = mine;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        double t = 0.0;
+        for (int i = 0; i < GROUPS; ++i) t += redd[i];
+        partial[blockIdx.x] = t;
+      }
+    } else if (threadIdx.x == 0) {
+      partial[blockIdx.x] = mine;
+    }
+  }
+}
+
+// Gradient of all rows from memory: per-row slopes (slope != null), or one slope per sequence with masked rows zero.  `upstream`
+// is the gradient of the loss, in device memory; with `unless_one` the whole kernel has nothing to do when it is 1, which is what
+// the forward pass has written the gradient for already.  Rows are walked from the last to the first.
+template <typename T, int TPR, int THREADS>
+__global__ void __launch_bounds__(THREADS) rows_grad_kernel(const RowArgs a, const float* __restrict__ lse, const float* __restrict__ slope,
+                                                            const float* __restrict__ seq_slope, const float* __restrict__ upstream, int unless_one,
+                                                            void* __restrict__ dlogits) {
+  const float g = *upstream;
+  if (unless_one && g == 1.f) return;
+  constexpr int GROUPS = THREADS / TPR;
+  const int lane = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
+  const int group = TPR == 32 ? (threadIdx.x >> 5) : 0;
+  for (long long i = (long long)blockIdx.x * GROUPS + group; i < a.rows; i += (long long)gridDim.x * GROUPS) {
+    const long long row = a.rows - 1 - i;
+    const Row r = locate(a, row);
+    T* o = out_row<T>(dlogits, row, a.V);
+    const bool hidden = a.mask && !a.mask[r.nt];
+    const float sl = hidden ? 0.f : g * (slope ? slope[row] : seq_slope[r.n]);
+    if (sl == 0.f) {
+      write_zeros<T, TPR>(o, a.V, lane);
+      continue;
+    }
+    const long long y64 = a.targets[row];
+    const int y = y64 >= 0 && y64 < a.V ? (int)y64 : -1;
+    grad_from_memory<T, TPR>(reinterpret_cast<const T*>(a.logits) + r.off, o, a.V, lane, y, sl, lse[row], 1.f);
+  }
+}
+
+__global__ void count_kernel(const uint8_t* __restrict__ mask, long long nt, int C, int* __restrict__ count) {
+  __shared__ int red[32];
+  long long n = 0;
+  for (long long i = threadIdx.x; i < nt; i += blockDim.x) n += mask ? mask[i] != 0 : 1;
+  int c = (int)n;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = c;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int t = 0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += red[i];
+    *count = t * C;
+  }
+}
+
+__global__ void policy_finish_kernel(const double* __restrict__ partial, int n, const int* __restrict__ count, float* __restrict__ loss) {
+  __shared__ double red[32];
+  double t = 0.0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) t += partial[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double u = 0.0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) u += red[i];
+    *loss = (float)(u / (double)max(1, *count));
+  }
+}
+
+// One block per sequence: ratio_i = sum of its rows' log ratios.
+__global__ void ratio_kernel(const double* __restrict__ ratio, long long per, double* __restrict__ total) {
+  __shared__ double red[32];
+  const double* p = ratio + (long long)blockIdx.x * per;
+  double t = 0.0;
+  for (long long i = threadIdx.x; i < per; i += blockDim.x) t += p[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double u = 0.0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) u += red[i];
+    total[blockIdx.x] = u;
+  }
+}
+
+// Scalar losses of all pairs, their mean, rewards beta * ratio and the slope of every sequence's positions.  One block.
+__global__ void preference_finish_kernel(const double* __restrict__ total, int pairs, int kind, float beta_f, const float* __restrict__ gap,
+                                         float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ seq_slope) {
+  __shared__ double red[32];
+  const double beta = (double)beta_f;
+  double mine = 0.0;
+  for (int n = threadIdx.x; n < pairs; n += blockDim.x) {
+    const double margin = total[n] - total[n + pairs];
+    double l, s;
+    if (kind == 0) {                                        // -log sigmoid(beta margin)
+      const double z = beta * margin;
+      l = log1p(exp(-fabs(z))) + (z < 0.0 ? -z : 0.0);
+      s = -beta / (1.0 + exp(z));
+    } else if (kind == 1) {
+      const double d = margin - 1.0 / (2.0 * beta);
+      l = d * d;
+      s = 2.0 * d;
+    } else {
+      const double d = beta * margin - (double)gap[n];
+      l = d * d;
+      s = 2.0 * beta * d;
+    }
+    mine += l;
+    seq_slope[n] = (float)(s / pairs);
+    seq_slope[n + pairs] = (float)(-s / pairs);
+    rewards[n] = (float)(beta * total[n]);
+    rewards[n + pairs] = (float)(beta * total[n + pairs]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mine;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double u = 0.0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) u += red[i];
+    *loss = (float)(u / pairs);
+  }
+}
+
+constexpr int MAX_BLOCKS = 148 * 8;
+
+template <typename T, int MODE, int TPR, int NV, int THREADS>
+int run_forward(const RowArgs& a, const int* count, float* logp, float* lse, float* slope, void* dlogits, double* partial, double* ratio, int* blocks,
+                cudaStream_t stream) {
+  long long need = (a.rows + THREADS / TPR - 1) / (THREADS / TPR);
+  const long long cap = (long long)sb_num_sms() * 8 < MAX_BLOCKS ? (long long)sb_num_sms() * 8 : MAX_BLOCKS;
+  *blocks = (int)(need < cap ? need : cap);
+  rows_forward_kernel<T, MODE, TPR, NV, THREADS><<<*blocks, THREADS, 0, stream>>>(a, count, logp, lse, slope, dlogits, partial, ratio);
+  return (int)cudaGetLastError();
+}
+
+template <typename T, int MODE>
+int forward(const RowArgs& a, const int* count, float* logp, float* lse, float* slope, void* dlogits, double* partial, double* ratio, int* blocks,
+            cudaStream_t stream) {
+  // a row that fits eight 16-byte groups per lane of a warp, or per thread of a block, stays in registers
+  const long long groups = a.V / Vec<T>::N;
+  if (groups <= 32 * 2) return run_forward<T, MODE, 32, 2, 256>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
+  if (groups <= 32 * 8) return run_forward<T, MODE, 32, 8, 256>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
+  if (groups <= 256 * 8) return run_forward<T, MODE, 256, 8, 256>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
+  return run_forward<T, MODE, 512, 0, 512>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
+}
+
+template <typename T>
+int gradient(const RowArgs& a, const float* lse, const float* slope, const float* seq_slope, const float* upstream, int unless_one, void* dlogits,
+             cudaStream_t stream) {
+  const long long cap = (long long)sb_num_sms() * 8;
+  if (a.V / Vec<T>::N <= 32 * 16) {
+    const long long need = (a.rows + 7) / 8;
+    rows_grad_kernel<T, 32, 256><<<(int)(need < cap ? need : cap), 256, 0, stream>>>(a, lse, slope, seq_slope, upstream, unless_one, dlogits);
+  } else {
+    rows_grad_kernel<T, 256, 256><<<(int)(a.rows < cap ? a.rows : cap), 256, 0, stream>>>(a, lse, slope, seq_slope, upstream, unless_one, dlogits);
+  }
+  return (int)cudaGetLastError();
+}
+
+bool fill(RowArgs& a, const void* logits, long long sn, long long st, long long sc, const long long* targets, const uint8_t* mask, long long N, int T, int C,
+          int V) {
+  if (!logits || !targets || N <= 0 || T <= 0 || C <= 0 || V <= 0) return false;
+  a = RowArgs{};
+  a.logits = logits; a.sn = sn; a.st = st; a.sc = sc;
+  a.targets = targets; a.mask = mask;
+  a.rows = N * T * C;
+  a.T = T; a.C = C; a.V = V;
+  return a.rows < (1ll << 31);      // counted positions are held in 32 bits
+}
+
+}  // namespace
+
+// Logit types: 0 = bf16, 1 = fp16, 2 = fp32.  `partial`: at least sb_sequence_loss_blocks() doubles.
+SB_API int sb_sequence_loss_blocks() { return MAX_BLOCKS; }
+
+SB_API int sb_policy_loss_fwd(const void* logits, int type, long long sn, long long st, long long sc, const long long* targets, const uint8_t* mask,
+                              const float* old_logp, const float* ref_logp, const float* adv, long long N, int T, int C, int V, float clip_lo,
+                              float clip_hi, float kl_beta, int* count, double* partial, float* loss, float* logp, float* lse, float* slope,
+                              void* dlogits, cudaStream_t stream) {
+  RowArgs a;
+  if (!fill(a, logits, sn, st, sc, targets, mask, N, T, C, V) || !old_logp || !adv || !count || !partial || !loss || !logp || !lse || !slope)
+    return SB_BAD_ARGUMENT;
+  a.old = old_logp; a.ref = ref_logp; a.adv = adv;
+  a.clip_lo = clip_lo; a.clip_hi = clip_hi; a.kl_beta = kl_beta;
+  count_kernel<<<1, 1024, 0, stream>>>(mask, N * T, C, count);
+  int blocks = 0, rc;
+  if (type == 0) rc = forward<__nv_bfloat16, LOSS_POLICY>(a, count, logp, lse, slope, dlogits, partial, nullptr, &blocks, stream);
+  else if (type == 1) rc = forward<__half, LOSS_POLICY>(a, count, logp, lse, slope, dlogits, partial, nullptr, &blocks, stream);
+  else if (type == 2) rc = forward<float, LOSS_POLICY>(a, count, logp, lse, slope, dlogits, partial, nullptr, &blocks, stream);
+  else return SB_BAD_ARGUMENT;
+  if (rc) return rc;
+  policy_finish_kernel<<<1, 256, 0, stream>>>(partial, blocks, count, loss);
+  return (int)cudaGetLastError();
+}
+
+SB_API int sb_preference_loss_fwd(const void* logits, int type, long long sn, long long st, long long sc, const long long* targets, const uint8_t* mask,
+                                  const float* ref_logp, long long N, int T, int C, int V, int kind, float beta, const float* gap, double* ratio,
+                                  double* total, float* loss, float* rewards, float* seq_slope, float* lse, cudaStream_t stream) {
+  RowArgs a;
+  if (!fill(a, logits, sn, st, sc, targets, mask, N, T, C, V) || (N & 1) || N > (1 << 30) || !ref_logp || !ratio || !total || !loss || !rewards || !seq_slope ||
+      !lse || kind < 0 || kind > 2 || (kind == 2 && !gap))
+    return SB_BAD_ARGUMENT;
+  a.ref = ref_logp;
+  int blocks = 0, rc;
+  if (type == 0) rc = forward<__nv_bfloat16, LOSS_PREFERENCE>(a, nullptr, nullptr, lse, nullptr, nullptr, nullptr, ratio, &blocks, stream);
+  else if (type == 1) rc = forward<__half, LOSS_PREFERENCE>(a, nullptr, nullptr, lse, nullptr, nullptr, nullptr, ratio, &blocks, stream);
+  else if (type == 2) rc = forward<float, LOSS_PREFERENCE>(a, nullptr, nullptr, lse, nullptr, nullptr, nullptr, ratio, &blocks, stream);
+  else return SB_BAD_ARGUMENT;
+  if (rc) return rc;
+  ratio_kernel<<<(int)N, 256, 0, stream>>>(ratio, (long long)T * C, total);
+  rc = (int)cudaGetLastError();
+  if (rc) return rc;
+  preference_finish_kernel<<<1, 256, 0, stream>>>(total, (int)(N / 2), kind, beta, gap, loss, rewards, seq_slope);
+  return (int)cudaGetLastError();
+}
+
+SB_API int sb_sequence_loss_bwd(const void* logits, int type, long long sn, long long st, long long sc, const long long* targets, const uint8_t* mask,
+                                long long N, int T, int C, int V, const float* lse, const float* slope, const float* seq_slope, const float* upstream,
+                                int unless_one, void* dlogits, cudaStream_t stream) {
+  RowArgs a;
+  if (!fill(a, logits, sn, st, sc, targets, mask, N, T, C, V) || !lse || (!slope && !seq_slope) || !upstream || !dlogits) return SB_BAD_ARGUMENT;
+  if (type == 0) return gradient<__nv_bfloat16>(a, lse, slope, seq_slope, upstream, unless_one, dlogits, stream);
+  if (type == 1) return gradient<__half>(a, lse, slope, seq_slope, upstream, unless_one, dlogits, stream);
+  if (type == 2) return gradient<float>(a, lse, slope, seq_slope, upstream, unless_one, dlogits, stream);
+  return SB_BAD_ARGUMENT;
+}

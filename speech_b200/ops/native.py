@@ -422,6 +422,7 @@ from .native_transducer import transducer_joint_loss, transducer_loss_from_logit
 from .native_lstm import lstm  # noqa: E402,F401
 from .native_ctc import ctc_loss  # noqa: E402,F401
 from .native_logmel import logmel  # noqa: E402,F401
+from .native_sequence_loss import policy_loss, preference_loss  # noqa: E402,F401
 
 
 def __getattr__(name):

@@ -397,3 +397,140 @@ def ngram_advance(states, arc_keys, arc_w, arc_to, backoff_w, backoff_to, V: int
         cur = backoff_to[cur]
     scores = torch.where(done, scores, acc + default_score)
     return scores, nxt
+
+
+# ----------------------------------------------------------------------------- attention over an encoder's states / a shared prompt
+def check_cross_attention(q, k, v, key_lengths=None, key_mask=None):
+    """Argument checks shared by both implementations; returns (memories, rows per memory, query heads per key head)."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError(f"cross_attention takes [batch, time, heads, dim] tensors, got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape != v.shape or q.shape[3] != k.shape[3]:
+        raise ValueError(f"keys {tuple(k.shape)} and values {tuple(v.shape)} must agree, with the queries' head size {q.shape[3]}")
+    if not (q.dtype == k.dtype == v.dtype) or not q.is_floating_point():
+        raise ValueError(f"queries, keys and values must have one floating-point type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if not (q.device == k.device == v.device):
+        raise ValueError("queries, keys and values must be on one device")
+    B, M, H, Hk = q.shape[0], k.shape[0], q.shape[2], k.shape[2]
+    if M == 0 or Hk == 0 or q.shape[3] == 0 or B % M or H % Hk:
+        raise ValueError(f"{B} query rows and {H} heads must be whole multiples of {M} memories and {Hk} key heads")
+    if key_lengths is not None and (key_lengths.shape != (M,) or key_lengths.is_floating_point() or key_lengths.dtype == torch.bool
+                                    or key_lengths.device != q.device):
+        raise ValueError(f"key_lengths must be {M} integers on {q.device}, got {key_lengths.dtype} {tuple(key_lengths.shape)} on {key_lengths.device}")
+    if key_mask is not None and (key_mask.shape != (M, k.shape[1]) or key_mask.dtype != torch.bool or key_mask.device != q.device):
+        raise ValueError(f"key_mask must be bool {(M, k.shape[1])} on {q.device}, got {key_mask.dtype} {tuple(key_mask.shape)} on {key_mask.device}")
+    return M, B // M, H // Hk
+
+
+def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: Optional[float] = None):
+    """q [B, Tq, H, D]; k, v [M, Tk, Hk, D] -> [B, Tq, H*D]; see ``ops.cross_attention``."""
+    M, G, rep = check_cross_attention(q, k, v, key_lengths, key_mask)
+    B, Tq, H, D = q.shape
+    Tk, Hk = k.shape[1], k.shape[2]
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    hidden = torch.zeros((M, Tk), dtype=torch.bool, device=q.device) if key_mask is None else key_mask
+    if key_lengths is not None:
+        hidden = hidden | (torch.arange(Tk, device=q.device)[None, :] >= key_lengths[:, None])
+    kf = k.float().masked_fill(hidden[:, :, None, None], 0.0)          # whatever stands in a hidden place (NaN, too) has no influence
+    vf = v.float().masked_fill(hidden[:, :, None, None], 0.0)
+    qf = q.float().reshape(M, G, Tq, Hk, rep, D)
+    s = torch.einsum("mgthrd,mshd->mghrts", qf, kf) * scale
+    empty = hidden.all(dim=1, keepdim=True)
+    s = s.masked_fill((hidden & ~empty)[:, None, None, None, None, :], float("-inf"))
+    p = torch.softmax(s, dim=-1) if Tk > 0 else s
+    p = p.masked_fill(hidden[:, None, None, None, None, :], 0.0)
+    out = torch.einsum("mghrts,mshd->mgthrd", p, vf)
+    return out.reshape(B, Tq, H * D).to(q.dtype)
+
+
+def check_shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths=None):
+    P, G, rep = check_cross_attention(q, k_prefix, v_prefix, prefix_lengths)
+    B = q.shape[0]
+    if k.dim() != 4 or k.shape != v.shape or k.shape[0] != B or k.shape[2:] != k_prefix.shape[2:]:
+        raise ValueError(f"own keys {tuple(k.shape)} and values {tuple(v.shape)} must be [{B}, positions, {k_prefix.shape[2]}, {k_prefix.shape[3]}]")
+    if k.dtype != q.dtype or v.dtype != q.dtype or k.device != q.device or v.device != q.device:
+        raise ValueError("own keys and values must have the queries' type and device")
+    if lengths.shape != (B,) or lengths.is_floating_point() or lengths.dtype == torch.bool or lengths.device != q.device:
+        raise ValueError(f"lengths must be {B} integers on {q.device}, got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
+    return P, G, rep
+
+
+def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths=None, scale: Optional[float] = None):
+    """See ``ops.shared_prefix_attention``."""
+    P, G, rep = check_shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths)
+    B, Tq, H, D = q.shape
+    S, Smax, Hk, dev = k_prefix.shape[1], k.shape[1], k.shape[2], q.device
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+    hide_p = torch.zeros((P, S), dtype=torch.bool, device=dev)
+    if prefix_lengths is not None:
+        hide_p = torch.arange(S, device=dev)[None, :] >= prefix_lengths[:, None]
+    last = lengths.clamp(max=Smax)[:, None] - Tq + torch.arange(Tq, device=dev)[None, :]
+    hide_o = torch.arange(Smax, device=dev)[None, None, :] > last[:, :, None]                       # [B, Tq, Smax]
+    kp, vp = (x.float().masked_fill(hide_p[:, :, None, None], 0.0) for x in (k_prefix, v_prefix))
+    unused = hide_o.all(dim=1) if Tq else torch.ones((B, Smax), dtype=torch.bool, device=dev)
+    ko, vo = (x.float().masked_fill(unused[:, :, None, None], 0.0).view(P, G, Smax, Hk, D) for x in (k, v))
+    qf = q.float().reshape(P, G, Tq, Hk, rep, D)
+    s = torch.cat([torch.einsum("pgthrd,pshd->pghrts", qf, kp), torch.einsum("pgthrd,pgshd->pghrts", qf, ko)], dim=-1) * scale
+    hidden = torch.cat([hide_p[:, None, None, None, None, :].expand(P, G, 1, 1, Tq, S), hide_o.view(P, G, 1, 1, Tq, Smax)], dim=-1)
+    if S + Smax:
+        empty = hidden.all(dim=-1, keepdim=True)
+        s = torch.softmax(s.masked_fill(hidden & ~empty, float("-inf")), dim=-1)
+    w = s.masked_fill(hidden, 0.0)
+    out = torch.einsum("pghrts,pshd->pgthrd", w[..., :S], vp) + torch.einsum("pghrts,pgshd->pgthrd", w[..., S:], vo)
+    return out.reshape(B, Tq, H * D).to(q.dtype)
+
+
+# ----------------------------------------------------------------------------- losses of preference / policy optimisation
+def check_sequence_loss(name, logits, targets, mask, per_position, per_sequence):
+    if logits.dim() not in (3, 4) or not logits.is_floating_point() or logits.shape[-1] == 0:
+        raise ValueError(f"{name} takes floating-point logits [N, T, V] or [N, T, C, V], got {logits.dtype} {tuple(logits.shape)}")
+    if targets.shape != logits.shape[:-1] or targets.is_floating_point() or targets.dtype == torch.bool:
+        raise ValueError(f"targets must be integers {tuple(logits.shape[:-1])}, got {targets.dtype} {tuple(targets.shape)}")
+    if mask is not None and mask.shape != logits.shape[:2]:
+        raise ValueError(f"mask must be {tuple(logits.shape[:2])}, got {tuple(mask.shape)}")
+    for what, t in per_position:
+        if t is not None and t.shape != targets.shape:
+            raise ValueError(f"{what} must be {tuple(targets.shape)}, got {tuple(t.shape)}")
+    for what, t, n in per_sequence:
+        if t is not None and t.shape != (n,):
+            raise ValueError(f"{what} must be ({n},), got {tuple(t.shape)}")
+    for t in [targets, mask] + [t for _, t in per_position] + [t for _, t, _ in per_sequence]:
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"{name} takes tensors of one device, got {logits.device} and {t.device}")
+
+
+def _target_logprob(logits, targets, mask):
+    """fp64 log-probabilities of the targets, zero (and without gradient) where masked."""
+    counted = torch.ones(logits.shape[:2], dtype=torch.bool, device=logits.device) if mask is None else mask != 0
+    counted = counted.view(counted.shape + (1,) * (logits.dim() - 3)).expand(targets.shape)
+    x = logits.double().masked_fill(~counted.unsqueeze(-1), 0.0)
+    y = targets.long().masked_fill(~counted, 0)
+    logp = torch.log_softmax(x, dim=-1).gather(-1, y.unsqueeze(-1)).squeeze(-1)
+    return logp.masked_fill(~counted, 0.0), counted
+
+
+def policy_loss(logits, targets, mask, old_logp, advantages, ref_logp=None, clip: float = 0.2, clip_high: Optional[float] = None,
+                kl_beta: float = 0.0):
+    logp, counted = _target_logprob(logits, targets, mask)
+    zero = logp.new_zeros(())
+    ratio = torch.exp(torch.where(counted, logp - old_logp.detach().double(), zero))
+    adv = advantages.detach().double().view((-1,) + (1,) * (targets.dim() - 1))
+    term = -torch.minimum(ratio * adv, ratio.clamp(1.0 - clip, 1.0 + (clip if clip_high is None else clip_high)) * adv)
+    if kl_beta != 0.0:
+        d = torch.where(counted, ref_logp.detach().double() - logp, zero)
+        term = term + kl_beta * (torch.exp(d) - d - 1.0)
+    loss = torch.where(counted, term, zero).sum() / counted.sum().clamp(min=1)
+    return loss.float(), logp.detach().float()
+
+
+def preference_loss(logits, targets, mask, ref_logp, beta: float = 0.1, loss_type: str = "dpo", reward_gap=None):
+    logp, counted = _target_logprob(logits, targets, mask)
+    ratio = torch.where(counted, logp - ref_logp.detach().double(), logp.new_zeros(())).flatten(1).sum(1)
+    n = ratio.shape[0] // 2
+    margin = ratio[:n] - ratio[n:]
+    if loss_type == "dpo":
+        loss = -F.logsigmoid(beta * margin)
+    elif loss_type == "ipo":
+        loss = (margin - 1.0 / (2.0 * beta)) ** 2
+    else:
+        loss = (beta * margin - reward_gap.detach().double()) ** 2
+    return loss.mean().float(), (beta * ratio).detach().float()

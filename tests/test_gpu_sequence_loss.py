@@ -1,0 +1,237 @@
+"""Policy and preference loss kernels against a plain statement in 64 bits."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}      # half a step, relative
+
+
+def make(n, t, c, v, dtype, seed=0, scale=2.0, whole=False):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    shape = (n, t) if c is None else (n, t, c)
+    logits = (scale * torch.randn(shape + (v,), generator=g, device="cuda")).to(dtype)
+    targets = torch.randint(0, v, shape, generator=g, device="cuda")
+    mask = torch.rand((n, t), generator=g, device="cuda") < 0.7
+    mask[0, 0] = True
+    if n > 2:
+        mask[2] = False
+    if whole:
+        mask[:] = True
+    near = torch.log_softmax(logits.double(), -1).gather(-1, targets.unsqueeze(-1)).squeeze(-1)
+    old = (near + 0.2 * torch.randn(shape, generator=g, device="cuda")).float()
+    ref = (near + 0.2 * torch.randn(shape, generator=g, device="cuda")).float()
+    adv = torch.randn(n, generator=g, device="cuda")
+    return logits, targets, mask, old, ref, adv
+
+
+def plain_logp(logits, targets, mask):
+    m = mask.view(mask.shape + (1,) * (targets.dim() - 2)).expand(targets.shape)
+    x = logits.double().masked_fill(~m.unsqueeze(-1), 0.0)
+    lse = torch.logsumexp(x, -1)
+    lp = (x.gather(-1, targets.masked_fill(~m, 0).unsqueeze(-1)).squeeze(-1) - lse) * m
+    return lp, m, torch.exp(x - lse.unsqueeze(-1))
+
+
+def lp_tolerance(v):
+    # CUDA states 2 + floor(1.173 |x|) ulp (2^-23) for the fast exponential; weighted by the exponentials themselves, |x| averages to
+    # the distance from the largest logit, below 16 here: 21 * 2^-23 < 2^-18.  A thread adds up to max(64, v / 512) terms one by one,
+    # half a step each.  fp32 storage of a logp below 32 adds 2^-20.
+    return 2.0 ** -18 + max(64, v // 512 + 16) * 2.0 ** -24 + 2.0 ** -20
+
+
+def check_gradient(got, targets, weights, slope, dtype, v, upstream=1.0):
+    """slope: 64-bit dloss/dlogp per position (times the upstream gradient)."""
+    want = -weights * slope.unsqueeze(-1)
+    want.scatter_add_(-1, targets.clamp(0, v - 1).unsqueeze(-1), slope.unsqueeze(-1))
+    # one rounding of the result; softmax weights inherit the log-probability's error and one more exponential; the slope is fp32
+    # and for the policy loss its ratio inherits the log-probability's error as well
+    lp = 2 * lp_tolerance(v) + 2.0 ** -18
+    tol = EPS[dtype] * want.abs() + slope.abs().unsqueeze(-1) * (weights + (want.abs() > 0)) * 2 * lp + 2.0 ** -25 * (dtype == torch.float16) + 1e-38
+    assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
+
+
+SHAPES = [(2, 3, None, 2), (4, 5, 8, 130), (3, 4, None, 257), (4, 6, 8, 2024), (2, 3, 2, 2049), (2, 5, None, 16384), (2, 3, None, 20003), (2, 2, None, 151936), (1, 1, 1, 1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("kl", [0.0, 0.04])
+def test_policy_loss(shape, dtype, kl):
+    from speech_b200 import ops
+
+    n, t, c, v = shape
+    logits, targets, mask, old, ref, adv = make(n, t, c, v, dtype)
+    up = 512.0 if dtype == torch.float16 else 1.0
+    lp, m, w = plain_logp(logits, targets, mask)
+    for border in (0.8, 1.3):                                # no input lies on a clip border, where the slope jumps
+        old = torch.where((torch.exp(lp - old.double()) - border).abs() < 1e-3, old + 0.01, old)
+    x = logits.clone().requires_grad_()
+    loss, logp = ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref if kl else None, clip=0.2, clip_high=0.3, kl_beta=kl)
+    (g,) = torch.autograd.grad(loss, x, torch.tensor(up, device="cuda"))
+    tol = lp_tolerance(v)
+    assert bool(((logp.double() - lp).abs() <= tol + EPS[torch.float32] * lp.abs()).all())
+    assert bool((logp[~m] == 0).all())
+    a = adv.double().view((-1,) + (1,) * (targets.dim() - 1))
+    r = torch.exp(lp - old.double())
+    plain, clipped = r * a, r.clamp(0.8, 1.3) * a
+    term, slope = -torch.minimum(plain, clipped), torch.where(plain <= clipped, -plain, 0.0)
+    if kl:
+        d = ref.double() - lp
+        term, slope = term + kl * (torch.exp(d) - d - 1), slope + kl * (1 - torch.exp(d))
+    count = m.sum().clamp(min=1)
+    want = (term * m).sum() / count
+    reach = (((r * a).abs() + kl * (1 + torch.exp(ref.double() - lp))) * m).sum() / count          # how far the loss moves with the log-probabilities
+    assert abs(float(loss) - float(want)) <= 2.0 ** -23 * abs(float(want)) + float(reach) * tol
+    # the slope itself moves with the log-probability: r a and kl exp(d) by the same relative error
+    check_gradient(g, targets, w, slope * m / count * up, dtype, v)
+    hidden = ~m
+    assert bool((g[hidden] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES[:-1])
+@pytest.mark.parametrize("kind", ["dpo", "ipo", "rpo_sq"])
+def test_preference_loss(shape, dtype, kind):
+    from speech_b200 import ops
+
+    n, t, c, v = shape
+    n += n % 2
+    logits, targets, mask, _, ref, _ = make(n, t, c, v, dtype, seed=1)
+    beta, up, pairs = 0.1, 64.0 if dtype == torch.float16 else 1.0, n // 2
+    gap = torch.rand(pairs, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    x = logits.clone().requires_grad_()
+    loss, rewards = ops.preference_loss(x, targets, mask, ref, beta=beta, loss_type=kind, reward_gap=gap)
+    (g,) = torch.autograd.grad(loss, x, torch.tensor(up, device="cuda"))
+    lp, m, w = plain_logp(logits, targets, mask)
+    ratio = ((lp - ref.double()) * m).flatten(1).sum(1)
+    margin = ratio[:pairs] - ratio[pairs:]
+    tol = lp_tolerance(v) * m.flatten(1).sum(1).max()                                           # positions of a sequence, all off the same way
+    if kind == "dpo":
+        each, slope, bend = -torch.nn.functional.logsigmoid(beta * margin), -beta * torch.sigmoid(-beta * margin), beta ** 2
+    elif kind == "ipo":
+        each, slope, bend = (margin - 0.5 / beta) ** 2, 2 * (margin - 0.5 / beta), 2.0
+    else:
+        each, slope, bend = (beta * margin - gap.double()) ** 2, 2 * beta * (beta * margin - gap.double()), 2 * beta ** 2
+    assert bool(((rewards.double() - beta * ratio).abs() <= beta * tol + 2.0 ** -23 * (beta * ratio).abs()).all())
+    assert abs(float(loss) - float(each.mean())) <= float(slope.abs().max() * 2 * tol + bend * (2 * tol) ** 2) + 2.0 ** -23 * float(each.mean())
+    s = torch.cat([slope, -slope]).view((-1,) + (1,) * (targets.dim() - 1)) * m / pairs * up
+    want = -w * s.unsqueeze(-1)
+    want.scatter_add_(-1, targets.unsqueeze(-1), s.unsqueeze(-1))
+    one = lp_tolerance(v) * 2 + 2.0 ** -17
+    allow = EPS[dtype] * want.abs() + (s.abs() * one + m * bend * 2 * tol / pairs * up).unsqueeze(-1) * (w + torch.zeros_like(w).scatter_(-1, targets.unsqueeze(-1), 1.0)) \
+        + 2.0 ** -25 * (dtype == torch.float16) + 1e-38
+    assert bool(((g.double() - want).abs() <= allow).all()), float(((g.double() - want).abs() / allow).max())
+
+
+def test_strided_logits_and_hidden_garbage():
+    """Logits that are a slice of a longer tensor (rows at odd addresses), NaN and invalid targets at hidden positions."""
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(4, 7, 3, 333, torch.bfloat16)
+    longer = torch.full((4, 9, 3, 335), float("nan"), dtype=torch.bfloat16, device="cuda")
+    view = longer[:, 1:8, :, 1:334]
+    view.copy_(logits)
+    view[~mask] = float("nan")
+    t = targets.masked_fill(~mask.unsqueeze(-1), -100)
+
+    def policy(x, y):
+        return ops.policy_loss(x, y, mask, old, adv, ref_logp=ref, kl_beta=0.1)
+
+    for f in (policy, lambda x, y: ops.preference_loss(x, y, mask, ref)):
+        a, b = logits.clone().requires_grad_(), view.detach().requires_grad_()
+        (la, ea), (lb, eb) = f(a, targets), f(b, t)
+        # a row's groups start at another address, so its sum is taken in another order: both sides are within the log-probability's
+        # tolerance of the same value (times the 21 positions of a sequence for the rewards of the second loss, beta = 0.1)
+        assert bool(((ea.double() - eb.double()).abs() <= 2 * lp_tolerance(333) * (1 if f is policy else 2.1)).all())
+        assert bool((la.double() - lb.double()).abs() <= 2 * lp_tolerance(333) * 2.1 + 2.0 ** -23 * la.double().abs())
+        ga, gb = torch.autograd.grad(la, a)[0], torch.autograd.grad(lb, b)[0]
+        # and one step of the gradient's type
+        assert bool(((ga.double() - gb.double()).abs() <= 2.0 ** -7 * ga.double().abs() + 1e-12).all())
+
+
+def test_second_backward_other_upstream_and_determinism():
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(8, 33, 8, 2024, torch.bfloat16)
+    x = logits.clone().requires_grad_()
+
+    def f():
+        return ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.04)[0]
+
+    loss = f()
+    (a,) = torch.autograd.grad(loss, x, retain_graph=True)
+    kept = a.clone()
+    (b,) = torch.autograd.grad(loss, x, torch.tensor(0.5, device="cuda"), retain_graph=True)
+    assert torch.equal(a, kept), "a second backward pass has written into the first one's gradient"
+    (c,) = torch.autograd.grad(loss, x)
+    again = f()
+    (d,) = torch.autograd.grad(again, x)
+    assert torch.equal(loss, again) and torch.equal(a, d)
+    # recomputed from memory: another exponential, one step of the result's type apart at most
+    assert bool(((c.double() - a.double()).abs() <= 2.0 ** -7 * a.double().abs() + 1e-12).all())
+    assert bool(((2 * b.double() - a.double()).abs() <= 2.0 ** -7 * a.double().abs() + 1e-12).all())
+    p = ops.preference_loss(x, targets, mask, ref)[0]
+    assert torch.equal(torch.autograd.grad(p, x, retain_graph=True)[0], torch.autograd.grad(p, x)[0])
+
+
+def test_invalid_target_is_loud_and_stays_in_bounds():
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(2, 3, None, 64, torch.bfloat16, whole=True)
+    for bad in (-1, 64, 2 ** 40):
+        t = targets.clone()
+        t[0, 1] = bad
+        loss, logp = ops.policy_loss(logits, t, mask, old, adv)
+        assert bool(torch.isnan(loss)) and bool(torch.isnan(logp[0, 1])) and not bool(torch.isnan(logp[1]).any())
+
+
+def test_extreme_logits():
+    """The type's lowest value and -inf as vocabulary masks, a row that is all one value."""
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(2, 4, None, 500, torch.bfloat16, whole=True)
+    targets.clamp_(max=249)
+    logits[0, :, 250:] = float("-inf")
+    logits[1, :, 250:] = torch.finfo(torch.bfloat16).min
+    logits[1, 3] = 3.0
+    x = logits.clone().requires_grad_()
+    loss, logp = ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.1)
+    (g,) = torch.autograd.grad(loss, x)
+    assert bool(torch.isfinite(loss)) and bool(torch.isfinite(g).all())
+    assert bool((g[0, :, 250:] == 0).all()) and bool((g[1, :3, 250:] == 0).all())
+    lp, _, _ = plain_logp(logits, targets, mask)
+    assert bool(((logp.double() - lp).abs() <= lp_tolerance(500)).all())
+
+
+def test_captured_and_replayed():
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(4, 9, 2, 2024, torch.bfloat16)
+    x = logits.clone().requires_grad_()
+
+    def step():
+        loss, logp = ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.04)
+        (g,) = torch.autograd.grad(loss, x)
+        p, rewards = ops.preference_loss(x, targets, mask, ref)
+        (h,) = torch.autograd.grad(p, x)
+        return loss, logp, g, p, rewards, h
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    other = make(4, 9, 2, 2024, torch.bfloat16, seed=9)
+    with torch.no_grad():
+        x.copy_(other[0])
+    for a, b in zip((targets, mask, old, ref, adv), other[1:]):
+        a.copy_(b)
+    graph.replay()
+    want = [o.detach().clone() for o in step()]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
