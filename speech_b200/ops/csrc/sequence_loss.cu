@@ -12,12 +12,15 @@
 // slope needs both sequences of the pair, so the rows are read a second time; the gradient kernel walks them backwards, and what
 // the forward pass read last is then still in the L2.
 //
-// Rounding: exponentials and sums over a thread's share of a row are fp32, shares are joined in fp64, and logarithm, ratio,
-// clip decision and the sums over rows are fp64: a policy at its reference has log ratios near zero, and in fp32 the rounding of
-// a logp of -8 (5e-7) would be all that is left after a few thousand positions are summed.  The gradient is rounded once.
-// Every sum has a fixed order (no floating-point atomics).
+// Rounding: exponentials and a thread's share of a row's sum are fp32, shares are joined in fp64, and logp, the clip decision and
+// the sums over rows are fp64: a policy at its reference has log ratios near zero, and in fp32 the rounding of a logp of -8 (5e-7)
+// would be all that is left after a few thousand positions are summed.  For the same reason the exponent of a summed term is
+// t log2(e) with log2(e) in two parts: the fp32 constant alone is 1.3e-8 too small, which moves every row's log sum the same way.
+// log s = k ln 2 + log f with s = 2^k f, f in [0.71, 1.42): the fp32 logarithm of f is off by less than 2^-25.
+// The gradient is rounded once.  Every sum has a fixed order (no floating-point atomics).
 #include "common.cuh"
 #include <cuda_fp16.h>
+#include <math.h>
 
 namespace {
 
@@ -84,6 +87,7 @@ struct RowArgs {
   long long rows;
   int T, C, V;
   float clip_lo, clip_hi, kl_beta;
+  double log_lo, log_hi;             // log(1 - clip_lo), log(1 + clip_hi): the clip decision is taken on log ratios
 };
 
 struct Row { long long n, nt; long long off; };
@@ -112,30 +116,60 @@ template <typename T> __device__ __forceinline__ Span span_of(const T* p, int V)
 // (max, sum) pairs with sum taken relative to max; an empty share is (-inf, 0)
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.f : m; }
 
-// TPR threads work on a row: one warp (TPR = 32) or a whole block.  NV > 0: the row stays in registers, NV 16-byte groups per
-// thread; NV = 0: rows of any length, read again (from the L2: 148 rows of 300 KB in flight are a third of it) for the gradient.
-template <int TPR> __device__ __forceinline__ float group_max(float v, float* red) {
-  v = warp_max(v);
-  if (TPR == 32) return v;
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = red[0];
-#pragma unroll
-  for (int i = 1; i < TPR / 32; ++i) r = fmaxf(r, red[i]);
-  return r;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-template <int TPR> __device__ __forceinline__ double group_sum(double v, double* red) {
+constexpr float LOG2E_HI = 1.44269502f, LOG2E_LO = 1.92596303e-8f;
+__device__ __forceinline__ float exp_exact(float t) { return ex2(fmaf(t, LOG2E_HI, t * LOG2E_LO)); }
+
+// Softmax weights of the gradient, times `inv`: exp(x - shift).  For 16-bit logits one fused multiply-add gives the exponent (the
+// product shift log2(e), rounded to fp32, makes a weight off by less than 2^-18, far below half a step of the result).
+template <typename T> struct Weight {
+  float shift;
+  __device__ __forceinline__ explicit Weight(float s) : shift(s * LOG2E_HI) {}
+  __device__ __forceinline__ float operator()(float x) const { return ex2(fmaf(x, LOG2E_HI, -shift)); }
+};
+template <> struct Weight<float> {
+  float shift;
+  __device__ __forceinline__ explicit Weight(float s) : shift(s) {}
+  __device__ __forceinline__ float operator()(float x) const { return exp_exact(x - shift); }
+};
+
+// Joins the (max, sum) shares of the TPR threads of a row: one warp (TPR = 32) or a whole block.
+template <int TPR> __device__ __forceinline__ void join(float& m, double& sum, float share, float* redf, double* redd) {
+  const float wm = warp_max(m);
+  double v = (double)(share * exp_exact(finite_or_zero(m) - finite_or_zero(wm)));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (TPR == 32) return v;
+  if (TPR == 32) {
+    m = finite_or_zero(wm);
+    sum = v;
+    return;
+  }
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  if ((threadIdx.x & 31) == 0) {
+    redf[threadIdx.x >> 5] = wm;
+    redd[threadIdx.x >> 5] = v;
+  }
   __syncthreads();
-  double r = red[0];
+  float bm = redf[0];
 #pragma unroll
-  for (int i = 1; i < TPR / 32; ++i) r += red[i];
-  return r;
+  for (int i = 1; i < TPR / 32; ++i) bm = fmaxf(bm, redf[i]);
+  m = finite_or_zero(bm);
+  sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < TPR / 32; ++i) sum += redd[i] * (double)exp_exact(finite_or_zero(redf[i]) - m);
+}
+
+__device__ __forceinline__ double log_of_sum(double s) {
+  // s = 2^k f; also right for 0 (-inf), infinity and NaN, which the scaling leaves alone
+  if (!(s > 1e-30 && s < 1e30)) return (double)logf((float)s);
+  const float f = (float)s;
+  int k = ((__float_as_int(f) - 0x3f350000) >> 23);
+  const double scaled = s * __longlong_as_double((long long)(1023 - k) << 52);
+  return (double)k * 0.693147180559945309417 + (double)logf((float)scaled);
 }
 
 template <typename T> __device__ __forceinline__ T* out_row(void* d, long long row, int V) { return reinterpret_cast<T*>(d) + row * V; }
@@ -150,13 +184,13 @@ template <typename T, int TPR> __device__ __forceinline__ void write_zeros(T* o,
 
 // Gradient of a row read again from memory: slope * (1[v = y] - exp(x - shift) * inv).  Input and output may be aligned differently
 // (logits that are a slice of a longer tensor): groups are formed on the output where the input allows it, else one by one.
+// The thread that wrote the target's element writes it once more, with its 1.
 template <typename T, int TPR>
 __device__ __forceinline__ void grad_from_memory(const T* x, T* o, int V, int lane, int y, float slope, float shift, float inv) {
   const bool same = ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
-  auto one = [&](int v) {
-    const float p = __expf(Vec<T>::up(x[v]) - shift) * inv;
-    o[v] = Vec<T>::down(slope * ((v == y ? 1.f : 0.f) - p));
-  };
+  const Weight<T> weight(shift);
+  const float k = -slope * inv;
+  auto one = [&](int v) { o[v] = Vec<T>::down(fmaf(k, weight(Vec<T>::up(x[v])), v == y ? slope : 0.f)); };
   if (!same) {
     for (int v = lane; v < V; v += TPR) one(v);
     return;
@@ -164,23 +198,27 @@ __device__ __forceinline__ void grad_from_memory(const T* x, T* o, int V, int la
   constexpr int E = Vec<T>::N;
   const Span s = span_of(x, V);
   if (lane < s.head) one(lane);
+  if (lane < s.tail) one(s.head + s.nv * E + lane);
   const uint4* xv = reinterpret_cast<const uint4*>(x + s.head);
   uint4* ov = reinterpret_cast<uint4*>(o + s.head);
+#pragma unroll 4
   for (int i = lane; i < s.nv; i += TPR) {
     float f[E];
     Vec<T>::unpack(xv[i], f);
-    const int v0 = s.head + i * E;
 #pragma unroll
-    for (int u = 0; u < E; ++u) f[u] = slope * ((v0 + u == y ? 1.f : 0.f) - __expf(f[u] - shift) * inv);
+    for (int u = 0; u < E; ++u) f[u] = k * weight(f[u]);
     ov[i] = Vec<T>::pack(f);
   }
-  if (lane < s.tail) one(s.head + s.nv * E + lane);
+  const int yv = y - s.head;
+  if (yv >= 0 && yv < s.nv * E && (yv / E) % TPR == lane) one(y);
 }
 
 enum { LOSS_POLICY = 0, LOSS_PREFERENCE = 1 };
 
-// Forward pass over all rows.  lse / logp / slope: fp32 [rows]; dlogits: contiguous [rows, V] or null (no gradient wanted now);
-// partial: fp64, per block the sum of its policy terms; ratio: fp64 [rows], preference only.
+// Forward pass over all rows.  TPR threads work on a row; NV > 0: it stays in registers as it was read, NV 16-byte groups per thread;
+// NV = 0: rows of any length, read again for the gradient, from the L2 (148 rows of 300 KB in flight are a third of it).
+// lse / logp / slope: fp32 [rows]; dlogits: contiguous [rows, V] or null (no gradient wanted now); partial: fp64, per block the sum of
+// its policy terms; ratio: fp64 [rows], preference only.
 template <typename T, int MODE, int TPR, int NV, int THREADS>
 __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, const int* __restrict__ count_p, float* __restrict__ logp_out, float* __restrict__ lse_out,
                                                                float* __restrict__ slope_out, void* __restrict__ dlogits, double* __restrict__ partial,
@@ -190,7 +228,7 @@ __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, 
   __shared__ double redd[32];
   const int lane = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
   const int group = TPR == 32 ? (threadIdx.x >> 5) : 0;
-  const double inv_count = MODE == LOSS_POLICY ? 1.0 / (double)max(1, *count_p) : 0.0;
+  const float inv_count = MODE == LOSS_POLICY ? (float)(1.0 / (double)max(1, *count_p)) : 0.f;
   double mine = 0.0;                                     // same value in every thread of the group
   for (long long row = (long long)blockIdx.x * GROUPS + group; row < a.rows; row += (long long)gridDim.x * GROUPS) {
     const Row r = locate(a, row);
@@ -205,84 +243,79 @@ __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, 
       continue;
     }
     const T* x = reinterpret_cast<const T*>(a.logits) + r.off;
+    const Span s = span_of(x, a.V);
+    const uint4* xv = reinterpret_cast<const uint4*>(x + s.head);
+    const int vt = s.head + s.nv * E;
+    uint4 raw[NV > 0 ? NV : 1];
+    if (NV > 0) {
+#pragma unroll
+      for (int k = 0; k < NV; ++k)
+        if (lane + k * TPR < s.nv) raw[k] = __ldcs(xv + lane + k * TPR);
+    }
     const long long y64 = a.targets[row];
     const bool known = y64 >= 0 && y64 < a.V;            // a target outside the vocabulary makes the row's results NaN
     const int y = known ? (int)y64 : -1;
     const float xy = known ? Vec<T>::up(x[y]) : NAN;
-    const Span s = span_of(x, a.V);
-    const uint4* xv = reinterpret_cast<const uint4*>(x + s.head);
-    const int vt = s.head + s.nv * E;
-    float hx = lane < s.head ? Vec<T>::up(x[lane]) : -INFINITY;
-    float tx = lane < s.tail ? Vec<T>::up(x[vt + lane]) : -INFINITY;
-    float m, share;
-    float e[NV > 0 ? NV : 1][E];
+    const float old = MODE == LOSS_POLICY ? a.old[row] : 0.f, ref = a.ref ? a.ref[row] : 0.f, A = MODE == LOSS_POLICY ? a.adv[r.n] : 0.f;
+    const float hx = lane < s.head ? Vec<T>::up(x[lane]) : -INFINITY;
+    const float tx = lane < s.tail ? Vec<T>::up(x[vt + lane]) : -INFINITY;
+    float m = fmaxf(hx, tx), share;
     if (NV > 0) {
-      uint4 raw[NV > 0 ? NV : 1];
 #pragma unroll
       for (int k = 0; k < NV; ++k)
-        if (lane + k * TPR < s.nv) raw[k] = xv[lane + k * TPR];
-      m = fmaxf(hx, tx);
+        if (lane + k * TPR < s.nv) {
+          float f[E];
+          Vec<T>::unpack(raw[k], f);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        if (lane + k * TPR < s.nv) Vec<T>::unpack(raw[k], e[k]);
-        else {
-#pragma unroll
-          for (int u = 0; u < E; ++u) e[k][u] = -INFINITY;
+          for (int u = 0; u < E; ++u) m = fmaxf(m, f[u]);
         }
+      const float base = finite_or_zero(m);
+      share = exp_exact(hx - base) + exp_exact(tx - base);
 #pragma unroll
-        for (int u = 0; u < E; ++u) m = fmaxf(m, e[k][u]);
-      }
-      m = finite_or_zero(group_max<TPR>(m, redf));
-      hx = __expf(hx - m);
-      tx = __expf(tx - m);
-      share = hx + tx;
+      for (int k = 0; k < NV; ++k)
+        if (lane + k * TPR < s.nv) {
+          float f[E], part = 0.f;
+          Vec<T>::unpack(raw[k], f);
 #pragma unroll
-      for (int k = 0; k < NV; ++k) {
-        float part = 0.f;
-#pragma unroll
-        for (int u = 0; u < E; ++u) {
-          e[k][u] = __expf(e[k][u] - m);
-          part += e[k][u];
+          for (int u = 0; u < E; ++u) part += exp_exact(f[u] - base);
+          share += part;
         }
-        share += part;
-      }
     } else {
-      float tm = fmaxf(hx, tx), ts = 0.f;
-      ts = __expf(hx - finite_or_zero(tm)) + __expf(tx - finite_or_zero(tm));
+      share = exp_exact(hx - finite_or_zero(m)) + exp_exact(tx - finite_or_zero(m));
 #pragma unroll 4
       for (int i = lane; i < s.nv; i += TPR) {
-        float f[E];
+        float f[E], nm = m, part = 0.f;
         Vec<T>::unpack(xv[i], f);
-        float nm = tm;
 #pragma unroll
         for (int u = 0; u < E; ++u) nm = fmaxf(nm, f[u]);
-        const float ref_m = finite_or_zero(nm);
-        float part = 0.f;
+        const float base = finite_or_zero(nm);
+        if (nm > m) {                                    // rare after the first groups
+          share *= exp_exact(finite_or_zero(m) - base);
+          m = nm;
+        }
 #pragma unroll
-        for (int u = 0; u < E; ++u) part += __expf(f[u] - ref_m);
-        ts = ts * __expf(finite_or_zero(tm) - ref_m) + part;
-        tm = nm;
+        for (int u = 0; u < E; ++u) part += exp_exact(f[u] - base);
+        share += part;
       }
-      m = finite_or_zero(group_max<TPR>(tm, redf));
-      share = ts * __expf(finite_or_zero(tm) - m);
     }
-    const double sum = group_sum<TPR>((double)share, redd);
-    const double log_sum = log(sum);
+    double sum;
+    join<TPR>(m, sum, share, redf, redd);
+    const double log_sum = log_of_sum(sum);
     const double logp = (double)xy - (double)m - log_sum;
     float slope = 0.f;
     if (MODE == LOSS_POLICY) {
-      const double rt = exp(logp - (double)a.old[row]), A = (double)a.adv[r.n];
-      const double lo = 1.0 - (double)a.clip_lo, hi = 1.0 + (double)a.clip_hi;
-      const double plain = rt * A, clipped = (rt < lo ? lo : (rt > hi ? hi : rt)) * A;
-      const bool inside = plain <= clipped;
-      double term = -(inside || plain != plain ? plain : clipped), sl = inside || plain != plain ? -plain : 0.0;
+      const double d = logp - (double)old;
+      const float plain = expf((float)d) * A;
+      const bool above = A > 0.f && d > a.log_hi, below = A < 0.f && d < a.log_lo;   // NaN is neither
+      float term = above ? -(1.f + a.clip_hi) * A : below ? -(1.f - a.clip_lo) * A : -plain;
+      slope = above || below ? 0.f : -plain;
       if (a.ref && a.kl_beta != 0.f) {
-        const double d = (double)a.ref[row] - logp, ed = exp(d);
-        term += (double)a.kl_beta * (ed - d - 1.0);
-        sl += (double)a.kl_beta * (1.0 - ed);
+        const float kd = (float)((double)ref - logp), em = expm1f(kd);
+        term += a.kl_beta * (em - kd);
+        slope -= a.kl_beta * em;
       }
-      mine += term;
-      slope = (float)(sl * inv_count);
+      mine += (double)term;
+      slope *= inv_count;
     }
     if (lane == 0) {
       lse_out[row] = (float)((double)m + log_sum);
@@ -290,7 +323,7 @@ __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, 
         logp_out[row] = (float)logp;
         slope_out[row] = slope;
       } else {
-        ratio[row] = logp - (double)a.ref[row];
+        ratio[row] = logp - (double)ref;
       }
     }
     if (MODE == LOSS_POLICY && o) {
@@ -298,21 +331,25 @@ __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, 
         write_zeros<T, TPR>(o, a.V, lane);
         continue;
       }
-      const float inv = (float)(1.0 / sum);
+      const float inv = 1.f / (float)sum;
       if (NV > 0 && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
-        const float si = slope * inv;
+        const Weight<T> weight(m);
+        const float k0 = -slope * inv;
+        auto put = [&](int v, float xf) { o[v] = Vec<T>::down(fmaf(k0, weight(xf), v == y ? slope : 0.f)); };
         uint4* ov = reinterpret_cast<uint4*>(o + s.head);
-        if (lane < s.head) o[lane] = Vec<T>::down((lane == y ? slope : 0.f) - hx * si);
+        if (lane < s.head) put(lane, hx);
+        if (lane < s.tail) put(vt + lane, tx);
 #pragma unroll
         for (int k = 0; k < NV; ++k)
           if (lane + k * TPR < s.nv) {
-            const int v0 = s.head + (lane + k * TPR) * E;
             float f[E];
+            Vec<T>::unpack(raw[k], f);
 #pragma unroll
-            for (int u = 0; u < E; ++u) f[u] = (v0 + u == y ? slope : 0.f) - e[k][u] * si;
-            ov[lane + k * TPR] = Vec<T>::pack(f);
+            for (int u = 0; u < E; ++u) f[u] = k0 * weight(f[u]);
+            __stcs(ov + lane + k * TPR, Vec<T>::pack(f));
           }
-        if (lane < s.tail) o[vt + lane] = Vec<T>::down((vt + lane == y ? slope : 0.f) - tx * si);
+        const int yv = y - s.head;                        // the target's element once more, by the thread that wrote its group
+        if (yv >= 0 && yv < s.nv * E && (yv / E) % TPR == lane) put(y, xy);
       } else {
         grad_from_memory<T, TPR>(x, o, a.V, lane, y, slope, m, inv);
       }
@@ -450,13 +487,14 @@ __global__ void preference_finish_kernel(const double* __restrict__ total, int p
   }
 }
 
-constexpr int MAX_BLOCKS = 148 * 8;
+constexpr int MAX_BLOCKS = 148 * 16;
 
 template <typename T, int MODE, int TPR, int NV, int THREADS>
 int run_forward(const RowArgs& a, const int* count, float* logp, float* lse, float* slope, void* dlogits, double* partial, double* ratio, int* blocks,
                 cudaStream_t stream) {
   long long need = (a.rows + THREADS / TPR - 1) / (THREADS / TPR);
-  const long long cap = (long long)sb_num_sms() * 8 < MAX_BLOCKS ? (long long)sb_num_sms() * 8 : MAX_BLOCKS;
+  const long long fit = (long long)sb_num_sms() * (2048 / THREADS);
+  const long long cap = fit < MAX_BLOCKS ? fit : MAX_BLOCKS;
   *blocks = (int)(need < cap ? need : cap);
   rows_forward_kernel<T, MODE, TPR, NV, THREADS><<<*blocks, THREADS, 0, stream>>>(a, count, logp, lse, slope, dlogits, partial, ratio);
   return (int)cudaGetLastError();
@@ -465,11 +503,12 @@ int run_forward(const RowArgs& a, const int* count, float* logp, float* lse, flo
 template <typename T, int MODE>
 int forward(const RowArgs& a, const int* count, float* logp, float* lse, float* slope, void* dlogits, double* partial, double* ratio, int* blocks,
             cudaStream_t stream) {
-  // a row that fits eight 16-byte groups per lane of a warp, or per thread of a block, stays in registers
+  // a row that fits eight 16-byte groups per thread of a warp or block stays in registers
   const long long groups = a.V / Vec<T>::N;
   if (groups <= 32 * 2) return run_forward<T, MODE, 32, 2, 256>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
-  if (groups <= 32 * 8) return run_forward<T, MODE, 32, 8, 256>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
-  if (groups <= 256 * 8) return run_forward<T, MODE, 256, 8, 256>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
+  if (groups <= 32 * 8) return run_forward<T, MODE, 32, 8, 128>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
+  if (groups <= 128 * 8) return run_forward<T, MODE, 128, 8, 128>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
+  if (groups <= 512 * 8) return run_forward<T, MODE, 512, 8, 512>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
   return run_forward<T, MODE, 512, 0, 512>(a, count, logp, lse, slope, dlogits, partial, ratio, blocks, stream);
 }
 
@@ -511,6 +550,8 @@ SB_API int sb_policy_loss_fwd(const void* logits, int type, long long sn, long l
     return SB_BAD_ARGUMENT;
   a.old = old_logp; a.ref = ref_logp; a.adv = adv;
   a.clip_lo = clip_lo; a.clip_hi = clip_hi; a.kl_beta = kl_beta;
+  a.log_lo = clip_lo < 1.f ? log(1.0 - (double)clip_lo) : -HUGE_VAL;
+  a.log_hi = log(1.0 + (double)clip_hi);
   count_kernel<<<1, 1024, 0, stream>>>(mask, N * T, C, count);
   int blocks = 0, rc;
   if (type == 0) rc = forward<__nv_bfloat16, LOSS_POLICY>(a, count, logp, lse, slope, dlogits, partial, nullptr, &blocks, stream);
