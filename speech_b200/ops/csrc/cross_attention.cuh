@@ -1,0 +1,160 @@
+// Shared parts of the fused cross-attention kernels (cross_attention_fwd.cu, cross_attention_bwd.cu).
+//
+// All query rows that read the same memory and key head are packed: row r in [0, R), R = G * rep * Tq, is token t = r % Tq of query
+// head hk * rep + (r / Tq) % rep of batch row m * G + r / (Tq * rep).  A tile of 128 packed rows therefore never mixes memories,
+// short queries of several heads or beams fill one tile, and the sums over shared heads and shared rows need no second pass.
+#pragma once
+#include "tcgen05.cuh"
+#include <cuda_fp16.h>
+
+struct XAttnArgs {
+  const void* q;                       // [B, Tq, H, D], element strides below, D contiguous
+  long long q_sb, q_st, q_sh;
+  const int* lengths;                  // [M] visible keys, null = Tk; clamped to [0, Tk]
+  const uint8_t* mask;                 // [M, Tk] non-zero = hidden, or null
+  int M, G, rep, Tq, Tk, H, Hk, D;
+  int R;                               // packed rows of one (memory, key head)
+  float c;                             // softmax scale * log2(e): probabilities are powers of two of c * score
+  int* status;
+};
+
+namespace {
+
+template <typename T> struct Half2;    // 16-bit types of the tensor core
+template <> struct Half2<__nv_bfloat16> {
+  static constexpr uint32_t KIND = 1;  // operand type field of the instruction descriptor
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+};
+template <> struct Half2<__half> {
+  static constexpr uint32_t KIND = 0;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&t);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+};
+
+// D fp32, A and B of type KIND, B either K-major or MN-major, M = 128
+template <typename T> constexpr uint32_t instr_desc(int n, bool b_mn) {
+  return (1u << 4) | (Half2<T>::KIND << 7) | (Half2<T>::KIND << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// A operand in tensor memory (128 lanes, two 16-bit elements per column), B in shared memory
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Load and wait in one statement, so that no use of the registers can be scheduled before the wait.
+__device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+        "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// whole-warp bounded wait: the same answer in every lane, so that the .aligned instructions that follow stay converged
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* status, int code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code) ? 1 : 0) != 0;
+}
+
+struct RowAt { int b, t, h; };
+__device__ __forceinline__ RowAt row_at(const XAttnArgs& a, int m, int hk, int r) {
+  const int x = r / a.Tq, g = x / a.rep;
+  return {m * a.G + g, r - x * a.Tq, hk * a.rep + x - g * a.rep};
+}
+
+__device__ __forceinline__ int visible_keys(const XAttnArgs& a, int m) {
+  if (!a.lengths) return a.Tk;
+  const int n = a.lengths[m];
+  return n < 0 ? 0 : (n > a.Tk ? a.Tk : n);
+}
+
+// Bit i of the result: key first + i of memory m is hidden.  One word per call, the same in every lane.
+__device__ __forceinline__ uint32_t hidden_word(const XAttnArgs& a, int m, int len, int first, int lane) {
+  const int key = first + lane;
+  bool hide = key >= len;
+  if (a.mask && !hide) hide = a.mask[(long long)m * a.Tk + key] != 0;
+  return __ballot_sync(0xffffffffu, hide);
+}
+
+// Rows of a [rows, DP] operand tile in shared memory: 64-element halves of 128-byte rows, 16-byte chunks XORed with the row (the
+// 128-byte swizzle of TMA and of the matrix descriptors).
+__device__ __forceinline__ uint32_t tile_addr(uint32_t base, int rows, int row, int chunk) {
+  return base + (uint32_t)(chunk >> 3) * (uint32_t)(rows * 128) + (uint32_t)row * 128u + (uint32_t)(((chunk & 7) ^ (row & 7)) << 4);
+}
+
+// The four warps of a warpgroup copy packed rows [row0, row0 + 128) of a [B, Tq, H, D] tensor into a swizzled tile; rows beyond R
+// and columns beyond D become zero.
+template <int DP>
+__device__ __forceinline__ void load_rows(const XAttnArgs& a, const void* src, long long sb, long long st, long long sh, int m, int hk, int row0,
+                                          uint32_t tile, int wg_warp, int lane) {
+  constexpr int CH = DP / 8, RPI = 32 / CH;               // 16-byte chunks of a row, rows per instruction
+  const int sub = lane / CH, ch = lane % CH;
+#pragma unroll 4
+  for (int i = 0; i < 32; i += RPI) {
+    const int row = wg_warp * 32 + i + sub;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row0 + row < a.R && ch * 8 < a.D) {
+      const RowAt w = row_at(a, m, hk, row0 + row);
+      v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(src) + w.b * sb + w.t * st + w.h * sh + ch * 8);
+    }
+    st_shared_v4(tile_addr(tile, 128, row, ch), v.x, v.y, v.z, v.w);
+  }
+}
+
+// Zeroes the rows of a [rows, DP] tile whose keys are hidden (bits of `words`, 32 rows each): a hidden value of infinity or NaN would
+// turn its zero weight into NaN inside the matrix product.
+template <int DP>
+__device__ __forceinline__ void clear_rows(uint32_t tile, int rows, const uint32_t* words, int nwords, int lane) {
+  constexpr int CH = DP / 8;
+  for (int w = 0; w < nwords; ++w) {
+    uint32_t bits = words[w];
+    while (bits) {
+      const int row = w * 32 + __ffs(bits) - 1;
+      bits &= bits - 1;
+      if (lane < CH) st_shared_v4(tile_addr(tile, rows, row, lane), 0, 0, 0, 0);
+    }
+  }
+}
+
+}  // namespace

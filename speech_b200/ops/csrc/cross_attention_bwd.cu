@@ -1,0 +1,610 @@
+// Fused cross attention, backward:   p = 2^(c s - lse),  dp = do v^T,  ds = p (dp - delta),  delta = sum_d do o
+//   dq = scale ds k        (one CTA per 256 packed query rows, keys stream past: xattn_dq_kernel)
+//   dv = p^T do, dk = scale ds^T q   (one CTA per 128 keys, packed query rows stream past: xattn_dkv_kernel)
+//
+// Probabilities are computed again from the scores and the row's lse, in both kernels: seven products where one kernel with shared
+// sums of dq would need five, but every sum is taken by one CTA in a fixed order, so that gradients are the same every time, nothing
+// is accumulated in fp32 memory and converted afterwards, and gradients of shared heads and shared rows are sums over packed rows.
+//
+// Both kernels have the roles of the forward pass.  dq: two tiles of 128 rows take turns, 64 keys at a time (scores, dp: 64 columns of
+// tensor memory each, dq: DP columns, per tile).  dk / dv: tiles of 64 packed rows take turns in two sets of tensor memory columns,
+// transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax.
+//
+// Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
+// matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do| of the call to [8, 16), and
+// the sums are scaled back, so that neither small weights nor small upstream gradients fall below the type's normal range.
+#include "cross_attention.cuh"
+#include "cross_attention_host.h"
+
+namespace {
+
+constexpr int BWD_THREADS = 384;
+constexpr int MAX_PARTS = 592;        // blocks of the row kernel, whose maxima every block of the other kernels joins
+
+template <typename T> constexpr float p_shift() { return Half2<T>::KIND == 0 ? 12.f : 0.f; }
+
+struct BwdArgs {
+  const uint16_t* dout;               // contiguous [B, Tq, H, D]
+  const uint16_t* out;
+  const float* lse;                   // [M * Hk, R]
+  float* delta;                       // [M * Hk, R]
+  float* peak;                        // fp16: largest |do| of every block of the row kernel
+  int peaks;
+  float scale;
+};
+
+// delta of every packed row, and the largest |do|.  One warp per row of up to 128 elements.
+template <typename T>
+__global__ void __launch_bounds__(256) xattn_delta_kernel(const XAttnArgs a, const BwdArgs b) {
+  __shared__ float red[8];
+  const long long rows = (long long)a.M * a.Hk * a.R;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int sub = lane >> 4, ch = lane & 15;              // 16 lanes of 8 elements per row, two rows per warp
+  float peak = 0.f;
+  for (long long i0 = ((long long)blockIdx.x * 8 + warp) * 2; i0 < rows; i0 += (long long)gridDim.x * 16) {
+    const long long i = i0 + sub;
+    float d = 0.f;
+    if (i < rows && ch * 8 < a.D) {
+      const int unit = (int)(i / a.R);
+      const RowAt at = row_at(a, unit / a.Hk, unit % a.Hk, (int)(i - (long long)unit * a.R));
+      const long long off = (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D + ch * 8;
+      const uint4 x = *reinterpret_cast<const uint4*>(b.dout + off), y = *reinterpret_cast<const uint4*>(b.out + off);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = Half2<T>::unpack(xs[k]), e = Half2<T>::unpack(ys[k]);
+        d += f.x * e.x + f.y * e.y;
+        if (Half2<T>::KIND == 0) peak = fmaxf(peak, fmaxf(fabsf(f.x), fabsf(f.y)));
+      }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (i < rows && ch == 0) b.delta[i] = d;
+  }
+  if (Half2<T>::KIND == 0) {
+    peak = warp_max(peak);
+    if (lane == 0) red[warp] = peak;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int w = 1; w < 8; ++w) peak = fmaxf(peak, red[w]);
+      b.peak[blockIdx.x] = peak;
+    }
+  }
+}
+
+// Power of two that brings the largest |do| to [8, 16); 1 for bf16, whose range needs none.  One warp.
+template <typename T> __device__ __forceinline__ float ds_scale(const BwdArgs& b, int lane) {
+  if (Half2<T>::KIND != 0) return 1.f;
+  float peak = 0.f;
+  for (int i = lane; i < b.peaks; i += 32) peak = fmaxf(peak, b.peak[i]);
+  peak = warp_max(peak);
+  if (!(peak > 0.f) || !(peak < 3e38f)) return 1.f;
+  return __int_as_float((127 + 3 - ((__float_as_int(peak) >> 23) - 127)) << 23);   // |do| of fp16 lies between 2^-24 and 2^16
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack_ds(float x, float y) {
+  if (Half2<T>::KIND == 0) {                               // beyond the type's range only for values far above any activation: saturate
+    x = fminf(fmaxf(x, -65504.f), 65504.f);
+    y = fminf(fmaxf(y, -65504.f), 65504.f);
+  }
+  return Half2<T>::pack(x, y);
+}
+
+template <typename T> __device__ __forceinline__ void store_row32(uint16_t* dst, int col, int D, const uint32_t* r, float f) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 8)
+    if (col + k < D) {
+      uint4 v;
+      v.x = Half2<T>::pack(__uint_as_float(r[k]) * f, __uint_as_float(r[k + 1]) * f);
+      v.y = Half2<T>::pack(__uint_as_float(r[k + 2]) * f, __uint_as_float(r[k + 3]) * f);
+      v.z = Half2<T>::pack(__uint_as_float(r[k + 4]) * f, __uint_as_float(r[k + 5]) * f);
+      v.w = Half2<T>::pack(__uint_as_float(r[k + 6]) * f, __uint_as_float(r[k + 7]) * f);
+      *reinterpret_cast<uint4*>(dst + col + k) = v;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ dq
+template <int DP> struct DqSmem {
+  static constexpr int BN = 64;
+  static constexpr int STAGES = DP == 128 ? 3 : 4;
+  static constexpr int ROWS = 128 * DP * 2, KEYS = BN * DP * 2;
+  static constexpr int DO0 = 2 * ROWS, KV0 = 4 * ROWS, BAR = KV0 + STAGES * 2 * KEYS;
+  static constexpr int BYTES = BAR + 256 + 1024;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(BWD_THREADS, 1)
+xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq) {
+  using S = DqSmem<DP>;
+  constexpr int BN = S::BN, HALVES = DP / 64;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = base + S::BAR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto kv_full = [&](int s) { return bars + 8u * s; };
+  auto kv_clean = [&](int s) { return bars + 8u * (4 + s); };
+  auto kv_empty = [&](int s) { return bars + 8u * (8 + s); };
+  auto s_full = [&](int t) { return bars + 8u * (12 + t); };
+  auto ds_full = [&](int t) { return bars + 8u * (14 + t); };
+  auto dq_full = [&](int t) { return bars + 8u * (16 + t); };
+  const uint32_t rows_ready = bars + 8u * 18, tmem_slot = bars + 8u * 19, scale_slot = tmem_slot + 4;
+
+  const int pairs = (a.R + 255) / 256;
+  const int unit = blockIdx.x / pairs, m = unit / a.Hk, hk = unit % a.Hk;
+  const int row0 = (blockIdx.x - unit * pairs) * 256;
+  const int tiles = a.R - row0 > 128 ? 2 : 1;
+  const int len = visible_keys(a, m);
+  const int nt = (len + BN - 1) / BN;
+  const bool hide = a.mask != nullptr;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_clean(s), 1); mbar_init(kv_empty(s), 1); }
+    for (int t = 0; t < 2; ++t) { mbar_init(s_full(t), 1); mbar_init(ds_full(t), 4); mbar_init(dq_full(t), 1); }
+    mbar_init(rows_ready, 4 * tiles);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == 3) {
+    const float f = ds_scale<T>(b, lane);
+    if (lane == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale_slot), "f"(f) : "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
+
+  if (warp == 0) {
+    int s = 0, issued = 0;
+    uint32_t ph = 0;
+    for (int j = 0; j < nt; ++j) {
+      if (!warp_wait(kv_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY)) break;
+      if (elect_one()) {
+        const uint32_t kb = base + S::KV0 + s * 2 * S::KEYS;
+        mbar_expect_tx(kv_full(s), 2 * S::KEYS);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          tma_load_4d(kb + h * (BN * 128), &map_k, kv_full(s), h * 64, j * BN, hk, m);
+          tma_load_4d(kb + S::KEYS + h * (BN * 128), &map_v, kv_full(s), h * 64, j * BN, hk, m);
+        }
+      }
+      __syncwarp();
+      issued = j + 1;
+      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+    }
+    for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
+      warp_wait(kv_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = instr_desc<T>(BN, false), idesc_o = instr_desc<T>(DP, true);
+    const uint64_t qd = make_desc(base, 16, 1024), od = make_desc(base + S::DO0, 16, 1024);
+    const uint64_t kd = make_desc(base + S::KV0, 16, 1024), kn = make_desc(base + S::KV0, BN * 128, 1024);
+    auto scores = [&](int t, int s) {
+      if (elect_one()) {
+        const uint64_t st = (uint64_t)((s * 2 * S::KEYS) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t ro = (uint64_t)((t * S::ROWS + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+          umma_bf16(tmem + t * 64, qd + ro, kd + st + ko, idesc_s, kk > 0);
+        }
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t ro = (uint64_t)((t * S::ROWS + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+          umma_bf16(tmem + 128 + t * 64, od + ro, kd + st + (S::KEYS >> 4) + ko, idesc_s, kk > 0);
+        }
+        umma_commit(s_full(t));
+      }
+      __syncwarp();
+    };
+    bool ok = nt > 0 && warp_wait(rows_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL) && warp_wait(kv_clean(0), 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    if (ok) {
+      tc_fence_after();
+      for (int t = 0; t < tiles; ++t) scores(t, 0);
+    }
+    int s = 0;
+    uint32_t ph = 0;
+    for (int j = 0; j < nt && ok; ++j) {
+      const int s1 = s + 1 == S::STAGES ? 0 : s + 1;
+      const uint32_t ph1 = s1 == 0 ? ph ^ 1u : ph;
+      for (int t = 0; t < tiles && ok; ++t) {
+        ok = warp_wait(ds_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_EMPTY);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            umma_ts(tmem + 256 + t * DP, tmem + t * 64 + kk * 8, kn + (uint64_t)((s * 2 * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
+          if (t == tiles - 1) umma_commit(kv_empty(s));
+          if (j == nt - 1) umma_commit(dq_full(t));
+        }
+        __syncwarp();
+        if (j + 1 < nt) {
+          if (t == 0) {
+            ok = warp_wait(kv_clean(s1), ph1, a.status, SB_TIMEOUT_SMEM_FULL);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          scores(t, s1);
+        }
+      }
+      s = s1;
+      ph = ph1;
+    }
+  } else if (warp == 2) {
+    // hidden key rows are cleared: their ds is zero, and zero times NaN is not
+    int s = 0;
+    uint32_t ph = 0;
+    for (int j = 0; j < nt; ++j) {
+      if (!warp_wait(kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
+      if (hide || (j + 1) * BN > len) {
+        uint32_t w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
+        clear_rows<DP>(base + S::KV0 + s * 2 * S::KEYS, BN, w, 2, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kv_clean(s));
+      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+    }
+  } else if (warp >= 4 && (warp - 4) / 4 < tiles) {
+    const int t = (warp - 4) >> 2, quarter = warp & 3;
+    const int tile_row = row0 + t * 128, row = tile_row + quarter * 32 + lane;
+    const bool valid = row < a.R;
+    float dsf;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
+    const float lse = valid ? b.lse[(long long)unit * a.R + row] : INFINITY, delta = valid ? b.delta[(long long)unit * a.R + row] : 0.f;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_addr = lane_base + t * 64, dp_addr = lane_base + 128 + t * 64, dq_addr = lane_base + 256 + t * DP;
+    bool ok = true;
+    if (nt > 0) {
+      load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, tile_row, base + t * S::ROWS, quarter, lane);
+      const long long st = (long long)a.H * a.D;
+      load_rows<DP>(a, b.dout, st * a.Tq, st, a.D, m, hk, tile_row, base + S::DO0 + t * S::ROWS, quarter, lane);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(rows_ready);
+    }
+    for (int j = 0; j < nt; ++j) {
+      const bool some_hidden = hide || (j + 1) * BN > len;
+      uint32_t w[2] = {0, 0};
+      if (some_hidden) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
+      }
+      ok = warp_wait(s_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t sr[32], pr[32], o[16];
+        tmem_load32(s_addr + 32 * i, sr);
+        tmem_load32(dp_addr + 32 * i, pr);
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          float v[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float p = ex2(fmaf(__uint_as_float(sr[k + u]), a.c, -lse));
+            v[u] = p * (__uint_as_float(pr[k + u]) - delta) * dsf;
+            if (some_hidden && ((w[i] >> (k + u)) & 1u)) v[u] = 0.f;
+          }
+          o[k >> 1] = pack_ds<T>(v[0], v[1]);
+        }
+        tmem_store16(s_addr + 16 * i, o);
+      }
+      tmem_store_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full(t));
+    }
+    if (nt > 0 && ok) ok = warp_wait(dq_full(t), 0, a.status, SB_TIMEOUT_TMEM_FULL);
+    tc_fence_after();
+    uint16_t* dst = dq;
+    if (valid) {
+      const RowAt at = row_at(a, m, hk, row);
+      dst = dq + (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
+    }
+    const float f = b.scale / dsf;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+      uint32_t r[32];
+      if (nt > 0 && ok) {
+        tmem_load32(dq_addr + 32 * i, r);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) r[k] = 0u;
+      }
+      if (valid) store_row32<T>(dst, 32 * i, a.D, r, f);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------ dk, dv
+template <int DP> struct DkvSmem {
+  static constexpr int BQ = 64;                            // packed query rows of a step
+  static constexpr int STAGES = 4;
+  static constexpr int KEYS = 128 * DP * 2, ROWS = BQ * DP * 2;
+  static constexpr int Q0 = 2 * KEYS, STAT0 = Q0 + STAGES * 2 * ROWS, BAR = STAT0 + STAGES * 2 * BQ * 4;
+  static constexpr int BYTES = BAR + 256 + 1024;
+};
+constexpr int LOADERS = 96;                                // warps 0, 2, 3
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? 16 : 0;                               // 0 source bytes: the 16 bytes become zero
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(BWD_THREADS, 1)
+xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dk,
+                 uint16_t* __restrict__ dv) {
+  using S = DkvSmem<DP>;
+  constexpr int BQ = S::BQ, HALVES = DP / 64;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = base + S::BAR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto q_full = [&](int s) { return bars + 8u * s; };
+  auto q_empty = [&](int s) { return bars + 8u * (4 + s); };
+  auto s_full = [&](int u) { return bars + 8u * (8 + u); };
+  auto p_full = [&](int u) { return bars + 8u * (10 + u); };
+  const uint32_t kv_full = bars + 8u * 12, d_full = bars + 8u * 13, tmem_slot = bars + 8u * 14, scale_slot = tmem_slot + 4;
+
+  const int ktiles = (a.Tk + 127) / 128;
+  const int unit = blockIdx.x / ktiles, m = unit / a.Hk, hk = unit % a.Hk;
+  const int key0 = (blockIdx.x - unit * ktiles) * 128;
+  const int len = visible_keys(a, m);
+  const int nq = key0 < len ? (a.R + BQ - 1) / BQ : 0;     // nothing is visible here: gradients are zero
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) { mbar_init(q_full(s), 3); mbar_init(q_empty(s), 1); }
+    for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 1); mbar_init(p_full(u), 4); }
+    mbar_init(kv_full, 1);
+    mbar_init(d_full, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == 3) {
+    const float f = ds_scale<T>(b, lane);
+    if (lane == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale_slot), "f"(f) : "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
+
+  if (warp == 0 || warp == 2 || warp == 3) {
+    // ---------------------------------------------------------------- loads: keys and values once by TMA, packed rows by cp.async
+    if (warp == 0 && nq > 0 && elect_one()) {
+      mbar_expect_tx(kv_full, 2 * S::KEYS);
+#pragma unroll
+      for (int h = 0; h < HALVES; ++h) {
+        tma_load_4d(base + h * 16384, &map_k, kv_full, h * 64, key0, hk, m);
+        tma_load_4d(base + S::KEYS + h * 16384, &map_v, kv_full, h * 64, key0, hk, m);
+      }
+    }
+    __syncwarp();
+    const int id = (warp == 0 ? 0 : warp - 1) * 32 + lane;
+    constexpr int CH = DP / 8;
+    const long long o_st = (long long)a.H * a.D;
+    // a stage is announced one step after its copies were issued, when they have landed and are visible to the tensor core
+    bool ok = true;
+    for (int i = 0; i <= nq; ++i) {
+      if (i < nq) {
+        const int s = i % S::STAGES;
+        ok = warp_wait(q_empty(s), ((uint32_t)(i / S::STAGES) & 1u) ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY);
+        if (!ok) break;
+        const uint32_t qb = base + S::Q0 + s * 2 * S::ROWS;
+        for (int x = id; x < BQ * CH; x += LOADERS) {
+          const int rr = x / CH, ch = x % CH, r = i * BQ + rr;
+          const bool in = r < a.R && ch * 8 < a.D;
+          const RowAt at = row_at(a, m, hk, in ? r : 0);
+          const uint16_t* qs = reinterpret_cast<const uint16_t*>(a.q) + at.b * a.q_sb + at.t * a.q_st + at.h * a.q_sh + (in ? ch * 8 : 0);
+          const uint16_t* os = b.dout + ((long long)at.b * a.Tq + at.t) * o_st + (long long)at.h * a.D + (in ? ch * 8 : 0);
+          copy16(tile_addr(qb, BQ, rr, ch), qs, in);
+          copy16(tile_addr(qb + S::ROWS, BQ, rr, ch), os, in);
+        }
+        for (int rr = id; rr < BQ; rr += LOADERS) {
+          const int r = i * BQ + rr;
+          const float l = r < a.R ? b.lse[(long long)unit * a.R + r] - p_shift<T>() : INFINITY, d = r < a.R ? b.delta[(long long)unit * a.R + r] : 0.f;
+          const uint32_t st = base + S::STAT0 + (uint32_t)(s * 2 * BQ + rr) * 4u;
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(st), "f"(l) : "memory");
+          asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + BQ * 4), "f"(d) : "memory");
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (i > 0) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full((i - 1) % S::STAGES));
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (warp == 0 && nq > 0) warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- matrix products
+    constexpr uint32_t idesc_s = instr_desc<T>(BQ, false), idesc_o = instr_desc<T>(DP, true);
+    const uint64_t kd = make_desc(base, 16, 1024), vd = make_desc(base + S::KEYS, 16, 1024);
+    const uint64_t qd = make_desc(base + S::Q0, 16, 1024), qn = make_desc(base + S::Q0, BQ * 128, 1024);
+    auto scores = [&](int i) {                              // s^T = k q^T, dp^T = v do^T of step i
+      const uint64_t st = (uint64_t)(((i % S::STAGES) * 2 * S::ROWS) >> 4);
+      const uint32_t d = tmem + 256 + (i & 1) * 128;
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t ko = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ro = (uint64_t)(((kk >> 2) * (BQ * 128) + (kk & 3) * 32) >> 4);
+          umma_bf16(d, kd + ko, qd + st + ro, idesc_s, kk > 0);
+        }
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t ko = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ro = (uint64_t)(((kk >> 2) * (BQ * 128) + (kk & 3) * 32) >> 4);
+          umma_bf16(d + 64, vd + ko, qd + st + (S::ROWS >> 4) + ro, idesc_s, kk > 0);
+        }
+        umma_commit(s_full(i & 1));
+      }
+      __syncwarp();
+    };
+    bool ok = nq > 0 && warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    for (int i = 0; i < 2 && i < nq && ok; ++i) {
+      ok = warp_wait(q_full(i), 0, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      scores(i);
+    }
+    for (int i = 0; i < nq && ok; ++i) {
+      const int s = i % S::STAGES, u = i & 1;
+      ok = warp_wait(p_full(u), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t p = tmem + 256 + u * 128;
+        const uint64_t st = (uint64_t)((s * 2 * S::ROWS) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < BQ / 16; ++kk)
+          umma_ts(tmem, p + kk * 8, qn + st + (uint64_t)((S::ROWS + kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
+#pragma unroll
+        for (int kk = 0; kk < BQ / 16; ++kk)
+          umma_ts(tmem + 128, p + 64 + kk * 8, qn + st + (uint64_t)((kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
+        umma_commit(q_empty(s));
+        if (i == nq - 1) umma_commit(d_full);
+      }
+      __syncwarp();
+      if (i + 2 < nq) {
+        ok = warp_wait(q_full((i + 2) % S::STAGES), (uint32_t)((i + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+        if (!ok) break;
+        tc_fence_after();
+        scores(i + 2);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- p^T and ds^T; lanes are keys
+    const int u = (warp - 4) >> 2, quarter = warp & 3;
+    const int key = key0 + quarter * 32 + lane;
+    bool ok = true;
+    float dsf;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
+    const bool hidden = key >= len || (a.mask && a.mask[(long long)m * a.Tk + key] != 0);
+    const float k_ds = dsf * ex2(-p_shift<T>());
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_addr = lane_base + 256 + u * 128, dp_addr = s_addr + 64;
+    for (int i = u; i < nq; i += 2) {
+      ok = warp_wait(s_full(u), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
+      if (!ok) break;
+      // the loaders' statistics of this step: their arrivals were waited for by the issuer of the scores, and again here for their order
+      ok = warp_wait(q_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t stat = base + S::STAT0 + (uint32_t)((i % S::STAGES) * 2 * BQ) * 4u;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t sr[32], pr[32], po[16], so[16];
+        tmem_load32(s_addr + 32 * h, sr);
+        tmem_load32(dp_addr + 32 * h, pr);
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          float4 l, d;
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(l.x), "=f"(l.y), "=f"(l.z), "=f"(l.w) : "r"(stat + (32 * h + k) * 4));
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(d.x), "=f"(d.y), "=f"(d.z), "=f"(d.w) : "r"(stat + (BQ + 32 * h + k) * 4));
+          const float ls[4] = {l.x, l.y, l.z, l.w}, ds[4] = {d.x, d.y, d.z, d.w};
+          float p[4], g[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[e] = hidden ? 0.f : ex2(fmaf(__uint_as_float(sr[k + e]), a.c, -ls[e]));
+            g[e] = hidden ? 0.f : p[e] * (__uint_as_float(pr[k + e]) - ds[e]) * k_ds;
+          }
+          po[k >> 1] = Half2<T>::pack(p[0], p[1]);
+          po[(k >> 1) + 1] = Half2<T>::pack(p[2], p[3]);
+          so[k >> 1] = pack_ds<T>(g[0], g[1]);
+          so[(k >> 1) + 1] = pack_ds<T>(g[2], g[3]);
+        }
+        tmem_store16(s_addr + 16 * h, po);
+        tmem_store16(dp_addr + 16 * h, so);
+      }
+      tmem_store_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(u));
+    }
+    if (nq > 0 && ok) ok = warp_wait(d_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
+    tc_fence_after();
+    // one warpgroup writes dv, the other dk
+    uint16_t* dst = (u ? dk : dv) + (((long long)m * a.Tk + key) * a.Hk + hk) * a.D;
+    const float f = u ? b.scale / dsf : ex2(-p_shift<T>());
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+      uint32_t r[32];
+      if (nq > 0 && ok) {
+        tmem_load32(lane_base + u * 128 + 32 * i, r);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) r[k] = 0u;
+      }
+      if (key < a.Tk) store_row32<T>(dst, 32 * i, a.D, r, f);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <typename T, int DP>
+int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, void* dk, void* dv, cudaStream_t stream) {
+  CUtensorMap k64, v64, k128, v128;
+  int rc = sb_rows_map(&k64, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, DqSmem<DP>::BN);
+  if (!rc) rc = sb_rows_map(&v64, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, DqSmem<DP>::BN);
+  if (!rc) rc = sb_rows_map(&k128, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, 128);
+  if (!rc) rc = sb_rows_map(&v128, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, 128);
+  if (!rc) rc = sb_allow_smem((const void*)xattn_dq_kernel<T, DP>, DqSmem<DP>::BYTES);
+  if (!rc) rc = sb_allow_smem((const void*)xattn_dkv_kernel<T, DP>, DkvSmem<DP>::BYTES);
+  if (rc) return rc;
+  const long long units = (long long)a.M * a.Hk, gq = units * ((a.R + 255) / 256), gk = units * ((a.Tk + 127) / 128);
+  if (gq > 0x7fffffffll || gk > 0x7fffffffll) return SB_BAD_ARGUMENT;
+  const long long blocks = (units * a.R + 15) / 16;
+  b.peaks = (int)(blocks < MAX_PARTS ? blocks : MAX_PARTS);
+  xattn_delta_kernel<T><<<b.peaks, 256, 0, stream>>>(a, b);
+  rc = (int)cudaGetLastError();
+  if (!rc && dq) {
+    xattn_dq_kernel<T, DP><<<(unsigned)gq, BWD_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
+    rc = (int)cudaGetLastError();
+  }
+  if (!rc && dk) {
+    xattn_dkv_kernel<T, DP><<<(unsigned)gk, BWD_THREADS, DkvSmem<DP>::BYTES, stream>>>(k128, v128, a, b, (uint16_t*)dk, (uint16_t*)dv);
+    rc = (int)cudaGetLastError();
+  }
+  return rc;
+}
+
+}  // namespace
+
+// out, dout: contiguous [B, Tq, H, D]; lse: the forward pass's; ws: M * Hk * R + 592 floats; dq [B, Tq, H, D] or null; dk, dv
+// [M, Tk, Hk, D], both or neither.
+SB_API int sb_cross_attention_bwd(const SbCrossAttention* g, const void* out, const void* dout, const float* lse, float* ws, void* dq, void* dk, void* dv,
+                                  cudaStream_t stream) {
+  XAttnArgs a;
+  const int rc = sb_xattn_args(g, &a);
+  if (rc) return rc;
+  if (!out || !dout || !lse || !ws || (dk != nullptr) != (dv != nullptr) || ((uintptr_t)dout & 15)) return SB_BAD_ARGUMENT;
+  BwdArgs b = {};
+  b.dout = (const uint16_t*)dout;
+  b.out = (const uint16_t*)out;
+  b.lse = lse;
+  b.delta = ws;
+  b.peak = ws + (long long)a.M * a.Hk * a.R;
+  b.scale = g->scale;
+  if (g->type == 0)
+    return a.D <= 64 ? launch<__nv_bfloat16, 64>(g, a, b, dq, dk, dv, stream) : launch<__nv_bfloat16, 128>(g, a, b, dq, dk, dv, stream);
+  return a.D <= 64 ? launch<__half, 64>(g, a, b, dq, dk, dv, stream) : launch<__half, 128>(g, a, b, dq, dk, dv, stream);
+}

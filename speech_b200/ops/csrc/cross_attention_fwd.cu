@@ -1,0 +1,329 @@
+// Fused cross attention, forward, for many query rows:  o = softmax(scale q k^T) v  without the score matrix in memory.
+//
+// One pass over the keys with the running maximum m and sum l of every row; p = 2^(c s - c m) is held unnormalised:
+//   s = q k_j^T,  m' = max(m, max s),  o = o 2^(c (m - m')) + p v_j,  l = l 2^(c (m - m')) + sum p,  at the end o / l
+// and lse = c m + log2 l is kept for the backward pass (+inf for a row that sees nothing: its probabilities are then 2^-inf = 0).
+//
+// A CTA takes two tiles of 128 packed rows and streams the 128-key tiles of its memory and key head past both, so that keys and values
+// cross the L2 once per 256 rows.  Warp 0 loads keys and values by TMA, warp 1 issues all tcgen05.mma, warp 2 clears hidden value
+// rows, and one warpgroup per row tile does the softmax: scores and output accumulate in tensor memory (2 x (128 + DP) columns), the
+// probabilities go back there as 16-bit pairs over the scores they came from and are the A operand of the second product.  While one
+// tile's warpgroup works, the tensor core works for the other.  The output is rescaled only when a row's maximum has grown by more than
+// 2^8 since the last time; p then stays below 2^8, and the result does not depend on it beyond rounding.
+//
+// Rounding: scores, maxima, sums and output are fp32; p is rounded to the operands' 16-bit type, which is what the tensor core
+// multiplies (relative 2^-9 per weight in bf16, random, as large as the one rounding of the result); l sums the unrounded p.
+#include "cross_attention.cuh"
+#include "cross_attention_host.h"
+
+namespace {
+
+constexpr int FWD_THREADS = 384;
+constexpr int BN = 128;
+template <int DP> struct FwdSmem {
+  static constexpr int STAGES = DP == 128 ? 2 : 4;
+  static constexpr int TILE = 128 * DP * 2;               // a tile of 128 rows of q, k or v
+  static constexpr int K0 = 2 * TILE, V0 = K0 + STAGES * TILE, BAR = V0 + STAGES * TILE;
+  static constexpr int BYTES = BAR + 256 + 1024;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(FWD_THREADS, 1)
+xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, uint16_t* __restrict__ out,
+                 float* __restrict__ lse) {
+  using S = FwdSmem<DP>;
+  constexpr int HALVES = DP / 64;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t bars = base + S::BAR;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto k_full = [&](int s) { return bars + 8u * s; };
+  auto k_empty = [&](int s) { return bars + 8u * (4 + s); };
+  auto v_full = [&](int s) { return bars + 8u * (8 + s); };
+  auto v_clean = [&](int s) { return bars + 8u * (12 + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (16 + s); };
+  auto s_full = [&](int t) { return bars + 8u * (20 + t); };
+  auto p_full = [&](int t) { return bars + 8u * (22 + t); };
+  auto o_full = [&](int t) { return bars + 8u * (24 + t); };
+  const uint32_t q_ready = bars + 8u * 26, tmem_slot = bars + 8u * 27;
+
+  const int pairs = (a.R + 255) / 256;                    // row-tile pairs of a (memory, key head): neighbours in the grid, for the L2
+  const int unit = blockIdx.x / pairs, m = unit / a.Hk, hk = unit % a.Hk;
+  const int row0 = (blockIdx.x - unit * pairs) * 256;
+  const int tiles = a.R - row0 > 128 ? 2 : 1;
+  const int len = visible_keys(a, m);
+  const int nt = (len + BN - 1) / BN;
+  const bool hide = a.mask != nullptr;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::STAGES; ++s) {
+      mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1);
+      mbar_init(v_full(s), 1); mbar_init(v_clean(s), 1); mbar_init(v_empty(s), 1);
+    }
+    for (int t = 0; t < 2; ++t) { mbar_init(s_full(t), 1); mbar_init(p_full(t), 4); mbar_init(o_full(t), 1); }
+    mbar_init(q_ready, 4 * tiles);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loads
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    int issued = 0;
+    for (int j = 0; j < nt && ok; ++j) {
+      ok = warp_wait(k_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY);
+      if (!ok) break;
+      if (elect_one()) {
+        mbar_expect_tx(k_full(s), S::TILE);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::K0 + s * S::TILE + h * 16384, &map_k, k_full(s), h * 64, j * BN, hk, m);
+      }
+      __syncwarp();
+      ok = warp_wait(v_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY);
+      issued = j + 1;
+      if (!ok) break;
+      if (elect_one()) {
+        mbar_expect_tx(v_full(s), S::TILE);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::V0 + s * S::TILE + h * 16384, &map_v, v_full(s), h * 64, j * BN, hk, m);
+      }
+      __syncwarp();
+      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+    }
+    // no copy may be in flight when the block ends: the last one of every stage has landed (long since, unless a wait gave up)
+    for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i) {
+      warp_wait(k_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (ok || i + 1 < issued) warp_wait(v_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- matrix products
+    constexpr uint32_t idesc_s = instr_desc<T>(BN, false), idesc_o = instr_desc<T>(DP, true);
+    const uint64_t qd = make_desc(base, 16, 1024), kd = make_desc(base + S::K0, 16, 1024), vd = make_desc(base + S::V0, BN * 128, 1024);
+    auto scores = [&](int t, int s) {
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint64_t off = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
+          umma_bf16(tmem + t * 128, qd + ((t * S::TILE) >> 4) + off, kd + ((s * S::TILE) >> 4) + off, idesc_s, kk > 0);
+        }
+        umma_commit(s_full(t));
+      }
+      __syncwarp();
+    };
+    bool ok = nt > 0 && warp_wait(q_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL) && warp_wait(k_full(0), 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    if (ok) {
+      tc_fence_after();
+      for (int t = 0; t < tiles; ++t) scores(t, 0);
+      if (elect_one()) umma_commit(k_empty(0));
+      __syncwarp();
+    }
+    int s = 0;
+    uint32_t ph = 0;
+    for (int j = 0; j < nt && ok; ++j) {
+      const int s1 = s + 1 == S::STAGES ? 0 : s + 1;
+      const uint32_t ph1 = s1 == 0 ? ph ^ 1u : ph;
+      for (int t = 0; t < tiles && ok; ++t) {
+        ok = warp_wait(p_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_EMPTY);
+        if (ok && t == 0) ok = warp_wait(v_clean(s), ph, a.status, SB_TIMEOUT_SMEM_FULL);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < BN / 16; ++kk)
+            umma_ts(tmem + 256 + t * DP, tmem + t * 128 + kk * 8, vd + ((s * S::TILE) >> 4) + (uint64_t)(kk * (2048 >> 4)), idesc_o, (j > 0) | (kk > 0));
+          if (t == tiles - 1) umma_commit(v_empty(s));
+          if (j == nt - 1) umma_commit(o_full(t));
+        }
+        __syncwarp();
+        if (j + 1 < nt) {
+          if (t == 0) {
+            ok = warp_wait(k_full(s1), ph1, a.status, SB_TIMEOUT_SMEM_FULL);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          scores(t, s1);
+          if (t == tiles - 1 && elect_one()) umma_commit(k_empty(s1));
+          __syncwarp();
+        }
+      }
+      s = s1;
+      ph = ph1;
+    }
+  } else if (warp == 2) {
+    // ---------------------------------------------------------------- hidden value rows
+    int s = 0;
+    uint32_t ph = 0;
+    for (int j = 0; j < nt; ++j) {
+      if (!warp_wait(v_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
+      if (hide || (j + 1) * BN > len) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
+        clear_rows<DP>(base + S::V0 + s * S::TILE, BN, w, 4, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(v_clean(s));
+      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+    }
+  } else if (warp >= 4 && (warp - 4) / 4 < tiles) {
+    // ---------------------------------------------------------------- softmax and output of one row tile
+    const int t = (warp - 4) >> 2, quarter = warp & 3;
+    const int tile_row = row0 + t * 128, row = tile_row + quarter * 32 + lane;
+    bool ok = true;
+    float mx = -INFINITY, l = 0.f;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_addr = lane_base + t * 128, o_addr = lane_base + 256 + t * DP;
+    if (nt > 0) {
+      load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, tile_row, base + t * S::TILE, quarter, lane);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    }
+    for (int j = 0; j < nt; ++j) {
+      const bool some_hidden = hide || (j + 1) * BN > len;
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (some_hidden) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
+      }
+      ok = warp_wait(s_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      float tile_max = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t r[32];
+        tmem_load32(s_addr + 32 * i, r);
+        if (some_hidden) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) tile_max = fmaxf(tile_max, (w[i] >> k) & 1u ? -INFINITY : __uint_as_float(r[k]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) tile_max = fmaxf(tile_max, __uint_as_float(r[k]));
+        }
+      }
+      // the output keeps its scale until a row's maximum has grown by 2^8
+      const bool grow = mx == -INFINITY ? false : (tile_max - mx) * a.c > 8.f;
+      if (__any_sync(0xffffffffu, grow)) {
+        const float nm = fmaxf(mx, tile_max);
+        const float f = mx == -INFINITY ? 1.f : ex2((mx - nm) * a.c);
+        if (mx != -INFINITY) {
+          l *= f;
+          mx = nm;
+        }
+        if (j > 0) {
+#pragma unroll
+          for (int i = 0; i < DP / 32; ++i) {
+            uint32_t r[32];
+            tmem_load32(o_addr + 32 * i, r);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * f);
+            tmem_store32(o_addr + 32 * i, r);
+          }
+        }
+      }
+      if (mx == -INFINITY) mx = tile_max;                  // nothing seen so far: output and sum are zero at any scale
+      const float mc = mx == -INFINITY ? 0.f : mx * a.c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t r[32], p[16];
+        tmem_load32(s_addr + 32 * i, r);
+        float part = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          float x = __uint_as_float(r[k]), y = __uint_as_float(r[k + 1]);
+          if (some_hidden) {
+            if ((w[i] >> k) & 1u) x = -INFINITY;
+            if ((w[i] >> (k + 1)) & 1u) y = -INFINITY;
+          }
+          x = ex2(fmaf(x, a.c, -mc));
+          y = ex2(fmaf(y, a.c, -mc));
+          part += x + y;
+          p[k >> 1] = Half2<T>::pack(x, y);
+        }
+        l += part;
+        tmem_store16(s_addr + 16 * i, p);
+      }
+      tmem_store_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full(t));
+    }
+    if (nt > 0 && ok) ok = warp_wait(o_full(t), 0, a.status, SB_TIMEOUT_TMEM_FULL);
+    tc_fence_after();
+    const bool valid = row < a.R;
+    uint16_t* dst = out;
+    if (valid) {
+      const RowAt at = row_at(a, m, hk, row);
+      dst = out + (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
+      if (lse) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+      uint32_t r[32];
+      if (nt > 0 && ok) {
+        tmem_load32(o_addr + 32 * i, r);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) r[k] = 0u;
+      }
+      if (valid) {
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+          if (32 * i + k < a.D) {
+            uint4 v;
+            v.x = Half2<T>::pack(__uint_as_float(r[k]) * inv, __uint_as_float(r[k + 1]) * inv);
+            v.y = Half2<T>::pack(__uint_as_float(r[k + 2]) * inv, __uint_as_float(r[k + 3]) * inv);
+            v.z = Half2<T>::pack(__uint_as_float(r[k + 4]) * inv, __uint_as_float(r[k + 5]) * inv);
+            v.w = Half2<T>::pack(__uint_as_float(r[k + 6]) * inv, __uint_as_float(r[k + 7]) * inv);
+            *reinterpret_cast<uint4*>(dst + 32 * i + k) = v;
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <typename T, int DP>
+int launch(const XAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, void* out, float* lse, cudaStream_t stream) {
+  const long long grid = (long long)((a.R + 255) / 256) * a.M * a.Hk;
+  if (grid > 0x7fffffffll) return SB_BAD_ARGUMENT;
+  const int rc = sb_allow_smem((const void*)xattn_fwd_kernel<T, DP>, FwdSmem<DP>::BYTES);
+  if (rc) return rc;
+  xattn_fwd_kernel<T, DP><<<(unsigned)grid, FWD_THREADS, FwdSmem<DP>::BYTES, stream>>>(mk, mv, a, (uint16_t*)out, lse);
+  return (int)cudaGetLastError();
+}
+
+}  // namespace
+
+// q [B, Tq, H, D], k / v [M, Tk, Hk, D] by element strides (batch, time, head); out contiguous [B, Tq, H, D]; lse fp32 [M, Hk, R] or null;
+// ws: sb_cross_attention_workspace() bytes.
+SB_API int sb_cross_attention_fwd(const SbCrossAttention* g, void* out, float* lse, void* ws, cudaStream_t stream) {
+  XAttnArgs a;
+  int rc = sb_xattn_args(g, &a);
+  if (rc) return rc;
+  if (!out) return SB_BAD_ARGUMENT;
+  if (sb_few_rows(g)) return sb_step_cross_attention(g, out, lse, ws, stream);
+  CUtensorMap mk, mv;
+  rc = sb_rows_map(&mk, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, BN);
+  if (!rc) rc = sb_rows_map(&mv, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, BN);
+  if (rc) return rc;
+  if (g->type == 0) return a.D <= 64 ? launch<__nv_bfloat16, 64>(a, mk, mv, out, lse, stream) : launch<__nv_bfloat16, 128>(a, mk, mv, out, lse, stream);
+  return a.D <= 64 ? launch<__half, 64>(a, mk, mv, out, lse, stream) : launch<__half, 128>(a, mk, mv, out, lse, stream);
+}

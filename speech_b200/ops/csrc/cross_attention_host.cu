@@ -1,0 +1,73 @@
+// Host side shared by the cross-attention entry points.
+#include "cross_attention_host.h"
+
+namespace {
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) ptr = nullptr;
+    return (EncodeTiledFn)ptr;
+  }();
+  return fn;
+}
+bool aligned(const void* p, long long a, long long b, long long c) { return (((uintptr_t)p) & 15) == 0 && a % 8 == 0 && b % 8 == 0 && c % 8 == 0; }
+}  // namespace
+
+int sb_xattn_args(const SbCrossAttention* g, XAttnArgs* a) {
+  if (!g || !g->q || !g->k || !g->v || (g->type != 0 && g->type != 1)) return SB_BAD_ARGUMENT;
+  if (g->M <= 0 || g->G <= 0 || g->rep <= 0 || g->Tq <= 0 || g->Tk <= 0 || g->Hk <= 0 || g->D <= 0 || g->D > 128 || g->D % 8) return SB_BAD_ARGUMENT;
+  if (!(g->scale > 0.f) || !(g->scale < 3e38f)) return SB_BAD_ARGUMENT;
+  if (!aligned(g->q, g->q_sb, g->q_st, g->q_sh) || !aligned(g->k, g->k_sb, g->k_st, g->k_sh) || !aligned(g->v, g->v_sb, g->v_st, g->v_sh))
+    return SB_BAD_ARGUMENT;
+  a->q = g->q;
+  a->q_sb = g->q_sb; a->q_st = g->q_st; a->q_sh = g->q_sh;
+  a->lengths = g->lengths; a->mask = g->mask;
+  a->M = g->M; a->G = g->G; a->rep = g->rep; a->Tq = g->Tq; a->Tk = g->Tk; a->Hk = g->Hk; a->D = g->D;
+  a->H = g->Hk * g->rep;
+  const long long R = (long long)g->G * g->rep * g->Tq;
+  if (R > 0x7fffff00ll || (long long)g->M * g->Hk > 0x7fffffffll || (long long)g->M * g->G > 0x7fffffffll) return SB_BAD_ARGUMENT;
+  a->R = (int)R;
+  a->c = g->scale * 1.44269504088896f;
+  a->status = sb_status_ptr();
+  return a->status ? 0 : -2;
+}
+
+int sb_rows_map(CUtensorMap* map, const void* ptr, int type, int D, int T, int heads, int batch, long long st, long long sh, long long sb, int box) {
+  EncodeTiledFn enc = encode_fn();
+  if (!enc) return -100;
+  // the driver call below wants a current context, which a thread that has made no runtime call that needs one (autograd's) lacks
+  static thread_local int bound = -1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && bound != dev) e = cudaSetDevice(dev);
+  if (e != cudaSuccess) return (int)e;
+  bound = dev;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)T, (cuuint64_t)heads, (cuuint64_t)batch};
+  // a stride that is never used (extent 1, or a broadcast of 0 over extent 1) only has to be valid
+  const cuuint64_t any = (cuuint64_t)((D + 7) / 8 * 16);
+  if ((T > 1 && st <= 0) || (heads > 1 && sh <= 0) || (batch > 1 && sb <= 0)) return -101;
+  const cuuint64_t strides[3] = {T > 1 ? (cuuint64_t)st * 2 : any, heads > 1 ? (cuuint64_t)sh * 2 : any, batch > 1 ? (cuuint64_t)sb * 2 : any};
+  const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, type == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(ptr), dims, strides, boxes, ones,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -(200 + (int)r);
+}
+
+int sb_allow_smem(const void* kernel, int bytes) {
+  // a handful of kernels: remembered per device, so that a launch costs no driver call
+  struct Seen { const void* kernel; int device; };
+  static thread_local Seen seen[32];
+  static thread_local int n = 0;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  for (int i = 0; i < n; ++i)
+    if (seen[i].kernel == kernel && seen[i].device == dev) return 0;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return (int)e;
+  if (n < 32) seen[n++] = {kernel, dev};
+  return 0;
+}

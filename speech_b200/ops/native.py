@@ -423,6 +423,7 @@ from .native_lstm import lstm  # noqa: E402,F401
 from .native_ctc import ctc_loss  # noqa: E402,F401
 from .native_logmel import logmel  # noqa: E402,F401
 from .native_sequence_loss import policy_loss, preference_loss  # noqa: E402,F401
+from .native_cross_attention import cross_attention, shared_prefix_attention  # noqa: E402,F401
 
 
 def __getattr__(name):

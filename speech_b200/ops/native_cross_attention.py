@@ -1,0 +1,147 @@
+"""Autograd wrapper of the fused cross attention (``csrc/cross_attention_*.cu``) and of the decoding-step attention over a shared
+prompt (``csrc/step_attention.cu``)."""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import native as N
+from .native_sequence_loss import address, bind, current_stream, on_device
+
+_SIGNATURES = {                      # p: pointer; the stream is the last one
+    "sb_cross_attention_fwd": "ppppp",
+    "sb_cross_attention_bwd": "ppppppppp",
+    "sb_cross_attention_workspace": "p",
+    "sb_shared_prefix_workspace": "pp",
+    "sb_shared_prefix_attention": "ppppp",
+}
+_PEAKS = 592                         # floats of the backward pass's workspace behind the row sums
+
+
+class SbCrossAttention(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v")] + \
+               [(n, ctypes.c_longlong) for n in ("q_sb", "q_st", "q_sh", "k_sb", "k_st", "k_sh", "v_sb", "v_st", "v_sh")] + \
+               [("lengths", ctypes.c_void_p), ("mask", ctypes.c_void_p), ("type", ctypes.c_int)] + \
+               [(n, ctypes.c_int) for n in ("M", "G", "rep", "Tq", "Tk", "Hk", "D")] + [("scale", ctypes.c_float)]
+
+
+class SbOwnCache(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_longlong) for n in ("k_sb", "k_st", "k_sh", "v_sb", "v_st", "v_sh")] + \
+               [("lengths", ctypes.c_void_p), ("size", ctypes.c_int), ("pad", ctypes.c_int)]
+
+
+def _call(name):
+    f = bind(name, _SIGNATURES)
+    if name.endswith("_workspace"):
+        f.restype = ctypes.c_longlong
+    return f
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself if the kernels can address it (contiguous head rows on 16-byte boundaries), else a contiguous copy."""
+    sb, st, sh, sd = t.stride()
+    if sd == 1 and not (sb | st | sh) & 7 and not t.data_ptr() & 15:
+        nb, nt, nh, _ = t.shape
+        if (sb > 0 or nb == 1) and (st > 0 or nt == 1) and (sh > 0 or nh == 1):
+            return t
+    return t.contiguous()
+
+
+def _lengths(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if t is None or (t.dtype == torch.int32 and t.is_contiguous()):
+        return t
+    # clamped before the narrowing, so that a 64-bit length cannot wrap
+    return t.clamp(0, 2 ** 31 - 1).to(torch.int32).contiguous()
+
+
+def _block(q, k, v, lengths, mask, scale) -> SbCrossAttention:
+    B, Tq, H, D = q.shape
+    M, Tk, Hk, _ = k.shape
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    return SbCrossAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                            address(lengths), address(mask), 0 if q.dtype == torch.bfloat16 else 1, M, B // M, H // Hk, Tq, Tk, Hk, D, scale)
+
+
+def _scratch(nbytes: int, what: str, device) -> Optional[torch.Tensor]:
+    if nbytes < 0:
+        raise RuntimeError(f"speech_b200 native call {what} refused its arguments")
+    return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
+
+
+def _forward(q, k, v, lengths, mask, scale, want_lse):
+    B, Tq, H, D = q.shape
+    g = _block(q, k, v, lengths, mask, scale)
+    p = ctypes.byref(g)
+    out = torch.empty((B, Tq, H * D), dtype=q.dtype, device=q.device)
+    lse = torch.empty(B * Tq * H, dtype=torch.float32, device=q.device) if want_lse else None
+    ws = _scratch(_call("sb_cross_attention_workspace")(p), "sb_cross_attention_workspace", q.device)
+    N._check(_call("sb_cross_attention_fwd")(p, out.data_ptr(), address(lse), address(ws), current_stream()), "sb_cross_attention_fwd")
+    return out, lse
+
+
+class _CrossAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, mask, scale):
+        out, lse = _forward(q, k, v, lengths, mask, scale, True)
+        ctx.save_for_backward(q, k, v, out, lengths, mask)
+        ctx.lse, ctx.scale = lse, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lengths, mask = ctx.saved_tensors
+        if not dout.is_contiguous() or dout.data_ptr() & 15:
+            dout = dout.clone(memory_format=torch.contiguous_format)
+        want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        with on_device(q):
+            ws = torch.empty(ctx.lse.numel() + _PEAKS, dtype=torch.float32, device=q.device)
+            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_q else None
+            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_kv else None
+            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if want_kv else None
+            g = _block(q, k, v, lengths, mask, ctx.scale)
+            N._check(_call("sb_cross_attention_bwd")(ctypes.byref(g), out.data_ptr(), dout.data_ptr(), ctx.lse.data_ptr(), ws.data_ptr(), address(dq),
+                                                     address(dk), address(dv), current_stream()), "sb_cross_attention_bwd")
+        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None
+
+
+def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
+    D, Tk = q.shape[3], k.shape[1]
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if D % 8 or D > 128 or Tk == 0 or q.numel() == 0 or not 0.0 < scale < 1e30:
+        from . import reference
+
+        return reference.cross_attention(q, k, v, key_lengths, key_mask, scale)
+    with on_device(q):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        lengths, mask = _lengths(key_lengths), None if key_mask is None else key_mask.contiguous()
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            return _CrossAttentionFn.apply(q, k, v, lengths, mask, scale)
+        return _forward(q, k, v, lengths, mask, scale, False)[0]
+
+
+def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths=None, scale=None):
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_prefix, v_prefix, k, v)):
+        raise RuntimeError("shared_prefix_attention has no backward pass on GPUs: call it under torch.no_grad() or on detached tensors")
+    B, Tq, H, D = q.shape
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if D % 8 or D > 128 or q.numel() == 0 or k_prefix.shape[1] == 0 or k.shape[1] == 0 or not 0.0 < scale < 1e30:
+        from . import reference
+
+        return reference.shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths, scale)
+    with on_device(q):
+        q, kp, vp, k, v = _rows(q), _rows(k_prefix), _rows(v_prefix), _rows(k), _rows(v)
+        lengths, prefix_lengths = _lengths(lengths), _lengths(prefix_lengths)
+        g = _block(q, kp, vp, prefix_lengths, None, scale)
+        ks, vs = k.stride(), v.stride()
+        own = SbOwnCache(k.data_ptr(), v.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], lengths.data_ptr(), k.shape[1], 0)
+        p, o = ctypes.byref(g), ctypes.byref(own)
+        out = torch.empty((B, Tq, H * D), dtype=q.dtype, device=q.device)
+        ws = _scratch(_call("sb_shared_prefix_workspace")(p, o), "sb_shared_prefix_workspace", q.device)
+        N._check(_call("sb_shared_prefix_attention")(p, o, out.data_ptr(), address(ws), current_stream()), "sb_shared_prefix_attention")
+        return out

@@ -1,0 +1,329 @@
+"""Fused cross attention and shared-prefix attention against a plain statement in 64 bits, with bounds from the roundings made."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}      # half a step, relative
+FAST = 2.0 ** -16      # scores up to 2^6 in powers of two, held in fp32 (2^-18 off) and raised by the fast exponential, then summed
+
+
+def plain(q, k, v, hidden, scale, dout=None):
+    """64-bit forward, backward and the error bounds that follow from rounding weights, score gradients and results once each."""
+    B, Tq, H, D = q.shape
+    M, Tk, Hk, _ = k.shape
+    G, rep, e = B // M, H // Hk, EPS[q.dtype]
+    qd = q.double().view(M, G, Tq, Hk, rep, D)
+    clean = hidden[:, :, None, None]
+    kd, vd = k.double().masked_fill(clean, 0.0), v.double().masked_fill(clean, 0.0)
+    s = torch.einsum("mgthrd,mshd->mghrts", qd, kd) * scale
+    h = hidden[:, None, None, None, None, :]
+    s = s.masked_fill(h, -math.inf)
+    top = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(top == -math.inf, 0.0, top)).masked_fill(h, 0.0)
+    total = p.sum(-1, keepdim=True)
+    p = p / torch.where(total == 0, 1.0, total)
+    mix = lambda w, x: torch.einsum("mghrts,mshd->mgthrd", w, x).reshape(B, Tq, H, D)   # noqa: E731
+    out = mix(p, vd)
+    out_err = e * out.abs() + (e + FAST) * mix(p, vd.abs()) + 2.0 ** -25
+    if dout is None:
+        return out, out_err
+    do = dout.double().view(M, G, Tq, Hk, rep, D)
+    over = lambda w, x: torch.einsum("mghrts,mgthrd->mshd", w, x)                        # noqa: E731
+    dp = torch.einsum("mgthrd,mshd->mghrts", do, vd)
+    line = lambda x: torch.einsum("mgthrd,mgthrd->mghrt", do.abs(), x.view(M, G, Tq, Hk, rep, D)).unsqueeze(-1)   # noqa: E731
+    delta = torch.einsum("mgthrd,mgthrd->mghrt", do, out.view(M, G, Tq, Hk, rep, D)).unsqueeze(-1)
+    ds = p * (dp - delta)
+    # delta is computed from the rounded output; fp16 score gradients have an absolute step too, 2^-25 after scaling the largest |do| to 8 or more
+    ds_err = (e + 2 * FAST) * ds.abs() + p * (line(out_err) + FAST * (dp.abs() + delta.abs())) + (2.0 ** -28 * float(dout.abs().max()) if q.dtype == torch.float16 else 0.0)
+    ds_err = ds_err.masked_fill(h, 0.0)
+    dq, dk, dv = mix(ds, kd) * scale, over(ds, qd) * scale, over(p, do)
+    tiny = 2.0 ** -25 if q.dtype == torch.float16 else 1e-30
+    dq_err = e * dq.abs() + mix(ds_err, kd.abs()) * scale + FAST * mix(ds.abs(), kd.abs()) * scale + tiny
+    dk_err = e * dk.abs() + over(ds_err, qd.abs()) * scale + FAST * over(ds.abs(), qd.abs()) * scale + tiny
+    dv_err = e * dv.abs() + (e + 2 * FAST) * over(p, do.abs()) + tiny + (2.0 ** -37 * over((p > 0).double(), do.abs()) if q.dtype == torch.float16 else 0.0)
+    return out, out_err, (dq, dk, dv), (dq_err, dk_err, dv_err)
+
+
+def make(M, G, Tq, Tk, Hk, rep, D, dtype, hide, seed=0, fused=True):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = (1.5 * torch.randn(M * G, Tq, Hk * rep, D, generator=g, device="cuda")).to(dtype)
+    kv = torch.randn(M, Tk, 2, Hk, D, generator=g, device="cuda").to(dtype)
+    k, v = (kv[:, :, 0], kv[:, :, 1]) if fused else (kv[:, :, 0].contiguous(), kv[:, :, 1].contiguous())
+    lengths = mask = None
+    hidden = torch.zeros((M, Tk), dtype=torch.bool, device="cuda")
+    if hide in ("lengths", "both"):
+        lengths = torch.randint(0, Tk + 1, (M,), generator=g, device="cuda")
+        lengths[0] = Tk + 3                                     # beyond the end counts as the end
+        if M > 2:
+            lengths[2] = 0
+        hidden |= torch.arange(Tk, device="cuda")[None] >= lengths[:, None]
+    if hide in ("mask", "both"):
+        mask = torch.rand((M, Tk), generator=g, device="cuda") < 0.4
+        if M > 1:
+            mask[1] = True
+        hidden |= mask
+    k.masked_fill_(hidden[:, :, None, None], float("nan"))
+    v.masked_fill_(hidden[:, :, None, None], float("inf"))
+    return q, k, v, lengths, mask, hidden
+
+
+def check(got, want, err, what):
+    bad = (got.double() - want).abs() / err
+    assert bool(torch.isfinite(got).all()), what
+    assert float(bad.max()) <= 1.0, (what, float(bad.max()))
+
+
+#        M, G, Tq, Tk, Hk, rep, D
+SHAPES = [(1, 1, 1, 1, 1, 1, 8), (2, 1, 7, 33, 4, 1, 64), (3, 4, 1, 129, 2, 1, 128), (2, 16, 1, 300, 1, 4, 128), (3, 1, 64, 127, 2, 1, 40),
+          (3, 1, 65, 128, 2, 1, 96), (2, 2, 33, 260, 1, 2, 128), (1, 1, 128, 64, 1, 2, 64), (3, 1, 257, 65, 2, 1, 128), (2, 5, 31, 513, 2, 4, 64),
+          (1, 1, 300, 1, 3, 1, 72), (1, 3, 130, 1111, 1, 1, 128)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hide", ["none", "lengths", "mask", "both"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward(shape, hide, dtype):
+    from speech_b200 import ops
+
+    q, k, v, lengths, mask, hidden = make(*shape, dtype, hide)
+    out = ops.cross_attention(q, k, v, key_lengths=lengths, key_mask=mask)
+    want, err = plain(q, k, v, hidden, 1 / math.sqrt(shape[-1]))
+    check(out.view(want.shape), want, err, "out")
+    ops.native.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hide", ["none", "both"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_backward(shape, hide, dtype):
+    from speech_b200 import ops
+
+    q, k, v, lengths, mask, hidden = make(*shape, dtype, hide, seed=1)
+    dout = torch.randn(q.shape, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(dtype)
+    scale = 0.7 / math.sqrt(shape[-1])
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask, scale=scale)
+    grads = torch.autograd.grad(out, leaves, dout.flatten(2))
+    want, err, dwant, derr = plain(q, k, v, hidden, scale, dout)
+    check(out.view(want.shape), want, err, "out")
+    for g, w, e, n in zip(grads, dwant, derr, ("dq", "dk", "dv")):
+        check(g, w, e, n)
+    assert bool((grads[1][hidden] == 0).all()) and bool((grads[2][hidden] == 0).all())
+    ops.native.check_status()
+
+
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** 12])
+def test_fp16_gradients_of_any_size(size):
+    """Upstream gradients far from one keep their precision in fp16 (score gradients are scaled)."""
+    from speech_b200 import ops
+
+    q, k, v, _, _, hidden = make(1, 1, 130, 700, 2, 1, 64, torch.float16, "none")
+    dout = (size * torch.randn(q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2))).to(torch.float16)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.cross_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, dout.flatten(2))
+    _, _, dwant, derr = plain(q, k, v, hidden, 1 / 8, dout)
+    for g, w, e, n in zip(grads, dwant, derr, ("dq", "dk", "dv")):
+        check(g, w, e, n)
+
+
+def test_gradients_against_differences():
+    from speech_b200 import ops
+
+    q, k, v, lengths, mask, hidden = make(2, 2, 40, 90, 1, 2, 64, torch.bfloat16, "none")
+    w = torch.randn(q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(4)).to(torch.bfloat16)
+    leaves = [t.detach().contiguous().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.cross_attention(*leaves), leaves, w.flatten(2))
+    for i in range(3):
+        d = torch.randn(leaves[i].shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(i)).double()
+        h = 2.0 ** -10
+
+        def f(sign):
+            args = [x.detach().double() for x in leaves]
+            args[i] = args[i] + sign * h * d
+            s = torch.einsum("mgthrd,mshd->mghrts", args[0].view(2, 2, 40, 1, 2, 64), args[1]) / 8
+            return (torch.einsum("mghrts,mshd->mgthrd", torch.softmax(s, -1), args[2]).reshape(w.shape) * w.double()).sum()
+
+        slope, got = float((f(1) - f(-1)) / (2 * h)), float((grads[i].double() * d).sum())
+        # every gradient element is off by a few bf16 half steps of its own size and of the terms it sums (factor 8), at random signs against d
+        assert abs(got - slope) <= 8 * 2.0 ** -8 * float((grads[i].double() * d).norm()) + 1e-4 * abs(slope)
+
+
+def test_strides_and_unaligned_inputs():
+    """Heads-first caches, slices at odd offsets, broadcast memories: the same results as contiguous copies."""
+    from speech_b200 import ops
+
+    for Tq in (3, 140):
+        q, k, v, _, mask, _ = make(2, 2, Tq, 200, 2, 2, 64, torch.bfloat16, "mask", fused=False)
+        want = ops.cross_attention(q, k, v, key_mask=mask)
+        qh, kh, vh = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v))
+        assert torch.equal(ops.cross_attention(qh, kh, vh, key_mask=mask), want)
+        wide = torch.zeros(k.shape[:3] + (67,), dtype=k.dtype, device="cuda")
+        wide[..., 3:] = k
+        odd = wide[..., 3:]
+        assert odd.data_ptr() % 16 and torch.equal(ops.cross_attention(q, odd, v, key_mask=mask), want)
+        wide_mask = torch.zeros((2, 401), dtype=torch.bool, device="cuda")
+        wide_mask[:, 1::2] = mask
+        assert torch.equal(ops.cross_attention(q, k, v, key_mask=wide_mask[:, 1::2]), want)
+        one = k[:1].nan_to_num().expand(2, -1, -1, -1)
+        assert torch.equal(ops.cross_attention(q, one, one), ops.cross_attention(q, one.contiguous(), one.contiguous()))
+        longs = torch.tensor([150, 2 ** 40], device="cuda")
+        assert torch.equal(ops.cross_attention(q, k, v, key_lengths=longs, key_mask=mask),
+                           ops.cross_attention(q, k, v, key_lengths=torch.tensor([150, 200], dtype=torch.int32, device="cuda"), key_mask=mask))
+
+
+def test_partial_gradients_and_determinism():
+    from speech_b200 import ops
+
+    q, k, v, lengths, mask, _ = make(2, 3, 50, 333, 2, 2, 64, torch.bfloat16, "both")
+    dout = torch.randn(q.shape, device="cuda").to(torch.bfloat16).flatten(2)
+
+    def grads(want):
+        leaves = [t.detach().requires_grad_(w) for t, w in zip((q, k, v), want)]
+        out = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask)
+        return torch.autograd.grad(out, [x for x in leaves if x.requires_grad], dout)
+
+    full, again = grads((True, True, True)), grads((True, True, True))
+    assert all(torch.equal(a, b) for a, b in zip(full, again))
+    assert torch.equal(grads((True, False, False))[0], full[0])
+    assert torch.equal(grads((False, True, False))[0], full[1])
+    assert torch.equal(grads((False, False, True))[0], full[2])
+    # a gradient that arrives transposed, and one that is a broadcast scalar
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask)
+    odd = dout.transpose(0, 1).contiguous().transpose(0, 1)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, odd, retain_graph=True), full))
+    out.sum().backward()
+    assert bool(torch.isfinite(leaves[0].grad).all())
+
+
+def test_double_backward_is_refused():
+    from speech_b200 import ops
+
+    q = torch.randn(1, 3, 2, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    (g,) = torch.autograd.grad(ops.cross_attention(q, q, q).float().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.float().sum().backward()
+
+
+def test_other_stream_and_captured_graphs():
+    """Two captured graphs and an eager call in between, on inputs that change between replays."""
+    from speech_b200 import ops
+
+    cases = [make(2, 2, 1, 700, 2, 2, 128, torch.bfloat16, "lengths"), make(2, 1, 200, 300, 2, 2, 64, torch.bfloat16, "lengths")]
+    side = torch.cuda.Stream()
+    graphs, outs = [], []
+
+    def call(c):
+        leaves = [t.detach().requires_grad_() for t in c[:3]]
+        out = ops.cross_attention(*leaves, key_lengths=c[3])
+        return (out.detach(),) + torch.autograd.grad(out, leaves, torch.ones_like(out))
+
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for c in cases:
+            first = call(c)
+    torch.cuda.current_stream().wait_stream(side)
+    for c in cases:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(c))
+        graphs.append(graph)
+    for c, seed in zip(cases, (7, 8)):
+        for t in c[:3]:
+            t.copy_(torch.randn(t.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)))
+        c[3].copy_(torch.tensor([100, 250], device="cuda"))
+    graphs[0].replay()
+    graphs[1].replay()
+    want = [[x.clone() for x in call(c)] for c in cases]
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    ops.native.check_status()
+
+
+# ------------------------------------------------------------------------------------------------ shared prefix
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 1, 1, 1, 8, 1, 1, 8), (1, 4, 1, 129, 17, 8, 2, 128), (3, 16, 1, 700, 65, 2, 2, 128), (2, 3, 5, 40, 300, 2, 4, 64),
+                                   (2, 40, 2, 333, 16, 1, 1, 40), (5, 1, 1, 2000, 1000, 1, 4, 96)])
+def test_shared_prefix(shape, dtype):
+    from speech_b200 import ops
+
+    P, G, Tq, S, Smax, Hk, rep, D = shape
+    B = P * G
+    g = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)      # noqa: E731
+    q, kp, vp, k, v = 1.5 * r(B, Tq, Hk * rep, D), r(P, S, Hk, D), r(P, S, Hk, D), r(B, Hk, Smax, D).transpose(1, 2), r(B, Hk, Smax, D).transpose(1, 2)
+    plen = torch.randint(0, S + 1, (P,), generator=g, device="cuda")
+    plen[0] = S
+    lens = torch.randint(0, Smax + 1, (B,), generator=g, device="cuda")
+    lens[B // 2] = Smax + 5
+    lens[0] = Tq - 1                                            # the first new token sees the prompt alone
+    for b in range(B):                                          # what lies behind the lengths is garbage
+        k[b, int(lens[b]):] = float("nan")
+        v[b, int(lens[b]):] = float("inf")
+    for p in range(P):
+        kp[p, int(plen[p]):] = float("inf")
+        vp[p, int(plen[p]):] = float("nan")
+    out = ops.shared_prefix_attention(q, kp, vp, k, v, lens, prefix_lengths=plen).view(B, Tq, Hk * rep, D)
+    for b in range(B):
+        n, own = int(plen[b // G]), min(int(lens[b]), Smax)
+        for t in range(Tq):
+            upto = max(0, own - Tq + 1 + t)
+            kk = torch.cat([kp[b // G, :n], k[b, :upto]])[None]
+            vv = torch.cat([vp[b // G, :n], v[b, :upto]])[None]
+            if kk.shape[1] == 0:
+                assert bool((out[b, t] == 0).all())
+                continue
+            want, err = plain(q[b:b + 1, t:t + 1], kk, vv, torch.zeros((1, kk.shape[1]), dtype=torch.bool, device="cuda"), 1 / math.sqrt(D))
+            check(out[b:b + 1, t:t + 1], want, err, (b, t))
+
+
+def test_shared_prefix_refuses_gradients_and_takes_empty_caches():
+    from speech_b200 import ops
+
+    q, k = torch.randn(4, 1, 2, 64, device="cuda", dtype=torch.bfloat16), torch.randn(2, 9, 2, 64, device="cuda", dtype=torch.bfloat16)
+    own, n = torch.randn(4, 5, 2, 64, device="cuda", dtype=torch.bfloat16), torch.tensor([1, 2, 3, 5], device="cuda")
+    with pytest.raises(RuntimeError, match="no backward"):
+        ops.shared_prefix_attention(q.requires_grad_(), k, k, own, own, n)
+    with torch.no_grad():
+        ops.shared_prefix_attention(q, k, k, own, own, n)
+    q = q.detach()
+    a = ops.shared_prefix_attention(q, k[:, :0], k[:, :0], own, own, n)
+    b = ops.cross_attention(q, own, own, key_lengths=n)
+    # one is the plain form in fp32, the other the kernel: both within a bf16 step of the same value
+    assert bool(((a.float() - b.float()).abs() <= 2.0 ** -6 * (1 + b.float().abs())).all())
+
+
+def test_run_of_the_operators_together():
+    """A group of answers per memory: decoding steps over the shared states and the shared prompt, teacher forcing over the same states,
+    policy loss and gradients down to queries, keys and values."""
+    from speech_b200 import ops
+
+    M, G, T, Tk, H, D, V = 2, 4, 6, 90, 4, 64, 130
+    q, k, v, lengths, _, hidden = make(M, G, T, Tk, H, 1, D, torch.bfloat16, "lengths", fused=False)
+    full = ops.cross_attention(q, k, v, key_lengths=lengths)
+    steps = torch.cat([ops.cross_attention(q[:, t:t + 1], k, v, key_lengths=lengths) for t in range(T)], dim=1)
+    want, err = plain(q, k, v, hidden, 1 / 8)
+    check(full.view(want.shape), want, err, "all at once")
+    check(steps.view(want.shape), want, err, "one at a time")
+    own = torch.randn(M * G, T, H, D, device="cuda").to(torch.bfloat16)
+    both = ops.shared_prefix_attention(q[:, -1:], k, v, own, own, torch.full((M * G,), T, device="cuda"), prefix_lengths=lengths)
+    assert bool(torch.isfinite(both).all())
+    head = (0.1 * torch.randn(V, H * D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))).to(torch.bfloat16)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    logits = torch.nn.functional.linear(ops.cross_attention(*leaves, key_lengths=lengths), head)
+    targets = torch.randint(0, V, (M * G, T), device="cuda")
+    mask = torch.ones((M * G, T), dtype=torch.bool, device="cuda")
+    with torch.no_grad():
+        old = torch.log_softmax(logits.double(), -1).gather(-1, targets.unsqueeze(-1)).squeeze(-1).float()
+    loss, logp = ops.policy_loss(logits, targets, mask, old, torch.randn(M * G, device="cuda"), ref_logp=old, kl_beta=0.04)
+    loss.backward()
+    assert torch.allclose(logp, old, atol=1e-5) and all(bool(torch.isfinite(x.grad).all()) and float(x.grad.abs().max()) > 0 for x in leaves)
+    pref, _ = ops.preference_loss(logits.detach().requires_grad_(), targets, mask, old)
+    assert abs(float(pref) - math.log(2)) < 1e-4
+    ops.native.check_status()
