@@ -7,8 +7,9 @@
 // is accumulated in fp32 memory and converted afterwards, and gradients of shared heads and shared rows are sums over packed rows.
 //
 // Both kernels have the roles of the forward pass.  dq: two tiles of 128 rows take turns, 64 keys at a time (scores, dp: 64 columns of
-// tensor memory each, dq: DP columns, per tile).  dk / dv: tiles of 64 packed rows take turns in two sets of tensor memory columns,
-// transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax.
+// tensor memory each, dq: DP columns, per tile).  dk / dv: tiles of 64 query rows of one head take turns in two sets of tensor memory
+// columns, transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; rows come by TMA, their
+// statistics by bulk copies, for which a row kernel lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
 //
 // Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
 // matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do| of the call to [8, 16), and
@@ -25,41 +26,48 @@ template <typename T> constexpr float p_shift() { return Half2<T>::KIND == 0 ? 1
 
 struct BwdArgs {
   const uint16_t* dout;               // contiguous [B, Tq, H, D]
-  const uint16_t* out;
+  const uint16_t *out, *rest;         // the forward pass's result and what its rounding took away
   const float* lse;                   // [M * Hk, R]
-  float* delta;                       // [M * Hk, R]
+  float *nlse, *ndelta;               // [M * Hk, G * rep, Tqp]: -lse (-inf behind the last row, too) and -delta (0 there)
+  int Tqp;                            // Tq rounded up to 64
   float* peak;                        // fp16: largest |do| of every block of the row kernel
   int peaks;
   float scale;
 };
 
-// delta of every packed row, and the largest |do|.  One warp per row of up to 128 elements.
+// -lse and -delta of every row, and the largest |do|.  Sixteen lanes per row of up to 128 elements.
 template <typename T>
 __global__ void __launch_bounds__(256) xattn_delta_kernel(const XAttnArgs a, const BwdArgs b) {
   __shared__ float red[8];
-  const long long rows = (long long)a.M * a.Hk * a.R;
+  const int segs = a.G * a.rep;
+  const long long rows = (long long)a.M * a.Hk * segs * b.Tqp;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = lane >> 4, ch = lane & 15;              // 16 lanes of 8 elements per row, two rows per warp
+  const int sub = lane >> 4, ch = lane & 15;
   float peak = 0.f;
   for (long long i0 = ((long long)blockIdx.x * 8 + warp) * 2; i0 < rows; i0 += (long long)gridDim.x * 16) {
     const long long i = i0 + sub;
+    const int line = (int)(i / b.Tqp), t = (int)(i - (long long)line * b.Tqp);
+    const int unit = line / segs, seg = line - unit * segs;
+    const bool in = i < rows && t < a.Tq;
     float d = 0.f;
-    if (i < rows && ch * 8 < a.D) {
-      const int unit = (int)(i / a.R);
-      const RowAt at = row_at(a, unit / a.Hk, unit % a.Hk, (int)(i - (long long)unit * a.R));
-      const long long off = (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D + ch * 8;
-      const uint4 x = *reinterpret_cast<const uint4*>(b.dout + off), y = *reinterpret_cast<const uint4*>(b.out + off);
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    if (in && ch * 8 < a.D) {
+      const int g = seg / a.rep, m = unit / a.Hk;
+      const long long off = (((long long)(m * a.G + g) * a.Tq + t) * a.H + (unit - m * a.Hk) * a.rep + seg - g * a.rep) * a.D + ch * 8;
+      const uint4 x = *reinterpret_cast<const uint4*>(b.dout + off), y = *reinterpret_cast<const uint4*>(b.out + off), z = *reinterpret_cast<const uint4*>(b.rest + off);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 f = Half2<T>::unpack(xs[k]), e = Half2<T>::unpack(ys[k]);
-        d += f.x * e.x + f.y * e.y;
+        const float2 f = Half2<T>::unpack(xs[k]), e = Half2<T>::unpack(ys[k]), c = Half2<T>::unpack(zs[k]);
+        d += f.x * (e.x + c.x) + f.y * (e.y + c.y);
         if (Half2<T>::KIND == 0) peak = fmaxf(peak, fmaxf(fabsf(f.x), fabsf(f.y)));
       }
     }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (i < rows && ch == 0) b.delta[i] = d;
+    if (i < rows && ch == 0) {
+      b.ndelta[i] = -d;
+      b.nlse[i] = in ? -b.lse[(long long)unit * a.R + seg * a.Tq + t] : -INFINITY;
+    }
   }
   if (Half2<T>::KIND == 0) {
     peak = warp_max(peak);
@@ -256,7 +264,9 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const bool valid = row < a.R;
     float dsf;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
-    const float lse = valid ? b.lse[(long long)unit * a.R + row] : INFINITY, delta = valid ? b.delta[(long long)unit * a.R + row] : 0.f;
+    const long long stat = valid ? ((long long)unit * (a.G * a.rep) + row / a.Tq) * b.Tqp + row % a.Tq : 0;
+    const float nlse = valid ? b.nlse[stat] : -INFINITY;
+    float ndelta = valid ? b.ndelta[stat] : 0.f;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_addr = lane_base + t * 64, dp_addr = lane_base + 128 + t * 64, dq_addr = lane_base + 256 + t * DP;
     bool ok = true;
@@ -278,21 +288,44 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       ok = warp_wait(s_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
+      uint32_t sr[64], pr[64];
+      tmem_load64(s_addr, sr);
+      tmem_load64(dp_addr, pr);
+      const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse);
+#pragma unroll
+      for (int k = 0; k < 64; k += 2) {                    // p over s
+        float x, y;
+        split(fma2(pair(sr[k], sr[k + 1]), c2, nl2), x, y);
+        sr[k] = __float_as_uint(ex2(x));
+        sr[k + 1] = __float_as_uint(ex2(y));
+      }
+      if (some_hidden) {
+#pragma unroll
+        for (int k = 0; k < 64; ++k)
+          if ((w[k >> 5] >> (k & 31)) & 1u) sr[k] = pr[k] = 0u;
+      }
+      if (nt == 1) {
+        // all keys are in this tile: delta = sum p dp from the values that it is subtracted from, instead of the rounded output
+        uint64_t d2[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 64; k += 2) d2[(k >> 1) & 1] = fma2(pair(sr[k], sr[k + 1]), pair(pr[k], pr[k + 1]), d2[(k >> 1) & 1]);
+        float x, y;
+        split(add2(d2[0], d2[1]), x, y);
+        ndelta = -(x + y);
+        if (valid) b.ndelta[stat] = ndelta;
+      }
+      const uint64_t nd2 = pair(ndelta, ndelta), f2 = pair(dsf, dsf);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint32_t sr[32], pr[32], o[16];
-        tmem_load32(s_addr + 32 * i, sr);
-        tmem_load32(dp_addr + 32 * i, pr);
+        uint32_t o[16];
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          float v[2];
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const float p = ex2(fmaf(__uint_as_float(sr[k + u]), a.c, -lse));
-            v[u] = p * (__uint_as_float(pr[k + u]) - delta) * dsf;
-            if (some_hidden && ((w[i] >> (k + u)) & 1u)) v[u] = 0.f;
-          }
-          o[k >> 1] = pack_ds<T>(v[0], v[1]);
+        for (int k = 0; k < 16; ++k) {
+          const int e = 32 * i + 2 * k;
+          uint64_t v = mul2(pair(sr[e], sr[e + 1]), add2(pair(pr[e], pr[e + 1]), nd2));
+          if (Half2<T>::KIND == 0) v = mul2(v, f2);
+          float x, y;
+          split(v, x, y);
+          o[k] = pack_ds<T>(x, y);
         }
         tmem_store16(s_addr + 16 * i, o);
       }
@@ -318,7 +351,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
         for (int k = 0; k < 32; ++k) r[k] = 0u;
       }
-      if (valid) store_row32<T>(dst, 32 * i, a.D, r, f);
+      if (valid && dq) store_row32<T>(dst, 32 * i, a.D, r, f);
     }
   }
   tc_fence_before();
@@ -328,23 +361,17 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
 // ------------------------------------------------------------------------------------------------ dk, dv
 template <int DP> struct DkvSmem {
-  static constexpr int BQ = 64;                            // packed query rows of a step
+  static constexpr int BQ = 64;                            // query rows of a step
   static constexpr int STAGES = 4;
-  static constexpr int KEYS = 128 * DP * 2, ROWS = BQ * DP * 2;
-  static constexpr int Q0 = 2 * KEYS, STAT0 = Q0 + STAGES * 2 * ROWS, BAR = STAT0 + STAGES * 2 * BQ * 4;
+  static constexpr int KEYS = 128 * DP * 2, ROWS = BQ * DP * 2, STAT = 2 * BQ * 4;
+  static constexpr int Q0 = 2 * KEYS, STAT0 = Q0 + STAGES * 2 * ROWS, BAR = STAT0 + STAGES * STAT;
   static constexpr int BYTES = BAR + 256 + 1024;
 };
-constexpr int LOADERS = 96;                                // warps 0, 2, 3
-
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
-  const int n = ok ? 16 : 0;                               // 0 source bytes: the 16 bytes become zero
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
-xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dk,
-                 uint16_t* __restrict__ dv) {
+xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
+                 const __grid_constant__ CUtensorMap map_do, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv) {
   using S = DkvSmem<DP>;
   constexpr int BQ = S::BQ, HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -361,10 +388,11 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   const int unit = blockIdx.x / ktiles, m = unit / a.Hk, hk = unit % a.Hk;
   const int key0 = (blockIdx.x - unit * ktiles) * 128;
   const int len = visible_keys(a, m);
-  const int nq = key0 < len ? (a.R + BQ - 1) / BQ : 0;     // nothing is visible here: gradients are zero
+  const int segs = a.G * a.rep, lines = b.Tqp / BQ;        // (row, head) pairs that read these keys, steps of each
+  const int nq = key0 < len ? segs * lines : 0;            // 0: nothing is visible here, gradients are zero
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::STAGES; ++s) { mbar_init(q_full(s), 3); mbar_init(q_empty(s), 1); }
+    for (int s = 0; s < S::STAGES; ++s) { mbar_init(q_full(s), 1); mbar_init(q_empty(s), 1); }
     for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 1); mbar_init(p_full(u), 4); }
     mbar_init(kv_full, 1);
     mbar_init(d_full, 1);
@@ -385,9 +413,9 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
 
-  if (warp == 0 || warp == 2 || warp == 3) {
-    // ---------------------------------------------------------------- loads: keys and values once by TMA, packed rows by cp.async
-    if (warp == 0 && nq > 0 && elect_one()) {
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loads
+    if (nq > 0 && elect_one()) {
       mbar_expect_tx(kv_full, 2 * S::KEYS);
 #pragma unroll
       for (int h = 0; h < HALVES; ++h) {
@@ -396,44 +424,34 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
     }
     __syncwarp();
-    const int id = (warp == 0 ? 0 : warp - 1) * 32 + lane;
-    constexpr int CH = DP / 8;
-    const long long o_st = (long long)a.H * a.D;
-    // a stage is announced one step after its copies were issued, when they have landed and are visible to the tensor core
-    bool ok = true;
-    for (int i = 0; i <= nq; ++i) {
-      if (i < nq) {
-        const int s = i % S::STAGES;
-        ok = warp_wait(q_empty(s), ((uint32_t)(i / S::STAGES) & 1u) ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY);
-        if (!ok) break;
-        const uint32_t qb = base + S::Q0 + s * 2 * S::ROWS;
-        for (int x = id; x < BQ * CH; x += LOADERS) {
-          const int rr = x / CH, ch = x % CH, r = i * BQ + rr;
-          const bool in = r < a.R && ch * 8 < a.D;
-          const RowAt at = row_at(a, m, hk, in ? r : 0);
-          const uint16_t* qs = reinterpret_cast<const uint16_t*>(a.q) + at.b * a.q_sb + at.t * a.q_st + at.h * a.q_sh + (in ? ch * 8 : 0);
-          const uint16_t* os = b.dout + ((long long)at.b * a.Tq + at.t) * o_st + (long long)at.h * a.D + (in ? ch * 8 : 0);
-          copy16(tile_addr(qb, BQ, rr, ch), qs, in);
-          copy16(tile_addr(qb + S::ROWS, BQ, rr, ch), os, in);
+    int s = 0, issued = 0, t0 = 0, head = 0, g = 0;        // step i: rows t0 .. of head hk * rep + head of batch row m * G + g
+    uint32_t ph = 0;
+    for (int i = 0; i < nq; ++i) {
+      if (!warp_wait(q_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY)) break;
+      if (elect_one()) {
+        const uint32_t qb = base + S::Q0 + s * 2 * S::ROWS, st = base + S::STAT0 + s * S::STAT;
+        const long long line = ((long long)unit * segs + g * a.rep + head) * b.Tqp + t0;
+        mbar_expect_tx(q_full(s), 2 * S::ROWS + S::STAT);
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          tma_load_4d(qb + h * (BQ * 128), &map_q, q_full(s), h * 64, t0, hk * a.rep + head, m * a.G + g);
+          tma_load_4d(qb + S::ROWS + h * (BQ * 128), &map_do, q_full(s), h * 64, t0, hk * a.rep + head, m * a.G + g);
         }
-        for (int rr = id; rr < BQ; rr += LOADERS) {
-          const int r = i * BQ + rr;
-          const float l = r < a.R ? b.lse[(long long)unit * a.R + r] - p_shift<T>() : INFINITY, d = r < a.R ? b.delta[(long long)unit * a.R + r] : 0.f;
-          const uint32_t st = base + S::STAT0 + (uint32_t)(s * 2 * BQ + rr) * 4u;
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(st), "f"(l) : "memory");
-          asm volatile("st.shared.f32 [%0], %1;" ::"r"(st + BQ * 4), "f"(d) : "memory");
-        }
+        bulk_load(st, b.nlse + line, BQ * 4, q_full(s));
+        bulk_load(st + BQ * 4, b.ndelta + line, BQ * 4, q_full(s));
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (i > 0) {
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full((i - 1) % S::STAGES));
+      __syncwarp();
+      issued = i + 1;
+      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+      t0 += BQ;
+      if (t0 >= a.Tq) {
+        t0 = 0;
+        if (++head == a.rep) { head = 0; ++g; }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-    if (warp == 0 && nq > 0) warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    if (nq > 0) warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
+      warp_wait(q_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
   } else if (warp == 1) {
     // ---------------------------------------------------------------- matrix products
     constexpr uint32_t idesc_s = instr_desc<T>(BQ, false), idesc_o = instr_desc<T>(DP, true);
@@ -489,7 +507,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         scores(i + 2);
       }
     }
-  } else {
+  } else if (warp >= 4) {
     // ---------------------------------------------------------------- p^T and ds^T; lanes are keys
     const int u = (warp - 4) >> 2, quarter = warp & 3;
     const int key = key0 + quarter * 32 + lane;
@@ -497,41 +515,51 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     float dsf;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
     const bool hidden = key >= len || (a.mask && a.mask[(long long)m * a.Tk + key] != 0);
+    const bool some_hidden = __any_sync(0xffffffffu, hidden);
     const float k_ds = dsf * ex2(-p_shift<T>());
+    const uint64_t c2 = pair(a.c, a.c), shift2 = pair(p_shift<T>(), p_shift<T>()), f2 = pair(k_ds, k_ds);
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_addr = lane_base + 256 + u * 128, dp_addr = s_addr + 64;
+    const uint32_t s_addr = lane_base + 256 + u * 128;
     for (int i = u; i < nq; i += 2) {
       ok = warp_wait(s_full(u), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
-      // the loaders' statistics of this step: their arrivals were waited for by the issuer of the scores, and again here for their order
+      // the statistics of this step have landed with its rows; waiting on their barrier makes them visible here
       ok = warp_wait(q_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t stat = base + S::STAT0 + (uint32_t)((i % S::STAGES) * 2 * BQ) * 4u;
+      const uint32_t stat = base + S::STAT0 + (i % S::STAGES) * S::STAT;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t sr[32], pr[32], po[16], so[16];
         tmem_load32(s_addr + 32 * h, sr);
-        tmem_load32(dp_addr + 32 * h, pr);
+        tmem_load32(s_addr + 64 + 32 * h, pr);
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
-          float4 l, d;
-          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(l.x), "=f"(l.y), "=f"(l.z), "=f"(l.w) : "r"(stat + (32 * h + k) * 4));
-          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(d.x), "=f"(d.y), "=f"(d.z), "=f"(d.w) : "r"(stat + (BQ + 32 * h + k) * 4));
-          const float ls[4] = {l.x, l.y, l.z, l.w}, ds[4] = {d.x, d.y, d.z, d.w};
-          float p[4], g[4];
+          uint64_t l[2], d[2];
+          asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(l[0]), "=l"(l[1]) : "r"(stat + (32 * h + k) * 4));
+          asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(d[0]), "=l"(d[1]) : "r"(stat + (BQ + 32 * h + k) * 4));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[e] = hidden ? 0.f : ex2(fmaf(__uint_as_float(sr[k + e]), a.c, -ls[e]));
-            g[e] = hidden ? 0.f : p[e] * (__uint_as_float(pr[k + e]) - ds[e]) * k_ds;
+          for (int e = 0; e < 2; ++e) {
+            const int j = k + 2 * e;
+            if (Half2<T>::KIND == 0) l[e] = add2(l[e], shift2);
+            float x, y;
+            split(fma2(pair(sr[j], sr[j + 1]), c2, l[e]), x, y);
+            x = ex2(x);
+            y = ex2(y);
+            uint64_t v = mul2(pair(x, y), add2(pair(pr[j], pr[j + 1]), d[e]));
+            if (Half2<T>::KIND == 0) v = mul2(v, f2);
+            po[j >> 1] = Half2<T>::pack(x, y);
+            split(v, x, y);
+            so[j >> 1] = pack_ds<T>(x, y);
           }
-          po[k >> 1] = Half2<T>::pack(p[0], p[1]);
-          po[(k >> 1) + 1] = Half2<T>::pack(p[2], p[3]);
-          so[k >> 1] = pack_ds<T>(g[0], g[1]);
-          so[(k >> 1) + 1] = pack_ds<T>(g[2], g[3]);
         }
+        if (some_hidden && hidden) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) po[k] = so[k] = 0u;
+        }
+        __syncwarp();
         tmem_store16(s_addr + 16 * h, po);
-        tmem_store16(dp_addr + 16 * h, so);
+        tmem_store16(s_addr + 64 + 16 * h, so);
       }
       tmem_store_wait();
       tc_fence_before();
@@ -562,26 +590,28 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
 template <typename T, int DP>
 int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, void* dk, void* dv, cudaStream_t stream) {
-  CUtensorMap k64, v64, k128, v128;
+  CUtensorMap k64, v64, k128, v128, q64, do64;
   int rc = sb_rows_map(&k64, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, DqSmem<DP>::BN);
   if (!rc) rc = sb_rows_map(&v64, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, DqSmem<DP>::BN);
   if (!rc) rc = sb_rows_map(&k128, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, 128);
   if (!rc) rc = sb_rows_map(&v128, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, 128);
+  if (!rc) rc = sb_rows_map(&q64, g->q, g->type, a.D, a.Tq, a.H, a.M * a.G, g->q_st, g->q_sh, g->q_sb, DkvSmem<DP>::BQ);
+  if (!rc) rc = sb_rows_map(&do64, b.dout, g->type, a.D, a.Tq, a.H, a.M * a.G, (long long)a.H * a.D, a.D, (long long)a.Tq * a.H * a.D, DkvSmem<DP>::BQ);
   if (!rc) rc = sb_allow_smem((const void*)xattn_dq_kernel<T, DP>, DqSmem<DP>::BYTES);
   if (!rc) rc = sb_allow_smem((const void*)xattn_dkv_kernel<T, DP>, DkvSmem<DP>::BYTES);
   if (rc) return rc;
   const long long units = (long long)a.M * a.Hk, gq = units * ((a.R + 255) / 256), gk = units * ((a.Tk + 127) / 128);
   if (gq > 0x7fffffffll || gk > 0x7fffffffll) return SB_BAD_ARGUMENT;
-  const long long blocks = (units * a.R + 15) / 16;
+  const long long blocks = (units * a.G * a.rep * b.Tqp + 15) / 16;
   b.peaks = (int)(blocks < MAX_PARTS ? blocks : MAX_PARTS);
   xattn_delta_kernel<T><<<b.peaks, 256, 0, stream>>>(a, b);
   rc = (int)cudaGetLastError();
-  if (!rc && dq) {
+  if (!rc && (dq || a.Tk <= DqSmem<DP>::BN)) {                // for up to 64 keys it also refines delta, whichever gradients are wanted
     xattn_dq_kernel<T, DP><<<(unsigned)gq, BWD_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
     rc = (int)cudaGetLastError();
   }
   if (!rc && dk) {
-    xattn_dkv_kernel<T, DP><<<(unsigned)gk, BWD_THREADS, DkvSmem<DP>::BYTES, stream>>>(k128, v128, a, b, (uint16_t*)dk, (uint16_t*)dv);
+    xattn_dkv_kernel<T, DP><<<(unsigned)gk, BWD_THREADS, DkvSmem<DP>::BYTES, stream>>>(k128, v128, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv);
     rc = (int)cudaGetLastError();
   }
   return rc;
@@ -589,20 +619,23 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
 
 }  // namespace
 
-// out, dout: contiguous [B, Tq, H, D]; lse: the forward pass's; ws: M * Hk * R + 592 floats; dq [B, Tq, H, D] or null; dk, dv
+// out, rest, dout: contiguous [B, Tq, H, D]; out, rest, lse: the forward pass's; ws: 2 * B * H * (Tq rounded up to 64) + 592 floats; dq [B, Tq, H, D] or null; dk, dv
 // [M, Tk, Hk, D], both or neither.
-SB_API int sb_cross_attention_bwd(const SbCrossAttention* g, const void* out, const void* dout, const float* lse, float* ws, void* dq, void* dk, void* dv,
+SB_API int sb_cross_attention_bwd(const SbCrossAttention* g, const void* out, const void* rest, const void* dout, const float* lse, float* ws, void* dq, void* dk, void* dv,
                                   cudaStream_t stream) {
   XAttnArgs a;
   const int rc = sb_xattn_args(g, &a);
   if (rc) return rc;
-  if (!out || !dout || !lse || !ws || (dk != nullptr) != (dv != nullptr) || ((uintptr_t)dout & 15)) return SB_BAD_ARGUMENT;
+  if (!out || !rest || !dout || !lse || !ws || (dk != nullptr) != (dv != nullptr) || (((uintptr_t)dout | (uintptr_t)ws) & 15)) return SB_BAD_ARGUMENT;
   BwdArgs b = {};
   b.dout = (const uint16_t*)dout;
   b.out = (const uint16_t*)out;
+  b.rest = (const uint16_t*)rest;
   b.lse = lse;
-  b.delta = ws;
-  b.peak = ws + (long long)a.M * a.Hk * a.R;
+  b.Tqp = (a.Tq + 63) / 64 * 64;
+  b.nlse = ws;
+  b.ndelta = ws + (long long)a.M * a.G * a.H * b.Tqp;
+  b.peak = b.ndelta + (long long)a.M * a.G * a.H * b.Tqp;
   b.scale = g->scale;
   if (g->type == 0)
     return a.D <= 64 ? launch<__nv_bfloat16, 64>(g, a, b, dq, dk, dv, stream) : launch<__nv_bfloat16, 128>(g, a, b, dq, dk, dv, stream);

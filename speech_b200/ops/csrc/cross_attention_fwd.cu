@@ -30,7 +30,7 @@ template <int DP> struct FwdSmem {
 template <typename T, int DP>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, uint16_t* __restrict__ out,
-                 float* __restrict__ lse) {
+                 uint16_t* __restrict__ rest, float* __restrict__ lse) {
   using S = FwdSmem<DP>;
   constexpr int HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -201,19 +201,19 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       ok = warp_wait(s_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      float tile_max = -INFINITY;
+      uint32_t r[128];
+      tmem_load128(s_addr, r);
+      if (some_hidden) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t r[32];
-        tmem_load32(s_addr + 32 * i, r);
-        if (some_hidden) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) tile_max = fmaxf(tile_max, (w[i] >> k) & 1u ? -INFINITY : __uint_as_float(r[k]));
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) tile_max = fmaxf(tile_max, __uint_as_float(r[k]));
-        }
+        for (int k = 0; k < 128; ++k)
+          if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = 0xff800000u;
       }
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int k = 0; k < 128; k += 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = max3(top[i], __uint_as_float(r[k + 2 * i]), __uint_as_float(r[k + 2 * i + 1]));
+      const float tile_max = fmaxf(max3(top[0], top[1], top[2]), top[3]);
       // the output keeps its scale until a row's maximum has grown by 2^8
       const bool grow = mx == -INFINITY ? false : (tile_max - mx) * a.c > 8.f;
       if (__any_sync(0xffffffffu, grow)) {
@@ -226,35 +226,36 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (j > 0) {
 #pragma unroll
           for (int i = 0; i < DP / 32; ++i) {
-            uint32_t r[32];
-            tmem_load32(o_addr + 32 * i, r);
+            uint32_t x[32];
+            tmem_load32(o_addr + 32 * i, x);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * f);
-            tmem_store32(o_addr + 32 * i, r);
+            for (int k = 0; k < 32; ++k) x[k] = __float_as_uint(__uint_as_float(x[k]) * f);
+            tmem_store32(o_addr + 32 * i, x);
           }
         }
       }
       if (mx == -INFINITY) mx = tile_max;                  // nothing seen so far: output and sum are zero at any scale
       const float mc = mx == -INFINITY ? 0.f : mx * a.c;
+      const uint64_t c2 = pair(a.c, a.c), shift2 = pair(-mc, -mc);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        uint32_t r[32], p[16];
-        tmem_load32(s_addr + 32 * i, r);
-        float part = 0.f;
+        uint32_t p[16];
 #pragma unroll
-        for (int k = 0; k < 32; k += 2) {
-          float x = __uint_as_float(r[k]), y = __uint_as_float(r[k + 1]);
-          if (some_hidden) {
-            if ((w[i] >> k) & 1u) x = -INFINITY;
-            if ((w[i] >> (k + 1)) & 1u) y = -INFINITY;
-          }
-          x = ex2(fmaf(x, a.c, -mc));
-          y = ex2(fmaf(y, a.c, -mc));
-          part += x + y;
-          p[k >> 1] = Half2<T>::pack(x, y);
+        for (int k = 0; k < 16; ++k) {
+          float x, y;
+          split(fma2(pair(r[32 * i + 2 * k], r[32 * i + 2 * k + 1]), c2, shift2), x, y);
+          x = ex2(x);
+          y = ex2(y);
+          sum[k & 1] = add2(sum[k & 1], pair(x, y));
+          p[k] = Half2<T>::pack(x, y);
         }
-        l += part;
         tmem_store16(s_addr + 16 * i, p);
+      }
+      {
+        float x, y;
+        split(add2(sum[0], sum[1]), x, y);
+        l += x + y;
       }
       tmem_store_wait();
       tc_fence_before();
@@ -264,10 +265,10 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     if (nt > 0 && ok) ok = warp_wait(o_full(t), 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
     const bool valid = row < a.R;
-    uint16_t* dst = out;
+    long long at_row = 0;
     if (valid) {
       const RowAt at = row_at(a, m, hk, row);
-      dst = out + (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
+      at_row = (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
       if (lse) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -280,19 +281,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
         for (int k = 0; k < 32; ++k) r[k] = 0u;
       }
-      if (valid) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          if (32 * i + k < a.D) {
-            uint4 v;
-            v.x = Half2<T>::pack(__uint_as_float(r[k]) * inv, __uint_as_float(r[k + 1]) * inv);
-            v.y = Half2<T>::pack(__uint_as_float(r[k + 2]) * inv, __uint_as_float(r[k + 3]) * inv);
-            v.z = Half2<T>::pack(__uint_as_float(r[k + 4]) * inv, __uint_as_float(r[k + 5]) * inv);
-            v.w = Half2<T>::pack(__uint_as_float(r[k + 6]) * inv, __uint_as_float(r[k + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + 32 * i + k) = v;
-          }
-        }
-      }
+      if (valid) store_out32<T>(out + at_row, rest ? rest + at_row : nullptr, 32 * i, a.D, r, inv);
     }
   }
   tc_fence_before();
@@ -301,29 +290,29 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 }
 
 template <typename T, int DP>
-int launch(const XAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, void* out, float* lse, cudaStream_t stream) {
+int launch(const XAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, void* out, void* rest, float* lse, cudaStream_t stream) {
   const long long grid = (long long)((a.R + 255) / 256) * a.M * a.Hk;
   if (grid > 0x7fffffffll) return SB_BAD_ARGUMENT;
   const int rc = sb_allow_smem((const void*)xattn_fwd_kernel<T, DP>, FwdSmem<DP>::BYTES);
   if (rc) return rc;
-  xattn_fwd_kernel<T, DP><<<(unsigned)grid, FWD_THREADS, FwdSmem<DP>::BYTES, stream>>>(mk, mv, a, (uint16_t*)out, lse);
+  xattn_fwd_kernel<T, DP><<<(unsigned)grid, FWD_THREADS, FwdSmem<DP>::BYTES, stream>>>(mk, mv, a, (uint16_t*)out, (uint16_t*)rest, lse);
   return (int)cudaGetLastError();
 }
 
 }  // namespace
 
-// q [B, Tq, H, D], k / v [M, Tk, Hk, D] by element strides (batch, time, head); out contiguous [B, Tq, H, D]; lse fp32 [M, Hk, R] or null;
-// ws: sb_cross_attention_workspace() bytes.
-SB_API int sb_cross_attention_fwd(const SbCrossAttention* g, void* out, float* lse, void* ws, cudaStream_t stream) {
+// q [B, Tq, H, D], k / v [M, Tk, Hk, D] by element strides (batch, time, head); out contiguous [B, Tq, H, D]; for a backward pass
+// rest [B, Tq, H, D], what rounding took from out, and lse fp32 [M, Hk, R], else both null; ws: sb_cross_attention_workspace() bytes.
+SB_API int sb_cross_attention_fwd(const SbCrossAttention* g, void* out, void* rest, float* lse, void* ws, cudaStream_t stream) {
   XAttnArgs a;
   int rc = sb_xattn_args(g, &a);
   if (rc) return rc;
-  if (!out) return SB_BAD_ARGUMENT;
-  if (sb_few_rows(g)) return sb_step_cross_attention(g, out, lse, ws, stream);
+  if (!out || (rest != nullptr) != (lse != nullptr)) return SB_BAD_ARGUMENT;
+  if (sb_few_rows(g)) return sb_step_cross_attention(g, out, rest, lse, ws, stream);
   CUtensorMap mk, mv;
   rc = sb_rows_map(&mk, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, BN);
   if (!rc) rc = sb_rows_map(&mv, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, BN);
   if (rc) return rc;
-  if (g->type == 0) return a.D <= 64 ? launch<__nv_bfloat16, 64>(a, mk, mv, out, lse, stream) : launch<__nv_bfloat16, 128>(a, mk, mv, out, lse, stream);
-  return a.D <= 64 ? launch<__half, 64>(a, mk, mv, out, lse, stream) : launch<__half, 128>(a, mk, mv, out, lse, stream);
+  if (g->type == 0) return a.D <= 64 ? launch<__nv_bfloat16, 64>(a, mk, mv, out, rest, lse, stream) : launch<__nv_bfloat16, 128>(a, mk, mv, out, rest, lse, stream);
+  return a.D <= 64 ? launch<__half, 64>(a, mk, mv, out, rest, lse, stream) : launch<__half, 128>(a, mk, mv, out, rest, lse, stream);
 }

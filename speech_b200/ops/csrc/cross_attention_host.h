@@ -23,4 +23,4 @@ int sb_allow_smem(const void* kernel, int bytes);
 
 // Whether a call has few enough query rows per key head for the decoding-step kernel (step_attention.cu).
 bool sb_few_rows(const SbCrossAttention* g);
-int sb_step_cross_attention(const SbCrossAttention* g, void* out, float* lse, void* ws, cudaStream_t stream);
+int sb_step_cross_attention(const SbCrossAttention* g, void* out, void* rest, float* lse, void* ws, cudaStream_t stream);

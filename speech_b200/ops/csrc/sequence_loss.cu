@@ -14,10 +14,10 @@
 //
 // Rounding: exponentials and a thread's share of a row's sum are fp32, shares are joined in fp64, and logp, the clip decision and
 // the sums over rows are fp64: a policy at its reference has log ratios near zero, and in fp32 the rounding of a logp of -8 (5e-7)
-// would be all that is left after a few thousand positions are summed.  For the same reason the exponent of a summed term is
-// t log2(e) with log2(e) in two parts: the fp32 constant alone is 1.3e-8 too small, which moves every row's log sum the same way.
-// log s = k ln 2 + log f with s = 2^k f, f in [0.71, 1.42): the fp32 logarithm of f is off by less than 2^-25.
-// The gradient is rounded once.  Every sum has a fixed order (no floating-point atomics).
+// would be all that is left after a few thousand positions are summed.  For the same reason the preference loss sums expf, whose
+// errors have no common sign; the approximate power of two moves every row's log sum the same way (7e-8), which a sum over a sequence
+// multiplies and the mean of the policy loss does not.  log s = k ln 2 + log f with s = 2^k f, f in [0.71, 1.42): the fp32 logarithm
+// of f is off by less than 2^-24.  The gradient is rounded once.  Every sum has a fixed order (no floating-point atomics).
 #include "common.cuh"
 #include <cuda_fp16.h>
 #include <math.h>
@@ -121,26 +121,28 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-constexpr float LOG2E_HI = 1.44269502f, LOG2E_LO = 1.92596303e-8f;
-__device__ __forceinline__ float exp_exact(float t) { return ex2(fmaf(t, LOG2E_HI, t * LOG2E_LO)); }
+constexpr float LOG2E = 1.44269504f;
+enum { LOSS_POLICY = 0, LOSS_PREFERENCE = 1 };
+// a summed term: exp(t), t <= 0
+template <int MODE> __device__ __forceinline__ float term(float t) { return MODE == LOSS_PREFERENCE ? expf(t) : ex2(t * LOG2E); }
 
 // Softmax weights of the gradient, times `inv`: exp(x - shift).  For 16-bit logits one fused multiply-add gives the exponent (the
 // product shift log2(e), rounded to fp32, makes a weight off by less than 2^-18, far below half a step of the result).
 template <typename T> struct Weight {
   float shift;
-  __device__ __forceinline__ explicit Weight(float s) : shift(s * LOG2E_HI) {}
-  __device__ __forceinline__ float operator()(float x) const { return ex2(fmaf(x, LOG2E_HI, -shift)); }
+  __device__ __forceinline__ explicit Weight(float s) : shift(s * LOG2E) {}
+  __device__ __forceinline__ float operator()(float x) const { return ex2(fmaf(x, LOG2E, -shift)); }
 };
 template <> struct Weight<float> {
   float shift;
   __device__ __forceinline__ explicit Weight(float s) : shift(s) {}
-  __device__ __forceinline__ float operator()(float x) const { return exp_exact(x - shift); }
+  __device__ __forceinline__ float operator()(float x) const { return ex2((x - shift) * LOG2E); }
 };
 
 // Joins the (max, sum) shares of the TPR threads of a row: one warp (TPR = 32) or a whole block.
 template <int TPR> __device__ __forceinline__ void join(float& m, double& sum, float share, float* redf, double* redd) {
   const float wm = warp_max(m);
-  double v = (double)(share * exp_exact(finite_or_zero(m) - finite_or_zero(wm)));
+  double v = (double)(share * expf(finite_or_zero(m) - finite_or_zero(wm)));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (TPR == 32) {
@@ -160,7 +162,7 @@ template <int TPR> __device__ __forceinline__ void join(float& m, double& sum, f
   m = finite_or_zero(bm);
   sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < TPR / 32; ++i) sum += redd[i] * (double)exp_exact(finite_or_zero(redf[i]) - m);
+  for (int i = 0; i < TPR / 32; ++i) sum += redd[i] * (double)expf(finite_or_zero(redf[i]) - m);
 }
 
 __device__ __forceinline__ double log_of_sum(double s) {
@@ -212,8 +214,6 @@ __device__ __forceinline__ void grad_from_memory(const T* x, T* o, int V, int la
   const int yv = y - s.head;
   if (yv >= 0 && yv < s.nv * E && (yv / E) % TPR == lane) one(y);
 }
-
-enum { LOSS_POLICY = 0, LOSS_PREFERENCE = 1 };
 
 // Forward pass over all rows.  TPR threads work on a row; NV > 0: it stays in registers as it was read, NV 16-byte groups per thread;
 // NV = 0: rows of any length, read again for the gradient, from the L2 (148 rows of 300 KB in flight are a third of it).
@@ -270,18 +270,18 @@ __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, 
           for (int u = 0; u < E; ++u) m = fmaxf(m, f[u]);
         }
       const float base = finite_or_zero(m);
-      share = exp_exact(hx - base) + exp_exact(tx - base);
+      share = term<MODE>(hx - base) + term<MODE>(tx - base);
 #pragma unroll
       for (int k = 0; k < NV; ++k)
         if (lane + k * TPR < s.nv) {
           float f[E], part = 0.f;
           Vec<T>::unpack(raw[k], f);
 #pragma unroll
-          for (int u = 0; u < E; ++u) part += exp_exact(f[u] - base);
+          for (int u = 0; u < E; ++u) part += term<MODE>(f[u] - base);
           share += part;
         }
     } else {
-      share = exp_exact(hx - finite_or_zero(m)) + exp_exact(tx - finite_or_zero(m));
+      share = term<MODE>(hx - finite_or_zero(m)) + term<MODE>(tx - finite_or_zero(m));
 #pragma unroll 4
       for (int i = lane; i < s.nv; i += TPR) {
         float f[E], nm = m, part = 0.f;
@@ -290,11 +290,11 @@ __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, 
         for (int u = 0; u < E; ++u) nm = fmaxf(nm, f[u]);
         const float base = finite_or_zero(nm);
         if (nm > m) {                                    // rare after the first groups
-          share *= exp_exact(finite_or_zero(m) - base);
+          share *= expf(finite_or_zero(m) - base);
           m = nm;
         }
 #pragma unroll
-        for (int u = 0; u < E; ++u) part += exp_exact(f[u] - base);
+        for (int u = 0; u < E; ++u) part += term<MODE>(f[u] - base);
         share += part;
       }
     }
@@ -307,14 +307,14 @@ __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, 
       const double d = logp - (double)old;
       const float plain = expf((float)d) * A;
       const bool above = A > 0.f && d > a.log_hi, below = A < 0.f && d < a.log_lo;   // NaN is neither
-      float term = above ? -(1.f + a.clip_hi) * A : below ? -(1.f - a.clip_lo) * A : -plain;
+      float each = above ? -(1.f + a.clip_hi) * A : below ? -(1.f - a.clip_lo) * A : -plain;
       slope = above || below ? 0.f : -plain;
       if (a.ref && a.kl_beta != 0.f) {
         const float kd = (float)((double)ref - logp), em = expm1f(kd);
-        term += a.kl_beta * (em - kd);
+        each += a.kl_beta * (em - kd);
         slope -= a.kl_beta * em;
       }
-      mine += (double)term;
+      mine += (double)each;
       slope *= inv_count;
     }
     if (lane == 0) {

@@ -42,7 +42,7 @@ struct StepArgs {
   float c;
   Segment seg[2];
   int slots;                // splits of both segments
-  uint16_t* out;            // [B, Tq, H, D]
+  uint16_t *out, *rest;     // [B, Tq, H, D]; rest: what rounding took from out, or null
   float* lse;               // packed rows of segment 0, or null
   float* part_o;            // [slots, B * Tq * H, D]
   float2* part_ml;          // [slots, B * Tq * H]
@@ -232,9 +232,11 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) step_kernel(const StepArgs a)
     const long long qrow = ((long long)(mem * s.rows_per + gr) * a.Tq + t) * a.H + hk * a.rep + y - gr * a.rep;
     if (a.slots == 1) {
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      *reinterpret_cast<uint4*>(a.out + qrow * a.D + d) =
-          make_uint4(Half2<T>::pack(v[0] * inv, v[1] * inv), Half2<T>::pack(v[2] * inv, v[3] * inv), Half2<T>::pack(v[4] * inv, v[5] * inv),
-                     Half2<T>::pack(v[6] * inv, v[7] * inv));
+      uint32_t o4[4], r4[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o4[k] = out_pair<T>(v[2 * k] * inv, v[2 * k + 1] * inv, r4[k]);
+      *reinterpret_cast<uint4*>(a.out + qrow * a.D + d) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
+      if (a.rest) *reinterpret_cast<uint4*>(a.rest + qrow * a.D + d) = make_uint4(r4[0], r4[1], r4[2], r4[3]);
       if (a.lse && d == 0) a.lse[((long long)mem * a.Hk + hk) * s.R + r] = sum > 0.f ? big + log2f(sum) : (sum == 0.f ? INFINITY : sum);
     } else {
       float* po = a.part_o + ((long long)slot * qrows + qrow) * a.D + d;
@@ -269,7 +271,10 @@ template <typename T> __global__ void __launch_bounds__(128) step_join_kernel(co
       const float4 p = *reinterpret_cast<const float4*>(a.part_o + (i * qrows + qrow) * a.D + 4 * lane);
       v.x += f * p.x; v.y += f * p.y; v.z += f * p.z; v.w += f * p.w;
     }
-    *reinterpret_cast<uint2*>(a.out + qrow * a.D + 4 * lane) = make_uint2(Half2<T>::pack(v.x * inv, v.y * inv), Half2<T>::pack(v.z * inv, v.w * inv));
+    uint32_t r0, r1;
+    const uint32_t o0 = out_pair<T>(v.x * inv, v.y * inv, r0), o1 = out_pair<T>(v.z * inv, v.w * inv, r1);
+    *reinterpret_cast<uint2*>(a.out + qrow * a.D + 4 * lane) = make_uint2(o0, o1);
+    if (a.rest) *reinterpret_cast<uint2*>(a.rest + qrow * a.D + 4 * lane) = make_uint2(r0, r1);
   }
   if (a.lse && lane == 0) {
     const int h = (int)(qrow % a.H), t = (int)(qrow / a.H % a.Tq), b = (int)(qrow / a.H / a.Tq);
@@ -362,13 +367,14 @@ int fill(StepArgs& a, const SbCrossAttention* g) {
 
 bool sb_few_rows(const SbCrossAttention* g) { return (long long)g->G * g->rep * g->Tq <= 64; }
 
-int sb_step_cross_attention(const SbCrossAttention* g, void* out, float* lse, void* ws, cudaStream_t stream) {
+int sb_step_cross_attention(const SbCrossAttention* g, void* out, void* rest, float* lse, void* ws, cudaStream_t stream) {
   StepArgs a;
   int rc = fill(a, g);
   if (rc) return rc;
   rc = plan(a, g->M, 0);
   if (rc) return rc;
   a.out = (uint16_t*)out;
+  a.rest = (uint16_t*)rest;
   a.lse = lse;
   return run(a, g->type, ws, stream);
 }

@@ -13,8 +13,8 @@ from . import native as N
 from .native_sequence_loss import address, bind, current_stream, on_device
 
 _SIGNATURES = {                      # p: pointer; the stream is the last one
-    "sb_cross_attention_fwd": "ppppp",
-    "sb_cross_attention_bwd": "ppppppppp",
+    "sb_cross_attention_fwd": "pppppp",
+    "sb_cross_attention_bwd": "pppppppppp",
     "sb_cross_attention_workspace": "p",
     "sb_shared_prefix_workspace": "pp",
     "sb_shared_prefix_attention": "ppppp",
@@ -78,18 +78,19 @@ def _forward(q, k, v, lengths, mask, scale, want_lse):
     g = _block(q, k, v, lengths, mask, scale)
     p = ctypes.byref(g)
     out = torch.empty((B, Tq, H * D), dtype=q.dtype, device=q.device)
+    rest = torch.empty_like(out) if want_lse else None          # what rounding took from the output: the backward pass sums both
     lse = torch.empty(B * Tq * H, dtype=torch.float32, device=q.device) if want_lse else None
     ws = _scratch(_call("sb_cross_attention_workspace")(p), "sb_cross_attention_workspace", q.device)
-    N._check(_call("sb_cross_attention_fwd")(p, out.data_ptr(), address(lse), address(ws), current_stream()), "sb_cross_attention_fwd")
-    return out, lse
+    N._check(_call("sb_cross_attention_fwd")(p, out.data_ptr(), address(rest), address(lse), address(ws), current_stream()), "sb_cross_attention_fwd")
+    return out, rest, lse
 
 
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask, scale):
-        out, lse = _forward(q, k, v, lengths, mask, scale, True)
+        out, rest, lse = _forward(q, k, v, lengths, mask, scale, True)
         ctx.save_for_backward(q, k, v, out, lengths, mask)
-        ctx.lse, ctx.scale = lse, scale
+        ctx.kept, ctx.scale = (rest, lse), scale
         return out
 
     @staticmethod
@@ -98,14 +99,16 @@ class _CrossAttentionFn(torch.autograd.Function):
         q, k, v, out, lengths, mask = ctx.saved_tensors
         if not dout.is_contiguous() or dout.data_ptr() & 15:
             dout = dout.clone(memory_format=torch.contiguous_format)
+        rest, lse = ctx.kept
         want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         with on_device(q):
-            ws = torch.empty(ctx.lse.numel() + _PEAKS, dtype=torch.float32, device=q.device)
+            B, Tq, H, _ = q.shape
+            ws = torch.empty(2 * B * H * ((Tq + 63) // 64 * 64) + _PEAKS, dtype=torch.float32, device=q.device)
             dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_q else None
             dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_kv else None
             dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if want_kv else None
             g = _block(q, k, v, lengths, mask, ctx.scale)
-            N._check(_call("sb_cross_attention_bwd")(ctypes.byref(g), out.data_ptr(), dout.data_ptr(), ctx.lse.data_ptr(), ws.data_ptr(), address(dq),
+            N._check(_call("sb_cross_attention_bwd")(ctypes.byref(g), out.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse.data_ptr(), ws.data_ptr(), address(dq),
                                                      address(dk), address(dv), current_stream()), "sb_cross_attention_bwd")
         return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None
 
