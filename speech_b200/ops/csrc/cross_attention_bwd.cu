@@ -1,15 +1,16 @@
 // Fused cross attention, backward:   p = 2^(c s - lse),  dp = do v^T,  ds = p (dp - delta),  delta = sum_d do o
-//   dq = scale ds k        (one CTA per 256 packed query rows, keys stream past: xattn_dq_kernel)
+//   dq = scale ds k        (one CTA per 128 packed query rows, keys stream past: xattn_dq_kernel)
 //   dv = p^T do, dk = scale ds^T q   (one CTA per 128 keys, packed query rows stream past: xattn_dkv_kernel)
 //
 // Probabilities are computed again from the scores and the row's lse, in both kernels: seven products where one kernel with shared
 // sums of dq would need five, but every sum is taken by one CTA in a fixed order, so that gradients are the same every time, nothing
 // is accumulated in fp32 memory and converted afterwards, and gradients of shared heads and shared rows are sums over packed rows.
 //
-// Both kernels have the roles of the forward pass.  dq: two tiles of 128 rows take turns, 64 keys at a time (scores, dp: 64 columns of
-// tensor memory each, dq: DP columns, per tile).  dk / dv: tiles of 64 query rows of one head take turns in two sets of tensor memory
-// columns, transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; rows come by TMA, their
-// statistics by bulk copies, for which a row kernel lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
+// Both kernels have the roles of the forward pass.  dq: blocks of 64 keys go through three sets of tensor memory columns (scores and dp,
+// 64 each), two warpgroups take them in turn, so that scores are computed ahead of them.  dk / dv: tiles of 64 query rows of one head
+// take turns in two such sets, transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; four
+// warpgroups, two per set with half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which a row kernel
+// lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
 //
 // Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
 // matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do| of the call to [8, 16), and
@@ -114,9 +115,9 @@ template <typename T> __device__ __forceinline__ void store_row32(uint16_t* dst,
 // ------------------------------------------------------------------------------------------------ dq
 template <int DP> struct DqSmem {
   static constexpr int BN = 64;
-  static constexpr int STAGES = DP == 128 ? 3 : 4;
+  static constexpr int STAGES = 5;
   static constexpr int ROWS = 128 * DP * 2, KEYS = BN * DP * 2;
-  static constexpr int DO0 = 2 * ROWS, KV0 = 4 * ROWS, BAR = KV0 + STAGES * 2 * KEYS;
+  static constexpr int DO0 = ROWS, KV0 = 2 * ROWS, BAR = KV0 + STAGES * 2 * KEYS;
   static constexpr int BYTES = BAR + 256 + 1024;
 };
 
@@ -130,25 +131,24 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const uint32_t bars = base + S::BAR;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto kv_full = [&](int s) { return bars + 8u * s; };
-  auto kv_clean = [&](int s) { return bars + 8u * (4 + s); };
-  auto kv_empty = [&](int s) { return bars + 8u * (8 + s); };
-  auto s_full = [&](int t) { return bars + 8u * (12 + t); };
-  auto ds_full = [&](int t) { return bars + 8u * (14 + t); };
-  auto dq_full = [&](int t) { return bars + 8u * (16 + t); };
-  const uint32_t rows_ready = bars + 8u * 18, tmem_slot = bars + 8u * 19, scale_slot = tmem_slot + 4;
+  auto kv_clean = [&](int s) { return bars + 8u * (5 + s); };
+  auto kv_empty = [&](int s) { return bars + 8u * (10 + s); };
+  auto s_full = [&](int u) { return bars + 8u * (15 + u); };
+  auto ds_full = [&](int u) { return bars + 8u * (18 + u); };
+  const uint32_t dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, scale_slot = tmem_slot + 4;
 
-  const int pairs = (a.R + 255) / 256;
-  const int unit = blockIdx.x / pairs, m = unit / a.Hk, hk = unit % a.Hk;
-  const int row0 = (blockIdx.x - unit * pairs) * 256;
-  const int tiles = a.R - row0 > 128 ? 2 : 1;
+  const int tiles = (a.R + 127) / 128;
+  const int unit = blockIdx.x / tiles, m = unit / a.Hk, hk = unit % a.Hk;
+  const int row0 = (blockIdx.x - unit * tiles) * 128;
   const int len = visible_keys(a, m);
   const int nt = (len + BN - 1) / BN;
   const bool hide = a.mask != nullptr;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_clean(s), 1); mbar_init(kv_empty(s), 1); }
-    for (int t = 0; t < 2; ++t) { mbar_init(s_full(t), 1); mbar_init(ds_full(t), 4); mbar_init(dq_full(t), 1); }
-    mbar_init(rows_ready, 4 * tiles);
+    for (int u = 0; u < 3; ++u) { mbar_init(s_full(u), 1); mbar_init(ds_full(u), 4); }
+    mbar_init(dq_full, 1);
+    mbar_init(rows_ready, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -190,56 +190,50 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     constexpr uint32_t idesc_s = instr_desc<T>(BN, false), idesc_o = instr_desc<T>(DP, true);
     const uint64_t qd = make_desc(base, 16, 1024), od = make_desc(base + S::DO0, 16, 1024);
     const uint64_t kd = make_desc(base + S::KV0, 16, 1024), kn = make_desc(base + S::KV0, BN * 128, 1024);
-    auto scores = [&](int t, int s) {
+    auto scores = [&](int j) {                              // s = q k^T, dp = do v^T of block j into buffer j % 3
+      const uint64_t st = (uint64_t)(((j % S::STAGES) * 2 * S::KEYS) >> 4);
+      const uint32_t d = tmem + 128 + (j % 3) * 128;
       if (elect_one()) {
-        const uint64_t st = (uint64_t)((s * 2 * S::KEYS) >> 4);
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t ro = (uint64_t)((t * S::ROWS + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
-          umma_bf16(tmem + t * 64, qd + ro, kd + st + ko, idesc_s, kk > 0);
+          const uint64_t ro = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+          umma_bf16(d, qd + ro, kd + st + ko, idesc_s, kk > 0);
         }
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t ro = (uint64_t)((t * S::ROWS + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
-          umma_bf16(tmem + 128 + t * 64, od + ro, kd + st + (S::KEYS >> 4) + ko, idesc_s, kk > 0);
+          const uint64_t ro = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+          umma_bf16(d + 64, od + ro, kd + st + (S::KEYS >> 4) + ko, idesc_s, kk > 0);
         }
-        umma_commit(s_full(t));
+        umma_commit(s_full(j % 3));
       }
       __syncwarp();
     };
-    bool ok = nt > 0 && warp_wait(rows_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL) && warp_wait(kv_clean(0), 0, a.status, SB_TIMEOUT_SMEM_FULL);
-    if (ok) {
+    bool ok = nt > 0 && warp_wait(rows_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    for (int j = 0; j < 3 && j < nt && ok; ++j) {
+      ok = warp_wait(kv_clean(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (!ok) break;
       tc_fence_after();
-      for (int t = 0; t < tiles; ++t) scores(t, 0);
+      scores(j);
     }
-    int s = 0;
-    uint32_t ph = 0;
     for (int j = 0; j < nt && ok; ++j) {
-      const int s1 = s + 1 == S::STAGES ? 0 : s + 1;
-      const uint32_t ph1 = s1 == 0 ? ph ^ 1u : ph;
-      for (int t = 0; t < tiles && ok; ++t) {
-        ok = warp_wait(ds_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_EMPTY);
+      const int s = j % S::STAGES, u = j % 3;
+      ok = warp_wait(ds_full(u), (uint32_t)(j / 3) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          umma_ts(tmem, tmem + 128 + u * 128 + kk * 8, kn + (uint64_t)((s * 2 * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
+        umma_commit(kv_empty(s));
+        if (j == nt - 1) umma_commit(dq_full);
+      }
+      __syncwarp();
+      if (j + 3 < nt) {
+        ok = warp_wait(kv_clean((j + 3) % S::STAGES), (uint32_t)((j + 3) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            umma_ts(tmem + 256 + t * DP, tmem + t * 64 + kk * 8, kn + (uint64_t)((s * 2 * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
-          if (t == tiles - 1) umma_commit(kv_empty(s));
-          if (j == nt - 1) umma_commit(dq_full(t));
-        }
-        __syncwarp();
-        if (j + 1 < nt) {
-          if (t == 0) {
-            ok = warp_wait(kv_clean(s1), ph1, a.status, SB_TIMEOUT_SMEM_FULL);
-            if (!ok) break;
-            tc_fence_after();
-          }
-          scores(t, s1);
-        }
+        scores(j + 3);
       }
-      s = s1;
-      ph = ph1;
     }
   } else if (warp == 2) {
     // hidden key rows are cleared: their ds is zero, and zero times NaN is not
@@ -258,9 +252,10 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (lane == 0) mbar_arrive(kv_clean(s));
       if (++s == S::STAGES) { s = 0; ph ^= 1u; }
     }
-  } else if (warp >= 4 && (warp - 4) / 4 < tiles) {
-    const int t = (warp - 4) >> 2, quarter = warp & 3;
-    const int tile_row = row0 + t * 128, row = tile_row + quarter * 32 + lane;
+  } else if (warp >= 4) {
+    // the two warpgroups take key blocks in turn; both load the rows
+    const int wg = (warp - 4) >> 2, quarter = warp & 3;
+    const int row = row0 + quarter * 32 + lane;
     const bool valid = row < a.R;
     float dsf;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
@@ -268,60 +263,63 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const float nlse = valid ? b.nlse[stat] : -INFINITY;
     float ndelta = valid ? b.ndelta[stat] : 0.f;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_addr = lane_base + t * 64, dp_addr = lane_base + 128 + t * 64, dq_addr = lane_base + 256 + t * DP;
     bool ok = true;
     if (nt > 0) {
-      load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, tile_row, base + t * S::ROWS, quarter, lane);
-      const long long st = (long long)a.H * a.D;
-      load_rows<DP>(a, b.dout, st * a.Tq, st, a.D, m, hk, tile_row, base + S::DO0 + t * S::ROWS, quarter, lane);
+      if (wg == 0) {
+        load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, row0, base, quarter, lane);
+      } else {
+        const long long st = (long long)a.H * a.D;
+        load_rows<DP>(a, b.dout, st * a.Tq, st, a.D, m, hk, row0, base + S::DO0, quarter, lane);
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(rows_ready);
     }
-    for (int j = 0; j < nt; ++j) {
+    const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse), f2 = pair(dsf, dsf);
+    for (int j = wg; j < nt; j += 2) {
       const bool some_hidden = hide || (j + 1) * BN > len;
       uint32_t w[2] = {0, 0};
       if (some_hidden) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
       }
-      ok = warp_wait(s_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_FULL);
+      const int u = j % 3;
+      const uint32_t s_addr = lane_base + 128 + u * 128;
+      ok = warp_wait(s_full(u), (uint32_t)(j / 3) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      uint32_t sr[64], pr[64];
-      tmem_load64(s_addr, sr);
-      tmem_load64(dp_addr, pr);
-      const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse);
+      uint32_t r[128];                                     // 64 scores, 64 dp
+      tmem_load128(s_addr, r);
 #pragma unroll
       for (int k = 0; k < 64; k += 2) {                    // p over s
         float x, y;
-        split(fma2(pair(sr[k], sr[k + 1]), c2, nl2), x, y);
-        sr[k] = __float_as_uint(ex2(x));
-        sr[k + 1] = __float_as_uint(ex2(y));
+        split(fma2(pair(r[k], r[k + 1]), c2, nl2), x, y);
+        r[k] = __float_as_uint(ex2(x));
+        r[k + 1] = __float_as_uint(ex2(y));
       }
       if (some_hidden) {
 #pragma unroll
         for (int k = 0; k < 64; ++k)
-          if ((w[k >> 5] >> (k & 31)) & 1u) sr[k] = pr[k] = 0u;
+          if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = r[64 + k] = 0u;
       }
       if (nt == 1) {
-        // all keys are in this tile: delta = sum p dp from the values that it is subtracted from, instead of the rounded output
+        // all keys are in this block: delta = sum p dp from the values that it is subtracted from, instead of the rounded output
         uint64_t d2[2] = {0, 0};
 #pragma unroll
-        for (int k = 0; k < 64; k += 2) d2[(k >> 1) & 1] = fma2(pair(sr[k], sr[k + 1]), pair(pr[k], pr[k + 1]), d2[(k >> 1) & 1]);
+        for (int k = 0; k < 64; k += 2) d2[(k >> 1) & 1] = fma2(pair(r[k], r[k + 1]), pair(r[64 + k], r[65 + k]), d2[(k >> 1) & 1]);
         float x, y;
         split(add2(d2[0], d2[1]), x, y);
         ndelta = -(x + y);
         if (valid) b.ndelta[stat] = ndelta;
       }
-      const uint64_t nd2 = pair(ndelta, ndelta), f2 = pair(dsf, dsf);
+      const uint64_t nd2 = pair(ndelta, ndelta);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t o[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const int e = 32 * i + 2 * k;
-          uint64_t v = mul2(pair(sr[e], sr[e + 1]), add2(pair(pr[e], pr[e + 1]), nd2));
+          uint64_t v = mul2(pair(r[e], r[e + 1]), add2(pair(r[64 + e], r[65 + e]), nd2));
           if (Half2<T>::KIND == 0) v = mul2(v, f2);
           float x, y;
           split(v, x, y);
@@ -332,26 +330,30 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       tmem_store_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full(t));
+      if (lane == 0) mbar_arrive(ds_full(u));
     }
-    if (nt > 0 && ok) ok = warp_wait(dq_full(t), 0, a.status, SB_TIMEOUT_TMEM_FULL);
+    if (nt > 0 && ok) ok = warp_wait(dq_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
-    uint16_t* dst = dq;
-    if (valid) {
-      const RowAt at = row_at(a, m, hk, row);
-      dst = dq + (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
-    }
-    const float f = b.scale / dsf;
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-      uint32_t r[32];
-      if (nt > 0 && ok) {
-        tmem_load32(dq_addr + 32 * i, r);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 32; ++k) r[k] = 0u;
+    if (dq) {
+      // each warpgroup writes half of the columns
+      uint16_t* dst = dq;
+      if (valid) {
+        const RowAt at = row_at(a, m, hk, row);
+        dst = dq + (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
       }
-      if (valid && dq) store_row32<T>(dst, 32 * i, a.D, r, f);
+      const float f = b.scale / dsf;
+#pragma unroll
+      for (int i = 0; i < DP / 64; ++i) {
+        const int col = wg * (DP / 2) + 32 * i;
+        uint32_t r[32];
+        if (nt > 0 && ok) {
+          tmem_load32(lane_base + col, r);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) r[k] = 0u;
+        }
+        if (valid) store_row32<T>(dst, col, a.D, r, f);
+      }
     }
   }
   tc_fence_before();
@@ -360,6 +362,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ dk, dv
+constexpr int DKV_THREADS = 640;
 template <int DP> struct DkvSmem {
   static constexpr int BQ = 64;                            // query rows of a step
   static constexpr int STAGES = 4;
@@ -369,7 +372,7 @@ template <int DP> struct DkvSmem {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(BWD_THREADS, 1)
+__global__ void __launch_bounds__(DKV_THREADS, 1)
 xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
                  const __grid_constant__ CUtensorMap map_do, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv) {
   using S = DkvSmem<DP>;
@@ -393,7 +396,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) { mbar_init(q_full(s), 1); mbar_init(q_empty(s), 1); }
-    for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 1); mbar_init(p_full(u), 4); }
+    for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 1); mbar_init(p_full(u), 8); }
     mbar_init(kv_full, 1);
     mbar_init(d_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -492,10 +495,10 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const uint64_t st = (uint64_t)((s * 2 * S::ROWS) >> 4);
 #pragma unroll
         for (int kk = 0; kk < BQ / 16; ++kk)
-          umma_ts(tmem, p + kk * 8, qn + st + (uint64_t)((S::ROWS + kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
+          umma_ts(tmem, p + (kk >> 1) * 32 + (kk & 1) * 8, qn + st + (uint64_t)((S::ROWS + kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
 #pragma unroll
         for (int kk = 0; kk < BQ / 16; ++kk)
-          umma_ts(tmem + 128, p + 64 + kk * 8, qn + st + (uint64_t)((kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
+          umma_ts(tmem + 128, p + 64 + (kk >> 1) * 32 + (kk & 1) * 8, qn + st + (uint64_t)((kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
         umma_commit(q_empty(s));
         if (i == nq - 1) umma_commit(d_full);
       }
@@ -509,7 +512,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
   } else if (warp >= 4) {
     // ---------------------------------------------------------------- p^T and ds^T; lanes are keys
-    const int u = (warp - 4) >> 2, quarter = warp & 3;
+    const int u = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3;
     const int key = key0 + quarter * 32 + lane;
     bool ok = true;
     float dsf;
@@ -519,7 +522,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const float k_ds = dsf * ex2(-p_shift<T>());
     const uint64_t c2 = pair(a.c, a.c), shift2 = pair(p_shift<T>(), p_shift<T>()), f2 = pair(k_ds, k_ds);
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_addr = lane_base + 256 + u * 128;
+    const uint32_t s_addr = lane_base + 256 + u * 128 + half * 32;
     for (int i = u; i < nq; i += 2) {
       ok = warp_wait(s_full(u), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
@@ -528,39 +531,37 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       const uint32_t stat = base + S::STAT0 + (i % S::STAGES) * S::STAT;
+      // p^T and ds^T of a half go over the scores and dp that it has read itself: 16 of its 32 columns
+      uint32_t sr[32], pr[32], po[16], so[16];
+      tmem_load32(s_addr, sr);
+      tmem_load32(s_addr + 64, pr);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t sr[32], pr[32], po[16], so[16];
-        tmem_load32(s_addr + 32 * h, sr);
-        tmem_load32(s_addr + 64 + 32 * h, pr);
+      for (int k = 0; k < 32; k += 4) {
+        uint64_t l[2], d[2];
+        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(l[0]), "=l"(l[1]) : "r"(stat + (32 * half + k) * 4));
+        asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(d[0]), "=l"(d[1]) : "r"(stat + (BQ + 32 * half + k) * 4));
 #pragma unroll
-        for (int k = 0; k < 32; k += 4) {
-          uint64_t l[2], d[2];
-          asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(l[0]), "=l"(l[1]) : "r"(stat + (32 * h + k) * 4));
-          asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(d[0]), "=l"(d[1]) : "r"(stat + (BQ + 32 * h + k) * 4));
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = k + 2 * e;
-            if (Half2<T>::KIND == 0) l[e] = add2(l[e], shift2);
-            float x, y;
-            split(fma2(pair(sr[j], sr[j + 1]), c2, l[e]), x, y);
-            x = ex2(x);
-            y = ex2(y);
-            uint64_t v = mul2(pair(x, y), add2(pair(pr[j], pr[j + 1]), d[e]));
-            if (Half2<T>::KIND == 0) v = mul2(v, f2);
-            po[j >> 1] = Half2<T>::pack(x, y);
-            split(v, x, y);
-            so[j >> 1] = pack_ds<T>(x, y);
-          }
+        for (int e = 0; e < 2; ++e) {
+          const int j = k + 2 * e;
+          if (Half2<T>::KIND == 0) l[e] = add2(l[e], shift2);
+          float x, y;
+          split(fma2(pair(sr[j], sr[j + 1]), c2, l[e]), x, y);
+          x = ex2(x);
+          y = ex2(y);
+          uint64_t v = mul2(pair(x, y), add2(pair(pr[j], pr[j + 1]), d[e]));
+          if (Half2<T>::KIND == 0) v = mul2(v, f2);
+          po[j >> 1] = Half2<T>::pack(x, y);
+          split(v, x, y);
+          so[j >> 1] = pack_ds<T>(x, y);
         }
-        if (some_hidden && hidden) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) po[k] = so[k] = 0u;
-        }
-        __syncwarp();
-        tmem_store16(s_addr + 16 * h, po);
-        tmem_store16(s_addr + 64 + 16 * h, so);
       }
+      if (some_hidden && hidden) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) po[k] = so[k] = 0u;
+      }
+      __syncwarp();
+      tmem_store16(s_addr, po);
+      tmem_store16(s_addr + 64, so);
       tmem_store_wait();
       tc_fence_before();
       __syncwarp();
@@ -568,19 +569,20 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (nq > 0 && ok) ok = warp_wait(d_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
-    // one warpgroup writes dv, the other dk
+    // two warpgroups write dv, the others dk, half of the columns each
     uint16_t* dst = (u ? dk : dv) + (((long long)m * a.Tk + key) * a.Hk + hk) * a.D;
     const float f = u ? b.scale / dsf : ex2(-p_shift<T>());
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
+    for (int i = 0; i < DP / 64; ++i) {
+      const int col = half * (DP / 2) + 32 * i;
       uint32_t r[32];
       if (nq > 0 && ok) {
-        tmem_load32(lane_base + u * 128 + 32 * i, r);
+        tmem_load32(lane_base + u * 128 + col, r);
       } else {
 #pragma unroll
         for (int k = 0; k < 32; ++k) r[k] = 0u;
       }
-      if (key < a.Tk) store_row32<T>(dst, 32 * i, a.D, r, f);
+      if (key < a.Tk) store_row32<T>(dst, col, a.D, r, f);
     }
   }
   tc_fence_before();
@@ -600,7 +602,7 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   if (!rc) rc = sb_allow_smem((const void*)xattn_dq_kernel<T, DP>, DqSmem<DP>::BYTES);
   if (!rc) rc = sb_allow_smem((const void*)xattn_dkv_kernel<T, DP>, DkvSmem<DP>::BYTES);
   if (rc) return rc;
-  const long long units = (long long)a.M * a.Hk, gq = units * ((a.R + 255) / 256), gk = units * ((a.Tk + 127) / 128);
+  const long long units = (long long)a.M * a.Hk, gq = units * ((a.R + 127) / 128), gk = units * ((a.Tk + 127) / 128);
   if (gq > 0x7fffffffll || gk > 0x7fffffffll) return SB_BAD_ARGUMENT;
   const long long blocks = (units * a.G * a.rep * b.Tqp + 15) / 16;
   b.peaks = (int)(blocks < MAX_PARTS ? blocks : MAX_PARTS);
@@ -611,7 +613,7 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
     rc = (int)cudaGetLastError();
   }
   if (!rc && dk) {
-    xattn_dkv_kernel<T, DP><<<(unsigned)gk, BWD_THREADS, DkvSmem<DP>::BYTES, stream>>>(k128, v128, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv);
+    xattn_dkv_kernel<T, DP><<<(unsigned)gk, DKV_THREADS, DkvSmem<DP>::BYTES, stream>>>(k128, v128, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv);
     rc = (int)cudaGetLastError();
   }
   return rc;

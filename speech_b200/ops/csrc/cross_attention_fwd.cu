@@ -4,12 +4,13 @@
 //   s = q k_j^T,  m' = max(m, max s),  o = o 2^(c (m - m')) + p v_j,  l = l 2^(c (m - m')) + sum p,  at the end o / l
 // and lse = c m + log2 l is kept for the backward pass (+inf for a row that sees nothing: its probabilities are then 2^-inf = 0).
 //
-// A CTA takes two tiles of 128 packed rows and streams the 128-key tiles of its memory and key head past both, so that keys and values
+// A CTA takes two tiles of 128 packed rows and streams blocks of 64 keys of its memory and key head past both, so that keys and values
 // cross the L2 once per 256 rows.  Warp 0 loads keys and values by TMA, warp 1 issues all tcgen05.mma, warp 2 clears hidden value
-// rows, and one warpgroup per row tile does the softmax: scores and output accumulate in tensor memory (2 x (128 + DP) columns), the
-// probabilities go back there as 16-bit pairs over the scores they came from and are the A operand of the second product.  While one
-// tile's warpgroup works, the tensor core works for the other.  The output is rescaled only when a row's maximum has grown by more than
-// 2^8 since the last time; p then stays below 2^8, and the result does not depend on it beyond rounding.
+// rows, and one warpgroup per row tile does the softmax: scores and output accumulate in tensor memory (per tile two buffers of 64
+// columns and DP columns), the probabilities go back there as 16-bit pairs over the scores they came from and are the A operand of
+// the second product.  The scores of the next block are there before the softmax of this one ends; with one buffer of 128 keys the
+// warpgroups waited for the tensor core and it for them (41 % of its cycles busy).  The output is rescaled only when a row's maximum
+// has grown by more than 2^8 since the last time; p then stays below 2^8, and the result does not depend on it beyond rounding.
 //
 // Rounding: scores, maxima, sums and output are fp32; p is rounded to the operands' 16-bit type, which is what the tensor core
 // multiplies (relative 2^-9 per weight in bf16, random, as large as the one rounding of the result); l sums the unrounded p.
@@ -19,12 +20,12 @@
 namespace {
 
 constexpr int FWD_THREADS = 384;
-constexpr int BN = 128;
+constexpr int BN = 64;
 template <int DP> struct FwdSmem {
-  static constexpr int STAGES = DP == 128 ? 2 : 4;
-  static constexpr int TILE = 128 * DP * 2;               // a tile of 128 rows of q, k or v
-  static constexpr int K0 = 2 * TILE, V0 = K0 + STAGES * TILE, BAR = V0 + STAGES * TILE;
-  static constexpr int BYTES = BAR + 256 + 1024;
+  static constexpr int STAGES = 4;
+  static constexpr int TILE = 128 * DP * 2, KEYS = BN * DP * 2;      // 128 query rows, a block of keys or values
+  static constexpr int K0 = 2 * TILE, V0 = K0 + STAGES * KEYS, BAR = V0 + STAGES * KEYS;
+  static constexpr int BYTES = BAR + 512 + 1024;
 };
 
 template <typename T, int DP>
@@ -42,10 +43,11 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto v_full = [&](int s) { return bars + 8u * (8 + s); };
   auto v_clean = [&](int s) { return bars + 8u * (12 + s); };
   auto v_empty = [&](int s) { return bars + 8u * (16 + s); };
-  auto s_full = [&](int t) { return bars + 8u * (20 + t); };
-  auto p_full = [&](int t) { return bars + 8u * (22 + t); };
-  auto o_full = [&](int t) { return bars + 8u * (24 + t); };
-  const uint32_t q_ready = bars + 8u * 26, tmem_slot = bars + 8u * 27;
+  auto s_full = [&](int t, int u) { return bars + 8u * (20 + 2 * t + u); };
+  auto p_full = [&](int t, int u) { return bars + 8u * (24 + 2 * t + u); };
+  auto pv_done = [&](int t) { return bars + 8u * (28 + t); };   // every block's product: at most one is outstanding when it is waited for
+  auto o_full = [&](int t) { return bars + 8u * (32 + t); };    // the last one
+  const uint32_t q_ready = bars + 8u * 30, tmem_slot = bars + 8u * 31;
 
   const int pairs = (a.R + 255) / 256;                    // row-tile pairs of a (memory, key head): neighbours in the grid, for the L2
   const int unit = blockIdx.x / pairs, m = unit / a.Hk, hk = unit % a.Hk;
@@ -60,7 +62,11 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1);
       mbar_init(v_full(s), 1); mbar_init(v_clean(s), 1); mbar_init(v_empty(s), 1);
     }
-    for (int t = 0; t < 2; ++t) { mbar_init(s_full(t), 1); mbar_init(p_full(t), 4); mbar_init(o_full(t), 1); }
+    for (int t = 0; t < 2; ++t) {
+      for (int u = 0; u < 2; ++u) { mbar_init(s_full(t, u), 1); mbar_init(p_full(t, u), 4); }
+      mbar_init(pv_done(t), 1);
+      mbar_init(o_full(t), 1);
+    }
     mbar_init(q_ready, 4 * tiles);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -85,18 +91,18 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       ok = warp_wait(k_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY);
       if (!ok) break;
       if (elect_one()) {
-        mbar_expect_tx(k_full(s), S::TILE);
+        mbar_expect_tx(k_full(s), S::KEYS);
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::K0 + s * S::TILE + h * 16384, &map_k, k_full(s), h * 64, j * BN, hk, m);
+        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::K0 + s * S::KEYS + h * (BN * 128), &map_k, k_full(s), h * 64, j * BN, hk, m);
       }
       __syncwarp();
       ok = warp_wait(v_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY);
       issued = j + 1;
       if (!ok) break;
       if (elect_one()) {
-        mbar_expect_tx(v_full(s), S::TILE);
+        mbar_expect_tx(v_full(s), S::KEYS);
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::V0 + s * S::TILE + h * 16384, &map_v, v_full(s), h * 64, j * BN, hk, m);
+        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::V0 + s * S::KEYS + h * (BN * 128), &map_v, v_full(s), h * 64, j * BN, hk, m);
       }
       __syncwarp();
       if (++s == S::STAGES) { s = 0; ph ^= 1u; }
@@ -110,55 +116,50 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     // ---------------------------------------------------------------- matrix products
     constexpr uint32_t idesc_s = instr_desc<T>(BN, false), idesc_o = instr_desc<T>(DP, true);
     const uint64_t qd = make_desc(base, 16, 1024), kd = make_desc(base + S::K0, 16, 1024), vd = make_desc(base + S::V0, BN * 128, 1024);
-    auto scores = [&](int t, int s) {
+    auto scores = [&](int t, int j) {                       // s = q k^T of block j into buffer j & 1
+      const uint64_t st = (uint64_t)(((j % S::STAGES) * S::KEYS) >> 4);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t off = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4);
-          umma_bf16(tmem + t * 128, qd + ((t * S::TILE) >> 4) + off, kd + ((s * S::TILE) >> 4) + off, idesc_s, kk > 0);
+          const uint64_t ro = (uint64_t)((t * S::TILE + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+          umma_bf16(tmem + t * 128 + (j & 1) * 64, qd + ro, kd + st + ko, idesc_s, kk > 0);
         }
-        umma_commit(s_full(t));
+        umma_commit(s_full(t, j & 1));
+        if (t == tiles - 1) umma_commit(k_empty(j % S::STAGES));
       }
       __syncwarp();
     };
-    bool ok = nt > 0 && warp_wait(q_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL) && warp_wait(k_full(0), 0, a.status, SB_TIMEOUT_SMEM_FULL);
-    if (ok) {
+    bool ok = nt > 0 && warp_wait(q_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    for (int j = 0; j < 2 && j < nt && ok; ++j) {
+      ok = warp_wait(k_full(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (!ok) break;
       tc_fence_after();
-      for (int t = 0; t < tiles; ++t) scores(t, 0);
-      if (elect_one()) umma_commit(k_empty(0));
-      __syncwarp();
+      for (int t = 0; t < tiles; ++t) scores(t, j);
     }
-    int s = 0;
-    uint32_t ph = 0;
     for (int j = 0; j < nt && ok; ++j) {
-      const int s1 = s + 1 == S::STAGES ? 0 : s + 1;
-      const uint32_t ph1 = s1 == 0 ? ph ^ 1u : ph;
+      const int s = j % S::STAGES;
       for (int t = 0; t < tiles && ok; ++t) {
-        ok = warp_wait(p_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_EMPTY);
-        if (ok && t == 0) ok = warp_wait(v_clean(s), ph, a.status, SB_TIMEOUT_SMEM_FULL);
+        ok = warp_wait(p_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
+        if (ok && t == 0) ok = warp_wait(v_clean(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < BN / 16; ++kk)
-            umma_ts(tmem + 256 + t * DP, tmem + t * 128 + kk * 8, vd + ((s * S::TILE) >> 4) + (uint64_t)(kk * (2048 >> 4)), idesc_o, (j > 0) | (kk > 0));
+            umma_ts(tmem + 256 + t * DP, tmem + t * 128 + (j & 1) * 64 + kk * 8, vd + (uint64_t)((s * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
           if (t == tiles - 1) umma_commit(v_empty(s));
-          if (j == nt - 1) umma_commit(o_full(t));
+          umma_commit(j == nt - 1 ? o_full(t) : pv_done(t));
         }
         __syncwarp();
-        if (j + 1 < nt) {
+        if (j + 2 < nt) {
           if (t == 0) {
-            ok = warp_wait(k_full(s1), ph1, a.status, SB_TIMEOUT_SMEM_FULL);
+            ok = warp_wait(k_full((j + 2) % S::STAGES), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
             if (!ok) break;
             tc_fence_after();
           }
-          scores(t, s1);
-          if (t == tiles - 1 && elect_one()) umma_commit(k_empty(s1));
-          __syncwarp();
+          scores(t, j + 2);
         }
       }
-      s = s1;
-      ph = ph1;
     }
   } else if (warp == 2) {
     // ---------------------------------------------------------------- hidden value rows
@@ -167,10 +168,10 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     for (int j = 0; j < nt; ++j) {
       if (!warp_wait(v_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
       if (hide || (j + 1) * BN > len) {
-        uint32_t w[4];
+        uint32_t w[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
-        clear_rows<DP>(base + S::V0 + s * S::TILE, BN, w, 4, lane);
+        for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
+        clear_rows<DP>(base + S::V0 + s * S::KEYS, BN, w, 2, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -184,7 +185,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     bool ok = true;
     float mx = -INFINITY, l = 0.f;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_addr = lane_base + t * 128, o_addr = lane_base + 256 + t * DP;
+    const uint32_t o_addr = lane_base + 256 + t * DP;
     if (nt > 0) {
       load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, tile_row, base + t * S::TILE, quarter, lane);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -193,24 +194,25 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     for (int j = 0; j < nt; ++j) {
       const bool some_hidden = hide || (j + 1) * BN > len;
-      uint32_t w[4] = {0, 0, 0, 0};
+      const uint32_t s_addr = lane_base + t * 128 + (j & 1) * 64;
+      uint32_t w[2] = {0, 0};
       if (some_hidden) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
+        for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
       }
-      ok = warp_wait(s_full(t), j & 1, a.status, SB_TIMEOUT_TMEM_FULL);
+      ok = warp_wait(s_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      uint32_t r[128];
-      tmem_load128(s_addr, r);
+      uint32_t r[BN];
+      tmem_load64(s_addr, r);
       if (some_hidden) {
 #pragma unroll
-        for (int k = 0; k < 128; ++k)
+        for (int k = 0; k < BN; ++k)
           if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = 0xff800000u;
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int k = 0; k < 128; k += 8)
+      for (int k = 0; k < BN; k += 8)
 #pragma unroll
         for (int i = 0; i < 4; ++i) top[i] = max3(top[i], __uint_as_float(r[k + 2 * i]), __uint_as_float(r[k + 2 * i + 1]));
       const float tile_max = fmaxf(max3(top[0], top[1], top[2]), top[3]);
@@ -224,6 +226,11 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           mx = nm;
         }
         if (j > 0) {
+          // products up to block j - 1 have been added: those up to j - 2 have (the scores of block j were issued behind them), and the
+          // last one is waited for here
+          ok = warp_wait(pv_done(t), (uint32_t)(j - 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
           for (int i = 0; i < DP / 32; ++i) {
             uint32_t x[32];
@@ -239,7 +246,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const uint64_t c2 = pair(a.c, a.c), shift2 = pair(-mc, -mc);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < BN / 32; ++i) {
         uint32_t p[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -260,7 +267,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       tmem_store_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full(t));
+      if (lane == 0) mbar_arrive(p_full(t, j & 1));
     }
     if (nt > 0 && ok) ok = warp_wait(o_full(t), 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
