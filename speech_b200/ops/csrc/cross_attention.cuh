@@ -249,18 +249,13 @@ template <typename T> __device__ __forceinline__ void store_out32(uint16_t* out,
     }
 }
 
-// Zeroes the rows of a [rows, DP] tile whose keys are hidden (bits of `words`, 32 rows each): a hidden value of infinity or NaN would
-// turn its zero weight into NaN inside the matrix product.
-template <int DP>
-__device__ __forceinline__ void clear_rows(uint32_t tile, int rows, const uint32_t* words, int nwords, int lane) {
+// Zeroes the rows of a [64, DP] tile whose keys are hidden (bits of words[0..1]): a hidden value of infinity or NaN would turn its zero
+// weight into NaN inside the matrix product.  `threads` threads with numbers `id` share the work.
+template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, int rows, const uint32_t* words, int id, int threads) {
   constexpr int CH = DP / 8;
-  for (int w = 0; w < nwords; ++w) {
-    uint32_t bits = words[w];
-    while (bits) {
-      const int row = w * 32 + __ffs(bits) - 1;
-      bits &= bits - 1;
-      if (lane < CH) st_shared_v4(tile_addr(tile, rows, row, lane), 0, 0, 0, 0);
-    }
+  for (int i = id; i < rows * CH; i += threads) {
+    const int row = i / CH;
+    if (((row < 32 ? words[0] : words[1]) >> (row & 31)) & 1u) st_shared_v4(tile_addr(tile, rows, row, i % CH), 0, 0, 0, 0);
   }
 }
 

@@ -6,8 +6,11 @@
 // sums of dq would need five, but every sum is taken by one CTA in a fixed order, so that gradients are the same every time, nothing
 // is accumulated in fp32 memory and converted afterwards, and gradients of shared heads and shared rows are sums over packed rows.
 //
-// Both kernels have the roles of the forward pass.  dq: blocks of 64 keys go through three sets of tensor memory columns (scores and dp,
-// 64 each), two warpgroups take them in turn, so that scores are computed ahead of them.  dk / dv: tiles of 64 query rows of one head
+// The products into 64 columns have a warp each that issues them: such an instruction takes the tensor core 32 cycles, and issuing it
+// costs a warp twice that, so that one issuer for all of them left the tensor core idle more than half of the time.
+//
+// Both kernels have the roles of the forward pass otherwise.  dq: blocks of 64 keys go through three sets of tensor memory columns (scores and dp,
+// 64 each), with a warpgroup for each.  dk / dv: tiles of 64 query rows of one head
 // take turns in two such sets, transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; four
 // warpgroups, two per set with half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which a row kernel
 // lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
@@ -20,7 +23,7 @@
 
 namespace {
 
-constexpr int BWD_THREADS = 384;
+constexpr int DQ_THREADS = 512, DKV_THREADS = 640;     // 16 warps of 128 registers, 20 of 96
 constexpr int MAX_PARTS = 592;        // blocks of the row kernel, whose maxima every block of the other kernels joins
 
 template <typename T> constexpr float p_shift() { return Half2<T>::KIND == 0 ? 12.f : 0.f; }
@@ -122,7 +125,7 @@ template <int DP> struct DqSmem {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(BWD_THREADS, 1)
+__global__ void __launch_bounds__(DQ_THREADS, 1)
 xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq) {
   using S = DqSmem<DP>;
   constexpr int BN = S::BN, HALVES = DP / 64;
@@ -131,11 +134,11 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const uint32_t bars = base + S::BAR;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto kv_full = [&](int s) { return bars + 8u * s; };
-  auto kv_clean = [&](int s) { return bars + 8u * (5 + s); };
   auto kv_empty = [&](int s) { return bars + 8u * (10 + s); };
   auto s_full = [&](int u) { return bars + 8u * (15 + u); };
   auto ds_full = [&](int u) { return bars + 8u * (18 + u); };
-  const uint32_t dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, scale_slot = tmem_slot + 4;
+  auto s_empty = [&](int u) { return bars + 8u * (21 + u); };
+  const uint32_t dq_full = bars + 8u * 24, rows_ready = bars + 8u * 25, tmem_slot = bars + 8u * 26, scale_slot = tmem_slot + 4;
 
   const int tiles = (a.R + 127) / 128;
   const int unit = blockIdx.x / tiles, m = unit / a.Hk, hk = unit % a.Hk;
@@ -145,10 +148,10 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const bool hide = a.mask != nullptr;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::STAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_clean(s), 1); mbar_init(kv_empty(s), 1); }
-    for (int u = 0; u < 3; ++u) { mbar_init(s_full(u), 1); mbar_init(ds_full(u), 4); }
+    for (int s = 0; s < S::STAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
+    for (int u = 0; u < 3; ++u) { mbar_init(s_full(u), 2); mbar_init(ds_full(u), 4); mbar_init(s_empty(u), 1); }
     mbar_init(dq_full, 1);
-    mbar_init(rows_ready, 8);
+    mbar_init(rows_ready, 12);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -186,74 +189,57 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
     for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
       warp_wait(kv_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
-  } else if (warp == 1) {
-    constexpr uint32_t idesc_s = instr_desc<T>(BN, false), idesc_o = instr_desc<T>(DP, true);
-    const uint64_t qd = make_desc(base, 16, 1024), od = make_desc(base + S::DO0, 16, 1024);
-    const uint64_t kd = make_desc(base + S::KV0, 16, 1024), kn = make_desc(base + S::KV0, BN * 128, 1024);
-    auto scores = [&](int j) {                              // s = q k^T, dp = do v^T of block j into buffer j % 3
-      const uint64_t st = (uint64_t)(((j % S::STAGES) * 2 * S::KEYS) >> 4);
-      const uint32_t d = tmem + 128 + (j % 3) * 128;
+  } else if (warp == 1 || warp == 3) {
+    // s = q k^T (warp 1) and dp = do v^T (warp 3) of block j into buffer j % 3
+    const bool second = warp == 3;
+    constexpr uint32_t idesc_s = instr_desc<T>(BN, false);
+    const uint64_t rd = make_desc(base + (second ? S::DO0 : 0), 16, 1024), kd = make_desc(base + S::KV0 + (second ? S::KEYS : 0), 16, 1024);
+    bool ok = nt > 0 && warp_wait(rows_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    int s = 0, u = 0;
+    uint32_t ph = 0, uph = 1;
+    for (int j = 0; j < nt && ok; ++j) {
+      ok = warp_wait(s_empty(u), uph, a.status, SB_TIMEOUT_TMEM_EMPTY) && warp_wait(kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t st = (uint64_t)((s * 2 * S::KEYS) >> 4);
+      const uint32_t d = tmem + 128 + u * 128 + (second ? 64 : 0);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           const uint64_t ro = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
-          umma_bf16(d, qd + ro, kd + st + ko, idesc_s, kk > 0);
+          umma_bf16(d, rd + ro, kd + st + ko, idesc_s, kk > 0);
         }
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t ro = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
-          umma_bf16(d + 64, od + ro, kd + st + (S::KEYS >> 4) + ko, idesc_s, kk > 0);
-        }
-        umma_commit(s_full(j % 3));
+        umma_commit(s_full(u));
       }
       __syncwarp();
-    };
-    bool ok = nt > 0 && warp_wait(rows_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
-    for (int j = 0; j < 3 && j < nt && ok; ++j) {
-      ok = warp_wait(kv_clean(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
-      if (!ok) break;
-      tc_fence_after();
-      scores(j);
+      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+      if (++u == 3) { u = 0; uph ^= 1u; }
     }
+  } else if (warp == 2) {
+    // dq += ds k
+    constexpr uint32_t idesc_o = instr_desc<T>(DP, true);
+    const uint64_t kn = make_desc(base + S::KV0, BN * 128, 1024);
+    bool ok = true;
+    int s = 0, u = 0;
+    uint32_t uph = 0;
     for (int j = 0; j < nt && ok; ++j) {
-      const int s = j % S::STAGES, u = j % 3;
-      ok = warp_wait(ds_full(u), (uint32_t)(j / 3) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
+      ok = warp_wait(ds_full(u), uph, a.status, SB_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
           umma_ts(tmem, tmem + 128 + u * 128 + kk * 8, kn + (uint64_t)((s * 2 * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
+        umma_commit(s_empty(u));
         umma_commit(kv_empty(s));
         if (j == nt - 1) umma_commit(dq_full);
       }
       __syncwarp();
-      if (j + 3 < nt) {
-        ok = warp_wait(kv_clean((j + 3) % S::STAGES), (uint32_t)((j + 3) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
-        if (!ok) break;
-        tc_fence_after();
-        scores(j + 3);
-      }
+      if (++s == S::STAGES) s = 0;
+      if (++u == 3) { u = 0; uph ^= 1u; }
     }
-  } else if (warp == 2) {
-    // hidden key rows are cleared: their ds is zero, and zero times NaN is not
-    int s = 0;
-    uint32_t ph = 0;
-    for (int j = 0; j < nt; ++j) {
-      if (!warp_wait(kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
-      if (hide || (j + 1) * BN > len) {
-        uint32_t w[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
-        clear_rows<DP>(base + S::KV0 + s * 2 * S::KEYS, BN, w, 2, lane);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(kv_clean(s));
-      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
-    }
-  } else if (warp >= 4) {
-    // the two warpgroups take key blocks in turn; both load the rows
+  } else {
+    // three warpgroups take key blocks, and the three sets of columns with them, in turn
     const int wg = (warp - 4) >> 2, quarter = warp & 3;
     const int row = row0 + quarter * 32 + lane;
     const bool valid = row < a.R;
@@ -265,31 +251,29 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     bool ok = true;
     if (nt > 0) {
-      if (wg == 0) {
-        load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, row0, base, quarter, lane);
-      } else {
-        const long long st = (long long)a.H * a.D;
-        load_rows<DP>(a, b.dout, st * a.Tq, st, a.D, m, hk, row0, base + S::DO0, quarter, lane);
-      }
+      const long long st = (long long)a.H * a.D;
+      if (wg == 0) load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, row0, base, quarter, lane);
+      if (wg == 1) load_rows<DP>(a, b.dout, st * a.Tq, st, a.D, m, hk, row0, base + S::DO0, quarter, lane);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(rows_ready);
     }
     const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse), f2 = pair(dsf, dsf);
-    for (int j = wg; j < nt; j += 2) {
+    const uint32_t s_addr = lane_base + 128 + wg * 128;
+    uint32_t ph = 0;
+    for (int j = wg; j < nt; j += 3) {
       const bool some_hidden = hide || (j + 1) * BN > len;
       uint32_t w[2] = {0, 0};
       if (some_hidden) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
       }
-      const int u = j % 3;
-      const uint32_t s_addr = lane_base + 128 + u * 128;
-      ok = warp_wait(s_full(u), (uint32_t)(j / 3) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
+      ok = warp_wait(s_full(wg), ph, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
+      ph ^= 1u;
       tc_fence_after();
-      uint32_t r[128];                                     // 64 scores, 64 dp
-      tmem_load128(s_addr, r);
+      uint32_t r[64];
+      tmem_load64(s_addr, r);
 #pragma unroll
       for (int k = 0; k < 64; k += 2) {                    // p over s
         float x, y;
@@ -300,26 +284,39 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (some_hidden) {
 #pragma unroll
         for (int k = 0; k < 64; ++k)
-          if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = r[64 + k] = 0u;
+          if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = 0u;
+        // hidden key rows are cleared before dq sums over them: their ds is zero, and zero times NaN is not
+        clear_rows<DP>(base + S::KV0 + (j % S::STAGES) * 2 * S::KEYS, BN, w, quarter * 32 + lane, 128);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       if (nt == 1) {
         // all keys are in this block: delta = sum p dp from the values that it is subtracted from, instead of the rounded output
-        uint64_t d2[2] = {0, 0};
+        float d = 0.f;
 #pragma unroll
-        for (int k = 0; k < 64; k += 2) d2[(k >> 1) & 1] = fma2(pair(r[k], r[k + 1]), pair(r[64 + k], r[65 + k]), d2[(k >> 1) & 1]);
-        float x, y;
-        split(add2(d2[0], d2[1]), x, y);
-        ndelta = -(x + y);
+        for (int i = 0; i < 2; ++i) {
+          uint32_t g[32];
+          tmem_load32(s_addr + 64 + 32 * i, g);
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (!((w[i] >> k) & 1u)) d = fmaf(__uint_as_float(r[32 * i + k]), __uint_as_float(g[k]), d);
+        }
+        ndelta = -d;
         if (valid) b.ndelta[stat] = ndelta;
       }
       const uint64_t nd2 = pair(ndelta, ndelta);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint32_t o[16];
+        uint32_t g[32], o[16];
+        tmem_load32(s_addr + 64 + 32 * i, g);
+        if (some_hidden) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if ((w[i] >> k) & 1u) g[k] = 0u;
+        }
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const int e = 32 * i + 2 * k;
-          uint64_t v = mul2(pair(r[e], r[e + 1]), add2(pair(r[64 + e], r[65 + e]), nd2));
+          uint64_t v = mul2(pair(r[e], r[e + 1]), add2(pair(g[2 * k], g[2 * k + 1]), nd2));
           if (Half2<T>::KIND == 0) v = mul2(v, f2);
           float x, y;
           split(v, x, y);
@@ -330,21 +327,18 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       tmem_store_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full(u));
+      if (lane == 0) mbar_arrive(ds_full(wg));
     }
     if (nt > 0 && ok) ok = warp_wait(dq_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
     if (dq) {
-      // each warpgroup writes half of the columns
       uint16_t* dst = dq;
       if (valid) {
         const RowAt at = row_at(a, m, hk, row);
         dst = dq + (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
       }
       const float f = b.scale / dsf;
-#pragma unroll
-      for (int i = 0; i < DP / 64; ++i) {
-        const int col = wg * (DP / 2) + 32 * i;
+      for (int col = wg * 32; col < DP; col += 96) {        // 32 columns at a time, warpgroups in turn
         uint32_t r[32];
         if (nt > 0 && ok) {
           tmem_load32(lane_base + col, r);
@@ -362,7 +356,6 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 }
 
 // ------------------------------------------------------------------------------------------------ dk, dv
-constexpr int DKV_THREADS = 640;
 template <int DP> struct DkvSmem {
   static constexpr int BQ = 64;                            // query rows of a step
   static constexpr int STAGES = 4;
@@ -385,7 +378,8 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto q_empty = [&](int s) { return bars + 8u * (4 + s); };
   auto s_full = [&](int u) { return bars + 8u * (8 + u); };
   auto p_full = [&](int u) { return bars + 8u * (10 + u); };
-  const uint32_t kv_full = bars + 8u * 12, d_full = bars + 8u * 13, tmem_slot = bars + 8u * 14, scale_slot = tmem_slot + 4;
+  auto s_empty = [&](int u) { return bars + 8u * (12 + u); };
+  const uint32_t kv_full = bars + 8u * 14, d_full = bars + 8u * 15, tmem_slot = bars + 8u * 16, scale_slot = tmem_slot + 4;
 
   const int ktiles = (a.Tk + 127) / 128;
   const int unit = blockIdx.x / ktiles, m = unit / a.Hk, hk = unit % a.Hk;
@@ -396,7 +390,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) { mbar_init(q_full(s), 1); mbar_init(q_empty(s), 1); }
-    for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 1); mbar_init(p_full(u), 8); }
+    for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 2); mbar_init(p_full(u), 8); mbar_init(s_empty(u), 1); }
     mbar_init(kv_full, 1);
     mbar_init(d_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -406,7 +400,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  if (warp == 3) {
+  if (warp == 2) {
     const float f = ds_scale<T>(b, lane);
     if (lane == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale_slot), "f"(f) : "memory");
   }
@@ -455,43 +449,43 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     if (nq > 0) warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
     for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
       warp_wait(q_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- matrix products
-    constexpr uint32_t idesc_s = instr_desc<T>(BQ, false), idesc_o = instr_desc<T>(DP, true);
-    const uint64_t kd = make_desc(base, 16, 1024), vd = make_desc(base + S::KEYS, 16, 1024);
-    const uint64_t qd = make_desc(base + S::Q0, 16, 1024), qn = make_desc(base + S::Q0, BQ * 128, 1024);
-    auto scores = [&](int i) {                              // s^T = k q^T, dp^T = v do^T of step i
-      const uint64_t st = (uint64_t)(((i % S::STAGES) * 2 * S::ROWS) >> 4);
-      const uint32_t d = tmem + 256 + (i & 1) * 128;
+  } else if (warp == 1 || warp == 2) {
+    // ---------------------------------------------------------------- s^T = k q^T (warp 1), dp^T = v do^T (warp 2) of step i into set i & 1
+    const bool second = warp == 2;
+    constexpr uint32_t idesc_s = instr_desc<T>(BQ, false);
+    const uint64_t kd = make_desc(base + (second ? S::KEYS : 0), 16, 1024), qd = make_desc(base + S::Q0 + (second ? S::ROWS : 0), 16, 1024);
+    bool ok = nq > 0 && warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int i = 0; i < nq && ok; ++i) {
+      ok = warp_wait(s_empty(i & 1), ((uint32_t)(i >> 1) & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY) && warp_wait(q_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      const uint64_t st = (uint64_t)((s * 2 * S::ROWS) >> 4);
+      const uint32_t d = tmem + 256 + (i & 1) * 128 + (second ? 64 : 0);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           const uint64_t ko = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ro = (uint64_t)(((kk >> 2) * (BQ * 128) + (kk & 3) * 32) >> 4);
           umma_bf16(d, kd + ko, qd + st + ro, idesc_s, kk > 0);
         }
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t ko = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ro = (uint64_t)(((kk >> 2) * (BQ * 128) + (kk & 3) * 32) >> 4);
-          umma_bf16(d + 64, vd + ko, qd + st + (S::ROWS >> 4) + ro, idesc_s, kk > 0);
-        }
         umma_commit(s_full(i & 1));
       }
       __syncwarp();
-    };
-    bool ok = nq > 0 && warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
-    for (int i = 0; i < 2 && i < nq && ok; ++i) {
-      ok = warp_wait(q_full(i), 0, a.status, SB_TIMEOUT_SMEM_FULL);
-      if (!ok) break;
-      tc_fence_after();
-      scores(i);
+      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
     }
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- dv += p^T do, dk += ds^T q
+    constexpr uint32_t idesc_o = instr_desc<T>(DP, true);
+    const uint64_t qn = make_desc(base + S::Q0, BQ * 128, 1024);
+    bool ok = true;
+    int s = 0;
     for (int i = 0; i < nq && ok; ++i) {
-      const int s = i % S::STAGES, u = i & 1;
-      ok = warp_wait(p_full(u), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
+      ok = warp_wait(p_full(i & 1), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t p = tmem + 256 + u * 128;
+        const uint32_t p = tmem + 256 + (i & 1) * 128;
         const uint64_t st = (uint64_t)((s * 2 * S::ROWS) >> 4);
 #pragma unroll
         for (int kk = 0; kk < BQ / 16; ++kk)
@@ -499,18 +493,14 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
         for (int kk = 0; kk < BQ / 16; ++kk)
           umma_ts(tmem + 128, p + 64 + (kk >> 1) * 32 + (kk & 1) * 8, qn + st + (uint64_t)((kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
+        umma_commit(s_empty(i & 1));
         umma_commit(q_empty(s));
         if (i == nq - 1) umma_commit(d_full);
       }
       __syncwarp();
-      if (i + 2 < nq) {
-        ok = warp_wait(q_full((i + 2) % S::STAGES), (uint32_t)((i + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
-        if (!ok) break;
-        tc_fence_after();
-        scores(i + 2);
-      }
+      if (++s == S::STAGES) s = 0;
     }
-  } else if (warp >= 4) {
+  } else {
     // ---------------------------------------------------------------- p^T and ds^T; lanes are keys
     const int u = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1, quarter = warp & 3;
     const int key = key0 + quarter * 32 + lane;
@@ -609,7 +599,7 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   xattn_delta_kernel<T><<<b.peaks, 256, 0, stream>>>(a, b);
   rc = (int)cudaGetLastError();
   if (!rc && (dq || a.Tk <= DqSmem<DP>::BN)) {                // for up to 64 keys it also refines delta, whichever gradients are wanted
-    xattn_dq_kernel<T, DP><<<(unsigned)gq, BWD_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
+    xattn_dq_kernel<T, DP><<<(unsigned)gq, DQ_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
     rc = (int)cudaGetLastError();
   }
   if (!rc && dk) {

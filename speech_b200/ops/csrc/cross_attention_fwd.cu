@@ -59,8 +59,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
-      mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1);
-      mbar_init(v_full(s), 1); mbar_init(v_clean(s), 1); mbar_init(v_empty(s), 1);
+      mbar_init(k_full(s), 1); mbar_init(k_empty(s), tiles);
+      mbar_init(v_full(s), 1); mbar_init(v_clean(s), 1); mbar_init(v_empty(s), tiles);
     }
     for (int t = 0; t < 2; ++t) {
       for (int u = 0; u < 2; ++u) { mbar_init(s_full(t, u), 1); mbar_init(p_full(t, u), 4); }
@@ -112,20 +112,21 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       warp_wait(k_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
       if (ok || i + 1 < issued) warp_wait(v_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
     }
-  } else if (warp == 1) {
-    // ---------------------------------------------------------------- matrix products
+  } else if (warp == 1 || (warp == 3 && tiles == 2)) {
+    // ---------------------------------------------------------------- matrix products of one row tile
+    const int t = warp >> 1;
     constexpr uint32_t idesc_s = instr_desc<T>(BN, false), idesc_o = instr_desc<T>(DP, true);
-    const uint64_t qd = make_desc(base, 16, 1024), kd = make_desc(base + S::K0, 16, 1024), vd = make_desc(base + S::V0, BN * 128, 1024);
-    auto scores = [&](int t, int j) {                       // s = q k^T of block j into buffer j & 1
+    const uint64_t qd = make_desc(base + t * S::TILE, 16, 1024), kd = make_desc(base + S::K0, 16, 1024), vd = make_desc(base + S::V0, BN * 128, 1024);
+    auto scores = [&](int j) {                              // s = q k^T of block j into buffer j & 1
       const uint64_t st = (uint64_t)(((j % S::STAGES) * S::KEYS) >> 4);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t ro = (uint64_t)((t * S::TILE + (kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
+          const uint64_t ro = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
           umma_bf16(tmem + t * 128 + (j & 1) * 64, qd + ro, kd + st + ko, idesc_s, kk > 0);
         }
         umma_commit(s_full(t, j & 1));
-        if (t == tiles - 1) umma_commit(k_empty(j % S::STAGES));
+        umma_commit(k_empty(j % S::STAGES));
       }
       __syncwarp();
     };
@@ -134,31 +135,27 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       ok = warp_wait(k_full(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      for (int t = 0; t < tiles; ++t) scores(t, j);
+      scores(j);
     }
     for (int j = 0; j < nt && ok; ++j) {
       const int s = j % S::STAGES;
-      for (int t = 0; t < tiles && ok; ++t) {
-        ok = warp_wait(p_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
-        if (ok && t == 0) ok = warp_wait(v_clean(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+      ok = warp_wait(v_clean(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL) &&
+           warp_wait(p_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
+      if (!ok) break;
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          umma_ts(tmem + 256 + t * DP, tmem + t * 128 + (j & 1) * 64 + kk * 8, vd + (uint64_t)((s * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
+        umma_commit(v_empty(s));
+        umma_commit(j == nt - 1 ? o_full(t) : pv_done(t));
+      }
+      __syncwarp();
+      if (j + 2 < nt) {
+        ok = warp_wait(k_full((j + 2) % S::STAGES), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            umma_ts(tmem + 256 + t * DP, tmem + t * 128 + (j & 1) * 64 + kk * 8, vd + (uint64_t)((s * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
-          if (t == tiles - 1) umma_commit(v_empty(s));
-          umma_commit(j == nt - 1 ? o_full(t) : pv_done(t));
-        }
-        __syncwarp();
-        if (j + 2 < nt) {
-          if (t == 0) {
-            ok = warp_wait(k_full((j + 2) % S::STAGES), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
-            if (!ok) break;
-            tc_fence_after();
-          }
-          scores(t, j + 2);
-        }
+        scores(j + 2);
       }
     }
   } else if (warp == 2) {
@@ -171,7 +168,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         uint32_t w[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
-        clear_rows<DP>(base + S::V0 + s * S::KEYS, BN, w, 2, lane);
+        clear_rows<DP>(base + S::V0 + s * S::KEYS, BN, w, lane, 32);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
