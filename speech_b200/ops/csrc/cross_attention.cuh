@@ -210,43 +210,69 @@ __device__ __forceinline__ uint32_t tile_addr(uint32_t base, int rows, int row, 
   return base + (uint32_t)(chunk >> 3) * (uint32_t)(rows * 128) + (uint32_t)row * 128u + (uint32_t)(((chunk & 7) ^ (row & 7)) << 4);
 }
 
-// The four warps of a warpgroup copy packed rows [row0, row0 + 128) of a [B, Tq, H, D] tensor into a swizzled tile; rows beyond R
-// and columns beyond D become zero.
+// Element offset of this lane's packed row (row0 + lane) in a [B, Tq, H, D] tensor, -1 behind the last row.
+__device__ __forceinline__ long long row_offset(const XAttnArgs& a, long long sb, long long st, long long sh, int m, int hk, int row) {
+  if (row >= a.R) return -1;
+  const RowAt w = row_at(a, m, hk, row);
+  return w.b * sb + w.t * st + w.h * sh;
+}
+
+// A warp copies its 32 packed rows (offsets by lane, -1: zeros) into rows [quarter * 32, + 32) of a swizzled [128, DP] tile, columns
+// beyond D as zeros; whole rows per instruction.
 template <int DP>
-__device__ __forceinline__ void load_rows(const XAttnArgs& a, const void* src, long long sb, long long st, long long sh, int m, int hk, int row0,
-                                          uint32_t tile, int wg_warp, int lane) {
+__device__ __forceinline__ void load_rows(const void* src, long long off, int D, uint32_t tile, int quarter, int lane) {
   constexpr int CH = DP / 8, RPI = 32 / CH;               // 16-byte chunks of a row, rows per instruction
   const int sub = lane / CH, ch = lane % CH;
-#pragma unroll 4
+#pragma unroll 8
   for (int i = 0; i < 32; i += RPI) {
-    const int row = wg_warp * 32 + i + sub;
+    const long long o = __shfl_sync(0xffffffffu, off, i + sub);
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (row0 + row < a.R && ch * 8 < a.D) {
-      const RowAt w = row_at(a, m, hk, row0 + row);
-      v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(src) + w.b * sb + w.t * st + w.h * sh + ch * 8);
-    }
-    st_shared_v4(tile_addr(tile, 128, row, ch), v.x, v.y, v.z, v.w);
+    if (o >= 0 && ch * 8 < D) v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(src) + o + ch * 8);
+    st_shared_v4(tile_addr(tile, 128, quarter * 32 + i + sub, ch), v.x, v.y, v.z, v.w);
   }
 }
 
-// 32 columns of an output row, times f, and (rest != null) what the rounding to 16 bits took away, in 16 bits again: the backward
-// pass needs sum(do * o) to more than 16 bits, because it is subtracted from values of its own size.
+// This lane's row of such a tile into tensor memory as an A operand: DP / 2 columns of two 16-bit elements.
+template <int DP> __device__ __forceinline__ void row_to_tmem(uint32_t tile, int row, uint32_t taddr) {
+#pragma unroll
+  for (int h = 0; h < DP / 64; ++h) {
+    uint32_t r[32];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[4 * k]), "=r"(r[4 * k + 1]), "=r"(r[4 * k + 2]), "=r"(r[4 * k + 3])
+                   : "r"(tile_addr(tile, 128, row, 8 * h + k)) : "memory");
+    tmem_store32(taddr + 32 * h, r);
+  }
+}
+
+// What the rounding of a pair to 16 bits took away, in 16 bits again: the backward pass needs sum(do * o) to more than 16 bits, because
+// it is subtracted from values of its own size.
 template <typename T> __device__ __forceinline__ uint32_t out_pair(float x, float y, uint32_t& rest) {
   const uint32_t v = Half2<T>::pack(x, y);
   const float2 back = Half2<T>::unpack(v);
   rest = Half2<T>::pack(x - back.x, y - back.y);
   return v;
 }
-template <typename T> __device__ __forceinline__ void store_out32(uint16_t* out, uint16_t* rest, int col, int D, const uint32_t* r, float f) {
+
+// A warp writes 64 columns (128 bytes) of its 32 rows: lane l holds row l, packed; `off` is its row's element offset, -1 for none.  The
+// rows pass through 4 KB of shared memory so that an instruction writes four whole 128-byte lines; 16 bytes of 32 different rows per
+// instruction cost several times as much.  `buf`: this warp's, 128-byte aligned; columns [col, col + 64) below D are written.
+__device__ __forceinline__ void store_rows64(uint32_t buf, const uint32_t* packed, uint16_t* dst, long long off, int col, int D, int lane) {
 #pragma unroll
-  for (int k = 0; k < 32; k += 8)
-    if (col + k < D) {
-      uint32_t v[4], w[4];
+  for (int k = 0; k < 8; ++k)
+    st_shared_v4(buf + (uint32_t)lane * 128u + (uint32_t)((k ^ (lane & 7)) << 4), packed[4 * k], packed[4 * k + 1], packed[4 * k + 2], packed[4 * k + 3]);
+  __syncwarp();
+  const int sub = lane >> 3, ch = lane & 7;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = out_pair<T>(__uint_as_float(r[k + 2 * u]) * f, __uint_as_float(r[k + 2 * u + 1]) * f, w[u]);
-      *reinterpret_cast<uint4*>(out + col + k) = make_uint4(v[0], v[1], v[2], v[3]);
-      if (rest) *reinterpret_cast<uint4*>(rest + col + k) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
+  for (int i = 0; i < 32; i += 4) {
+    const int row = i + sub;
+    const long long o = __shfl_sync(0xffffffffu, off, row);
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(buf + (uint32_t)row * 128u + (uint32_t)((ch ^ (row & 7)) << 4)) : "memory");
+    if (o >= 0 && col + ch * 8 < D) *reinterpret_cast<uint4*>(dst + o + col + ch * 8) = v;
+  }
+  __syncwarp();
 }
 
 // Zeroes the rows of a [64, DP] tile whose keys are hidden (bits of words[0..1]): a hidden value of infinity or NaN would turn its zero

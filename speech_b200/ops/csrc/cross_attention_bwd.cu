@@ -9,8 +9,9 @@
 // The products into 64 columns have a warp each that issues them: such an instruction takes the tensor core 32 cycles, and issuing it
 // costs a warp twice that, so that one issuer for all of them left the tensor core idle more than half of the time.
 //
-// Both kernels have the roles of the forward pass otherwise.  dq: blocks of 64 keys go through three sets of tensor memory columns (scores and dp,
-// 64 each), with a warpgroup for each.  dk / dv: tiles of 64 query rows of one head
+// Both kernels have the roles of the forward pass otherwise.  dq: blocks of 64 keys go through two or three sets of tensor memory columns (scores
+// and dp, 64 each), with a warpgroup for each; q and do are A operands in tensor memory, because a product of 128 x 64 x 16 that reads
+// 6 KB from shared memory takes 60 cycles there, not 32.  dk / dv: tiles of 64 query rows of one head
 // take turns in two such sets, transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; four
 // warpgroups, two per set with half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which a row kernel
 // lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
@@ -23,7 +24,7 @@
 
 namespace {
 
-constexpr int DQ_THREADS = 512, DKV_THREADS = 640;     // 16 warps of 128 registers, 20 of 96
+constexpr int DKV_THREADS = 640;       // 20 warps of 96 registers
 constexpr int MAX_PARTS = 592;        // blocks of the row kernel, whose maxima every block of the other kernels joins
 
 template <typename T> constexpr float p_shift() { return Half2<T>::KIND == 0 ? 12.f : 0.f; }
@@ -102,17 +103,19 @@ template <typename T> __device__ __forceinline__ uint32_t pack_ds(float x, float
   return Half2<T>::pack(x, y);
 }
 
-template <typename T> __device__ __forceinline__ void store_row32(uint16_t* dst, int col, int D, const uint32_t* r, float f) {
+// 64 accumulator columns of a warp's 32 rows, times f, rounded and written.
+template <typename T>
+__device__ __forceinline__ void store_acc64(uint32_t buf, uint32_t taddr, bool have, float f, uint16_t* dst, long long off, int col, int D, int lane) {
+  uint32_t r[64], v[32];
+  if (have) {
+    tmem_load64(taddr, r);
+  } else {
 #pragma unroll
-  for (int k = 0; k < 32; k += 8)
-    if (col + k < D) {
-      uint4 v;
-      v.x = Half2<T>::pack(__uint_as_float(r[k]) * f, __uint_as_float(r[k + 1]) * f);
-      v.y = Half2<T>::pack(__uint_as_float(r[k + 2]) * f, __uint_as_float(r[k + 3]) * f);
-      v.z = Half2<T>::pack(__uint_as_float(r[k + 4]) * f, __uint_as_float(r[k + 5]) * f);
-      v.w = Half2<T>::pack(__uint_as_float(r[k + 6]) * f, __uint_as_float(r[k + 7]) * f);
-      *reinterpret_cast<uint4*>(dst + col + k) = v;
-    }
+    for (int k = 0; k < 64; ++k) r[k] = 0u;
+  }
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v[k] = Half2<T>::pack(__uint_as_float(r[2 * k]) * f, __uint_as_float(r[2 * k + 1]) * f);
+  store_rows64(buf, v, dst, off, col, D, lane);
 }
 
 // ------------------------------------------------------------------------------------------------ dq
@@ -122,10 +125,13 @@ template <int DP> struct DqSmem {
   static constexpr int ROWS = 128 * DP * 2, KEYS = BN * DP * 2;
   static constexpr int DO0 = ROWS, KV0 = 2 * ROWS, BAR = KV0 + STAGES * 2 * KEYS;
   static constexpr int BYTES = BAR + 256 + 1024;
+  // tensor memory: dq, q, do, then sets of 64 columns of scores and 64 of dp, one warpgroup for each
+  static constexpr int Q_COL = DP, DO_COL = DP + DP / 2, SET_COL = 2 * DP, SETS = (512 - SET_COL) / 128;
+  static constexpr int THREADS = 128 + SETS * 128;
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(DQ_THREADS, 1)
+__global__ void __launch_bounds__(DqSmem<DP>::THREADS, 1)
 xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq) {
   using S = DqSmem<DP>;
   constexpr int BN = S::BN, HALVES = DP / 64;
@@ -149,9 +155,9 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
-    for (int u = 0; u < 3; ++u) { mbar_init(s_full(u), 2); mbar_init(ds_full(u), 4); mbar_init(s_empty(u), 1); }
+    for (int u = 0; u < S::SETS; ++u) { mbar_init(s_full(u), 2); mbar_init(ds_full(u), 4); mbar_init(s_empty(u), 1); }
     mbar_init(dq_full, 1);
-    mbar_init(rows_ready, 12);
+    mbar_init(rows_ready, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -190,10 +196,11 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
       warp_wait(kv_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
   } else if (warp == 1 || warp == 3) {
-    // s = q k^T (warp 1) and dp = do v^T (warp 3) of block j into buffer j % 3
+    // s = q k^T (warp 1) and dp = do v^T (warp 3) of block j into set j % SETS
     const bool second = warp == 3;
     constexpr uint32_t idesc_s = instr_desc<T>(BN, false);
-    const uint64_t rd = make_desc(base + (second ? S::DO0 : 0), 16, 1024), kd = make_desc(base + S::KV0 + (second ? S::KEYS : 0), 16, 1024);
+    const uint32_t rows = tmem + (second ? S::DO_COL : S::Q_COL);
+    const uint64_t kd = make_desc(base + S::KV0 + (second ? S::KEYS : 0), 16, 1024);
     bool ok = nt > 0 && warp_wait(rows_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
     int s = 0, u = 0;
     uint32_t ph = 0, uph = 1;
@@ -202,18 +209,16 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (!ok) break;
       tc_fence_after();
       const uint64_t st = (uint64_t)((s * 2 * S::KEYS) >> 4);
-      const uint32_t d = tmem + 128 + u * 128 + (second ? 64 : 0);
+      const uint32_t d = tmem + S::SET_COL + u * 128 + (second ? 64 : 0);
       if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint64_t ro = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
-          umma_bf16(d, rd + ro, kd + st + ko, idesc_s, kk > 0);
-        }
+        for (int kk = 0; kk < DP / 16; ++kk)
+          umma_ts(d, rows + kk * 8, kd + st + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
         umma_commit(s_full(u));
       }
       __syncwarp();
       if (++s == S::STAGES) { s = 0; ph ^= 1u; }
-      if (++u == 3) { u = 0; uph ^= 1u; }
+      if (++u == S::SETS) { u = 0; uph ^= 1u; }
     }
   } else if (warp == 2) {
     // dq += ds k
@@ -229,17 +234,17 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          umma_ts(tmem, tmem + 128 + u * 128 + kk * 8, kn + (uint64_t)((s * 2 * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
+          umma_ts(tmem, tmem + S::SET_COL + u * 128 + kk * 8, kn + (uint64_t)((s * 2 * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
         umma_commit(s_empty(u));
         umma_commit(kv_empty(s));
         if (j == nt - 1) umma_commit(dq_full);
       }
       __syncwarp();
       if (++s == S::STAGES) s = 0;
-      if (++u == 3) { u = 0; uph ^= 1u; }
+      if (++u == S::SETS) { u = 0; uph ^= 1u; }
     }
   } else {
-    // three warpgroups take key blocks, and the three sets of columns with them, in turn
+    // the warpgroups take key blocks, and the sets of columns with them, in turn
     const int wg = (warp - 4) >> 2, quarter = warp & 3;
     const int row = row0 + quarter * 32 + lane;
     const bool valid = row < a.R;
@@ -251,17 +256,23 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     bool ok = true;
     if (nt > 0) {
-      const long long st = (long long)a.H * a.D;
-      if (wg == 0) load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, row0, base, quarter, lane);
-      if (wg == 1) load_rows<DP>(a, b.dout, st * a.Tq, st, a.D, m, hk, row0, base + S::DO0, quarter, lane);
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (wg < 2) {                                        // q by the first, do by the second, through shared memory into tensor memory
+        const uint32_t tile = base + wg * S::DO0;
+        const long long st = (long long)a.H * a.D;
+        const long long off = wg ? row_offset(a, st * a.Tq, st, a.D, m, hk, row) : row_offset(a, a.q_sb, a.q_st, a.q_sh, m, hk, row);
+        load_rows<DP>(wg ? (const void*)b.dout : a.q, off, a.D, tile, quarter, lane);
+        __syncwarp();
+        row_to_tmem<DP>(tile, quarter * 32 + lane, lane_base + (wg ? S::DO_COL : S::Q_COL));
+        tmem_store_wait();
+        tc_fence_before();
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(rows_ready);
+      if (wg < 2 && lane == 0) mbar_arrive(rows_ready);
     }
     const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse), f2 = pair(dsf, dsf);
-    const uint32_t s_addr = lane_base + 128 + wg * 128;
+    const uint32_t s_addr = lane_base + S::SET_COL + wg * 128;
     uint32_t ph = 0;
-    for (int j = wg; j < nt; j += 3) {
+    for (int j = wg; j < nt; j += S::SETS) {
       const bool some_hidden = hide || (j + 1) * BN > len;
       uint32_t w[2] = {0, 0};
       if (some_hidden) {
@@ -332,21 +343,9 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     if (nt > 0 && ok) ok = warp_wait(dq_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
     if (dq) {
-      uint16_t* dst = dq;
-      if (valid) {
-        const RowAt at = row_at(a, m, hk, row);
-        dst = dq + (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
-      }
-      const float f = b.scale / dsf;
-      for (int col = wg * 32; col < DP; col += 96) {        // 32 columns at a time, warpgroups in turn
-        uint32_t r[32];
-        if (nt > 0 && ok) {
-          tmem_load32(lane_base + col, r);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) r[k] = 0u;
-        }
-        if (valid) store_row32<T>(dst, col, a.D, r, f);
+      if (wg < DP / 64) {                                  // 64 columns a warpgroup
+        const long long off = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
+        store_acc64<T>(base + (wg * 4 + quarter) * 4096, lane_base + 64 * wg, nt > 0 && ok, b.scale / dsf, dq, off, 64 * wg, a.D, lane);
       }
     }
   }
@@ -559,20 +558,11 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (nq > 0 && ok) ok = warp_wait(d_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
-    // two warpgroups write dv, the others dk, half of the columns each
-    uint16_t* dst = (u ? dk : dv) + (((long long)m * a.Tk + key) * a.Hk + hk) * a.D;
-    const float f = u ? b.scale / dsf : ex2(-p_shift<T>());
-#pragma unroll
-    for (int i = 0; i < DP / 64; ++i) {
-      const int col = half * (DP / 2) + 32 * i;
-      uint32_t r[32];
-      if (nq > 0 && ok) {
-        tmem_load32(lane_base + u * 128 + col, r);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 32; ++k) r[k] = 0u;
-      }
-      if (key < a.Tk) store_row32<T>(dst, col, a.D, r, f);
+    // dv by two warpgroups, dk by the others, 64 columns each (DP = 64: one of the two)
+    if (half < DP / 64) {
+      const long long off = key < a.Tk ? (((long long)m * a.Tk + key) * a.Hk + hk) * a.D : -1;
+      store_acc64<T>(base + ((u * 2 + half) * 4 + quarter) * 4096, lane_base + u * 128 + half * 64, nq > 0 && ok, u ? b.scale / dsf : ex2(-p_shift<T>()),
+                     u ? dk : dv, off, half * 64, a.D, lane);
     }
   }
   tc_fence_before();
@@ -599,7 +589,7 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   xattn_delta_kernel<T><<<b.peaks, 256, 0, stream>>>(a, b);
   rc = (int)cudaGetLastError();
   if (!rc && (dq || a.Tk <= DqSmem<DP>::BN)) {                // for up to 64 keys it also refines delta, whichever gradients are wanted
-    xattn_dq_kernel<T, DP><<<(unsigned)gq, DQ_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
+    xattn_dq_kernel<T, DP><<<(unsigned)gq, DqSmem<DP>::THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
     rc = (int)cudaGetLastError();
   }
   if (!rc && dk) {

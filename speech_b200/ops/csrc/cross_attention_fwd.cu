@@ -184,7 +184,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t o_addr = lane_base + 256 + t * DP;
     if (nt > 0) {
-      load_rows<DP>(a, a.q, a.q_sb, a.q_st, a.q_sh, m, hk, tile_row, base + t * S::TILE, quarter, lane);
+      load_rows<DP>(a.q, row_offset(a, a.q_sb, a.q_st, a.q_sh, m, hk, row), a.D, base + t * S::TILE, quarter, lane);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
@@ -268,24 +268,23 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (nt > 0 && ok) ok = warp_wait(o_full(t), 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
-    const bool valid = row < a.R;
-    long long at_row = 0;
-    if (valid) {
-      const RowAt at = row_at(a, m, hk, row);
-      at_row = (((long long)at.b * a.Tq + at.t) * a.H + at.h) * a.D;
-      if (lse) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
-    }
+    const long long at_row = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
+    if (lse && row < a.R) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
     const float inv = l == 0.f ? 0.f : 1.f / l;
+    const uint32_t buf = base + t * S::TILE + quarter * 4096;      // the tile's queries have been read
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-      uint32_t r[32];
+    for (int i = 0; i < DP / 64; ++i) {
+      uint32_t r[64], v[32], w[32];
       if (nt > 0 && ok) {
-        tmem_load32(o_addr + 32 * i, r);
+        tmem_load64(o_addr + 64 * i, r);
       } else {
 #pragma unroll
-        for (int k = 0; k < 32; ++k) r[k] = 0u;
+        for (int k = 0; k < 64; ++k) r[k] = 0u;
       }
-      if (valid) store_out32<T>(out + at_row, rest ? rest + at_row : nullptr, 32 * i, a.D, r, inv);
+#pragma unroll
+      for (int k = 0; k < 32; ++k) v[k] = out_pair<T>(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv, w[k]);
+      store_rows64(buf, v, out, at_row, 64 * i, a.D, lane);
+      if (rest) store_rows64(buf, w, rest, at_row, 64 * i, a.D, lane);
     }
   }
   tc_fence_before();
