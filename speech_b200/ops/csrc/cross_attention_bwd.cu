@@ -9,9 +9,9 @@
 // The products into 64 columns have a warp each that issues them: such an instruction takes the tensor core 32 cycles, and issuing it
 // costs a warp twice that, so that one issuer for all of them left the tensor core idle more than half of the time.
 //
-// Both kernels have the roles of the forward pass otherwise.  dq: blocks of 64 keys go through two or three sets of tensor memory columns (scores
-// and dp, 64 each), with a warpgroup for each; q and do are A operands in tensor memory, because a product of 128 x 64 x 16 that reads
-// 6 KB from shared memory takes 60 cycles there, not 32.  dk / dv: tiles of 64 query rows of one head
+// Both kernels have the roles of the forward pass otherwise.  dq: two warpgroups take blocks of 64 keys in turn; scores and dp leave tensor memory
+// for registers at once, so that those of the next block are computed under this one's exponentials; q and do are A operands in tensor
+// memory, because a product of 128 x 64 x 16 that reads 6 KB from shared memory takes 60 cycles, not 32.  dk / dv: tiles of 64 query rows of one head
 // take turns in two such sets, transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; four
 // warpgroups, two per set with half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which a row kernel
 // lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
@@ -125,13 +125,13 @@ template <int DP> struct DqSmem {
   static constexpr int ROWS = 128 * DP * 2, KEYS = BN * DP * 2;
   static constexpr int DO0 = ROWS, KV0 = 2 * ROWS, BAR = KV0 + STAGES * 2 * KEYS;
   static constexpr int BYTES = BAR + 256 + 1024;
-  // tensor memory: dq, q, do, then sets of 64 columns of scores and 64 of dp, one warpgroup for each
-  static constexpr int Q_COL = DP, DO_COL = DP + DP / 2, SET_COL = 2 * DP, SETS = (512 - SET_COL) / 128;
-  static constexpr int THREADS = 128 + SETS * 128;
+  // tensor memory: dq, q, do, scores of even and odd blocks, dp, ds of even and odd blocks
+  static constexpr int Q_COL = DP, DO_COL = DP + DP / 2, S_COL = 2 * DP, DP_COL = S_COL + 128, DS_COL = DP_COL + 64;
 };
+constexpr int DQ_THREADS = 384;
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(DqSmem<DP>::THREADS, 1)
+__global__ void __launch_bounds__(DQ_THREADS, 1)
 xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq) {
   using S = DqSmem<DP>;
   constexpr int BN = S::BN, HALVES = DP / 64;
@@ -140,11 +140,13 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const uint32_t bars = base + S::BAR;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto kv_full = [&](int s) { return bars + 8u * s; };
-  auto kv_empty = [&](int s) { return bars + 8u * (10 + s); };
-  auto s_full = [&](int u) { return bars + 8u * (15 + u); };
-  auto ds_full = [&](int u) { return bars + 8u * (18 + u); };
-  auto s_empty = [&](int u) { return bars + 8u * (21 + u); };
-  const uint32_t dq_full = bars + 8u * 24, rows_ready = bars + 8u * 25, tmem_slot = bars + 8u * 26, scale_slot = tmem_slot + 4;
+  auto kv_empty = [&](int s) { return bars + 8u * (5 + s); };
+  auto s_full = [&](int u) { return bars + 8u * (10 + u); };
+  auto s_read = [&](int u) { return bars + 8u * (12 + u); };
+  auto ds_full = [&](int u) { return bars + 8u * (14 + u); };
+  auto ds_read = [&](int u) { return bars + 8u * (16 + u); };
+  auto dp_full = [&](int u) { return bars + 8u * (18 + u); };     // one per warpgroup: each sees every other block only
+  const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, scale_slot = tmem_slot + 4;
 
   const int tiles = (a.R + 127) / 128;
   const int unit = blockIdx.x / tiles, m = unit / a.Hk, hk = unit % a.Hk;
@@ -155,7 +157,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
-    for (int u = 0; u < S::SETS; ++u) { mbar_init(s_full(u), 2); mbar_init(ds_full(u), 4); mbar_init(s_empty(u), 1); }
+    for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 1); mbar_init(s_read(u), 4); mbar_init(ds_full(u), 4); mbar_init(ds_read(u), 1); mbar_init(dp_full(u), 1); }
+    mbar_init(dp_read, 4);
     mbar_init(dq_full, 1);
     mbar_init(rows_ready, 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -196,55 +199,55 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
       warp_wait(kv_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
   } else if (warp == 1 || warp == 3) {
-    // s = q k^T (warp 1) and dp = do v^T (warp 3) of block j into set j % SETS
+    // s = q k^T (warp 1) into the columns of block j & 1, dp = do v^T (warp 3) into its only ones: each as soon as the columns have been
+    // read, which happens right before a warpgroup starts on them
     const bool second = warp == 3;
     constexpr uint32_t idesc_s = instr_desc<T>(BN, false);
     const uint32_t rows = tmem + (second ? S::DO_COL : S::Q_COL);
     const uint64_t kd = make_desc(base + S::KV0 + (second ? S::KEYS : 0), 16, 1024);
     bool ok = nt > 0 && warp_wait(rows_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
-    int s = 0, u = 0;
-    uint32_t ph = 0, uph = 1;
+    int s = 0;
+    uint32_t ph = 0;
     for (int j = 0; j < nt && ok; ++j) {
-      ok = warp_wait(s_empty(u), uph, a.status, SB_TIMEOUT_TMEM_EMPTY) && warp_wait(kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL);
+      ok = warp_wait(kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL) &&
+           (second ? warp_wait(dp_read, ((uint32_t)j & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY)
+                   : warp_wait(s_read(j & 1), ((uint32_t)(j >> 1) & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY));
       if (!ok) break;
       tc_fence_after();
       const uint64_t st = (uint64_t)((s * 2 * S::KEYS) >> 4);
-      const uint32_t d = tmem + S::SET_COL + u * 128 + (second ? 64 : 0);
+      const uint32_t d = tmem + (second ? S::DP_COL : S::S_COL + (j & 1) * 64);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
           umma_ts(d, rows + kk * 8, kd + st + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
-        umma_commit(s_full(u));
+        umma_commit(second ? dp_full(j & 1) : s_full(j & 1));
       }
       __syncwarp();
       if (++s == S::STAGES) { s = 0; ph ^= 1u; }
-      if (++u == S::SETS) { u = 0; uph ^= 1u; }
     }
   } else if (warp == 2) {
     // dq += ds k
     constexpr uint32_t idesc_o = instr_desc<T>(DP, true);
     const uint64_t kn = make_desc(base + S::KV0, BN * 128, 1024);
     bool ok = true;
-    int s = 0, u = 0;
-    uint32_t uph = 0;
+    int s = 0;
     for (int j = 0; j < nt && ok; ++j) {
-      ok = warp_wait(ds_full(u), uph, a.status, SB_TIMEOUT_TMEM_EMPTY);
+      ok = warp_wait(ds_full(j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          umma_ts(tmem, tmem + S::SET_COL + u * 128 + kk * 8, kn + (uint64_t)((s * 2 * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
-        umma_commit(s_empty(u));
+          umma_ts(tmem, tmem + S::DS_COL + (j & 1) * 32 + kk * 8, kn + (uint64_t)((s * 2 * S::KEYS + kk * 2048) >> 4), idesc_o, (j > 0) | (kk > 0));
+        umma_commit(ds_read(j & 1));
         umma_commit(kv_empty(s));
         if (j == nt - 1) umma_commit(dq_full);
       }
       __syncwarp();
       if (++s == S::STAGES) s = 0;
-      if (++u == S::SETS) { u = 0; uph ^= 1u; }
     }
   } else {
-    // the warpgroups take key blocks, and the sets of columns with them, in turn
+    // two warpgroups take even and odd key blocks
     const int wg = (warp - 4) >> 2, quarter = warp & 3;
     const int row = row0 + quarter * 32 + lane;
     const bool valid = row < a.R;
@@ -254,37 +257,52 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const float nlse = valid ? b.nlse[stat] : -INFINITY;
     float ndelta = valid ? b.ndelta[stat] : 0.f;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_addr = lane_base + S::S_COL + wg * 64, dp_addr = lane_base + S::DP_COL, ds_addr = lane_base + S::DS_COL + wg * 32;
     bool ok = true;
     if (nt > 0) {
-      if (wg < 2) {                                        // q by the first, do by the second, through shared memory into tensor memory
-        const uint32_t tile = base + wg * S::DO0;
-        const long long st = (long long)a.H * a.D;
-        const long long off = wg ? row_offset(a, st * a.Tq, st, a.D, m, hk, row) : row_offset(a, a.q_sb, a.q_st, a.q_sh, m, hk, row);
-        load_rows<DP>(wg ? (const void*)b.dout : a.q, off, a.D, tile, quarter, lane);
-        __syncwarp();
-        row_to_tmem<DP>(tile, quarter * 32 + lane, lane_base + (wg ? S::DO_COL : S::Q_COL));
-        tmem_store_wait();
-        tc_fence_before();
-      }
+      // q by the first, do by the second, through shared memory into tensor memory
+      const uint32_t tile = base + wg * S::DO0;
+      const long long st = (long long)a.H * a.D;
+      const long long off = wg ? row_offset(a, st * a.Tq, st, a.D, m, hk, row) : row_offset(a, a.q_sb, a.q_st, a.q_sh, m, hk, row);
+      load_rows<DP>(wg ? (const void*)b.dout : a.q, off, a.D, tile, quarter, lane);
       __syncwarp();
-      if (wg < 2 && lane == 0) mbar_arrive(rows_ready);
+      row_to_tmem<DP>(tile, quarter * 32 + lane, lane_base + (wg ? S::DO_COL : S::Q_COL));
+      tmem_store_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(rows_ready);
     }
     const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse), f2 = pair(dsf, dsf);
-    const uint32_t s_addr = lane_base + S::SET_COL + wg * 128;
     uint32_t ph = 0;
-    for (int j = wg; j < nt; j += S::SETS) {
+    for (int j = wg; j < nt; j += 2) {
       const bool some_hidden = hide || (j + 1) * BN > len;
       uint32_t w[2] = {0, 0};
       if (some_hidden) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
       }
+      uint32_t r[64], g[64];
       ok = warp_wait(s_full(wg), ph, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
-      ph ^= 1u;
       tc_fence_after();
-      uint32_t r[64];
       tmem_load64(s_addr, r);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read(wg));
+      ok = warp_wait(dp_full(wg), ph, a.status, SB_TIMEOUT_TMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      tmem_load64(dp_addr, g);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dp_read);
+      // Waited for here and not where ds is stored: the branches keep the arithmetic below from being scheduled before the arrivals above,
+      // which nothing in this warp depends on but the next products do (1480 -> 1200 cycles a block).
+      if (j >= 2) {
+        ok = warp_wait(ds_read(wg), ph ^ 1u, a.status, SB_TIMEOUT_TMEM_FULL);
+        if (!ok) break;
+        tc_fence_after();
+      }
 #pragma unroll
       for (int k = 0; k < 64; k += 2) {                    // p over s
         float x, y;
@@ -295,58 +313,47 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (some_hidden) {
 #pragma unroll
         for (int k = 0; k < 64; ++k)
-          if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = 0u;
+          if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = g[k] = 0u;
         // hidden key rows are cleared before dq sums over them: their ds is zero, and zero times NaN is not
         clear_rows<DP>(base + S::KV0 + (j % S::STAGES) * 2 * S::KEYS, BN, w, quarter * 32 + lane, 128);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       if (nt == 1) {
         // all keys are in this block: delta = sum p dp from the values that it is subtracted from, instead of the rounded output
-        float d = 0.f;
+        uint64_t d2[2] = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t g[32];
-          tmem_load32(s_addr + 64 + 32 * i, g);
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if (!((w[i] >> k) & 1u)) d = fmaf(__uint_as_float(r[32 * i + k]), __uint_as_float(g[k]), d);
-        }
-        ndelta = -d;
+        for (int k = 0; k < 64; k += 2) d2[(k >> 1) & 1] = fma2(pair(r[k], r[k + 1]), pair(g[k], g[k + 1]), d2[(k >> 1) & 1]);
+        float x, y;
+        split(add2(d2[0], d2[1]), x, y);
+        ndelta = -(x + y);
         if (valid) b.ndelta[stat] = ndelta;
       }
       const uint64_t nd2 = pair(ndelta, ndelta);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        uint32_t g[32], o[16];
-        tmem_load32(s_addr + 64 + 32 * i, g);
-        if (some_hidden) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k)
-            if ((w[i] >> k) & 1u) g[k] = 0u;
-        }
+        uint32_t o[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           const int e = 32 * i + 2 * k;
-          uint64_t v = mul2(pair(r[e], r[e + 1]), add2(pair(g[2 * k], g[2 * k + 1]), nd2));
+          uint64_t v = mul2(pair(r[e], r[e + 1]), add2(pair(g[e], g[e + 1]), nd2));
           if (Half2<T>::KIND == 0) v = mul2(v, f2);
           float x, y;
           split(v, x, y);
           o[k] = pack_ds<T>(x, y);
         }
-        tmem_store16(s_addr + 16 * i, o);
+        tmem_store16(ds_addr + 16 * i, o);
       }
       tmem_store_wait();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full(wg));
+      ph ^= 1u;
     }
     if (nt > 0 && ok) ok = warp_wait(dq_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
-    if (dq) {
-      if (wg < DP / 64) {                                  // 64 columns a warpgroup
-        const long long off = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
-        store_acc64<T>(base + (wg * 4 + quarter) * 4096, lane_base + 64 * wg, nt > 0 && ok, b.scale / dsf, dq, off, 64 * wg, a.D, lane);
-      }
+    if (dq && wg < DP / 64) {                              // 64 columns a warpgroup
+      const long long off = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
+      store_acc64<T>(base + (wg * 4 + quarter) * 4096, lane_base + 64 * wg, nt > 0 && ok, b.scale / dsf, dq, off, 64 * wg, a.D, lane);
     }
   }
   tc_fence_before();
@@ -589,7 +596,7 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   xattn_delta_kernel<T><<<b.peaks, 256, 0, stream>>>(a, b);
   rc = (int)cudaGetLastError();
   if (!rc && (dq || a.Tk <= DqSmem<DP>::BN)) {                // for up to 64 keys it also refines delta, whichever gradients are wanted
-    xattn_dq_kernel<T, DP><<<(unsigned)gq, DqSmem<DP>::THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
+    xattn_dq_kernel<T, DP><<<(unsigned)gq, DQ_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
     rc = (int)cudaGetLastError();
   }
   if (!rc && dk) {

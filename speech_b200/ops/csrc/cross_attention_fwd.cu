@@ -248,9 +248,14 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           float x, y;
-          split(fma2(pair(r[32 * i + 2 * k], r[32 * i + 2 * k + 1]), c2, shift2), x, y);
-          x = ex2(x);
-          y = ex2(y);
+          const uint64_t e = fma2(pair(r[32 * i + 2 * k], r[32 * i + 2 * k + 1]), c2, shift2);
+          if (k % 8 >= 5) {                                 // three pairs of eight: see the head of this file
+            ex2_poly(e, x, y);
+          } else {
+            split(e, x, y);
+            x = ex2(x);
+            y = ex2(y);
+          }
           sum[k & 1] = add2(sum[k & 1], pair(x, y));
           p[k] = Half2<T>::pack(x, y);
         }
