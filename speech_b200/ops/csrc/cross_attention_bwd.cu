@@ -11,9 +11,9 @@
 //
 // Both kernels have the roles of the forward pass otherwise.  dq: two warpgroups take blocks of 64 keys in turn; scores and dp leave tensor memory
 // for registers at once, so that those of the next block are computed under this one's exponentials; q and do are A operands in tensor
-// memory, because a product of 128 x 64 x 16 that reads 6 KB from shared memory takes 60 cycles, not 32.  dk / dv: tiles of 64 query rows of one head
-// take turns in two such sets, transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; four
-// warpgroups, two per set with half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which a row kernel
+// memory, because a product of 128 x 64 x 16 that reads 6 KB from shared memory takes 60 cycles, not 32.  dk / dv: tiles of 64 query rows of one head,
+// transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; two pairs of warpgroups take them in
+// turn, half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which a row kernel
 // lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
 //
 // Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
@@ -368,6 +368,10 @@ template <int DP> struct DkvSmem {
   static constexpr int KEYS = 128 * DP * 2, ROWS = BQ * DP * 2, STAT = 2 * BQ * 4;
   static constexpr int Q0 = 2 * KEYS, STAT0 = Q0 + STAGES * 2 * ROWS, BAR = STAT0 + STAGES * STAT;
   static constexpr int BYTES = BAR + 256 + 1024;
+  // tensor memory: dv, dk, k (and v for DP = 64, where there is room) as A operands, scores, dp, p and ds
+  static constexpr bool V_TMEM = DP == 64;
+  static constexpr int DK_COL = DP, K_COL = 2 * DP, V_COL = K_COL + DP / 2, S_COL = V_COL + (V_TMEM ? DP / 2 : 0), DP_COL = S_COL + 64, P_COL = DP_COL + 64,
+                       DS_COL = P_COL + 32;
 };
 
 template <typename T, int DP>
@@ -382,10 +386,12 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto q_full = [&](int s) { return bars + 8u * s; };
   auto q_empty = [&](int s) { return bars + 8u * (4 + s); };
-  auto s_full = [&](int u) { return bars + 8u * (8 + u); };
-  auto p_full = [&](int u) { return bars + 8u * (10 + u); };
-  auto s_empty = [&](int u) { return bars + 8u * (12 + u); };
-  const uint32_t kv_full = bars + 8u * 14, d_full = bars + 8u * 15, tmem_slot = bars + 8u * 16, scale_slot = tmem_slot + 4;
+  auto s_full = [&](int u) { return bars + 8u * (8 + u); };           // one per pair of warpgroups: each sees every other step only
+  auto dp_full = [&](int u) { return bars + 8u * (10 + u); };
+  auto p_full = [&](int u) { return bars + 8u * (12 + u); };
+  auto p_read = [&](int u) { return bars + 8u * (14 + u); };
+  const uint32_t s_read = bars + 8u * 16, dp_read = bars + 8u * 17, kv_full = bars + 8u * 18, kv_tmem = bars + 8u * 19, d_full = bars + 8u * 20,
+                 tmem_slot = bars + 8u * 21, scale_slot = tmem_slot + 4;
 
   const int ktiles = (a.Tk + 127) / 128;
   const int unit = blockIdx.x / ktiles, m = unit / a.Hk, hk = unit % a.Hk;
@@ -396,8 +402,11 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) { mbar_init(q_full(s), 1); mbar_init(q_empty(s), 1); }
-    for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 2); mbar_init(p_full(u), 8); mbar_init(s_empty(u), 1); }
+    for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 1); mbar_init(dp_full(u), 1); mbar_init(p_full(u), 8); mbar_init(p_read(u), 1); }
+    mbar_init(s_read, 8);
+    mbar_init(dp_read, 8);
     mbar_init(kv_full, 1);
+    mbar_init(kv_tmem, S::V_TMEM ? 8 : 4);
     mbar_init(d_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -456,26 +465,29 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
       warp_wait(q_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
   } else if (warp == 1 || warp == 2) {
-    // ---------------------------------------------------------------- s^T = k q^T (warp 1), dp^T = v do^T (warp 2) of step i into set i & 1
+    // ---------------------------------------------------------------- s^T = k q^T (warp 1), dp^T = v do^T (warp 2) of every step, each as soon
+    // as its columns have been read
     const bool second = warp == 2;
     constexpr uint32_t idesc_s = instr_desc<T>(BQ, false);
-    const uint64_t kd = make_desc(base + (second ? S::KEYS : 0), 16, 1024), qd = make_desc(base + S::Q0 + (second ? S::ROWS : 0), 16, 1024);
-    bool ok = nq > 0 && warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+    const uint64_t vd = make_desc(base + S::KEYS, 16, 1024), qd = make_desc(base + S::Q0 + (second ? S::ROWS : 0), 16, 1024);
+    const uint32_t d = tmem + (second ? S::DP_COL : S::S_COL), keys = tmem + (second ? S::V_COL : S::K_COL);
+    bool ok = nq > 0 && warp_wait(second && !S::V_TMEM ? kv_full : kv_tmem, 0, a.status, SB_TIMEOUT_SMEM_FULL);
     int s = 0;
     uint32_t ph = 0;
     for (int i = 0; i < nq && ok; ++i) {
-      ok = warp_wait(s_empty(i & 1), ((uint32_t)(i >> 1) & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY) && warp_wait(q_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL);
+      ok = warp_wait(q_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL) &&
+           warp_wait(second ? dp_read : s_read, ((uint32_t)i & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
       tc_fence_after();
       const uint64_t st = (uint64_t)((s * 2 * S::ROWS) >> 4);
-      const uint32_t d = tmem + 256 + (i & 1) * 128 + (second ? 64 : 0);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk) {
           const uint64_t ko = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ro = (uint64_t)(((kk >> 2) * (BQ * 128) + (kk & 3) * 32) >> 4);
-          umma_bf16(d, kd + ko, qd + st + ro, idesc_s, kk > 0);
+          if (second && !S::V_TMEM) umma_bf16(d, vd + ko, qd + st + ro, idesc_s, kk > 0);
+          else umma_ts(d, keys + kk * 8, qd + st + ro, idesc_s, kk > 0);
         }
-        umma_commit(s_full(i & 1));
+        umma_commit(second ? dp_full(i & 1) : s_full(i & 1));
       }
       __syncwarp();
       if (++s == S::STAGES) { s = 0; ph ^= 1u; }
@@ -491,15 +503,14 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t p = tmem + 256 + (i & 1) * 128;
         const uint64_t st = (uint64_t)((s * 2 * S::ROWS) >> 4);
 #pragma unroll
         for (int kk = 0; kk < BQ / 16; ++kk)
-          umma_ts(tmem, p + (kk >> 1) * 32 + (kk & 1) * 8, qn + st + (uint64_t)((S::ROWS + kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
+          umma_ts(tmem, tmem + S::P_COL + kk * 8, qn + st + (uint64_t)((S::ROWS + kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
 #pragma unroll
         for (int kk = 0; kk < BQ / 16; ++kk)
-          umma_ts(tmem + 128, p + 64 + (kk >> 1) * 32 + (kk & 1) * 8, qn + st + (uint64_t)((kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
-        umma_commit(s_empty(i & 1));
+          umma_ts(tmem + S::DK_COL, tmem + S::DS_COL + kk * 8, qn + st + (uint64_t)((kk * 2048) >> 4), idesc_o, (i > 0) | (kk > 0));
+        umma_commit(p_read(i & 1));
         umma_commit(q_empty(s));
         if (i == nq - 1) umma_commit(d_full);
       }
@@ -518,19 +529,36 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const float k_ds = dsf * ex2(-p_shift<T>());
     const uint64_t c2 = pair(a.c, a.c), shift2 = pair(p_shift<T>(), p_shift<T>()), f2 = pair(k_ds, k_ds);
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-    const uint32_t s_addr = lane_base + 256 + u * 128 + half * 32;
-    for (int i = u; i < nq; i += 2) {
-      ok = warp_wait(s_full(u), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
-      if (!ok) break;
+    if (nq > 0 && u == 0 && (half == 0 || S::V_TMEM)) {      // keys (and values) into tensor memory, by the first warpgroups
+      ok = warp_wait(kv_full, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+      row_to_tmem<DP>(base + half * S::KEYS, quarter * 32 + lane, lane_base + (half ? S::V_COL : S::K_COL));
+      tmem_store_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kv_tmem);
+    }
+    const uint32_t s_addr = lane_base + S::S_COL + half * 32, dp_addr = lane_base + S::DP_COL + half * 32;
+    const uint32_t p_addr = lane_base + S::P_COL + half * 16, ds_addr = lane_base + S::DS_COL + half * 16;
+    for (int i = u; i < nq && ok; i += 2) {
+      uint32_t sr[32], pr[32], po[16], so[16];
       // the statistics of this step have landed with its rows; waiting on their barrier makes them visible here
-      ok = warp_wait(q_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+      ok = warp_wait(q_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL) &&
+           warp_wait(s_full(u), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t stat = base + S::STAT0 + (i % S::STAGES) * S::STAT;
-      // p^T and ds^T of a half go over the scores and dp that it has read itself: 16 of its 32 columns
-      uint32_t sr[32], pr[32], po[16], so[16];
       tmem_load32(s_addr, sr);
-      tmem_load32(s_addr + 64, pr);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_read);
+      ok = warp_wait(dp_full(u), (uint32_t)(i >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
+      if (!ok) break;
+      tc_fence_after();
+      tmem_load32(dp_addr, pr);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(dp_read);
+      if (a.Tk <= 0) break;                                 // never: a branch keeps the arithmetic below behind the arrivals (see the dq kernel)
+      const uint32_t stat = base + S::STAT0 + (i % S::STAGES) * S::STAT;
 #pragma unroll
       for (int k = 0; k < 32; k += 4) {
         uint64_t l[2], d[2];
@@ -556,8 +584,13 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         for (int k = 0; k < 16; ++k) po[k] = so[k] = 0u;
       }
       __syncwarp();
-      tmem_store16(s_addr, po);
-      tmem_store16(s_addr + 64, so);
+      if (i > 0) {                                          // p and ds of the step before have been multiplied
+        ok = warp_wait(p_read(u ^ 1), (uint32_t)((i - 1) >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      tmem_store16(p_addr, po);
+      tmem_store16(ds_addr, so);
       tmem_store_wait();
       tc_fence_before();
       __syncwarp();
@@ -568,7 +601,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     // dv by two warpgroups, dk by the others, 64 columns each (DP = 64: one of the two)
     if (half < DP / 64) {
       const long long off = key < a.Tk ? (((long long)m * a.Tk + key) * a.Hk + hk) * a.D : -1;
-      store_acc64<T>(base + ((u * 2 + half) * 4 + quarter) * 4096, lane_base + u * 128 + half * 64, nq > 0 && ok, u ? b.scale / dsf : ex2(-p_shift<T>()),
+      store_acc64<T>(base + ((u * 2 + half) * 4 + quarter) * 4096, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok, u ? b.scale / dsf : ex2(-p_shift<T>()),
                      u ? dk : dv, off, half * 64, a.D, lane);
     }
   }

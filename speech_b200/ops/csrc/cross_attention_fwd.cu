@@ -249,7 +249,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         for (int k = 0; k < 16; ++k) {
           float x, y;
           const uint64_t e = fma2(pair(r[32 * i + 2 * k], r[32 * i + 2 * k + 1]), c2, shift2);
-          if (k % 8 >= 5) {                                 // three pairs of eight: see the head of this file
+          if (k % 8 >= 6) {                                 // a quarter: 120 us, none 129, half 130 (1024 queries, 7500 keys, 32 heads)
             ex2_poly(e, x, y);
           } else {
             split(e, x, y);
