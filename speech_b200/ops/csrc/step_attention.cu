@@ -1,19 +1,16 @@
 // Attention for a few query rows per key head: one decoding step over an encoder's states, or over a prompt that a group of rows
 // shares together with every row's own cache; also the forward pass of short queries in training.
 //
-// Keys and values are read once and little is computed on them, so bytes bound it, and what counts is how many loads are in flight:
-// the keys of a (memory, key head) are split over blocks and over the warps of a block, every warp streams 16 keys at a time straight
-// into registers in the fragment order of mma.m16n8k16, and the parts (running maximum m, sum l, unnormalised output) are joined in
-// the block and, for more than one block, by a second small kernel:  o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+// Keys and values are read once and little is computed on them, so bytes bound it, and what counts is how many loads are in flight.
+// The keys of a (memory, key head) are split over blocks and over the four warps of a block; every warp streams tiles of 16 keys through
+// a ring of its own in shared memory (cp.async, 24 KB per warp ahead of the arithmetic, 190 KB per SM; no barrier between warps), takes
+// its fragments of mma.m16n8k16 from there with ldmatrix, and keeps running maximum m, sum l and the unnormalised output in registers.
+// The parts are joined in the block and, for more than one block, by a second small kernel:
+//   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+// Loads straight into registers (16 keys ahead, 228 registers, or fewer and spills) reached a third of this.
 //
-// Fragment order without shared memory: a sum over d may take d in any order as long as both operands use the same one, so lane
-// (g, c) = (lane / 4, lane % 4) reads 16 contiguous bytes (8 d) of key g and uses them as the k indices {2c, 2c+1, 2c+8, 2c+9} of two
-// successive products; and a tile of 8 output columns may be any 8 d, so that lane reads 8 contiguous d of each of its four value
-// rows and hands element j of them to output tile j.  All loads are whole 32-byte sectors, 16 bytes a lane.
-//
-// Sixteen packed rows (rows that read the same keys: group x heads of a key head x tokens, as in cross_attention.cuh) make a row
-// block.  Up to four row blocks run in one block of threads, one per warp, so that the L1 serves their common keys; the rest of the
-// four warps split the keys.
+// Packed rows (rows that read the same keys: group x heads of a key head x tokens, as in cross_attention.cuh) fill blocks of 16, one or
+// two per warp; more rows than 32 read the keys again, from the L2.
 //
 // Rounding: as in cross_attention_fwd.cu (weights rounded to 16 bits for the second product, all else fp32).
 #include "cross_attention_host.h"
@@ -29,7 +26,6 @@ struct Segment {
   int rows_per;             // batch rows of a memory (G; 1 for own caches)
   int causal;               // token t sees its row's first length - Tq + 1 + t positions
   int R;                    // packed rows of a (memory, key head)
-  int row_warps;            // warps of a block that take different row blocks
   int row_groups;           // blocks over the rows
   int splits, chunk;        // blocks over the keys, keys of one
   int blocks;
@@ -58,18 +54,36 @@ template <> __device__ __forceinline__ void mma16816<__half>(float* d, const uin
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-__device__ __forceinline__ uint4 load16(const uint16_t* p, bool ok) {
-  return ok ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0);
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes from global to shared memory, or 16 zero bytes
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+// 16-byte chunk `ch` of row `row` in a tile of rows of DP 16-bit elements; the XOR spreads the eight rows of an ldmatrix over all banks
+template <int DP> __device__ __forceinline__ uint32_t row_addr(uint32_t base, int row, int ch) {
+  return base + (uint32_t)(row * DP * 2) + (uint32_t)((ch ^ (row & 7)) << 4);
 }
 
 constexpr int STEP_THREADS = 128;
+template <int DP, int MT> struct StepSmem {
+  static constexpr int HALF = 16 * DP * 2;                 // 16 rows of keys or values
+  static constexpr int RING = DP == 128 ? 3 : 6;           // tiles of keys and values per warp
+  static constexpr int Q0 = 4 * RING * 2 * HALF, BYTES = Q0 + MT * HALF + 16;
+};
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(STEP_THREADS, 3) step_kernel(const StepArgs a) {
-  constexpr int KS = DP / 32, HV = DP / 64, NT = DP / 8;
-  __shared__ float s_m[4][16], s_l[4][16];
-  extern __shared__ float s_o[];                         // [4][16][DP + 4]
+// MT: row blocks of 16 per warp
+template <typename T, int DP, int MT>
+__global__ void __launch_bounds__(STEP_THREADS, 2) step_kernel(const StepArgs a) {
+  using S = StepSmem<DP, MT>;
+  constexpr int CH = DP / 8, NT = DP / 8, KS = DP / 16;
+  __shared__ float s_m[4][16 * MT], s_l[4][16 * MT];
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  const uint32_t base = smem_u32(smem_raw), qs = base + S::Q0;
   const int second = blockIdx.x >= a.seg[0].blocks ? 1 : 0;
   const Segment& s = a.seg[second];
   int x = blockIdx.x - (second ? a.seg[0].blocks : 0);
@@ -79,152 +93,194 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) step_kernel(const StepArgs a)
   x /= s.row_groups;
   const int hk = x % a.Hk, mem = x / a.Hk;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int row_warp = warp % s.row_warps, key_warp = warp / s.row_warps, key_warps = 4 / s.row_warps;
-  const int row0 = (rg * s.row_warps + row_warp) * 16;
+  const int row0 = rg * 16 * MT;
 
   int len = s.size;
   if (s.lengths) len = min(max(s.lengths[mem], 0), s.size);
   const int key_begin = split * s.chunk, key_end = min(len, key_begin + s.chunk);
-
-  // packed row -> (batch row, token, head); rows g and g + 8 of the block
-  int seen[2];
-  uint4 q0[KS], q1[KS];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int r = row0 + g + 8 * u;
-    const bool ok = r < s.R;
-    const int y = r / a.Tq, t = r - y * a.Tq, gr = y / a.rep;
-    const uint16_t* p = a.q + (long long)(mem * s.rows_per + gr) * a.q_sb + (long long)t * a.q_st + (long long)(hk * a.rep + y - gr * a.rep) * a.q_sh + 8 * c;
-    seen[u] = !ok ? 0 : (s.causal ? len - a.Tq + 1 + t : len);
-#pragma unroll
-    for (int k = 0; k < KS; ++k) (u ? q1 : q0)[k] = load16(p + 32 * k, ok && 32 * k + 8 * c < a.D);
-  }
-  const uint16_t* kp = s.k + (long long)mem * s.k_sb + (long long)hk * s.k_sh + 8 * c;
-  const uint16_t* vp = s.v + (long long)mem * s.v_sb + (long long)hk * s.v_sh + 8 * g;
+  const int tiles = key_end > key_begin ? (key_end - key_begin + 15) / 16 : 0;
   const uint8_t* mask = s.mask ? s.mask + (long long)mem * s.size : nullptr;
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[NT][4];
+  // ---- the ring: tile i of the block belongs to warp i % 4
+  const int sub = lane / CH, ch = lane % CH;               // 32 / CH rows per instruction
+  const uint16_t* kp = s.k + (long long)mem * s.k_sb + (long long)hk * s.k_sh + ch * 8;
+  const uint16_t* vp = s.v + (long long)mem * s.v_sb + (long long)hk * s.v_sh + ch * 8;
+  const uint32_t ring = base + warp * (S::RING * 2 * S::HALF);
+  auto fetch = [&](int i, int slot) {                      // one commit group per call, empty behind the last tile
+    if (i < tiles) {
+      const int key0 = key_begin + i * 16;
+      const uint32_t kt = ring + slot * (2 * S::HALF), vt = kt + S::HALF;
 #pragma unroll
-  for (int i = 0; i < NT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-
-  uint4 kr[2][KS];
-  auto load_keys = [&](int key0) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      const int key = key0 + 8 * n + g;
-      const uint16_t* p = kp + (long long)key * s.k_st;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) kr[n][k] = load16(p + 32 * k, key < key_end && 32 * k + 8 * c < a.D);
+      for (int r = 0; r < 16; r += 32 / CH) {
+        const int row = r + sub, key = min(key0 + row, key_end - 1);
+        const bool in = key0 + row < key_end && ch * 8 < a.D;
+        const bool see = in && !(mask && mask[key]);        // a hidden value never meets its zero weight
+        copy16(row_addr<DP>(kt, row, ch), ch * 8 < a.D ? kp + (long long)key * s.k_st : kp - ch * 8, in);
+        copy16(row_addr<DP>(vt, row, ch), ch * 8 < a.D ? vp + (long long)key * s.v_st : vp - ch * 8, see);
+      }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  int key0 = key_begin + key_warp * 16;
-  if (row0 < s.R && key0 < key_end) load_keys(key0);
-  for (; row0 < s.R && key0 < key_end; key0 += key_warps * 16) {
-    // this lane's four keys, in score columns and in value rows alike: key0 + {2c, 2c+1, 2c+8, 2c+9}
-    bool see[4];
-    uint4 vr[4][HV];
+  int next = warp;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = key0 + 2 * c + (i & 1) + 8 * (i >> 1);
-      see[i] = key < key_end && !(mask && mask[key]);
-      const uint16_t* p = vp + (long long)key * s.v_st;
-#pragma unroll
-      for (int h = 0; h < HV; ++h) vr[i][h] = load16(p + 64 * h, see[i] && 64 * h + 8 * g < a.D);   // a hidden value never meets its zero weight
+  for (int i = 0; i < S::RING - 1; ++i, next += 4) fetch(next, i);
+
+  // ---- query rows: packed row -> (batch row, token, head)
+  for (int i = threadIdx.x; i < MT * 16 * CH; i += STEP_THREADS) {
+    const int lr = i / CH, qc = i % CH, r = row0 + lr;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < s.R && qc * 8 < a.D) {
+      const int y = r / a.Tq, t = r - y * a.Tq, gr = y / a.rep;
+      v = *reinterpret_cast<const uint4*>(a.q + (long long)(mem * s.rows_per + gr) * a.q_sb + (long long)t * a.q_st + (long long)(hk * a.rep + y - gr * a.rep) * a.q_sh + qc * 8);
     }
-    float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    st_shared_v4(row_addr<DP>(qs, lr, qc), v.x, v.y, v.z, v.w);
+  }
+  int seen[MT][2];                                         // keys that rows g and g + 8 of each row block see
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = row0 + 16 * t + g + 8 * u;
+      seen[t][u] = r >= s.R ? 0 : (s.causal ? len - a.Tq + 1 + r % a.Tq : len);
+    }
+  __syncthreads();
+
+  const int mrow = (lane & 7) + ((lane >> 3) & 1) * 8, mch = lane >> 4;      // ldmatrix rows of Q and V: (row half, chunk) by lane group
+  uint32_t qf[MT == 1 ? KS : 1][4];
+  if (MT == 1) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) ldmatrix4(row_addr<DP>(qs, mrow, 2 * k + mch), qf[MT == 1 ? k : 0]);
+  }
+  float m[MT][2], l[MT][2], o[MT][NT][4];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    m[t][0] = m[t][1] = -INFINITY;
+    l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
+  }
+
+  int slot = 0;
+  for (int i = warp; i < tiles; i += 4) {
+    {
+      int free_slot = slot + S::RING - 1;
+      if (free_slot >= S::RING) free_slot -= S::RING;
+      __syncwarp();                                        // the whole warp is done with the tile that is overwritten
+      fetch(next, free_slot);
+      next += 4;
+    }
+    asm volatile("cp.async.wait_group %0;" ::"n"(S::RING - 1) : "memory");
+    __syncwarp();
+    const uint32_t kt = ring + slot * (2 * S::HALF), vt = kt + S::HALF;
+    if (++slot == S::RING) slot = 0;
+    const int key0 = key_begin + i * 16;
+    // this lane's columns of the scores: keys key0 + {2c, 2c+1, 2c+8, 2c+9}
+    int kcol[4];
+    bool see[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      kcol[e] = key0 + 2 * c + (e & 1) + 8 * (e >> 1);
+      see[e] = kcol[e] < key_end && !(mask && mask[kcol[e]]);
+    }
+    float sc[MT][2][4];
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) sc[t][n][0] = sc[t][n][1] = sc[t][n][2] = sc[t][n][3] = 0.f;
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const uint32_t a0[4] = {q0[k].x, q1[k].x, q0[k].y, q1[k].y}, a1[4] = {q0[k].z, q1[k].z, q0[k].w, q1[k].w};
+      uint32_t kf[4];
+      ldmatrix4(row_addr<DP>(kt, (lane & 7) + mch * 8, 2 * k + ((lane >> 3) & 1)), kf);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        mma16816<T>(sc[n], a0, kr[n][k].x, kr[n][k].y);
-        mma16816<T>(sc[n], a1, kr[n][k].z, kr[n][k].w);
+      for (int t = 0; t < MT; ++t) {
+        uint32_t q2[4];
+        if (MT > 1) ldmatrix4(row_addr<DP>(qs, 16 * t + mrow, 2 * k + mch), q2);
+        const uint32_t* q = MT == 1 ? qf[MT == 1 ? k : 0] : q2;
+        mma16816<T>(sc[t][0], q, kf[0], kf[1]);
+        mma16816<T>(sc[t][1], q, kf[2], kf[3]);
       }
     }
-    if (key0 + key_warps * 16 < key_end) load_keys(key0 + key_warps * 16);
-    uint32_t p[4];
+    uint32_t p[MT][4];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {                         // row g + 8 u: columns sc[n][2u], sc[n][2u + 1]
-      float v[4];
-      float mx = -INFINITY;
+    for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = key0 + 2 * c + (i & 1) + 8 * (i >> 1);
-        v[i] = see[i] && key < seen[u] ? sc[i >> 1][2 * u + (i & 1)] * a.c : -INFINITY;
-        mx = fmaxf(mx, v[i]);
-      }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const bool grow = mx > m[u] + 8.f && m[u] != -INFINITY;
-      if (__any_sync(0xffffffffu, grow)) {                // rare: the output keeps its scale until a maximum has grown by 2^8
-        const float nm = m[u] == -INFINITY ? m[u] : fmaxf(m[u], mx);
-        const float f = m[u] == -INFINITY ? 1.f : ex2(m[u] - nm);
-        m[u] = nm;
-        l[u] *= f;
+      for (int u = 0; u < 2; ++u) {                        // row g + 8 u: columns sc[.][n][2u], sc[.][n][2u + 1]
+        float v[4], mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          o[i][2 * u] *= f;
-          o[i][2 * u + 1] *= f;
+        for (int e = 0; e < 4; ++e) {
+          v[e] = see[e] && kcol[e] < seen[t][u] ? sc[t][e >> 1][2 * u + (e & 1)] * a.c : -INFINITY;
+          mx = fmaxf(mx, v[e]);
         }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const bool grow = mx > m[t][u] + 8.f && m[t][u] != -INFINITY;
+        if (__any_sync(0xffffffffu, grow)) {               // rare: the output keeps its scale until a maximum has grown by 2^8
+          const float nm = m[t][u] == -INFINITY ? m[t][u] : fmaxf(m[t][u], mx);
+          const float f = m[t][u] == -INFINITY ? 1.f : ex2(m[t][u] - nm);
+          m[t][u] = nm;
+          l[t][u] *= f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            o[t][n][2 * u] *= f;
+            o[t][n][2 * u + 1] *= f;
+          }
+        }
+        if (m[t][u] == -INFINITY) m[t][u] = mx;
+        const float from = m[t][u] == -INFINITY ? 0.f : m[t][u];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = ex2(v[e] - from);
+        l[t][u] += (v[0] + v[1]) + (v[2] + v[3]);
+        p[t][u] = Half2<T>::pack(v[0], v[1]);
+        p[t][2 + u] = Half2<T>::pack(v[2], v[3]);
       }
-      if (m[u] == -INFINITY) m[u] = mx;
-      const float base = m[u] == -INFINITY ? 0.f : m[u];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = ex2(v[i] - base);
-      l[u] += (v[0] + v[1]) + (v[2] + v[3]);
-      p[u] = Half2<T>::pack(v[0], v[1]);
-      p[2 + u] = Half2<T>::pack(v[2], v[3]);
-    }
+    for (int n = 0; n < NT; n += 2) {
+      uint32_t vf[4];
+      ldmatrix4t(row_addr<DP>(vt, mrow, n + mch), vf);
 #pragma unroll
-    for (int h = 0; h < HV; ++h)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t sel = j & 1 ? 0x7632 : 0x5410;
-        const uint32_t b0 = __byte_perm(word_of(vr[0][h], j >> 1), word_of(vr[1][h], j >> 1), sel);
-        const uint32_t b1 = __byte_perm(word_of(vr[2][h], j >> 1), word_of(vr[3][h], j >> 1), sel);
-        mma16816<T>(o[8 * h + j], p, b0, b1);
+      for (int t = 0; t < MT; ++t) {
+        mma16816<T>(o[t][n], p[t], vf[0], vf[1]);
+        mma16816<T>(o[t][n + 1], p[t], vf[2], vf[3]);
       }
-  }
-  // join the warps that split the keys of a row block; lane (g, c) holds, of rows g and g + 8, columns 64 h + 16 c + 0 .. 15
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-    l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-    if (c == 0) {
-      s_m[warp][g + 8 * u] = m[u];
-      s_l[warp][g + 8 * u] = l[u];
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+
+  // ---- join the four warps; lane (g, c) holds columns 8 n + 2c, + 1 of rows g and g + 8
+  __syncthreads();                                         // the rings become the exchange buffer
   constexpr int LD = DP + 4;
-  float* mine = s_o + warp * 16 * LD;
+  float* s_o = reinterpret_cast<float*>(smem_raw);
+  float* mine = s_o + warp * 16 * MT * LD;
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int t = 0; t < MT; ++t)
 #pragma unroll
-    for (int h = 0; h < HV; ++h)
+    for (int u = 0; u < 2; ++u) {
+      l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], 1);
+      l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], 2);
+      const int lr = 16 * t + g + 8 * u;
+      if (c == 0) {
+        s_m[warp][lr] = m[t][u];
+        s_l[warp][lr] = l[t][u];
+      }
 #pragma unroll
-      for (int n = 0; n < 2; ++n)                          // column 2c + n of tile j is d = 64 h + 8 (2c + n) + j
-#pragma unroll
-        for (int j = 0; j < 8; j += 4)
-          *reinterpret_cast<float4*>(mine + (g + 8 * u) * LD + 64 * h + 16 * c + 8 * n + j) =
-              make_float4(o[8 * h + j][2 * u + n], o[8 * h + j + 1][2 * u + n], o[8 * h + j + 2][2 * u + n], o[8 * h + j + 3][2 * u + n]);
+      for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(mine + lr * LD + 8 * n + 2 * c) = make_float2(o[t][n][2 * u], o[t][n][2 * u + 1]);
+    }
   __syncthreads();
-  const int slot = split + (second ? a.seg[0].splits : 0);
+  const int slot_out = split + (second ? a.seg[0].splits : 0);
   const long long qrows = (long long)a.B * a.Tq * a.H;
-  const int per_row = a.D / 8;
-  for (int i = threadIdx.x; i < s.row_warps * 16 * per_row; i += STEP_THREADS) {
-    const int rr = i / per_row, d = (i - rr * per_row) * 8, rw = rr >> 4, lr = rr & 15;
-    const int r = (rg * s.row_warps + rw) * 16 + lr;
-    if (r >= s.R) continue;
+  const int per_row = a.D / 8, rows_here = min(16 * MT, s.R - row0);
+  for (int i = threadIdx.x; i < rows_here * per_row; i += STEP_THREADS) {
+    const int lr = i / per_row, d = (i - lr * per_row) * 8, r = row0 + lr;
     float big = -INFINITY;
-    for (int w = 0; w < key_warps; ++w) big = fmaxf(big, s_m[rw + w * s.row_warps][lr]);
-    const float base = big == -INFINITY ? 0.f : big;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) big = fmaxf(big, s_m[w][lr]);
+    const float from = big == -INFINITY ? 0.f : big;
     float sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int w = 0; w < key_warps; ++w) {
-      const int src = rw + w * s.row_warps;
-      const float f = ex2(s_m[src][lr] - base);
-      sum += f * s_l[src][lr];
-      const float* po = s_o + src * 16 * LD + lr * LD + d;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = ex2(s_m[w][lr] - from);
+      sum += f * s_l[w][lr];
+      const float* po = s_o + (w * 16 * MT + lr) * LD + d;
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += f * po[k];
     }
@@ -239,10 +295,10 @@ __global__ void __launch_bounds__(STEP_THREADS, 3) step_kernel(const StepArgs a)
       if (a.rest) *reinterpret_cast<uint4*>(a.rest + qrow * a.D + d) = make_uint4(r4[0], r4[1], r4[2], r4[3]);
       if (a.lse && d == 0) a.lse[((long long)mem * a.Hk + hk) * s.R + r] = sum > 0.f ? big + log2f(sum) : (sum == 0.f ? INFINITY : sum);
     } else {
-      float* po = a.part_o + ((long long)slot * qrows + qrow) * a.D + d;
+      float* po = a.part_o + ((long long)slot_out * qrows + qrow) * a.D + d;
       *reinterpret_cast<float4*>(po) = make_float4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<float4*>(po + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      if (d == 0) a.part_ml[slot * qrows + qrow] = make_float2(big, sum);
+      if (d == 0) a.part_ml[slot_out * qrows + qrow] = make_float2(big, sum);
     }
   }
 }
@@ -284,29 +340,26 @@ template <typename T> __global__ void __launch_bounds__(128) step_join_kernel(co
   }
 }
 
-void plan_rows(Segment& s) {
-  const int blocks16 = (s.R + 15) / 16;
-  s.row_warps = blocks16 >= 4 ? 4 : (blocks16 >= 2 ? 2 : 1);
-  s.row_groups = (blocks16 + s.row_warps - 1) / s.row_warps;
-}
+// Row blocks per warp: two where either segment has more than 16 packed rows.
+int row_blocks(const StepArgs& a) { return a.seg[0].R > 16 || a.seg[1].R > 16 ? 2 : 1; }
 
-// Splits both segments' keys so that about three blocks per SM have equal shares.  A share is at least 64 keys (16 per warp).
+// Splits both segments' keys so that the two blocks that fit an SM get equal shares, of at most MAX_SHARE keys: beyond one wave, short
+// shares keep the last wave short (and are what lengths far below the cache's size leave empty).  At least 64 keys, 16 per warp.
+constexpr int MAX_SHARE = 512;
 int plan(StepArgs& a, int memories0, int memories1) {
-  plan_rows(a.seg[0]);
-  if (memories1) plan_rows(a.seg[1]);
+  const int rows = 16 * row_blocks(a);
+  for (int i = 0; i < 2; ++i) a.seg[i].row_groups = (a.seg[i].R + rows - 1) / rows;
   const long long u0 = (long long)memories0 * a.Hk * a.seg[0].row_groups, u1 = memories1 ? (long long)memories1 * a.Hk * a.seg[1].row_groups : 0;
   const long long total = u0 * a.seg[0].size + u1 * a.seg[1].size;
-  long long chunk = (total / (148 * 3) + 63) / 64 * 64;
-  if (chunk < 64) chunk = 64;
+  long long chunk = (total / (sb_num_sms() * 2) + 63) / 64 * 64;
+  chunk = chunk < 64 ? 64 : (chunk > MAX_SHARE ? MAX_SHARE : chunk);
   a.slots = 0;
   long long blocks = 0;
   for (int i = 0; i < 2; ++i) {
     Segment& s = a.seg[i];
     const long long units = i ? u1 : u0;
     s.splits = units ? (int)((s.size + chunk - 1) / chunk) : 0;
-    if (units && s.splits < 1) s.splits = 1;
-    s.chunk = s.splits ? (int)(((s.size + s.splits - 1) / s.splits + 15) / 16 * 16) : 0;
-    if (s.chunk < 16) s.chunk = 16;
+    s.chunk = s.splits ? (int)(((s.size + s.splits - 1) / s.splits + 63) / 64 * 64) : 64;
     if (units * s.splits > 0x7fffffffll) return SB_BAD_ARGUMENT;
     s.blocks = (int)(units * s.splits);
     blocks += s.blocks;
@@ -319,10 +372,14 @@ long long workspace(const StepArgs& a) {
   return a.slots <= 1 ? 0 : (long long)a.slots * a.B * a.Tq * a.H * (a.D + 2) * 4;
 }
 
+template <typename T, int DP, int MT> int launch_rows(const StepArgs& a, cudaStream_t stream) {
+  const int rc = sb_allow_smem((const void*)step_kernel<T, DP, MT>, StepSmem<DP, MT>::BYTES);
+  if (rc) return rc;
+  step_kernel<T, DP, MT><<<(unsigned)(a.seg[0].blocks + a.seg[1].blocks), STEP_THREADS, StepSmem<DP, MT>::BYTES, stream>>>(a);
+  return (int)cudaGetLastError();
+}
 template <typename T, int DP> int launch_step(const StepArgs& a, cudaStream_t stream) {
-  constexpr int SMEM = 4 * 16 * (DP + 4) * 4;
-  step_kernel<T, DP><<<(unsigned)(a.seg[0].blocks + a.seg[1].blocks), STEP_THREADS, SMEM, stream>>>(a);
-  int rc = (int)cudaGetLastError();
+  const int rc = row_blocks(a) == 1 ? launch_rows<T, DP, 1>(a, stream) : launch_rows<T, DP, 2>(a, stream);
   if (rc || a.slots == 1) return rc;
   const long long qrows = (long long)a.B * a.Tq * a.H;
   step_join_kernel<T><<<(unsigned)((qrows + 3) / 4), 128, 0, stream>>>(a);
