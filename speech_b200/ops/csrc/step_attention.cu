@@ -3,7 +3,7 @@
 //
 // Keys and values are read once and little is computed on them, so bytes bound it, and what counts is how many loads are in flight.
 // The keys of a (memory, key head) are split over blocks and over the four warps of a block; every warp streams tiles of 16 keys through
-// a ring of its own in shared memory (cp.async, 24 KB per warp ahead of the arithmetic, 190 KB per SM; no barrier between warps), takes
+// a ring of its own in shared memory (cp.async, 16 or 24 KB per warp, 190 KB per SM; no barrier between warps), takes
 // its fragments of mma.m16n8k16 from there with ldmatrix, and keeps running maximum m, sum l and the unnormalised output in registers.
 // The parts are joined in the block and, for more than one block, by a second small kernel:
 //   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
@@ -72,13 +72,14 @@ template <int DP> __device__ __forceinline__ uint32_t row_addr(uint32_t base, in
 constexpr int STEP_THREADS = 128;
 template <int DP, int MT> struct StepSmem {
   static constexpr int HALF = 16 * DP * 2;                 // 16 rows of keys or values
-  static constexpr int RING = DP == 128 ? 3 : 6;           // tiles of keys and values per warp
+  static constexpr int RING = (DP == 128 ? 1 : 2) * (MT == 1 ? 2 : 3);      // tiles of keys and values per warp
   static constexpr int Q0 = 4 * RING * 2 * HALF, BYTES = Q0 + MT * HALF + 16;
+  static constexpr int BLOCKS = MT == 1 ? 3 : 2;           // per SM
 };
 
 // MT: row blocks of 16 per warp
 template <typename T, int DP, int MT>
-__global__ void __launch_bounds__(STEP_THREADS, 2) step_kernel(const StepArgs a) {
+__global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step_kernel(const __grid_constant__ StepArgs a) {
   using S = StepSmem<DP, MT>;
   constexpr int CH = DP / 8, NT = DP / 8, KS = DP / 16;
   __shared__ float s_m[4][16 * MT], s_l[4][16 * MT];
@@ -103,21 +104,45 @@ __global__ void __launch_bounds__(STEP_THREADS, 2) step_kernel(const StepArgs a)
 
   // ---- the ring: tile i of the block belongs to warp i % 4
   const int sub = lane / CH, ch = lane % CH;               // 32 / CH rows per instruction
-  const uint16_t* kp = s.k + (long long)mem * s.k_sb + (long long)hk * s.k_sh + ch * 8;
-  const uint16_t* vp = s.v + (long long)mem * s.v_sb + (long long)hk * s.v_sh + ch * 8;
+  const bool on = ch * 8 < a.D;                            // chunks behind the head size are zeros
+  const uint16_t* kp = s.k + (long long)mem * s.k_sb + (long long)hk * s.k_sh;
+  const uint16_t* vp = s.v + (long long)mem * s.v_sb + (long long)hk * s.v_sh;
+  const uint16_t *k_at = kp, *v_at = vp;                   // this lane's first chunk of tile `next`
+  if (on) {
+    k_at += (long long)(key_begin + warp * 16 + sub) * s.k_st + ch * 8;
+    v_at += (long long)(key_begin + warp * 16 + sub) * s.v_st + ch * 8;
+  }
+  const long long k_step = on ? s.k_st * (32 / CH) : 0, v_step = on ? s.v_st * (32 / CH) : 0;
   const uint32_t ring = base + warp * (S::RING * 2 * S::HALF);
+  const uint32_t lane_at = (uint32_t)(sub * DP * 2);
   auto fetch = [&](int i, int slot) {                      // one commit group per call, empty behind the last tile
     if (i < tiles) {
-      const int key0 = key_begin + i * 16;
-      const uint32_t kt = ring + slot * (2 * S::HALF), vt = kt + S::HALF;
+      const int left = key_end - (key_begin + i * 16);     // keys from this tile on
+      const uint32_t kt = ring + slot * (2 * S::HALF) + lane_at, vt = kt + S::HALF;
+      const uint16_t *kq = k_at, *vq = v_at;
+      if (left >= 16 && !mask) {
 #pragma unroll
-      for (int r = 0; r < 16; r += 32 / CH) {
-        const int row = r + sub, key = min(key0 + row, key_end - 1);
-        const bool in = key0 + row < key_end && ch * 8 < a.D;
-        const bool see = in && !(mask && mask[key]);        // a hidden value never meets its zero weight
-        copy16(row_addr<DP>(kt, row, ch), ch * 8 < a.D ? kp + (long long)key * s.k_st : kp - ch * 8, in);
-        copy16(row_addr<DP>(vt, row, ch), ch * 8 < a.D ? vp + (long long)key * s.v_st : vp - ch * 8, see);
+        for (int r = 0; r < 16; r += 32 / CH) {
+          const uint32_t x = (uint32_t)(r * DP * 2) + (uint32_t)((ch ^ ((r + sub) & 7)) << 4);
+          copy16(kt + x, kq, on);
+          copy16(vt + x, vq, on);
+          kq += k_step;
+          vq += v_step;
+        }
+      } else {
+#pragma unroll 1
+        for (int r = 0; r < 16; r += 32 / CH) {
+          const uint32_t x = (uint32_t)(r * DP * 2) + (uint32_t)((ch ^ ((r + sub) & 7)) << 4);
+          const bool in = on && r + sub < left;
+          const bool see = in && !(mask && mask[key_begin + i * 16 + r + sub]);      // a hidden value never meets its zero weight
+          copy16(kt + x, in ? kq : kp, in);
+          copy16(vt + x, see ? vq : vp, see);
+          kq += k_step;
+          vq += v_step;
+        }
       }
+      k_at += k_step * (2 * CH);                           // 64 rows on
+      v_at += v_step * (2 * CH);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -161,6 +186,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2) step_kernel(const StepArgs a)
   }
 
   int slot = 0;
+  const int all_see = mask ? 0 : min(key_end, s.causal ? len - a.Tq + 1 : len);      // every row sees the keys below
   for (int i = warp; i < tiles; i += 4) {
     {
       int free_slot = slot + S::RING - 1;
@@ -174,14 +200,6 @@ __global__ void __launch_bounds__(STEP_THREADS, 2) step_kernel(const StepArgs a)
     const uint32_t kt = ring + slot * (2 * S::HALF), vt = kt + S::HALF;
     if (++slot == S::RING) slot = 0;
     const int key0 = key_begin + i * 16;
-    // this lane's columns of the scores: keys key0 + {2c, 2c+1, 2c+8, 2c+9}
-    int kcol[4];
-    bool see[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      kcol[e] = key0 + 2 * c + (e & 1) + 8 * (e >> 1);
-      see[e] = kcol[e] < key_end && !(mask && mask[kcol[e]]);
-    }
     float sc[MT][2][4];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
@@ -200,19 +218,28 @@ __global__ void __launch_bounds__(STEP_THREADS, 2) step_kernel(const StepArgs a)
         mma16816<T>(sc[t][1], q, kf[2], kf[3]);
       }
     }
+    if (key0 + 16 > all_see) {
+      // this lane's columns of the scores are keys key0 + {2c, 2c+1, 2c+8, 2c+9}
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + 2 * c + (e & 1) + 8 * (e >> 1);
+        const bool see = key < key_end && !(mask && mask[key]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (!(see && key < seen[t][u])) sc[t][e >> 1][2 * u + (e & 1)] = -INFINITY;
+      }
+    }
     uint32_t p[MT][4];
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {                        // row g + 8 u: columns sc[.][n][2u], sc[.][n][2u + 1]
-        float v[4], mx = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] = see[e] && kcol[e] < seen[t][u] ? sc[t][e >> 1][2 * u + (e & 1)] * a.c : -INFINITY;
-          mx = fmaxf(mx, v[e]);
-        }
+        float v[4] = {sc[t][0][2 * u], sc[t][0][2 * u + 1], sc[t][1][2 * u], sc[t][1][2 * u + 1]};
+        float mx = fmaxf(max3(v[0], v[1], v[2]), v[3]);
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2)) * a.c;
         const bool grow = mx > m[t][u] + 8.f && m[t][u] != -INFINITY;
         if (__any_sync(0xffffffffu, grow)) {               // rare: the output keeps its scale until a maximum has grown by 2^8
           const float nm = m[t][u] == -INFINITY ? m[t][u] : fmaxf(m[t][u], mx);
@@ -228,7 +255,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2) step_kernel(const StepArgs a)
         if (m[t][u] == -INFINITY) m[t][u] = mx;
         const float from = m[t][u] == -INFINITY ? 0.f : m[t][u];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = ex2(v[e] - from);
+        for (int e = 0; e < 4; ++e) v[e] = ex2(fmaf(v[e], a.c, -from));
         l[t][u] += (v[0] + v[1]) + (v[2] + v[3]);
         p[t][u] = Half2<T>::pack(v[0], v[1]);
         p[t][2 + u] = Half2<T>::pack(v[2], v[3]);
@@ -340,10 +367,11 @@ template <typename T> __global__ void __launch_bounds__(128) step_join_kernel(co
   }
 }
 
-// Row blocks per warp: two where either segment has more than 16 packed rows.
-int row_blocks(const StepArgs& a) { return a.seg[0].R > 16 || a.seg[1].R > 16 ? 2 : 1; }
+// Row blocks per warp: two where a segment has more than 32 packed rows; up to there a second block of threads that reads the same keys
+// from the L2 is faster than fewer and larger blocks for all (three to an SM, not two).
+int row_blocks(const StepArgs& a) { return a.seg[0].R > 32 || a.seg[1].R > 32 ? 2 : 1; }
 
-// Splits both segments' keys so that the two blocks that fit an SM get equal shares, of at most MAX_SHARE keys: beyond one wave, short
+// Splits both segments' keys so that the blocks that fit the SMs at once get equal shares, of at most MAX_SHARE keys: beyond one wave, short
 // shares keep the last wave short (and are what lengths far below the cache's size leave empty).  At least 64 keys, 16 per warp.
 constexpr int MAX_SHARE = 512;
 int plan(StepArgs& a, int memories0, int memories1) {
@@ -351,7 +379,7 @@ int plan(StepArgs& a, int memories0, int memories1) {
   for (int i = 0; i < 2; ++i) a.seg[i].row_groups = (a.seg[i].R + rows - 1) / rows;
   const long long u0 = (long long)memories0 * a.Hk * a.seg[0].row_groups, u1 = memories1 ? (long long)memories1 * a.Hk * a.seg[1].row_groups : 0;
   const long long total = u0 * a.seg[0].size + u1 * a.seg[1].size;
-  long long chunk = (total / (sb_num_sms() * 2) + 63) / 64 * 64;
+  long long chunk = (total / (sb_num_sms() * (row_blocks(a) == 1 ? 3 : 2)) + 63) / 64 * 64;
   chunk = chunk < 64 ? 64 : (chunk > MAX_SHARE ? MAX_SHARE : chunk);
   a.slots = 0;
   long long blocks = 0;
