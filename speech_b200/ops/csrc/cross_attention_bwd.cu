@@ -431,8 +431,11 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       mbar_expect_tx(kv_full, 2 * S::KEYS);
 #pragma unroll
       for (int h = 0; h < HALVES; ++h) {
-        tma_load_4d(base + h * 16384, &map_k, kv_full, h * 64, key0, hk, m);
-        tma_load_4d(base + S::KEYS + h * 16384, &map_v, kv_full, h * 64, key0, hk, m);
+#pragma unroll
+        for (int r = 0; r < 128; r += 64) {                  // the dq kernel's boxes of 64 rows, two of them
+          tma_load_4d(base + h * 16384 + r * 128, &map_k, kv_full, h * 64, key0 + r, hk, m);
+          tma_load_4d(base + S::KEYS + h * 16384 + r * 128, &map_v, kv_full, h * 64, key0 + r, hk, m);
+        }
       }
     }
     __syncwarp();
@@ -612,11 +615,9 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
 template <typename T, int DP>
 int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, void* dk, void* dv, cudaStream_t stream) {
-  CUtensorMap k64, v64, k128, v128, q64, do64;
+  CUtensorMap k64, v64, q64, do64;
   int rc = sb_rows_map(&k64, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, DqSmem<DP>::BN);
   if (!rc) rc = sb_rows_map(&v64, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, DqSmem<DP>::BN);
-  if (!rc) rc = sb_rows_map(&k128, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, 128);
-  if (!rc) rc = sb_rows_map(&v128, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, 128);
   if (!rc) rc = sb_rows_map(&q64, g->q, g->type, a.D, a.Tq, a.H, a.M * a.G, g->q_st, g->q_sh, g->q_sb, DkvSmem<DP>::BQ);
   if (!rc) rc = sb_rows_map(&do64, b.dout, g->type, a.D, a.Tq, a.H, a.M * a.G, (long long)a.H * a.D, a.D, (long long)a.Tq * a.H * a.D, DkvSmem<DP>::BQ);
   if (!rc) rc = sb_allow_smem((const void*)xattn_dq_kernel<T, DP>, DqSmem<DP>::BYTES);
@@ -633,7 +634,7 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
     rc = (int)cudaGetLastError();
   }
   if (!rc && dk) {
-    xattn_dkv_kernel<T, DP><<<(unsigned)gk, DKV_THREADS, DkvSmem<DP>::BYTES, stream>>>(k128, v128, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv);
+    xattn_dkv_kernel<T, DP><<<(unsigned)gk, DKV_THREADS, DkvSmem<DP>::BYTES, stream>>>(k64, v64, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv);
     rc = (int)cudaGetLastError();
   }
   return rc;

@@ -215,12 +215,39 @@ __device__ __forceinline__ void grad_from_memory(const T* x, T* o, int V, int la
   if (yv >= 0 && yv < s.nv * E && (yv / E) % TPR == lane) one(y);
 }
 
+// Counted positions, by a whole block.  Every block counts for itself up to this many bytes of mask (a few loads per thread); beyond,
+// a kernel does it first.
+constexpr long long COUNT_LIMIT = 64 * 1024;
+__device__ int count_mask(const uint8_t* __restrict__ mask, long long rows, int C, int* red) {
+  if (!mask) return (int)rows;
+  const long long nt = rows / C;
+  int n = 0;
+  const long long head = min(nt, (long long)((16 - (reinterpret_cast<uintptr_t>(mask) & 15)) & 15)), groups = (nt - head) / 16;
+  if (threadIdx.x < head) n += mask[threadIdx.x] != 0;
+  const uint4* g = reinterpret_cast<const uint4*>(mask + head);
+  for (long long i = threadIdx.x; i < groups; i += blockDim.x) {
+    const uint4 v = g[i];
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) n += __popc(__vsetne4(w[k], 0u));
+  }
+  for (long long i = head + groups * 16 + threadIdx.x; i < nt; i += blockDim.x) n += mask[i] != 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = n;
+  __syncthreads();
+  int t = 0;
+  for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += red[i];
+  __syncthreads();
+  return t * C;
+}
+
 // Forward pass over all rows.  TPR threads work on a row; NV > 0: it stays in registers as it was read, NV 16-byte groups per thread;
 // NV = 0: rows of any length, read again for the gradient, from the L2 (148 rows of 300 KB in flight are a third of it).
 // lse / logp / slope: fp32 [rows]; dlogits: contiguous [rows, V] or null (no gradient wanted now); partial: fp64, per block the sum of
 // its policy terms; ratio: fp64 [rows], preference only.
-template <typename T, int MODE, int TPR, int NV, int THREADS>
-__global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, const int* __restrict__ count_p, float* __restrict__ logp_out, float* __restrict__ lse_out,
+template <typename T, int MODE, int TPR, int NV, int THREADS, bool COUNT_HERE>
+__global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, int* __restrict__ count_p, float* __restrict__ logp_out, float* __restrict__ lse_out,
                                                                float* __restrict__ slope_out, void* __restrict__ dlogits, double* __restrict__ partial,
                                                                double* __restrict__ ratio) {
   constexpr int E = Vec<T>::N, GROUPS = THREADS / TPR;
@@ -228,7 +255,10 @@ __global__ void __launch_bounds__(THREADS) rows_forward_kernel(const RowArgs a, 
   __shared__ double redd[32];
   const int lane = TPR == 32 ? (threadIdx.x & 31) : threadIdx.x;
   const int group = TPR == 32 ? (threadIdx.x >> 5) : 0;
-  const float inv_count = MODE == LOSS_POLICY ? (float)(1.0 / (double)max(1, *count_p)) : 0.f;
+  int count = 0;
+  if (MODE == LOSS_POLICY) count = COUNT_HERE ? count_mask(a.mask, a.rows, a.C, reinterpret_cast<int*>(redf)) : *count_p;
+  const float inv_count = (float)(1.0 / (double)max(1, count));
+  if (COUNT_HERE && blockIdx.x == 0 && threadIdx.x == 0) *count_p = count;
   double mine = 0.0;                                     // same value in every thread of the group
   for (long long row = (long long)blockIdx.x * GROUPS + group; row < a.rows; row += (long long)gridDim.x * GROUPS) {
     const Row r = locate(a, row);
@@ -400,20 +430,10 @@ __global__ void __launch_bounds__(THREADS) rows_grad_kernel(const RowArgs a, con
   }
 }
 
-__global__ void count_kernel(const uint8_t* __restrict__ mask, long long nt, int C, int* __restrict__ count) {
+__global__ void __launch_bounds__(1024) count_kernel(const uint8_t* __restrict__ mask, long long rows, int C, int* __restrict__ count) {
   __shared__ int red[32];
-  long long n = 0;
-  for (long long i = threadIdx.x; i < nt; i += blockDim.x) n += mask ? mask[i] != 0 : 1;
-  int c = (int)n;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) c += __shfl_xor_sync(0xffffffffu, c, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = c;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    int t = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) t += red[i];
-    *count = t * C;
-  }
+  const int n = count_mask(mask, rows, C, red);
+  if (threadIdx.x == 0) *count = n;
 }
 
 __global__ void policy_finish_kernel(const double* __restrict__ partial, int n, const int* __restrict__ count, float* __restrict__ loss) {
@@ -448,12 +468,34 @@ __global__ void ratio_kernel(const double* __restrict__ ratio, long long per, do
   }
 }
 
+// The same sums by one warp per sequence, in the block that goes on with them: for up to this many positions in all one kernel less is
+// worth more than the wider sum.
+constexpr long long ONE_BLOCK_ROWS = 64 * 1024;
+__device__ void ratio_sums(const double* __restrict__ ratio, long long per, int n, double* total) {
+  for (int s = threadIdx.x >> 5; s < n; s += blockDim.x >> 5) {
+    const double* p = ratio + (long long)s * per;
+    double t[4] = {0.0, 0.0, 0.0, 0.0};
+    long long i = threadIdx.x & 31;
+    for (; i + 96 < per; i += 128) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t[k] += p[i + 32 * k];
+    }
+    for (; i < per; i += 32) t[0] += p[i];
+    double u = (t[0] + t[1]) + (t[2] + t[3]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    if ((threadIdx.x & 31) == 0) total[s] = u;
+  }
+  __syncthreads();
+}
+
 // Scalar losses of all pairs, their mean, rewards beta * ratio and the slope of every sequence's positions.  One block.
-__global__ void preference_finish_kernel(const double* __restrict__ total, int pairs, int kind, float beta_f, const float* __restrict__ gap,
+__global__ void __launch_bounds__(1024) preference_finish_kernel(const double* __restrict__ ratio, long long per, double* total, int pairs, int kind, float beta_f, const float* __restrict__ gap,
                                          float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ seq_slope) {
   __shared__ double red[32];
   const double beta = (double)beta_f;
   double mine = 0.0;
+  if (ratio) ratio_sums(ratio, per, 2 * pairs, total);
   for (int n = threadIdx.x; n < pairs; n += blockDim.x) {
     const double margin = total[n] - total[n + pairs];
     double l, s;
@@ -490,18 +532,21 @@ __global__ void preference_finish_kernel(const double* __restrict__ total, int p
 constexpr int MAX_BLOCKS = 148 * 16;
 
 template <typename T, int MODE, int TPR, int NV, int THREADS>
-int run_forward(const RowArgs& a, const int* count, float* logp, float* lse, float* slope, void* dlogits, double* partial, double* ratio, int* blocks,
+int run_forward(const RowArgs& a, int* count, float* logp, float* lse, float* slope, void* dlogits, double* partial, double* ratio, int* blocks,
                 cudaStream_t stream) {
   long long need = (a.rows + THREADS / TPR - 1) / (THREADS / TPR);
   const long long fit = (long long)sb_num_sms() * (2048 / THREADS);
   const long long cap = fit < MAX_BLOCKS ? fit : MAX_BLOCKS;
   *blocks = (int)(need < cap ? need : cap);
-  rows_forward_kernel<T, MODE, TPR, NV, THREADS><<<*blocks, THREADS, 0, stream>>>(a, count, logp, lse, slope, dlogits, partial, ratio);
+  if (MODE == LOSS_POLICY && (!a.mask || a.rows / a.C <= COUNT_LIMIT))
+    rows_forward_kernel<T, MODE, TPR, NV, THREADS, MODE == LOSS_POLICY><<<*blocks, THREADS, 0, stream>>>(a, count, logp, lse, slope, dlogits, partial, ratio);
+  else
+    rows_forward_kernel<T, MODE, TPR, NV, THREADS, false><<<*blocks, THREADS, 0, stream>>>(a, count, logp, lse, slope, dlogits, partial, ratio);
   return (int)cudaGetLastError();
 }
 
 template <typename T, int MODE>
-int forward(const RowArgs& a, const int* count, float* logp, float* lse, float* slope, void* dlogits, double* partial, double* ratio, int* blocks,
+int forward(const RowArgs& a, int* count, float* logp, float* lse, float* slope, void* dlogits, double* partial, double* ratio, int* blocks,
             cudaStream_t stream) {
   // a row that fits eight 16-byte groups per thread of a warp or block stays in registers
   const long long groups = a.V / Vec<T>::N;
@@ -552,7 +597,7 @@ SB_API int sb_policy_loss_fwd(const void* logits, int type, long long sn, long l
   a.clip_lo = clip_lo; a.clip_hi = clip_hi; a.kl_beta = kl_beta;
   a.log_lo = clip_lo < 1.f ? log(1.0 - (double)clip_lo) : -HUGE_VAL;
   a.log_hi = log(1.0 + (double)clip_hi);
-  count_kernel<<<1, 1024, 0, stream>>>(mask, N * T, C, count);
+  if (mask && N * T > COUNT_LIMIT) count_kernel<<<1, 1024, 0, stream>>>(mask, a.rows, C, count);
   int blocks = 0, rc;
   if (type == 0) rc = forward<__nv_bfloat16, LOSS_POLICY>(a, count, logp, lse, slope, dlogits, partial, nullptr, &blocks, stream);
   else if (type == 1) rc = forward<__half, LOSS_POLICY>(a, count, logp, lse, slope, dlogits, partial, nullptr, &blocks, stream);
@@ -577,10 +622,13 @@ SB_API int sb_preference_loss_fwd(const void* logits, int type, long long sn, lo
   else if (type == 2) rc = forward<float, LOSS_PREFERENCE>(a, nullptr, nullptr, lse, nullptr, nullptr, nullptr, ratio, &blocks, stream);
   else return SB_BAD_ARGUMENT;
   if (rc) return rc;
-  ratio_kernel<<<(int)N, 256, 0, stream>>>(ratio, (long long)T * C, total);
-  rc = (int)cudaGetLastError();
-  if (rc) return rc;
-  preference_finish_kernel<<<1, 256, 0, stream>>>(total, (int)(N / 2), kind, beta, gap, loss, rewards, seq_slope);
+  const bool one = a.rows <= ONE_BLOCK_ROWS;
+  if (!one) {
+    ratio_kernel<<<(int)N, 256, 0, stream>>>(ratio, (long long)T * C, total);
+    rc = (int)cudaGetLastError();
+    if (rc) return rc;
+  }
+  preference_finish_kernel<<<1, one ? 1024 : 256, 0, stream>>>(one ? ratio : nullptr, (long long)T * C, total, (int)(N / 2), kind, beta, gap, loss, rewards, seq_slope);
   return (int)cudaGetLastError();
 }
 

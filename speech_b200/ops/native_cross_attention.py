@@ -7,10 +7,9 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import native as N
-from .native_sequence_loss import address, bind, current_stream, on_device
+from .native_sequence_loss import address, bind, current_stream, first_derivative, on_device
 
 _SIGNATURES = {                      # p: pointer; the stream is the last one
     "sb_cross_attention_fwd": "pppppp",
@@ -73,44 +72,53 @@ def _scratch(nbytes: int, what: str, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes // 4, dtype=torch.float32, device=device) if nbytes else None
 
 
-def _forward(q, k, v, lengths, mask, scale, want_lse):
+def _forward(q, k, v, lengths, mask, scale, for_backward):
+    """The output and, for a backward pass, one buffer: what rounding took from the output (16 bits), then lse."""
     B, Tq, H, D = q.shape
     g = _block(q, k, v, lengths, mask, scale)
     p = ctypes.byref(g)
     out = torch.empty((B, Tq, H * D), dtype=q.dtype, device=q.device)
-    rest = torch.empty_like(out) if want_lse else None          # what rounding took from the output: the backward pass sums both
-    lse = torch.empty(B * Tq * H, dtype=torch.float32, device=q.device) if want_lse else None
+    kept, rest, lse = None, 0, 0
+    if for_backward:
+        rows = B * Tq * H
+        kept = torch.empty(rows * (D // 2 + 1), dtype=torch.float32, device=q.device)
+        rest = kept.data_ptr()
+        lse = rest + rows * D * 2
     ws = _scratch(_call("sb_cross_attention_workspace")(p), "sb_cross_attention_workspace", q.device)
-    N._check(_call("sb_cross_attention_fwd")(p, out.data_ptr(), address(rest), address(lse), address(ws), current_stream()), "sb_cross_attention_fwd")
-    return out, rest, lse
+    N._check(_call("sb_cross_attention_fwd")(p, out.data_ptr(), rest, lse, address(ws), current_stream()), "sb_cross_attention_fwd")
+    return out, kept
+
+
+def _backward(ctx, dout):
+    q, k, v, out, lengths, mask = ctx.saved_tensors
+    kept = ctx.kept
+    if not dout.is_contiguous() or dout.data_ptr() & 15:
+        dout = dout.clone(memory_format=torch.contiguous_format)
+    want_q, want_k, want_v = ctx.needs_input_grad[:3]
+    B, Tq, H, D = q.shape
+    with on_device(q):
+        ws = torch.empty(2 * B * H * ((Tq + 63) // 64 * 64) + _PEAKS, dtype=torch.float32, device=q.device)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_q else None
+        dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_k or want_v else None
+        dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if want_k or want_v else None
+        g = _block(q, k, v, lengths, mask, ctx.scale)
+        rest = kept.data_ptr()
+        N._check(_call("sb_cross_attention_bwd")(ctypes.byref(g), out.data_ptr(), rest, dout.data_ptr(), rest + B * Tq * H * D * 2, ws.data_ptr(),
+                                                 address(dq), address(dk), address(dv), current_stream()), "sb_cross_attention_bwd")
+    return dq, dk if want_k else None, dv if want_v else None, None, None, None
 
 
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask, scale):
-        out, rest, lse = _forward(q, k, v, lengths, mask, scale, True)
+        out, ctx.kept = _forward(q, k, v, lengths, mask, scale, True)
         ctx.save_for_backward(q, k, v, out, lengths, mask)
-        ctx.kept, ctx.scale = (rest, lse), scale
+        ctx.scale = scale
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lengths, mask = ctx.saved_tensors
-        if not dout.is_contiguous() or dout.data_ptr() & 15:
-            dout = dout.clone(memory_format=torch.contiguous_format)
-        rest, lse = ctx.kept
-        want_q, want_kv = ctx.needs_input_grad[0], ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        with on_device(q):
-            B, Tq, H, _ = q.shape
-            ws = torch.empty(2 * B * H * ((Tq + 63) // 64 * 64) + _PEAKS, dtype=torch.float32, device=q.device)
-            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_q else None
-            dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_kv else None
-            dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if want_kv else None
-            g = _block(q, k, v, lengths, mask, ctx.scale)
-            N._check(_call("sb_cross_attention_bwd")(ctypes.byref(g), out.data_ptr(), rest.data_ptr(), dout.data_ptr(), lse.data_ptr(), ws.data_ptr(), address(dq),
-                                                     address(dk), address(dv), current_stream()), "sb_cross_attention_bwd")
-        return dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None
+        return first_derivative(_backward, ctx, dout)
 
 
 def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):

@@ -43,6 +43,13 @@ def on_device(t: torch.Tensor):
     return contextlib.nullcontext() if index == current else torch.cuda.device(index)
 
 
+def first_derivative(f, ctx, *grads):
+    """Runs a backward pass that cannot be differentiated itself: under ``create_graph`` its results raise when that is tried."""
+    if torch.is_grad_enabled():
+        return once_differentiable(f)(ctx, *grads)
+    return f(ctx, *grads)
+
+
 def address(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -79,12 +86,23 @@ def _blocks() -> int:
 
 
 def _gradient(upstream, logits, targets, mask, lse, slope, seq_slope, out, unless_one):
+    """``lse``, ``slope``, ``seq_slope``: addresses."""
     layout, sizes = _layout(logits)
     g = _plain(upstream, torch.float32)
     with on_device(logits):
-        N._check(bind("sb_sequence_loss_bwd")(address(logits), *layout, address(targets), address(mask), *sizes, address(lse), address(slope),
-                                              address(seq_slope), address(g), unless_one, address(out), current_stream()), "sb_sequence_loss_bwd")
+        N._check(bind("sb_sequence_loss_bwd")(logits.data_ptr(), *layout, targets.data_ptr(), address(mask), *sizes, lse, slope, seq_slope, g.data_ptr(),
+                                              unless_one, out.data_ptr(), current_stream()), "sb_sequence_loss_bwd")
     return out
+
+
+def _policy_backward(ctx, dloss, _):
+    logits, targets, mask = ctx.saved_tensors
+    out, ctx.grad = ctx.grad, None
+    first = out is not None
+    if not first:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    lse = ctx.kept.data_ptr() + 8 * _blocks() + 8
+    return _gradient(dloss, logits, targets, mask, lse, lse + 4 * targets.numel(), 0, out, int(first)), None, None, None, None, None, None, None, None, None
 
 
 class _PolicyLossFn(torch.autograd.Function):
@@ -96,30 +114,32 @@ class _PolicyLossFn(torch.autograd.Function):
         dev, rows = logits.device, targets.numel()
         loss = torch.empty((), dtype=torch.float32, device=dev)
         logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-        lse = torch.empty(rows, dtype=torch.float32, device=dev)
-        slope = torch.empty(rows, dtype=torch.float32, device=dev)
-        ws = torch.empty(_blocks() + 1, dtype=torch.float64, device=dev)          # sums of the blocks, and the count
+        kept = torch.empty(2 * _blocks() + 2 + 2 * rows, dtype=torch.float32, device=dev)       # fp64 sums of the blocks and the count, lse, slopes
+        ws = kept.data_ptr()
+        lse = ws + 8 * _blocks() + 8
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
         layout, sizes = _layout(logits)
-        N._check(bind("sb_policy_loss_fwd")(address(logits), *layout, address(targets), address(mask), address(old), address(ref), address(adv), *sizes,
-                                            lo, hi, kl_beta, ws.data_ptr() + 8 * _blocks(), ws.data_ptr(), loss.data_ptr(), logp.data_ptr(),
-                                            lse.data_ptr(), slope.data_ptr(), address(grad), current_stream()), "sb_policy_loss_fwd")
+        N._check(bind("sb_policy_loss_fwd")(logits.data_ptr(), *layout, targets.data_ptr(), address(mask), old.data_ptr(), address(ref), adv.data_ptr(), *sizes,
+                                            lo, hi, kl_beta, ws + 8 * _blocks(), ws, loss.data_ptr(), logp.data_ptr(), lse, lse + 4 * rows, address(grad),
+                                            current_stream()), "sb_policy_loss_fwd")
         if want_grad:
             ctx.save_for_backward(logits, targets, mask)
-            ctx.kept = lse, slope
+            ctx.kept = kept
             ctx.grad = grad
         ctx.mark_non_differentiable(logp)
         return loss, logp
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss, _):
-        logits, targets, mask = ctx.saved_tensors
-        out, ctx.grad = ctx.grad, None
-        first = out is not None
-        if not first:
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        return _gradient(dloss, logits, targets, mask, *ctx.kept, None, out, int(first)), None, None, None, None, None, None, None, None, None
+    def backward(ctx, dloss, dlogp):
+        return first_derivative(_policy_backward, ctx, dloss, dlogp)
+
+
+def _preference_backward(ctx, dloss, _):
+    logits, targets, mask = ctx.saved_tensors
+    rows = targets.numel()
+    slope = ctx.kept.data_ptr() + 8 * (rows + logits.shape[0])
+    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    return _gradient(dloss, logits, targets, mask, slope + 4 * logits.shape[0], 0, slope, out, 0), None, None, None, None, None, None
 
 
 class _PreferenceLossFn(torch.autograd.Function):
@@ -128,25 +148,21 @@ class _PreferenceLossFn(torch.autograd.Function):
         dev, rows, n = logits.device, targets.numel(), logits.shape[0]
         loss = torch.empty((), dtype=torch.float32, device=dev)
         rewards = torch.empty(n, dtype=torch.float32, device=dev)
-        seq_slope = torch.empty(n, dtype=torch.float32, device=dev)
-        lse = torch.empty(rows, dtype=torch.float32, device=dev)
-        ws = torch.empty(rows + n, dtype=torch.float64, device=dev)               # log ratios of the positions and of the sequences
+        # log ratios of the positions and of the sequences (fp64), slopes of the sequences, lse (fp32)
+        ctx.kept = torch.empty(3 * (rows + n), dtype=torch.float32, device=dev)
+        ws = ctx.kept.data_ptr()
+        slope = ws + 8 * (rows + n)
         layout, sizes = _layout(logits)
-        N._check(bind("sb_preference_loss_fwd")(address(logits), *layout, address(targets), address(mask), address(ref), *sizes, kind, beta, address(gap),
-                                                ws.data_ptr(), ws.data_ptr() + 8 * rows, loss.data_ptr(), rewards.data_ptr(), seq_slope.data_ptr(),
-                                                lse.data_ptr(), current_stream()), "sb_preference_loss_fwd")
+        N._check(bind("sb_preference_loss_fwd")(logits.data_ptr(), *layout, targets.data_ptr(), address(mask), ref.data_ptr(), *sizes, kind, beta, address(gap),
+                                                ws, ws + 8 * rows, loss.data_ptr(), rewards.data_ptr(), slope, slope + 4 * n, current_stream()),
+                 "sb_preference_loss_fwd")
         ctx.save_for_backward(logits, targets, mask)
-        ctx.kept = lse, seq_slope
         ctx.mark_non_differentiable(rewards)
         return loss, rewards
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dloss, _):
-        logits, targets, mask = ctx.saved_tensors
-        lse, seq_slope = ctx.kept
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        return _gradient(dloss, logits, targets, mask, lse, None, seq_slope, out, 0), None, None, None, None, None, None
+    def backward(ctx, dloss, drewards):
+        return first_derivative(_preference_backward, ctx, dloss, drewards)
 
 
 def policy_loss(logits, targets, mask, old_logp, advantages, ref_logp=None, clip=0.2, clip_high=None, kl_beta=0.0):
