@@ -216,12 +216,12 @@ __device__ __forceinline__ int visible_keys(const XAttnArgs& a, int m) {
   return n < 0 ? 0 : (n > a.Tk ? a.Tk : n);
 }
 
-// Bit i of the result: key first + i of memory m is hidden.  One word per call, the same in every lane.
+// Whether key `key` of memory m is hidden; and which of 32 keys from `first` on are, bit by bit, the same in every lane.
+__device__ __forceinline__ bool hidden_key(const XAttnArgs& a, int m, int len, int key) {
+  return key >= len || (a.mask && a.mask[(long long)m * a.Tk + key] != 0);
+}
 __device__ __forceinline__ uint32_t hidden_word(const XAttnArgs& a, int m, int len, int first, int lane) {
-  const int key = first + lane;
-  bool hide = key >= len;
-  if (a.mask && !hide) hide = a.mask[(long long)m * a.Tk + key] != 0;
-  return __ballot_sync(0xffffffffu, hide);
+  return __ballot_sync(0xffffffffu, hidden_key(a, m, len, first + lane));
 }
 
 // Rows of a [rows, DP] operand tile in shared memory: 64-element halves of 128-byte rows, 16-byte chunks XORed with the row (the

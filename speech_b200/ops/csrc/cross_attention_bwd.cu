@@ -13,8 +13,8 @@
 // for registers at once, so that those of the next block are computed under this one's exponentials; q and do are A operands in tensor
 // memory, because a product of 128 x 64 x 16 that reads 6 KB from shared memory takes 60 cycles, not 32.  dk / dv: tiles of 64 query rows of one head,
 // transposed (lanes are keys), so that p^T and ds^T are A operands as they come out of the softmax; two pairs of warpgroups take them in
-// turn, half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which a row kernel
-// lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
+// turn, half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which the dq kernel,
+// which comes first and computes delta as it loads do, lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
 //
 // Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
 // matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do| of the call to [8, 16), and
@@ -25,8 +25,6 @@
 namespace {
 
 constexpr int DKV_THREADS = 640;       // 20 warps of 96 registers
-constexpr int MAX_PARTS = 592;        // blocks of the row kernel, whose maxima every block of the other kernels joins
-
 template <typename T> constexpr float p_shift() { return Half2<T>::KIND == 0 ? 12.f : 0.f; }
 
 struct BwdArgs {
@@ -35,64 +33,47 @@ struct BwdArgs {
   const float* lse;                   // [M * Hk, R]
   float *nlse, *ndelta;               // [M * Hk, G * rep, Tqp]: -lse (-inf behind the last row, too) and -delta (0 there)
   int Tqp;                            // Tq rounded up to 64
-  float* peak;                        // fp16: largest |do| of every block of the row kernel
-  int peaks;
+  float* peak;                        // fp16: largest |do| of every block of the dq kernel
+  int tiles;                          // its blocks of a (memory, key head)
   float scale;
 };
 
-// -lse and -delta of every row, and the largest |do|.  Sixteen lanes per row of up to 128 elements.
-template <typename T>
-__global__ void __launch_bounds__(256) xattn_delta_kernel(const XAttnArgs a, const BwdArgs b) {
-  __shared__ float red[8];
-  const int segs = a.G * a.rep;
-  const long long rows = (long long)a.M * a.Hk * segs * b.Tqp;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int sub = lane >> 4, ch = lane & 15;
-  float peak = 0.f;
-  for (long long i0 = ((long long)blockIdx.x * 8 + warp) * 2; i0 < rows; i0 += (long long)gridDim.x * 16) {
-    const long long i = i0 + sub;
-    const int line = (int)(i / b.Tqp), t = (int)(i - (long long)line * b.Tqp);
-    const int unit = line / segs, seg = line - unit * segs;
-    const bool in = i < rows && t < a.Tq;
-    float d = 0.f;
-    if (in && ch * 8 < a.D) {
-      const int g = seg / a.rep, m = unit / a.Hk;
-      const long long off = (((long long)(m * a.G + g) * a.Tq + t) * a.H + (unit - m * a.Hk) * a.rep + seg - g * a.rep) * a.D + ch * 8;
-      const uint4 x = *reinterpret_cast<const uint4*>(b.dout + off), y = *reinterpret_cast<const uint4*>(b.out + off), z = *reinterpret_cast<const uint4*>(b.rest + off);
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = Half2<T>::unpack(xs[k]), e = Half2<T>::unpack(ys[k]), c = Half2<T>::unpack(zs[k]);
-        d += f.x * (e.x + c.x) + f.y * (e.y + c.y);
-        if (Half2<T>::KIND == 0) peak = fmaxf(peak, fmaxf(fabsf(f.x), fabsf(f.y)));
-      }
-    }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (i < rows && ch == 0) {
-      b.ndelta[i] = -d;
-      b.nlse[i] = in ? -b.lse[(long long)unit * a.R + seg * a.Tq + t] : -INFINITY;
-    }
-  }
-  if (Half2<T>::KIND == 0) {
-    peak = warp_max(peak);
-    if (lane == 0) red[warp] = peak;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int w = 1; w < 8; ++w) peak = fmaxf(peak, red[w]);
-      b.peak[blockIdx.x] = peak;
-    }
-  }
+// Power of two that brings the largest |do| of a (memory, key head) to [8, 16); 1 for bf16, whose range needs none.
+template <typename T> __device__ __forceinline__ float ds_scale(float peak) {
+  if (Half2<T>::KIND != 0 || !(peak > 0.f) || !(peak < 3e38f)) return 1.f;
+  return __int_as_float((127 + 3 - ((__float_as_int(peak) >> 23) - 127)) << 23);   // |do| of fp16 lies between 2^-24 and 2^16
 }
 
-// Power of two that brings the largest |do| to [8, 16); 1 for bf16, whose range needs none.  One warp.
-template <typename T> __device__ __forceinline__ float ds_scale(const BwdArgs& b, int lane) {
-  if (Half2<T>::KIND != 0) return 1.f;
-  float peak = 0.f;
-  for (int i = lane; i < b.peaks; i += 32) peak = fmaxf(peak, b.peak[i]);
-  peak = warp_max(peak);
-  if (!(peak > 0.f) || !(peak < 3e38f)) return 1.f;
-  return __int_as_float((127 + 3 - ((__float_as_int(peak) >> 23) - 127)) << 23);   // |do| of fp16 lies between 2^-24 and 2^16
+// A warp's 32 rows of do into a swizzled tile (as load_rows), with sum(do * (out + rest)) of this lane's row and the largest |do| of all.
+template <typename T, int DP>
+__device__ __forceinline__ void load_do_rows(const BwdArgs& b, long long off, int D, uint32_t tile, int quarter, int lane, float& delta, float& peak) {
+  constexpr int CH = DP / 8, RPI = 32 / CH;
+  const int sub = lane / CH, ch = lane % CH;
+  delta = peak = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < 32; i += RPI) {
+    const long long o = __shfl_sync(0xffffffffu, off, i + sub);
+    uint4 x = make_uint4(0, 0, 0, 0), y = x, z = x;
+    if (o >= 0 && ch * 8 < D) {
+      x = *reinterpret_cast<const uint4*>(b.dout + o + ch * 8);
+      y = *reinterpret_cast<const uint4*>(b.out + o + ch * 8);
+      z = *reinterpret_cast<const uint4*>(b.rest + o + ch * 8);
+    }
+    st_shared_v4(tile_addr(tile, 128, quarter * 32 + i + sub, ch), x.x, x.y, x.z, x.w);
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
+    float d = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = Half2<T>::unpack(xs[k]), e = Half2<T>::unpack(ys[k]), c = Half2<T>::unpack(zs[k]);
+      d += f.x * (e.x + c.x) + f.y * (e.y + c.y);
+      if (Half2<T>::KIND == 0) peak = fmaxf(peak, fmaxf(fabsf(f.x), fabsf(f.y)));
+    }
+#pragma unroll
+    for (int s = CH / 2; s > 0; s >>= 1) d += __shfl_xor_sync(0xffffffffu, d, s);
+    const float mine = __shfl_sync(0xffffffffu, d, ((lane - i) & (RPI - 1)) * CH);
+    if (lane >= i && lane < i + RPI) delta = mine;
+  }
+  if (Half2<T>::KIND == 0) peak = warp_max(peak);
 }
 
 template <typename T> __device__ __forceinline__ uint32_t pack_ds(float x, float y) {
@@ -124,7 +105,7 @@ template <int DP> struct DqSmem {
   static constexpr int STAGES = 5;
   static constexpr int ROWS = 128 * DP * 2, KEYS = BN * DP * 2;
   static constexpr int DO0 = ROWS, KV0 = 2 * ROWS, BAR = KV0 + STAGES * 2 * KEYS;
-  static constexpr int BYTES = BAR + 256 + 1024;
+  static constexpr int BYTES = BAR + 192 + 132 * 4 + 1024;
   // tensor memory: dq, q, do, scores of even and odd blocks, dp, ds of even and odd blocks
   static constexpr int Q_COL = DP, DO_COL = DP + DP / 2, S_COL = 2 * DP, DP_COL = S_COL + 128, DS_COL = DP_COL + 64;
 };
@@ -146,13 +127,14 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   auto ds_full = [&](int u) { return bars + 8u * (14 + u); };
   auto ds_read = [&](int u) { return bars + 8u * (16 + u); };
   auto dp_full = [&](int u) { return bars + 8u * (18 + u); };     // one per warpgroup: each sees every other block only
-  const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, scale_slot = tmem_slot + 4;
+  const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, stats = bars + 8u * 24;      // stats: -delta of the tile's rows, largest |do| of four warps
 
-  const int tiles = (a.R + 127) / 128;
+  const int tiles = b.tiles;
   const int unit = blockIdx.x / tiles, m = unit / a.Hk, hk = unit % a.Hk;
   const int row0 = (blockIdx.x - unit * tiles) * 128;
   const int len = visible_keys(a, m);
-  const int nt = (len + BN - 1) / BN;
+  const int blocks = (len + BN - 1) / BN;
+  const int nt = dq || blocks == 1 ? blocks : 0;            // without dq only the statistics are wanted, for which one block refines delta
   const bool hide = a.mask != nullptr;
 
   if (threadIdx.x == 0) {
@@ -167,10 +149,6 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tmem_slot) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  if (warp == 3) {
-    const float f = ds_scale<T>(b, lane);
-    if (lane == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale_slot), "f"(f) : "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -251,20 +229,33 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     const int wg = (warp - 4) >> 2, quarter = warp & 3;
     const int row = row0 + quarter * 32 + lane;
     const bool valid = row < a.R;
-    float dsf;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
-    const long long stat = valid ? ((long long)unit * (a.G * a.rep) + row / a.Tq) * b.Tqp + row % a.Tq : 0;
-    const float nlse = valid ? b.nlse[stat] : -INFINITY;
-    float ndelta = valid ? b.ndelta[stat] : 0.f;
+    const int line = row / a.Tq, t = row - line * a.Tq;
+    const long long stat = valid ? ((long long)unit * (a.G * a.rep) + line) * b.Tqp + t : 0;
+    const float nlse = valid ? -b.lse[(long long)unit * a.R + row] : -INFINITY;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_addr = lane_base + S::S_COL + wg * 64, dp_addr = lane_base + S::DP_COL, ds_addr = lane_base + S::DS_COL + wg * 32;
     bool ok = true;
+    // q by the first, do (and with it delta) by the second, through shared memory into tensor memory
+    const uint32_t tile = base + wg * S::DO0, stat_row = stats + (uint32_t)(quarter * 32 + lane) * 4u;
+    const long long st = (long long)a.H * a.D;
+    if (wg == 0) {
+      load_rows<DP>(a.q, row_offset(a, a.q_sb, a.q_st, a.q_sh, m, hk, row), a.D, tile, quarter, lane);
+    } else {
+      float delta, peak;
+      load_do_rows<T, DP>(b, row_offset(a, st * a.Tq, st, a.D, m, hk, row), a.D, tile, quarter, lane, delta, peak);
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(stat_row), "f"(-delta) : "memory");
+      if (lane == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(stats + (128 + quarter) * 4), "f"(peak) : "memory");
+      if (valid) {
+        b.nlse[stat] = nlse;
+        if (nt != 1) b.ndelta[stat] = -delta;
+        if (t == a.Tq - 1)                                   // the line's end, which the copies of the dk / dv kernel read
+          for (int x = 1; x < b.Tqp - t; ++x) {
+            b.nlse[stat + x] = -INFINITY;
+            b.ndelta[stat + x] = 0.f;
+          }
+      }
+    }
     if (nt > 0) {
-      // q by the first, do by the second, through shared memory into tensor memory
-      const uint32_t tile = base + wg * S::DO0;
-      const long long st = (long long)a.H * a.D;
-      const long long off = wg ? row_offset(a, st * a.Tq, st, a.D, m, hk, row) : row_offset(a, a.q_sb, a.q_st, a.q_sh, m, hk, row);
-      load_rows<DP>(wg ? (const void*)b.dout : a.q, off, a.D, tile, quarter, lane);
       __syncwarp();
       row_to_tmem<DP>(tile, quarter * 32 + lane, lane_base + (wg ? S::DO_COL : S::Q_COL));
       tmem_store_wait();
@@ -272,14 +263,26 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       __syncwarp();
       if (lane == 0) mbar_arrive(rows_ready);
     }
+    asm volatile("bar.sync 1, 256;" ::: "memory");           // both warpgroups: the statistics in shared memory
+    float ndelta, p4[4];
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ndelta) : "r"(stat_row) : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(p4[i]) : "r"(stats + (128 + i) * 4) : "memory");
+    const float peak = fmaxf(fmaxf(p4[0], p4[1]), fmaxf(p4[2], p4[3])), dsf = ds_scale<T>(peak);
+    if (Half2<T>::KIND == 0 && warp == 4 && lane == 0) b.peak[blockIdx.x] = peak;
     const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse), f2 = pair(dsf, dsf);
     uint32_t ph = 0;
+    bool hid[2] = {hidden_key(a, m, len, wg * BN + lane), hidden_key(a, m, len, wg * BN + 32 + lane)};      // of block j, read a turn ahead
     for (int j = wg; j < nt; j += 2) {
       const bool some_hidden = hide || (j + 1) * BN > len;
       uint32_t w[2] = {0, 0};
       if (some_hidden) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
+        for (int i = 0; i < 2; ++i) w[i] = __ballot_sync(0xffffffffu, hid[i]);
+      }
+      if (hide || (j + 3) * BN > len) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, (j + 2) * BN + 32 * i + lane);
       }
       uint32_t r[64], g[64];
       ok = warp_wait(s_full(wg), ph, a.status, SB_TIMEOUT_TMEM_FULL);
@@ -416,7 +419,10 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (warp == 2) {
-    const float f = ds_scale<T>(b, lane);
+    float peak = 0.f;
+    if (Half2<T>::KIND == 0)
+      for (int i = lane; i < b.tiles; i += 32) peak = fmaxf(peak, b.peak[(long long)unit * b.tiles + i]);
+    const float f = ds_scale<T>(warp_max(peak));
     if (lane == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(scale_slot), "f"(f) : "memory");
   }
   tc_fence_before();
@@ -623,16 +629,11 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   if (!rc) rc = sb_allow_smem((const void*)xattn_dq_kernel<T, DP>, DqSmem<DP>::BYTES);
   if (!rc) rc = sb_allow_smem((const void*)xattn_dkv_kernel<T, DP>, DkvSmem<DP>::BYTES);
   if (rc) return rc;
-  const long long units = (long long)a.M * a.Hk, gq = units * ((a.R + 127) / 128), gk = units * ((a.Tk + 127) / 128);
+  b.tiles = (a.R + 127) / 128;
+  const long long units = (long long)a.M * a.Hk, gq = units * b.tiles, gk = units * ((a.Tk + 127) / 128);
   if (gq > 0x7fffffffll || gk > 0x7fffffffll) return SB_BAD_ARGUMENT;
-  const long long blocks = (units * a.G * a.rep * b.Tqp + 15) / 16;
-  b.peaks = (int)(blocks < MAX_PARTS ? blocks : MAX_PARTS);
-  xattn_delta_kernel<T><<<b.peaks, 256, 0, stream>>>(a, b);
+  xattn_dq_kernel<T, DP><<<(unsigned)gq, DQ_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);      // also lays out the statistics
   rc = (int)cudaGetLastError();
-  if (!rc && (dq || a.Tk <= DqSmem<DP>::BN)) {                // for up to 64 keys it also refines delta, whichever gradients are wanted
-    xattn_dq_kernel<T, DP><<<(unsigned)gq, DQ_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);
-    rc = (int)cudaGetLastError();
-  }
   if (!rc && dk) {
     xattn_dkv_kernel<T, DP><<<(unsigned)gk, DKV_THREADS, DkvSmem<DP>::BYTES, stream>>>(k64, v64, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv);
     rc = (int)cudaGetLastError();
@@ -642,7 +643,8 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
 
 }  // namespace
 
-// out, rest, dout: contiguous [B, Tq, H, D]; out, rest, lse: the forward pass's; ws: 2 * B * H * (Tq rounded up to 64) + 592 floats; dq [B, Tq, H, D] or null; dk, dv
+// out, rest, dout: contiguous [B, Tq, H, D]; out, rest, lse: the forward pass's; ws: 2 * B * H * (Tq rounded up to 64) floats and
+// one per 128 packed rows of every (memory, key head); dq [B, Tq, H, D] or null; dk, dv
 // [M, Tk, Hk, D], both or neither.
 SB_API int sb_cross_attention_bwd(const SbCrossAttention* g, const void* out, const void* rest, const void* dout, const float* lse, float* ws, void* dq, void* dk, void* dv,
                                   cudaStream_t stream) {

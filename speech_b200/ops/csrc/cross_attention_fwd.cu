@@ -189,13 +189,18 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
+    bool hid[2] = {hidden_key(a, m, len, lane), hidden_key(a, m, len, 32 + lane)};      // this lane's keys of block j, read a block ahead
     for (int j = 0; j < nt; ++j) {
       const bool some_hidden = hide || (j + 1) * BN > len;
       const uint32_t s_addr = lane_base + t * 128 + (j & 1) * 64;
       uint32_t w[2] = {0, 0};
       if (some_hidden) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
+        for (int i = 0; i < 2; ++i) w[i] = __ballot_sync(0xffffffffu, hid[i]);
+      }
+      if (hide || (j + 2) * BN > len) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, (j + 1) * BN + 32 * i + lane);
       }
       ok = warp_wait(s_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;

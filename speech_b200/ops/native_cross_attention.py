@@ -18,7 +18,6 @@ _SIGNATURES = {                      # p: pointer; the stream is the last one
     "sb_shared_prefix_workspace": "pp",
     "sb_shared_prefix_attention": "ppppp",
 }
-_PEAKS = 592                         # floats of the backward pass's workspace behind the row sums
 
 
 class SbCrossAttention(ctypes.Structure):
@@ -97,7 +96,10 @@ def _backward(ctx, dout):
     want_q, want_k, want_v = ctx.needs_input_grad[:3]
     B, Tq, H, D = q.shape
     with on_device(q):
-        ws = torch.empty(2 * B * H * ((Tq + 63) // 64 * 64) + _PEAKS, dtype=torch.float32, device=q.device)
+        M, Hk = k.shape[0], k.shape[2]
+        units = M * Hk
+        # statistics in lines of a multiple of 64, and a maximum per 128 rows that read the same keys
+        ws = torch.empty(2 * B * H * ((Tq + 63) // 64 * 64) + units * ((B * H * Tq // units + 127) // 128), dtype=torch.float32, device=q.device)
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if want_q else None
         dk = torch.empty(k.shape, dtype=k.dtype, device=k.device) if want_k or want_v else None
         dv = torch.empty(v.shape, dtype=v.dtype, device=v.device) if want_k or want_v else None
