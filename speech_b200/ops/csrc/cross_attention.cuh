@@ -295,13 +295,34 @@ __device__ __forceinline__ void store_rows64(uint32_t buf, const uint32_t* packe
   __syncwarp();
 }
 
-// Zeroes the rows of a [64, DP] tile whose keys are hidden (bits of words[0..1]): a hidden value of infinity or NaN would turn its zero
-// weight into NaN inside the matrix product.  `threads` threads with numbers `id` share the work.
-template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, int rows, const uint32_t* words, int id, int threads) {
-  constexpr int CH = DP / 8;
-  for (int i = id; i < rows * CH; i += threads) {
-    const int row = i / CH;
-    if (((row < 32 ? words[0] : words[1]) >> (row & 31)) & 1u) st_shared_v4(tile_addr(tile, rows, row, i % CH), 0, 0, 0, 0);
+// A warp zeroes the hidden rows (bits of w[0], w[1]) of a [64, DP] tile: a hidden infinity or NaN would turn its zero weight into NaN
+// inside a matrix product.  (A loop over the set bits would find them with the unit that the exponentials keep busy.)
+template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, const uint32_t* w, int lane) {
+  constexpr int CH = DP / 8, RPI = 32 / CH;
+  const int sub = lane / CH, ch = lane % CH;
+#pragma unroll 4
+  for (int row = sub; row < 64; row += RPI)
+    if (((row < 32 ? w[0] : w[1]) >> (row & 31)) & 1u) st_shared_v4(tile_addr(tile, 64, row, ch), 0, 0, 0, 0);
+}
+
+// What is added to the scores of a block's 64 keys: 0, or -inf where hidden.  In shared memory, for all rows.
+__device__ __forceinline__ void store_score_mask(uint32_t addr, const uint32_t* w, int lane) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr + (uint32_t)(h * 32 + lane) * 4u), "f"((w[h] >> lane) & 1u ? -INFINITY : 0.f) : "memory");
+}
+__device__ __forceinline__ void add_score_mask(uint32_t addr, uint32_t* r) {
+#pragma unroll
+  for (int k = 0; k < 64; k += 4) {
+    uint64_t lo, hi;
+    float x, y;
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(addr + k * 4));
+    split(add2(pair(r[k], r[k + 1]), lo), x, y);
+    r[k] = __float_as_uint(x);
+    r[k + 1] = __float_as_uint(y);
+    split(add2(pair(r[k + 2], r[k + 3]), hi), x, y);
+    r[k + 2] = __float_as_uint(x);
+    r[k + 3] = __float_as_uint(y);
   }
 }
 

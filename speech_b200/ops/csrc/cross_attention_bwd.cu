@@ -78,8 +78,9 @@ __device__ __forceinline__ void load_do_rows(const BwdArgs& b, long long off, in
 
 template <typename T> __device__ __forceinline__ uint32_t pack_ds(float x, float y) {
   if (Half2<T>::KIND == 0) {                               // beyond the type's range only for values far above any activation: saturate
-    x = fminf(fmaxf(x, -65504.f), 65504.f);
-    y = fminf(fmaxf(y, -65504.f), 65504.f);
+    uint32_t v;
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(y), "f"(x));
+    return v;
   }
   return Half2<T>::pack(x, y);
 }
@@ -105,7 +106,7 @@ template <int DP> struct DqSmem {
   static constexpr int STAGES = 5;
   static constexpr int ROWS = 128 * DP * 2, KEYS = BN * DP * 2;
   static constexpr int DO0 = ROWS, KV0 = 2 * ROWS, BAR = KV0 + STAGES * 2 * KEYS;
-  static constexpr int BYTES = BAR + 192 + 132 * 4 + 1024;
+  static constexpr int MASK0 = BAR + 768, BYTES = MASK0 + STAGES * BN * 4 + 1024;
   // tensor memory: dq, q, do, scores of even and odd blocks, dp, ds of even and odd blocks
   static constexpr int Q_COL = DP, DO_COL = DP + DP / 2, S_COL = 2 * DP, DP_COL = S_COL + 128, DS_COL = DP_COL + 64;
 };
@@ -127,7 +128,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   auto ds_full = [&](int u) { return bars + 8u * (14 + u); };
   auto ds_read = [&](int u) { return bars + 8u * (16 + u); };
   auto dp_full = [&](int u) { return bars + 8u * (18 + u); };     // one per warpgroup: each sees every other block only
-  const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, stats = bars + 8u * 24;      // stats: -delta of the tile's rows, largest |do| of four warps
+  auto kv_clean = [&](int s) { return bars + 8u * (24 + s); };
+  const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, stats = bars + 240u;      // stats: -delta of the tile's rows, largest |do| of four warps
 
   const int tiles = b.tiles;
   const int unit = blockIdx.x / tiles, m = unit / a.Hk, hk = unit % a.Hk;
@@ -138,7 +140,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const bool hide = a.mask != nullptr;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::STAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_empty(s), 1); }
+    for (int s = 0; s < S::STAGES; ++s) { mbar_init(kv_full(s), 1); mbar_init(kv_clean(s), 1); mbar_init(kv_empty(s), 1); }
     for (int u = 0; u < 2; ++u) { mbar_init(s_full(u), 1); mbar_init(s_read(u), 4); mbar_init(ds_full(u), 4); mbar_init(ds_read(u), 1); mbar_init(dp_full(u), 1); }
     mbar_init(dp_read, 4);
     mbar_init(dq_full, 1);
@@ -157,10 +159,11 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot) : "memory");
 
   if (warp == 0) {
-    int s = 0, issued = 0;
-    uint32_t ph = 0;
-    for (int j = 0; j < nt; ++j) {
-      if (!warp_wait(kv_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY)) break;
+    // loads, up to STAGES - 2 blocks ahead, so that clearing runs two blocks ahead of dq; hidden keys' rows are cleared as they land (their
+    // ds is zero, and zero times NaN is not)
+    auto load = [&](int j) {
+      const int s = j % S::STAGES;
+      if (!warp_wait(kv_empty(s), ((uint32_t)(j / S::STAGES) & 1u) ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY)) return false;
       if (elect_one()) {
         const uint32_t kb = base + S::KV0 + s * 2 * S::KEYS;
         mbar_expect_tx(kv_full(s), 2 * S::KEYS);
@@ -171,9 +174,38 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         }
       }
       __syncwarp();
-      issued = j + 1;
-      if (++s == S::STAGES) { s = 0; ph ^= 1u; }
+      return true;
+    };
+    int issued = 0;
+    bool ok = true;
+    for (; issued < nt && issued < S::STAGES - 2 && ok; ++issued) ok = load(issued);
+    bool hid[2] = {hidden_key(a, m, len, lane), hidden_key(a, m, len, 32 + lane)};      // this lane's keys of block j, read a block ahead
+    for (int j = 0; j < nt && ok; ++j) {
+      const int s = j % S::STAGES;
+      const bool some = hide || (j + 1) * BN > len;
+      uint32_t w[2] = {0, 0};
+      if (some) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i] = __ballot_sync(0xffffffffu, hid[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, (j + 1) * BN + 32 * i + lane);
+      ok = warp_wait(kv_full(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (!ok) break;
+      if (some) {
+        clear_rows<DP>(base + S::KV0 + s * 2 * S::KEYS, w, lane);
+        clear_rows<DP>(base + S::KV0 + s * 2 * S::KEYS + S::KEYS, w, lane);
+        store_score_mask(base + S::MASK0 + s * BN * 4, w, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(kv_clean(s));
+      if (issued < nt) {
+        ok = load(issued);
+        if (ok) ++issued;
+      }
     }
+    // no copy may be in flight when the block ends (none is, unless a wait gave up)
     for (int i = issued > S::STAGES ? issued - S::STAGES : 0; i < issued; ++i)
       warp_wait(kv_full(i % S::STAGES), (uint32_t)(i / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
   } else if (warp == 1 || warp == 3) {
@@ -187,7 +219,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     int s = 0;
     uint32_t ph = 0;
     for (int j = 0; j < nt && ok; ++j) {
-      ok = warp_wait(kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL) &&
+      ok = warp_wait(hide || (j + 1) * BN > len ? kv_clean(s) : kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL) &&
            (second ? warp_wait(dp_read, ((uint32_t)j & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY)
                    : warp_wait(s_read(j & 1), ((uint32_t)(j >> 1) & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY));
       if (!ok) break;
@@ -272,18 +304,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     if (Half2<T>::KIND == 0 && warp == 4 && lane == 0) b.peak[blockIdx.x] = peak;
     const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse), f2 = pair(dsf, dsf);
     uint32_t ph = 0;
-    bool hid[2] = {hidden_key(a, m, len, wg * BN + lane), hidden_key(a, m, len, wg * BN + 32 + lane)};      // of block j, read a turn ahead
     for (int j = wg; j < nt; j += 2) {
-      const bool some_hidden = hide || (j + 1) * BN > len;
-      uint32_t w[2] = {0, 0};
-      if (some_hidden) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = __ballot_sync(0xffffffffu, hid[i]);
-      }
-      if (hide || (j + 3) * BN > len) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, (j + 2) * BN + 32 * i + lane);
-      }
       uint32_t r[64], g[64];
       ok = warp_wait(s_full(wg), ph, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
@@ -306,20 +327,17 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         if (!ok) break;
         tc_fence_after();
       }
+      if (hide || (j + 1) * BN > len) {
+        ok = warp_wait(kv_clean(j % S::STAGES), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+        if (!ok) break;
+        add_score_mask(base + S::MASK0 + (j % S::STAGES) * BN * 4, r);
+      }
 #pragma unroll
       for (int k = 0; k < 64; k += 2) {                    // p over s
         float x, y;
         split(fma2(pair(r[k], r[k + 1]), c2, nl2), x, y);
         r[k] = __float_as_uint(ex2(x));
         r[k + 1] = __float_as_uint(ex2(y));
-      }
-      if (some_hidden) {
-#pragma unroll
-        for (int k = 0; k < 64; ++k)
-          if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = g[k] = 0u;
-        // hidden key rows are cleared before dq sums over them: their ds is zero, and zero times NaN is not
-        clear_rows<DP>(base + S::KV0 + (j % S::STAGES) * 2 * S::KEYS, BN, w, quarter * 32 + lane, 128);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       if (nt == 1) {
         // all keys are in this block: delta = sum p dp from the values that it is subtracted from, instead of the rounded output

@@ -5,8 +5,8 @@
 // and lse = c m + log2 l is kept for the backward pass (+inf for a row that sees nothing: its probabilities are then 2^-inf = 0).
 //
 // A CTA takes two tiles of 128 packed rows and streams blocks of 64 keys of its memory and key head past both, so that keys and values
-// cross the L2 once per 256 rows.  Warp 0 loads keys and values by TMA, warp 1 issues all tcgen05.mma, warp 2 clears hidden value
-// rows, and one warpgroup per row tile does the softmax: scores and output accumulate in tensor memory (per tile two buffers of 64
+// cross the L2 once per 256 rows.  Warp 0 loads keys and values by TMA, warps 1 and 3 issue the tcgen05.mma of a tile each, warp 2
+// clears the rows of hidden keys and lays out what is added to their scores, and one warpgroup per row tile does the softmax: scores and output accumulate in tensor memory (per tile two buffers of 64
 // columns and DP columns), the probabilities go back there as 16-bit pairs over the scores they came from and are the A operand of
 // the second product.  The scores of the next block are there before the softmax of this one ends; with one buffer of 128 keys the
 // warpgroups waited for the tensor core and it for them (41 % of its cycles busy).  The output is rescaled only when a row's maximum
@@ -25,7 +25,7 @@ template <int DP> struct FwdSmem {
   static constexpr int STAGES = 4;
   static constexpr int TILE = 128 * DP * 2, KEYS = BN * DP * 2;      // 128 query rows, a block of keys or values
   static constexpr int K0 = 2 * TILE, V0 = K0 + STAGES * KEYS, BAR = V0 + STAGES * KEYS;
-  static constexpr int BYTES = BAR + 512 + 1024;
+  static constexpr int MASK0 = BAR + 512, BYTES = MASK0 + STAGES * BN * 4 + 1024;
 };
 
 template <typename T, int DP>
@@ -40,6 +40,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   auto k_full = [&](int s) { return bars + 8u * s; };
   auto k_empty = [&](int s) { return bars + 8u * (4 + s); };
+  auto k_clean = [&](int s) { return bars + 8u * (34 + s); };
   auto v_full = [&](int s) { return bars + 8u * (8 + s); };
   auto v_clean = [&](int s) { return bars + 8u * (12 + s); };
   auto v_empty = [&](int s) { return bars + 8u * (16 + s); };
@@ -59,7 +60,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
-      mbar_init(k_full(s), 1); mbar_init(k_empty(s), tiles);
+      mbar_init(k_full(s), 1); mbar_init(k_clean(s), 1); mbar_init(k_empty(s), tiles);
       mbar_init(v_full(s), 1); mbar_init(v_clean(s), 1); mbar_init(v_empty(s), tiles);
     }
     for (int t = 0; t < 2; ++t) {
@@ -132,14 +133,14 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     };
     bool ok = nt > 0 && warp_wait(q_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
     for (int j = 0; j < 2 && j < nt && ok; ++j) {
-      ok = warp_wait(k_full(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
+      ok = warp_wait(hide || (j + 1) * BN > len ? k_clean(j) : k_full(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
       if (!ok) break;
       tc_fence_after();
       scores(j);
     }
     for (int j = 0; j < nt && ok; ++j) {
       const int s = j % S::STAGES;
-      ok = warp_wait(v_clean(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL) &&
+      ok = warp_wait(hide || (j + 1) * BN > len ? v_clean(s) : v_full(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL) &&
            warp_wait(p_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
       tc_fence_after();
@@ -152,23 +153,37 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
       __syncwarp();
       if (j + 2 < nt) {
-        ok = warp_wait(k_full((j + 2) % S::STAGES), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+        ok = warp_wait(hide || (j + 3) * BN > len ? k_clean((j + 2) % S::STAGES) : k_full((j + 2) % S::STAGES), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
         scores(j + 2);
       }
     }
   } else if (warp == 2) {
-    // ---------------------------------------------------------------- hidden value rows
+    // ---------------------------------------------------------------- hidden keys: their rows cleared, their scores' addends
     int s = 0;
     uint32_t ph = 0;
+    bool hid[2] = {hidden_key(a, m, len, lane), hidden_key(a, m, len, 32 + lane)};      // this lane's keys of block j, read a block ahead
     for (int j = 0; j < nt; ++j) {
-      if (!warp_wait(v_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
-      if (hide || (j + 1) * BN > len) {
-        uint32_t w[2];
+      const bool some = hide || (j + 1) * BN > len;
+      uint32_t w[2] = {0, 0};
+      if (some) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = hidden_word(a, m, len, j * BN + 32 * i, lane);
-        clear_rows<DP>(base + S::V0 + s * S::KEYS, BN, w, lane, 32);
+        for (int i = 0; i < 2; ++i) w[i] = __ballot_sync(0xffffffffu, hid[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, (j + 1) * BN + 32 * i + lane);
+      if (!warp_wait(k_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
+      if (some) {
+        clear_rows<DP>(base + S::K0 + s * S::KEYS, w, lane);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(k_clean(s));
+      if (!warp_wait(v_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
+      if (some) {
+        clear_rows<DP>(base + S::V0 + s * S::KEYS, w, lane);
+        store_score_mask(base + S::MASK0 + s * BN * 4, w, lane);      // lives as long as the values: until the block's second product
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -189,28 +204,17 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       __syncwarp();
       if (lane == 0) mbar_arrive(q_ready);
     }
-    bool hid[2] = {hidden_key(a, m, len, lane), hidden_key(a, m, len, 32 + lane)};      // this lane's keys of block j, read a block ahead
     for (int j = 0; j < nt; ++j) {
-      const bool some_hidden = hide || (j + 1) * BN > len;
       const uint32_t s_addr = lane_base + t * 128 + (j & 1) * 64;
-      uint32_t w[2] = {0, 0};
-      if (some_hidden) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) w[i] = __ballot_sync(0xffffffffu, hid[i]);
-      }
-      if (hide || (j + 2) * BN > len) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, (j + 1) * BN + 32 * i + lane);
-      }
       ok = warp_wait(s_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_FULL);
       if (!ok) break;
       tc_fence_after();
       uint32_t r[BN];
       tmem_load64(s_addr, r);
-      if (some_hidden) {
-#pragma unroll
-        for (int k = 0; k < BN; ++k)
-          if ((w[k >> 5] >> (k & 31)) & 1u) r[k] = 0xff800000u;
+      if (hide || (j + 1) * BN > len) {
+        ok = warp_wait(v_clean(j % S::STAGES), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+        if (!ok) break;
+        add_score_mask(base + S::MASK0 + (j % S::STAGES) * BN * 4, r);
       }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
