@@ -4,6 +4,7 @@
 // head hk * rep + (r / Tq) % rep of batch row m * G + r / (Tq * rep).  A tile of 128 packed rows therefore never mixes memories,
 // short queries of several heads or beams fill one tile, and the sums over shared heads and shared rows need no second pass.
 #pragma once
+#include "packed_math.cuh"
 #include "tcgen05.cuh"
 #include <cuda_fp16.h>
 
@@ -139,45 +140,6 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) 
       : "memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// Two fp32 operations per instruction.
-__device__ __forceinline__ uint64_t pair(float lo, float hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ uint64_t pair(uint32_t lo, uint32_t hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  return v;
-}
-__device__ __forceinline__ void split(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 constexpr float EX2_C0 = 1.f, EX2_C1 = 0.693121045f, EX2_C2 = 0.24022349f, EX2_C3 = 0.0559219758f, EX2_C4 = 0.00966636852f;
 // 2^x for two values without the special-function unit: x = n + f with n the nearest integer, 2^f by a polynomial, times 2^n.

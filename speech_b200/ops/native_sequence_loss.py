@@ -102,7 +102,7 @@ def _policy_backward(ctx, dloss, _):
     if not first:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     lse = ctx.kept.data_ptr() + 8 * _blocks() + 8
-    return _gradient(dloss, logits, targets, mask, lse, lse + 4 * targets.numel(), 0, out, int(first)), None, None, None, None, None, None, None, None, None
+    return _gradient(dloss, logits, targets, mask, lse, lse + 8 * targets.numel(), 0, out, int(first)), None, None, None, None, None, None, None, None, None
 
 
 class _PolicyLossFn(torch.autograd.Function):
@@ -114,13 +114,13 @@ class _PolicyLossFn(torch.autograd.Function):
         dev, rows = logits.device, targets.numel()
         loss = torch.empty((), dtype=torch.float32, device=dev)
         logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-        kept = torch.empty(2 * _blocks() + 2 + 2 * rows, dtype=torch.float32, device=dev)       # fp64 sums of the blocks and the count, lse, slopes
+        kept = torch.empty(2 * _blocks() + 2 + 3 * rows, dtype=torch.float32, device=dev)       # fp64 sums of the blocks and the count, lse (two parts), slopes
         ws = kept.data_ptr()
         lse = ws + 8 * _blocks() + 8
         grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
         layout, sizes = _layout(logits)
         N._check(bind("sb_policy_loss_fwd")(logits.data_ptr(), *layout, targets.data_ptr(), address(mask), old.data_ptr(), address(ref), adv.data_ptr(), *sizes,
-                                            lo, hi, kl_beta, ws + 8 * _blocks(), ws, loss.data_ptr(), logp.data_ptr(), lse, lse + 4 * rows, address(grad),
+                                            lo, hi, kl_beta, ws + 8 * _blocks(), ws, loss.data_ptr(), logp.data_ptr(), lse, lse + 8 * rows, address(grad),
                                             current_stream()), "sb_policy_loss_fwd")
         if want_grad:
             ctx.save_for_backward(logits, targets, mask)
@@ -137,9 +137,9 @@ class _PolicyLossFn(torch.autograd.Function):
 def _preference_backward(ctx, dloss, _):
     logits, targets, mask = ctx.saved_tensors
     rows = targets.numel()
-    slope = ctx.kept.data_ptr() + 8 * (rows + logits.shape[0])
+    lse = ctx.kept.data_ptr() + 8 * (rows + logits.shape[0])
     out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    return _gradient(dloss, logits, targets, mask, slope + 4 * logits.shape[0], 0, slope, out, 0), None, None, None, None, None, None
+    return _gradient(dloss, logits, targets, mask, lse, 0, lse + 8 * rows, out, 0), None, None, None, None, None, None
 
 
 class _PreferenceLossFn(torch.autograd.Function):
@@ -148,13 +148,13 @@ class _PreferenceLossFn(torch.autograd.Function):
         dev, rows, n = logits.device, targets.numel(), logits.shape[0]
         loss = torch.empty((), dtype=torch.float32, device=dev)
         rewards = torch.empty(n, dtype=torch.float32, device=dev)
-        # log ratios of the positions and of the sequences (fp64), slopes of the sequences, lse (fp32)
-        ctx.kept = torch.empty(3 * (rows + n), dtype=torch.float32, device=dev)
+        # log ratios of the positions and of the sequences (fp64), lse (two parts) and the slopes of the sequences (fp32)
+        ctx.kept = torch.empty(4 * rows + 3 * n, dtype=torch.float32, device=dev)
         ws = ctx.kept.data_ptr()
-        slope = ws + 8 * (rows + n)
+        lse = ws + 8 * (rows + n)
         layout, sizes = _layout(logits)
         N._check(bind("sb_preference_loss_fwd")(logits.data_ptr(), *layout, targets.data_ptr(), address(mask), ref.data_ptr(), *sizes, kind, beta, address(gap),
-                                                ws, ws + 8 * rows, loss.data_ptr(), rewards.data_ptr(), slope, slope + 4 * n, current_stream()),
+                                                ws, ws + 8 * rows, loss.data_ptr(), rewards.data_ptr(), lse + 8 * rows, lse, current_stream()),
                  "sb_preference_loss_fwd")
         ctx.save_for_backward(logits, targets, mask)
         ctx.mark_non_differentiable(rewards)

@@ -202,6 +202,21 @@ def test_extreme_logits():
     assert bool((g[0, :, 250:] == 0).all()) and bool((g[1, :3, 250:] == 0).all())
     lp, _, _ = plain_logp(logits, targets, mask)
     assert bool(((logp.double() - lp).abs() <= lp_tolerance(500)).all())
+    # a row of nothing but the lowest value is uniform: weights of 1 / 500, in the gradient that forward writes and in the one read again
+    x = logits.clone()
+    x[1, 2] = torch.finfo(torch.bfloat16).min
+    x.requires_grad_()
+    loss, logp = ops.policy_loss(x, targets, mask, old, adv)
+    (g,) = torch.autograd.grad(loss, x, retain_graph=True)
+    (h,) = torch.autograd.grad(loss, x)
+    r = torch.exp(-torch.log(torch.tensor(500.0, dtype=torch.float64, device="cuda")) - old[1, 2].double())
+    slope = -float(r) * float(adv[1]) / mask.sum().item() if not (float(adv[1]) > 0 and float(r) > 1.2 or float(adv[1]) < 0 and float(r) < 0.8) else 0.0
+    for got in (g, h):
+        want = torch.full((500,), -slope / 500, dtype=torch.float64, device="cuda")
+        want[targets[1, 2]] += slope
+        assert bool(((got[1, 2].double() - want).abs() <= 2.0 ** -8 * want.abs() + abs(slope) * 2.0 ** -15).all())
+    p, _ = ops.preference_loss(x, targets, mask, old)
+    assert bool(torch.isfinite(torch.autograd.grad(p, x)[0]).all())
 
 
 def test_captured_and_replayed():
