@@ -17,8 +17,9 @@
 // which comes first and computes delta as it loads do, lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
 //
 // Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
-// matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do| of the call to [8, 16), and
-// the sums are scaled back, so that neither small weights nor small upstream gradients fall below the type's normal range.
+// matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do|, or a 64th of the largest
+// |delta| where the values are that large, to [8, 16), and the sums are scaled back, so that neither small weights nor small upstream
+// gradients fall below the type's normal range and ds stays below its end (behind which it is infinite).
 #include "cross_attention.cuh"
 #include "cross_attention_host.h"
 
@@ -33,18 +34,19 @@ struct BwdArgs {
   const float* lse;                   // [M * Hk, R]
   float *nlse, *ndelta;               // [M * Hk, G * rep, Tqp]: -lse (-inf behind the last row, too) and -delta (0 there)
   int Tqp;                            // Tq rounded up to 64
-  float* peak;                        // fp16: largest |do| of every block of the dq kernel
+  float* peak;                        // fp16: what ds_scale() takes, of every block of the dq kernel
   int tiles;                          // its blocks of a (memory, key head)
   float scale;
 };
 
-// Power of two that brings the largest |do| of a (memory, key head) to [8, 16); 1 for bf16, whose range needs none.
+// Power of two that brings the peak of a (memory, key head) to [8, 16); 1 for bf16, whose range needs none.  The peak is the largest
+// |do|, or |delta| / 64: ds is large only where p is, and there dp is of delta's size.
 template <typename T> __device__ __forceinline__ float ds_scale(float peak) {
   if (Half2<T>::KIND != 0 || !(peak > 0.f) || !(peak < 3e38f)) return 1.f;
-  return __int_as_float((127 + 3 - ((__float_as_int(peak) >> 23) - 127)) << 23);   // |do| of fp16 lies between 2^-24 and 2^16
+  return __int_as_float((127 + 3 - ((__float_as_int(fmaxf(peak, 1e-8f)) >> 23) - 127)) << 23);      // |do| of fp16 is at least 2^-24
 }
 
-// A warp's 32 rows of do into a swizzled tile (as load_rows), with sum(do * (out + rest)) of this lane's row and the largest |do| of all.
+// A warp's 32 rows of do into a swizzled tile (as load_rows), with sum(do * (out + rest)) of this lane's row and the peak of all.
 template <typename T, int DP>
 __device__ __forceinline__ void load_do_rows(const BwdArgs& b, long long off, int D, uint32_t tile, int quarter, int lane, float& delta, float& peak) {
   constexpr int CH = DP / 8, RPI = 32 / CH;
@@ -73,16 +75,7 @@ __device__ __forceinline__ void load_do_rows(const BwdArgs& b, long long off, in
     const float mine = __shfl_sync(0xffffffffu, d, ((lane - i) & (RPI - 1)) * CH);
     if (lane >= i && lane < i + RPI) delta = mine;
   }
-  if (Half2<T>::KIND == 0) peak = warp_max(peak);
-}
-
-template <typename T> __device__ __forceinline__ uint32_t pack_ds(float x, float y) {
-  if (Half2<T>::KIND == 0) {                               // beyond the type's range only for values far above any activation: saturate
-    uint32_t v;
-    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(y), "f"(x));
-    return v;
-  }
-  return Half2<T>::pack(x, y);
+  if (Half2<T>::KIND == 0) peak = warp_max(fmaxf(peak, fabsf(delta) * (1.f / 64.f)));
 }
 
 // 64 accumulator columns of a warp's 32 rows, times f, rounded and written.
@@ -360,7 +353,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           if (Half2<T>::KIND == 0) v = mul2(v, f2);
           float x, y;
           split(v, x, y);
-          o[k] = pack_ds<T>(x, y);
+          o[k] = Half2<T>::pack(x, y);
         }
         tmem_store16(ds_addr + 16 * i, o);
       }
@@ -603,7 +596,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           if (Half2<T>::KIND == 0) v = mul2(v, f2);
           po[j >> 1] = Half2<T>::pack(x, y);
           split(v, x, y);
-          so[j >> 1] = pack_ds<T>(x, y);
+          so[j >> 1] = Half2<T>::pack(x, y);
         }
       }
       if (some_hidden && hidden) {

@@ -28,7 +28,7 @@ int sb_xattn_args(const SbCrossAttention* g, XAttnArgs* a) {
   a->M = g->M; a->G = g->G; a->rep = g->rep; a->Tq = g->Tq; a->Tk = g->Tk; a->Hk = g->Hk; a->D = g->D;
   a->H = g->Hk * g->rep;
   const long long R = (long long)g->G * g->rep * g->Tq;
-  if (R > 0x7fffff00ll || (long long)g->M * g->Hk > 0x7fffffffll || (long long)g->M * g->G > 0x7fffffffll) return SB_BAD_ARGUMENT;
+  if (R > 0x7fffff00ll || g->Tk > 0x7fffff00 || (long long)g->M * g->Hk > 0x7fffffffll || (long long)g->M * g->G > 0x7fffffffll) return SB_BAD_ARGUMENT;
   a->R = (int)R;
   a->c = g->scale * 1.44269504088896f;
   a->status = sb_status_ptr();
