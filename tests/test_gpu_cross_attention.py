@@ -342,3 +342,59 @@ def test_run_of_the_operators_together():
     pref, _ = ops.preference_loss(logits.detach().requires_grad_(), targets, mask, old)
     assert abs(float(pref) - math.log(2)) < 1e-4
     ops.native.check_status()
+
+
+def test_offsets_beyond_32_bits():
+    """Memories and caches whose rows lie more than 2^31 elements apart."""
+    from speech_b200 import ops
+
+    q, k, v, lengths, mask, _ = make(2, 2, 70, 150, 2, 1, 64, torch.bfloat16, "both", fused=False)
+    far = torch.empty(2 ** 31 + 2 ** 20, dtype=torch.bfloat16, device="cuda")
+    apart = lambda t, at: far.as_strided(t.shape, (2 ** 31 + 2 ** 17,) + t.stride()[1:], at).copy_(t)       # noqa: E731
+
+    def run(k, v, mask):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask)
+        with torch.no_grad():
+            step = ops.cross_attention(q[:, :1], k, v, key_lengths=lengths, key_mask=mask)
+            both = ops.shared_prefix_attention(q[:2, :1], k, v, k, v, lengths.clamp(max=140), prefix_lengths=lengths)
+        return [t.detach().contiguous().view(torch.int16) for t in (out, step, both) + torch.autograd.grad(out, leaves, torch.ones_like(out))]
+
+    clean = lambda t: t.nan_to_num(1.0, 1.0, 1.0)           # noqa: E731
+    names = ("out", "step", "both", "dq", "dk", "dv")
+    for what, x, y, m in (("hidden garbage", k, v, mask), ("all but the lengths seen", clean(k), clean(v), None)):
+        near, at = run(x, y, m), run(apart(x, 0), apart(y, 2 ** 16), m)
+        assert [n for n, a, b in zip(names, near, at) if not torch.equal(a, b)] == [], what
+    ops.native.check_status()
+
+
+def test_calls_from_two_threads():
+    import threading
+
+    from speech_b200 import ops
+
+    cases, results = [make(2, 2, 130, t, 2, 1, 64, torch.float16, "lengths", seed=t) for t in (300, 77)], [[], []]
+
+    def call(c):
+        leaves = [t.detach().requires_grad_() for t in c[:3]]
+        out = ops.cross_attention(*leaves, key_lengths=c[3])
+        with torch.no_grad():
+            step = ops.cross_attention(c[0][:, :1], c[1], c[2], key_lengths=c[3])
+        return (out, step) + torch.autograd.grad(out, leaves, torch.ones_like(out))
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                results[i].append(call(cases[i]))
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for c, got in zip(cases, results):
+        want = call(c)
+        assert len(got) == 10 and all(torch.equal(a, b) for r in got for a, b in zip(r, want))
+    ops.native.check_status()

@@ -250,3 +250,85 @@ def test_captured_and_replayed():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("v", [130, 2024, 9000, 40001])
+def test_infinite_and_nan_logits(v):
+    """-inf logits (a masked vocabulary) have no weight and no gradient; a NaN or +inf logit shows in the loss and its sequence's reward."""
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(4, 5, None, v, torch.bfloat16)
+    mask[:] = True
+    hide = torch.rand(logits.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) < 0.5
+    hide[..., : v // 3] = True
+    hide.scatter_(-1, targets.unsqueeze(-1), False)
+    logits = logits.masked_fill(hide, float("-inf"))
+    lp, m, weights = plain_logp(logits, targets, mask)
+    old, tol = lp.float(), lp_tolerance(v)
+    x = logits.clone().requires_grad_()
+    loss, logp = ops.policy_loss(x, targets, mask, old, adv)
+    assert bool(((logp.double() - lp).abs() <= tol).all())
+    # the old log-probabilities are the new ones (to fp32): r = 1, the slope -A / count
+    g, slope = torch.autograd.grad(loss, x)[0], -adv.double().view(-1, 1) / m.sum()
+    check_gradient(g, targets, weights, slope.expand(targets.shape), torch.bfloat16, v)
+    assert bool((g[hide] == 0).all())
+    loss, rewards = ops.preference_loss(x, targets, mask, old)
+    # every position within the tolerance of its log-probability, and old's rounding (2^-20 below 32) on top
+    assert bool((rewards.double().abs() <= 0.1 * 5 * (tol + 2.0 ** -20)).all())
+    h = torch.autograd.grad(loss, x)[0]
+    assert bool((h[hide] == 0).all()) and bool(torch.isfinite(h).all())
+    for bad in (float("nan"), float("inf")):
+        for at in (0, v // 2, v - 1):
+            y = logits.clone()
+            y[1, 2, at] = bad
+            y.requires_grad_()
+            a, logp = ops.policy_loss(y, targets, mask, old, adv)
+            b, rewards = ops.preference_loss(y, targets, mask, old)
+            assert bool(torch.isnan(a)) and bool(torch.isnan(b)) and bool(torch.isnan(logp[1, 2])) and int(torch.isnan(logp).sum()) == 1
+            assert bool(torch.isnan(rewards[1])) and int(torch.isnan(rewards).sum()) == 1
+
+
+def test_rows_beyond_32_bit_offsets():
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(2, 3, None, 300, torch.bfloat16)
+    far = torch.empty(2 ** 31 + 4096, dtype=torch.bfloat16, device="cuda").as_strided((2, 3, 300), (2 ** 31 + 1024, 300, 1))
+    far.copy_(logits)
+    results = []
+    for t in (logits, far):
+        x = t.detach().requires_grad_()
+        loss, logp = ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.04)
+        p, rewards = ops.preference_loss(x, targets, mask, ref)
+        results.append([loss, logp, rewards, torch.autograd.grad(loss, x, retain_graph=True)[0], torch.autograd.grad(loss, x)[0], torch.autograd.grad(p, x)[0]])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_calls_from_two_threads():
+    import threading
+
+    from speech_b200 import ops
+
+    cases, results = [make(4, 50, 2, v, torch.bfloat16, seed=v) for v in (2024, 300)], [[], []]
+
+    def call(c):
+        logits, targets, mask, old, ref, adv = c
+        x = logits.detach().requires_grad_()
+        loss, _ = ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.04)
+        p, _ = ops.preference_loss(x, targets, mask, ref)
+        return torch.autograd.grad(loss, x)[0], torch.autograd.grad(p, x)[0]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                results[i].append(call(cases[i]))
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for c, got in zip(cases, results):
+        want = call(c)
+        assert len(got) == 10 and all(torch.equal(a, b) for r in got for a, b in zip(r, want))
