@@ -257,6 +257,48 @@ __device__ __forceinline__ void store_rows64(uint32_t buf, const uint32_t* packe
   __syncwarp();
 }
 
+// Blocks of a cluster that share one tile of results, each over its part of the summed axis: fp32 rows of DP values stand in every
+// block's shared memory, 16-byte pieces XORed with the row, and block r of n adds up and writes every n-th eight columns.
+__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+template <int DP> __device__ __forceinline__ uint32_t part_addr(uint32_t base, int row, int piece) {
+  return base + (uint32_t)row * (uint32_t)(DP * 4) + (uint32_t)((piece & ~7) | ((piece ^ row) & 7)) * 16u;
+}
+// 64 accumulator columns of this lane's row (zeros unless `have`)
+template <int DP> __device__ __forceinline__ void keep_part64(uint32_t base, int row, int col, uint32_t taddr, bool have) {
+  uint32_t r[64];
+  if (have) {
+    tmem_load64(taddr, r);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 64; ++k) r[k] = 0u;
+  }
+#pragma unroll
+  for (int k = 0; k < 16; ++k) st_shared_v4(part_addr<DP>(base, row, col / 4 + k), r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+}
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, int rank) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  return there;
+}
+__device__ __forceinline__ float2 load_remote2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+// sum[0 .. 7] += w * eight columns of a row in block `rank`
+template <int DP> __device__ __forceinline__ void add_part8(uint32_t base, int row, int c8, int rank, float w, float* sum) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(in_block(part_addr<DP>(base, row, 2 * c8 + h), rank)) : "memory");
+    sum[4 * h] = fmaf(w, v.x, sum[4 * h]);
+    sum[4 * h + 1] = fmaf(w, v.y, sum[4 * h + 1]);
+    sum[4 * h + 2] = fmaf(w, v.z, sum[4 * h + 2]);
+    sum[4 * h + 3] = fmaf(w, v.w, sum[4 * h + 3]);
+  }
+}
+
 // A warp zeroes the hidden rows (bits of w[0], w[1]) of a [64, DP] tile: a hidden infinity or NaN would turn its zero weight into NaN
 // inside a matrix product.  (A loop over the set bits would find them with the unit that the exponentials keep busy.)
 template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, const uint32_t* w, int lane) {

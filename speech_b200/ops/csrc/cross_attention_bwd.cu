@@ -16,6 +16,9 @@
 // turn, half of the columns each.  Rows come by TMA, their statistics by bulk copies, for which the dq kernel,
 // which comes first and computes delta as it loads do, lays out -lse and -delta in lines of a multiple of 64 per (memory, head).
 //
+// Where there are fewer tiles than SMs, up to eight CTAs of a cluster share one (keys of dq, query rows of dk / dv in parts) and add their
+// fp32 sums up through one another's shared memory, in a fixed order.
+//
 // Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
 // matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do|, or a 64th of the largest
 // |delta| where the values are that large, to [8, 16), and the sums are scaled back, so that neither small weights nor small upstream
@@ -26,6 +29,9 @@
 namespace {
 
 constexpr int DKV_THREADS = 640;       // 20 warps of 96 registers
+// What a CTA takes besides its blocks or steps, in those; a join takes half of it.  [dq, 100 queries, 8 heads of 128, 1 / 2 / 4 / 8 CTAs a
+// tile: 73 / 47 / 30 / 24 us for 7500 keys, 24 / 22 / 20 / 18 for 1500; dk / dv, 5 x 1500 queries against 100 keys: 102 / 57 / 36 / 28 us]
+constexpr int DQ_OWN_BLOCKS = 10, DKV_OWN_STEPS = 8;
 template <typename T> constexpr float p_shift() { return Half2<T>::KIND == 0 ? 12.f : 0.f; }
 
 struct BwdArgs {
@@ -78,6 +84,14 @@ __device__ __forceinline__ void load_do_rows(const BwdArgs& b, long long off, in
   if (Half2<T>::KIND == 0) peak = warp_max(fmaxf(peak, fabsf(delta) * (1.f / 64.f)));
 }
 
+// Eight columns of a row from all blocks of the cluster, in turn, times f, rounded and written.
+template <typename T, int DP> __device__ __forceinline__ void join_parts8(uint32_t base, int row, int c8, int splits, float f, uint16_t* dst) {
+  float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < splits; ++i) add_part8<DP>(base, row, c8, i, 1.f, o);
+  *reinterpret_cast<uint4*>(dst) = make_uint4(Half2<T>::pack(o[0] * f, o[1] * f), Half2<T>::pack(o[2] * f, o[3] * f), Half2<T>::pack(o[4] * f, o[5] * f),
+                                              Half2<T>::pack(o[6] * f, o[7] * f));
+}
+
 // 64 accumulator columns of a warp's 32 rows, times f, rounded and written.
 template <typename T>
 __device__ __forceinline__ void store_acc64(uint32_t buf, uint32_t taddr, bool have, float f, uint16_t* dst, long long off, int col, int D, int lane) {
@@ -107,7 +121,7 @@ constexpr int DQ_THREADS = 384;
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(DQ_THREADS, 1)
-xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq) {
+xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq, const int splits) {
   using S = DqSmem<DP>;
   constexpr int BN = S::BN, HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -125,11 +139,13 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, stats = bars + 240u;      // stats: -delta of the tile's rows, largest |do| of four warps
 
   const int tiles = b.tiles;
-  const int unit = blockIdx.x / tiles, m = unit / a.Hk, hk = unit % a.Hk;
-  const int row0 = (blockIdx.x - unit * tiles) * 128;
+  const int index = blockIdx.x / splits, rank = blockIdx.x - index * splits;      // block `rank` of a cluster takes its part of the keys
+  const int unit = index / tiles, m = unit / a.Hk, hk = unit % a.Hk;
+  const int row0 = (index - unit * tiles) * 128;
   const int len = visible_keys(a, m);
   const int blocks = (len + BN - 1) / BN;
-  const int nt = dq || blocks == 1 ? blocks : 0;            // without dq only the statistics are wanted, for which one block refines delta
+  const int share = (blocks + splits - 1) / splits, first = rank * share * BN;
+  const int nt = dq || blocks == 1 ? min(share, max(0, blocks - rank * share)) : 0;      // without dq only the statistics are wanted, for which one block refines delta
   const bool hide = a.mask != nullptr;
 
   if (threadIdx.x == 0) {
@@ -162,8 +178,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         mbar_expect_tx(kv_full(s), 2 * S::KEYS);
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
-          tma_load_4d(kb + h * (BN * 128), &map_k, kv_full(s), h * 64, j * BN, hk, m);
-          tma_load_4d(kb + S::KEYS + h * (BN * 128), &map_v, kv_full(s), h * 64, j * BN, hk, m);
+          tma_load_4d(kb + h * (BN * 128), &map_k, kv_full(s), h * 64, first + j * BN, hk, m);
+          tma_load_4d(kb + S::KEYS + h * (BN * 128), &map_v, kv_full(s), h * 64, first + j * BN, hk, m);
         }
       }
       __syncwarp();
@@ -172,17 +188,17 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     int issued = 0;
     bool ok = true;
     for (; issued < nt && issued < S::STAGES - 2 && ok; ++issued) ok = load(issued);
-    bool hid[2] = {hidden_key(a, m, len, lane), hidden_key(a, m, len, 32 + lane)};      // this lane's keys of block j, read a block ahead
+    bool hid[2] = {hidden_key(a, m, len, first + lane), hidden_key(a, m, len, first + 32 + lane)};      // this lane's keys of block j, read a block ahead
     for (int j = 0; j < nt && ok; ++j) {
       const int s = j % S::STAGES;
-      const bool some = hide || (j + 1) * BN > len;
+      const bool some = hide || first + (j + 1) * BN > len;
       uint32_t w[2] = {0, 0};
       if (some) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) w[i] = __ballot_sync(0xffffffffu, hid[i]);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, (j + 1) * BN + 32 * i + lane);
+      for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, first + (j + 1) * BN + 32 * i + lane);
       ok = warp_wait(kv_full(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
       if (!ok) break;
       if (some) {
@@ -212,7 +228,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     int s = 0;
     uint32_t ph = 0;
     for (int j = 0; j < nt && ok; ++j) {
-      ok = warp_wait(hide || (j + 1) * BN > len ? kv_clean(s) : kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL) &&
+      ok = warp_wait(hide || first + (j + 1) * BN > len ? kv_clean(s) : kv_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL) &&
            (second ? warp_wait(dp_read, ((uint32_t)j & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY)
                    : warp_wait(s_read(j & 1), ((uint32_t)(j >> 1) & 1u) ^ 1u, a.status, SB_TIMEOUT_TMEM_EMPTY));
       if (!ok) break;
@@ -270,9 +286,9 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       load_do_rows<T, DP>(b, row_offset(a, st * a.Tq, st, a.D, m, hk, row), a.D, tile, quarter, lane, delta, peak);
       asm volatile("st.shared.f32 [%0], %1;" ::"r"(stat_row), "f"(-delta) : "memory");
       if (lane == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(stats + (128 + quarter) * 4), "f"(peak) : "memory");
-      if (valid) {
+      if (valid && rank == 0) {
         b.nlse[stat] = nlse;
-        if (nt != 1) b.ndelta[stat] = -delta;
+        if (blocks != 1) b.ndelta[stat] = -delta;
         if (t == a.Tq - 1)                                   // the line's end, which the copies of the dk / dv kernel read
           for (int x = 1; x < b.Tqp - t; ++x) {
             b.nlse[stat + x] = -INFINITY;
@@ -294,7 +310,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(p4[i]) : "r"(stats + (128 + i) * 4) : "memory");
     const float peak = fmaxf(fmaxf(p4[0], p4[1]), fmaxf(p4[2], p4[3])), dsf = ds_scale<T>(peak);
-    if (Half2<T>::KIND == 0 && warp == 4 && lane == 0) b.peak[blockIdx.x] = peak;
+    if (Half2<T>::KIND == 0 && warp == 4 && lane == 0 && rank == 0) b.peak[index] = peak;
     const uint64_t c2 = pair(a.c, a.c), nl2 = pair(nlse, nlse), f2 = pair(dsf, dsf);
     uint32_t ph = 0;
     for (int j = wg; j < nt; j += 2) {
@@ -320,7 +336,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         if (!ok) break;
         tc_fence_after();
       }
-      if (hide || (j + 1) * BN > len) {
+      if (hide || first + (j + 1) * BN > len) {
         ok = warp_wait(kv_clean(j % S::STAGES), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         add_score_mask(base + S::MASK0 + (j % S::STAGES) * BN * 4, r);
@@ -332,7 +348,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         r[k] = __float_as_uint(ex2(x));
         r[k + 1] = __float_as_uint(ex2(y));
       }
-      if (nt == 1) {
+      if (blocks == 1) {
         // all keys are in this block: delta = sum p dp from the values that it is subtracted from, instead of the rounded output
         uint64_t d2[2] = {0, 0};
 #pragma unroll
@@ -365,10 +381,31 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
     if (nt > 0 && ok) ok = warp_wait(dq_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
-    if (dq && wg < DP / 64) {                              // 64 columns a warpgroup
+    if (splits > 1) {
+      if (wg < DP / 64) keep_part64<DP>(base, quarter * 32 + lane, 64 * wg, lane_base + 64 * wg, nt > 0 && ok);
+    } else if (dq && wg < DP / 64) {                       // 64 columns a warpgroup
       const long long off = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
       store_acc64<T>(base + (wg * 4 + quarter) * 4096, lane_base + 64 * wg, nt > 0 && ok, b.scale / dsf, dq, off, 64 * wg, a.D, lane);
     }
+  }
+  if (splits > 1) {                                        // only with dq
+    __syncthreads();
+    cluster_sync();
+    float peak = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float p;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(p) : "r"(stats + (128 + i) * 4) : "memory");
+      peak = fmaxf(peak, p);
+    }
+    const float f = b.scale / ds_scale<T>(peak);
+    constexpr int CH = DP / 8;
+    for (int x = rank * DQ_THREADS + threadIdx.x; x < 128 * CH; x += splits * DQ_THREADS) {
+      const int r = x / CH, c8 = x % CH;
+      if (row0 + r >= a.R || c8 * 8 >= a.D) continue;
+      join_parts8<T, DP>(base, r, c8, splits, f, dq + row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row0 + r) + c8 * 8);
+    }
+    cluster_sync();                                          // the others may still read this block's part
   }
   tc_fence_before();
   __syncthreads();
@@ -391,7 +428,8 @@ template <int DP> struct DkvSmem {
 template <typename T, int DP>
 __global__ void __launch_bounds__(DKV_THREADS, 1)
 xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
-                 const __grid_constant__ CUtensorMap map_do, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv) {
+                 const __grid_constant__ CUtensorMap map_do, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
+                 const int splits) {
   using S = DkvSmem<DP>;
   constexpr int BQ = S::BQ, HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -408,11 +446,13 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                  tmem_slot = bars + 8u * 21, scale_slot = tmem_slot + 4;
 
   const int ktiles = (a.Tk + 127) / 128;
-  const int unit = blockIdx.x / ktiles, m = unit / a.Hk, hk = unit % a.Hk;
-  const int key0 = (blockIdx.x - unit * ktiles) * 128;
+  const int index = blockIdx.x / splits, rank = blockIdx.x - index * splits;      // block `rank` of a cluster takes its part of the rows
+  const int unit = index / ktiles, m = unit / a.Hk, hk = unit % a.Hk;
+  const int key0 = (index - unit * ktiles) * 128;
   const int len = visible_keys(a, m);
   const int segs = a.G * a.rep, lines = b.Tqp / BQ;        // (row, head) pairs that read these keys, steps of each
-  const int nq = key0 < len ? segs * lines : 0;            // 0: nothing is visible here, gradients are zero
+  const int share = (segs * lines + splits - 1) / splits, step0 = rank * share;
+  const int nq = key0 < len ? min(share, max(0, segs * lines - step0)) : 0;        // 0: nothing is visible here, gradients are zero
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) { mbar_init(q_full(s), 1); mbar_init(q_empty(s), 1); }
@@ -456,7 +496,8 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
     }
     __syncwarp();
-    int s = 0, issued = 0, t0 = 0, head = 0, g = 0;        // step i: rows t0 .. of head hk * rep + head of batch row m * G + g
+    const int seg = step0 / lines;
+    int s = 0, issued = 0, t0 = (step0 - seg * lines) * BQ, g = seg / a.rep, head = seg - g * a.rep;      // step step0 + i: rows t0 .. of head hk * rep + head of batch row m * G + g
     uint32_t ph = 0;
     for (int i = 0; i < nq; ++i) {
       if (!warp_wait(q_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY)) break;
@@ -619,11 +660,27 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     if (nq > 0 && ok) ok = warp_wait(d_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
     // dv by two warpgroups, dk by the others, 64 columns each (DP = 64: one of the two)
-    if (half < DP / 64) {
+    if (splits > 1) {
+      if (half < DP / 64) keep_part64<DP>(base + u * 128 * DP * 4, quarter * 32 + lane, half * 64, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok);
+    } else if (half < DP / 64) {
       const long long off = key < a.Tk ? (((long long)m * a.Tk + key) * a.Hk + hk) * a.D : -1;
       store_acc64<T>(base + ((u * 2 + half) * 4 + quarter) * 4096, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok, u ? b.scale / dsf : ex2(-p_shift<T>()),
                      u ? dk : dv, off, half * 64, a.D, lane);
     }
+  }
+  if (splits > 1) {
+    __syncthreads();
+    cluster_sync();
+    float dsf;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
+    constexpr int CH = DP / 8;
+    for (int x = rank * DKV_THREADS + threadIdx.x; x < 2 * 128 * CH; x += splits * DKV_THREADS) {
+      const int u = x / (128 * CH), r = x / CH % 128, c8 = x % CH, key = key0 + r;
+      if (key >= a.Tk || c8 * 8 >= a.D) continue;
+      join_parts8<T, DP>(base + u * 128 * DP * 4, r, c8, splits, u ? b.scale / dsf : ex2(-p_shift<T>()),
+                         (u ? dk : dv) + (((long long)m * a.Tk + key) * a.Hk + hk) * a.D + c8 * 8);
+    }
+    cluster_sync();                                          // the others may still read this block's part
   }
   tc_fence_before();
   __syncthreads();
@@ -642,14 +699,17 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   if (rc) return rc;
   b.tiles = (a.R + 127) / 128;
   const long long units = (long long)a.M * a.Hk, gq = units * b.tiles, gk = units * ((a.Tk + 127) / 128);
-  if (gq > 0x7fffffffll || gk > 0x7fffffffll) return SB_BAD_ARGUMENT;
-  xattn_dq_kernel<T, DP><<<(unsigned)gq, DQ_THREADS, DqSmem<DP>::BYTES, stream>>>(k64, v64, a, b, (uint16_t*)dq);      // also lays out the statistics
-  rc = (int)cudaGetLastError();
-  if (!rc && dk) {
-    xattn_dkv_kernel<T, DP><<<(unsigned)gk, DKV_THREADS, DkvSmem<DP>::BYTES, stream>>>(k64, v64, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv);
-    rc = (int)cudaGetLastError();
-  }
-  return rc;
+  if (gq > 0x7ffffffll || gk > 0x7ffffffll) return SB_BAD_ARGUMENT;
+  const int sq = dq ? sb_cluster_splits((const void*)xattn_dq_kernel<T, DP>, DQ_THREADS, DqSmem<DP>::BYTES, gq, (a.Tk + DqSmem<DP>::BN - 1) / DqSmem<DP>::BN, DQ_OWN_BLOCKS,
+                                        DQ_OWN_BLOCKS / 2) : 1;
+  SbClusterLaunch lq(gq, sq, DQ_THREADS, DqSmem<DP>::BYTES, stream);
+  rc = (int)cudaLaunchKernelEx(&lq.config, xattn_dq_kernel<T, DP>, k64, v64, a, b, (uint16_t*)dq, sq);      // also lays out the statistics
+  if (rc || !dk) return rc;
+  const long long steps = (long long)a.G * a.rep * (b.Tqp / DkvSmem<DP>::BQ);
+  const int sk = sb_cluster_splits((const void*)xattn_dkv_kernel<T, DP>, DKV_THREADS, DkvSmem<DP>::BYTES, gk, (int)(steps < 0x7fffff00 ? steps : 0x7fffff00),
+                                   DKV_OWN_STEPS, DKV_OWN_STEPS / 2);
+  SbClusterLaunch lk(gk, sk, DKV_THREADS, DkvSmem<DP>::BYTES, stream);
+  return (int)cudaLaunchKernelEx(&lk.config, xattn_dkv_kernel<T, DP>, k64, v64, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv, sk);
 }
 
 }  // namespace

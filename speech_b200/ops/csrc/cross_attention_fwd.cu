@@ -11,6 +11,8 @@
 // the second product.  The scores of the next block are there before the softmax of this one ends; with one buffer of 128 keys the
 // warpgroups waited for the tensor core and it for them (41 % of its cycles busy).  The output is rescaled only when a row's maximum
 // has grown by more than 2^8 since the last time; p then stays below 2^8, and the result does not depend on it beyond rounding.
+// Where there are fewer tile pairs than SMs, up to eight CTAs of a cluster share one, each with its part of the keys; unnormalised outputs
+// and (m, l) meet in shared memory and are joined in a fixed order: w_i = 2^(c (m_i - max m)), o = sum w_i o_i / sum w_i l_i.
 //
 // Rounding: scores, maxima, sums and output are fp32; p is rounded to the operands' 16-bit type, which is what the tensor core
 // multiplies (relative 2^-9 per weight in bf16, random, as large as the one rounding of the result); l sums the unrounded p.
@@ -21,6 +23,9 @@ namespace {
 
 constexpr int FWD_THREADS = 384;
 constexpr int BN = 64;
+// What a CTA takes besides its blocks, and what a join takes, in blocks.  [1 x 100 queries, 8 heads of 128, 1 / 2 / 4 / 8 CTAs a tile:
+// 104 / 63 / 42 / 34 us for 7500 keys, 34 / 28 / 24 / 24 for 1500, 22 / 22 / 20 / 22 for 500]
+constexpr int OWN_BLOCKS = 9;
 template <int DP> struct FwdSmem {
   static constexpr int STAGES = 4;
   static constexpr int TILE = 128 * DP * 2, KEYS = BN * DP * 2;      // 128 query rows, a block of keys or values
@@ -31,7 +36,7 @@ template <int DP> struct FwdSmem {
 template <typename T, int DP>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, uint16_t* __restrict__ out,
-                 uint16_t* __restrict__ rest, float* __restrict__ lse) {
+                 uint16_t* __restrict__ rest, float* __restrict__ lse, const int splits) {
   using S = FwdSmem<DP>;
   constexpr int HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -51,11 +56,13 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   const uint32_t q_ready = bars + 8u * 30, tmem_slot = bars + 8u * 31;
 
   const int pairs = (a.R + 255) / 256;                    // row-tile pairs of a (memory, key head): neighbours in the grid, for the L2
-  const int unit = blockIdx.x / pairs, m = unit / a.Hk, hk = unit % a.Hk;
-  const int row0 = (blockIdx.x - unit * pairs) * 256;
+  const int index = blockIdx.x / splits, rank = blockIdx.x - index * splits;      // block `rank` of a cluster takes its part of the keys
+  const int unit = index / pairs, m = unit / a.Hk, hk = unit % a.Hk;
+  const int row0 = (index - unit * pairs) * 256;
   const int tiles = a.R - row0 > 128 ? 2 : 1;
   const int len = visible_keys(a, m);
-  const int nt = (len + BN - 1) / BN;
+  const int blocks = (len + BN - 1) / BN, share = (blocks + splits - 1) / splits, first = rank * share * BN;
+  const int nt = min(share, max(0, blocks - rank * share));
   const bool hide = a.mask != nullptr;
 
   if (threadIdx.x == 0) {
@@ -94,7 +101,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (elect_one()) {
         mbar_expect_tx(k_full(s), S::KEYS);
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::K0 + s * S::KEYS + h * (BN * 128), &map_k, k_full(s), h * 64, j * BN, hk, m);
+        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::K0 + s * S::KEYS + h * (BN * 128), &map_k, k_full(s), h * 64, first + j * BN, hk, m);
       }
       __syncwarp();
       ok = warp_wait(v_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY);
@@ -103,7 +110,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (elect_one()) {
         mbar_expect_tx(v_full(s), S::KEYS);
 #pragma unroll
-        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::V0 + s * S::KEYS + h * (BN * 128), &map_v, v_full(s), h * 64, j * BN, hk, m);
+        for (int h = 0; h < HALVES; ++h) tma_load_4d(base + S::V0 + s * S::KEYS + h * (BN * 128), &map_v, v_full(s), h * 64, first + j * BN, hk, m);
       }
       __syncwarp();
       if (++s == S::STAGES) { s = 0; ph ^= 1u; }
@@ -133,14 +140,14 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     };
     bool ok = nt > 0 && warp_wait(q_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
     for (int j = 0; j < 2 && j < nt && ok; ++j) {
-      ok = warp_wait(hide || (j + 1) * BN > len ? k_clean(j) : k_full(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
+      ok = warp_wait(hide || first + (j + 1) * BN > len ? k_clean(j) : k_full(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
       if (!ok) break;
       tc_fence_after();
       scores(j);
     }
     for (int j = 0; j < nt && ok; ++j) {
       const int s = j % S::STAGES;
-      ok = warp_wait(hide || (j + 1) * BN > len ? v_clean(s) : v_full(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL) &&
+      ok = warp_wait(hide || first + (j + 1) * BN > len ? v_clean(s) : v_full(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL) &&
            warp_wait(p_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
       tc_fence_after();
@@ -153,7 +160,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
       __syncwarp();
       if (j + 2 < nt) {
-        ok = warp_wait(hide || (j + 3) * BN > len ? k_clean((j + 2) % S::STAGES) : k_full((j + 2) % S::STAGES), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+        ok = warp_wait(hide || first + (j + 3) * BN > len ? k_clean((j + 2) % S::STAGES) : k_full((j + 2) % S::STAGES), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
         scores(j + 2);
@@ -163,16 +170,16 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     // ---------------------------------------------------------------- hidden keys: their rows cleared, their scores' addends
     int s = 0;
     uint32_t ph = 0;
-    bool hid[2] = {hidden_key(a, m, len, lane), hidden_key(a, m, len, 32 + lane)};      // this lane's keys of block j, read a block ahead
+    bool hid[2] = {hidden_key(a, m, len, first + lane), hidden_key(a, m, len, first + 32 + lane)};      // this lane's keys of block j, read a block ahead
     for (int j = 0; j < nt; ++j) {
-      const bool some = hide || (j + 1) * BN > len;
+      const bool some = hide || first + (j + 1) * BN > len;
       uint32_t w[2] = {0, 0};
       if (some) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) w[i] = __ballot_sync(0xffffffffu, hid[i]);
       }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, (j + 1) * BN + 32 * i + lane);
+      for (int i = 0; i < 2; ++i) hid[i] = hidden_key(a, m, len, first + (j + 1) * BN + 32 * i + lane);
       if (!warp_wait(k_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
       if (some) {
         clear_rows<DP>(base + S::K0 + s * S::KEYS, w, lane);
@@ -211,7 +218,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       tc_fence_after();
       uint32_t r[BN];
       tmem_load64(s_addr, r);
-      if (hide || (j + 1) * BN > len) {
+      if (hide || first + (j + 1) * BN > len) {
         ok = warp_wait(v_clean(j % S::STAGES), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         add_score_mask(base + S::MASK0 + (j % S::STAGES) * BN * 4, r);
@@ -282,24 +289,60 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (nt > 0 && ok) ok = warp_wait(o_full(t), 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
-    const long long at_row = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
-    if (lse && row < a.R) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const uint32_t buf = base + t * S::TILE + quarter * 4096;      // the tile's queries have been read
+    if (splits > 1) {
+      asm volatile("bar.sync 2, %0;" ::"r"(tiles * 128) : "memory");     // no product of either tile reads shared memory any more
+      const int r = t * 128 + quarter * 32 + lane;
 #pragma unroll
-    for (int i = 0; i < DP / 64; ++i) {
-      uint32_t r[64], v[32], w[32];
-      if (nt > 0 && ok) {
-        tmem_load64(o_addr + 64 * i, r);
-      } else {
+      for (int i = 0; i < DP / 64; ++i) keep_part64<DP>(base, r, 64 * i, o_addr + 64 * i, nt > 0 && ok);
+      asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(base + 256 * DP * 4 + r * 8), "f"(mx), "f"(l) : "memory");
+    } else {
+      const long long at_row = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
+      if (lse && row < a.R) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const uint32_t buf = base + t * S::TILE + quarter * 4096;      // the tile's queries have been read
 #pragma unroll
-        for (int k = 0; k < 64; ++k) r[k] = 0u;
+      for (int i = 0; i < DP / 64; ++i) {
+        uint32_t r[64], v[32], w[32];
+        if (nt > 0 && ok) {
+          tmem_load64(o_addr + 64 * i, r);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 64; ++k) r[k] = 0u;
+        }
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v[k] = out_pair<T>(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv, w[k]);
+        store_rows64(buf, v, out, at_row, 64 * i, a.D, lane);
+        if (rest) store_rows64(buf, w, rest, at_row, 64 * i, a.D, lane);
       }
-#pragma unroll
-      for (int k = 0; k < 32; ++k) v[k] = out_pair<T>(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv, w[k]);
-      store_rows64(buf, v, out, at_row, 64 * i, a.D, lane);
-      if (rest) store_rows64(buf, w, rest, at_row, 64 * i, a.D, lane);
     }
+  }
+  if (splits > 1) {
+    __syncthreads();
+    cluster_sync();
+    constexpr int CH = DP / 8;
+    for (int x = rank * FWD_THREADS + threadIdx.x; x < tiles * 128 * CH; x += splits * FWD_THREADS) {
+      const int r = x / CH, c8 = x % CH, row = row0 + r;
+      if (row >= a.R || c8 * 8 >= a.D) continue;
+      const uint32_t ml = base + 256 * DP * 4 + r * 8;
+      float top = -INFINITY, sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < splits; ++i) top = fmaxf(top, load_remote2(in_block(ml, i)).x);
+      for (int i = 0; i < splits; ++i) {
+        const float2 v = load_remote2(in_block(ml, i));
+        if (v.y == 0.f) continue;                            // saw nothing
+        const float w = ex2((v.x - top) * a.c);
+        sum = fmaf(w, v.y, sum);
+        add_part8<DP>(base, r, c8, i, w, o);
+      }
+      if (lse && c8 == 0) lse[(long long)unit * a.R + row] = sum > 0.f ? fmaf(top, a.c, log2f(sum)) : (sum == 0.f ? INFINITY : sum);
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+      const long long at = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row) + c8 * 8;
+      uint32_t v[4], w[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = out_pair<T>(o[2 * k] * inv, o[2 * k + 1] * inv, w[k]);
+      *reinterpret_cast<uint4*>(out + at) = make_uint4(v[0], v[1], v[2], v[3]);
+      if (rest) *reinterpret_cast<uint4*>(rest + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    cluster_sync();                                          // the others may still read this block's part
   }
   tc_fence_before();
   __syncthreads();
@@ -309,11 +352,12 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 template <typename T, int DP>
 int launch(const XAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, void* out, void* rest, float* lse, cudaStream_t stream) {
   const long long grid = (long long)((a.R + 255) / 256) * a.M * a.Hk;
-  if (grid > 0x7fffffffll) return SB_BAD_ARGUMENT;
+  if (grid > 0x7ffffffll) return SB_BAD_ARGUMENT;
   const int rc = sb_allow_smem((const void*)xattn_fwd_kernel<T, DP>, FwdSmem<DP>::BYTES);
   if (rc) return rc;
-  xattn_fwd_kernel<T, DP><<<(unsigned)grid, FWD_THREADS, FwdSmem<DP>::BYTES, stream>>>(mk, mv, a, (uint16_t*)out, (uint16_t*)rest, lse);
-  return (int)cudaGetLastError();
+  const int splits = sb_cluster_splits((const void*)xattn_fwd_kernel<T, DP>, FWD_THREADS, FwdSmem<DP>::BYTES, grid, (a.Tk + BN - 1) / BN, OWN_BLOCKS, OWN_BLOCKS);
+  SbClusterLaunch l(grid, splits, FWD_THREADS, FwdSmem<DP>::BYTES, stream);
+  return (int)cudaLaunchKernelEx(&l.config, xattn_fwd_kernel<T, DP>, mk, mv, a, (uint16_t*)out, (uint16_t*)rest, lse, splits);
 }
 
 }  // namespace

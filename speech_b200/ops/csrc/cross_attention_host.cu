@@ -56,6 +56,44 @@ int sb_rows_map(CUtensorMap* map, const void* ptr, int type, int D, int T, int h
   return r == CUDA_SUCCESS ? 0 : -(200 + (int)r);
 }
 
+namespace {
+// Clusters of n blocks of a kernel that the GPU holds at once; asked once per kernel, size and device.  (A cluster's SMs are in one part of
+// the GPU, and of the parts' 16 to 20 SMs a cluster of 8 leaves some unused.)
+int clusters_at_once(const void* kernel, int n, int threads, int smem) {
+  struct Seen { const void* kernel; int device, n, clusters; };
+  static thread_local Seen seen[64];
+  static thread_local int count = 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  for (int i = 0; i < count; ++i)
+    if (seen[i].kernel == kernel && seen[i].device == dev && seen[i].n == n) return seen[i].clusters;
+  SbClusterLaunch l(1, n, threads, smem, 0);
+  int clusters = 0;
+  if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &l.config) != cudaSuccess) {
+    cudaGetLastError();
+    clusters = 0;
+  }
+  if (count < 64) seen[count++] = {kernel, dev, n, clusters};
+  return clusters;
+}
+}  // namespace
+
+int sb_cluster_splits(const void* kernel, int threads, int smem, long long tiles, int steps, int own, int join) {
+  int best = 1;
+  const long long sms = sb_num_sms();
+  long long least = (tiles + sms - 1) / sms * (steps + own);
+  for (int n = 2; n <= 8 && steps >= 2 * n && tiles < sms; n *= 2) {
+    const int at_once = clusters_at_once(kernel, n, threads, smem);
+    if (at_once <= 0) break;
+    const long long cost = (tiles + at_once - 1) / at_once * ((steps + n - 1) / n + own + join);
+    if (cost < least) {
+      best = n;
+      least = cost;
+    }
+  }
+  return best;
+}
+
 int sb_allow_smem(const void* kernel, int bytes) {
   // a handful of kernels: remembered per device, so that a launch costs no driver call
   struct Seen { const void* kernel; int device; };

@@ -18,6 +18,25 @@ struct SbCrossAttention {
 int sb_xattn_args(const SbCrossAttention* g, XAttnArgs* a);
 // [T, heads, batch] rows of D 16-bit elements as a 4-D map (D, T, heads, batch) with a {64, box, 1, 1} box, 128-byte swizzle, zeros outside.
 int sb_rows_map(CUtensorMap* map, const void* ptr, int type, int D, int T, int heads, int batch, long long st, long long sh, long long sb, int box);
+struct SbClusterLaunch {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr[1];
+  SbClusterLaunch(long long tiles, int splits, int threads, int smem, cudaStream_t stream) {
+    config.gridDim = dim3((unsigned)(tiles * splits));
+    config.blockDim = dim3((unsigned)threads);
+    config.dynamicSmemBytes = (size_t)smem;
+    config.stream = stream;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = splits > 1 ? 1 : 0;
+  }
+};
+// How many blocks (1, 2, 4 or 8: a cluster) share the summed axis, `steps` long, of each of `tiles` result tiles: the number with the
+// shortest schedule.  `own`, `join`: what a block takes besides its steps, and with others for the join, in steps.  With a tile for every SM a
+// split costs more than the fuller last wave gives (dq, 4 x 1024 queries, 7500 keys, 256 tiles: 1 / 2 CTAs a tile 157 / 194 us).
+int sb_cluster_splits(const void* kernel, int threads, int smem, long long tiles, int steps, int own, int join);
 // Dynamic shared memory of a kernel, set once per kernel and device.
 int sb_allow_smem(const void* kernel, int bytes);
 

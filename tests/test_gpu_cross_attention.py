@@ -115,6 +115,35 @@ def test_backward(shape, hide, dtype):
     ops.native.check_status()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hide", ["none", "lengths", "both", "front"])
+@pytest.mark.parametrize("shape", [(1, 1, 100, 2500, 2, 1, 128), (2, 1, 70, 1100, 1, 2, 64), (1, 3, 500, 40, 1, 2, 72), (3, 1, 65, 600, 1, 1, 40)])
+def test_few_tiles_of_long_axes(shape, hide, dtype):
+    """Result tiles that several blocks share: parts of the keys that are hidden wholly, lengths that leave blocks without keys."""
+    from speech_b200 import ops
+
+    q, k, v, lengths, mask, hidden = make(*shape, dtype, "none" if hide == "front" else hide)
+    if hide == "front":
+        mask = torch.arange(k.shape[1], device="cuda")[None].expand(k.shape[0], -1) < k.shape[1] - 3
+        hidden = mask
+        k.masked_fill_(hidden[:, :, None, None], float("nan"))
+        v.masked_fill_(hidden[:, :, None, None], float("inf"))
+    dout = torch.randn(q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).to(dtype)
+    runs = []
+    for _ in range(2):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask)
+        runs.append((out.detach(),) + torch.autograd.grad(out, leaves, dout.flatten(2)))
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+    want, err, dwant, derr = plain(q, k, v, hidden, 1 / math.sqrt(q.shape[3]), dout)
+    with torch.no_grad():
+        check(ops.cross_attention(q, k, v, key_lengths=lengths, key_mask=mask).view(want.shape), want, err, "out without gradients")
+    check(runs[0][0].view(want.shape), want, err, "out")
+    for g, w, e, n in zip(runs[0][1:], dwant, derr, ("dq", "dk", "dv")):
+        check(g, w, e, n)
+    ops.native.check_status()
+
+
 @pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** 12])
 def test_fp16_gradients_of_any_size(size):
     """Upstream gradients far from one keep their precision in fp16 (score gradients are scaled)."""
