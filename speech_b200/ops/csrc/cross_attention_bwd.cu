@@ -121,7 +121,8 @@ constexpr int DQ_THREADS = 384;
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(DQ_THREADS, 1)
-xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq, const int splits) {
+xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq, const long long tile0,
+                const int splits) {
   using S = DqSmem<DP>;
   constexpr int BN = S::BN, HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -139,7 +140,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, stats = bars + 240u;      // stats: -delta of the tile's rows, largest |do| of four warps
 
   const int tiles = b.tiles;
-  const int index = blockIdx.x / splits, rank = blockIdx.x - index * splits;      // block `rank` of a cluster takes its part of the keys
+  const int local = blockIdx.x / splits, rank = blockIdx.x - local * splits;      // block `rank` of a cluster takes its part of the keys
+  const int index = (int)tile0 + local;
   const int unit = index / tiles, m = unit / a.Hk, hk = unit % a.Hk;
   const int row0 = (index - unit * tiles) * 128;
   const int len = visible_keys(a, m);
@@ -429,7 +431,7 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(DKV_THREADS, 1)
 xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
                  const __grid_constant__ CUtensorMap map_do, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dk, uint16_t* __restrict__ dv,
-                 const int splits) {
+                 const long long tile0, const int splits) {
   using S = DkvSmem<DP>;
   constexpr int BQ = S::BQ, HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -446,7 +448,8 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                  tmem_slot = bars + 8u * 21, scale_slot = tmem_slot + 4;
 
   const int ktiles = (a.Tk + 127) / 128;
-  const int index = blockIdx.x / splits, rank = blockIdx.x - index * splits;      // block `rank` of a cluster takes its part of the rows
+  const int local = blockIdx.x / splits, rank = blockIdx.x - local * splits;      // block `rank` of a cluster takes its part of the rows
+  const int index = (int)tile0 + local;
   const int unit = index / ktiles, m = unit / a.Hk, hk = unit % a.Hk;
   const int key0 = (index - unit * ktiles) * 128;
   const int len = visible_keys(a, m);
@@ -700,16 +703,16 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   b.tiles = (a.R + 127) / 128;
   const long long units = (long long)a.M * a.Hk, gq = units * b.tiles, gk = units * ((a.Tk + 127) / 128);
   if (gq > 0x7ffffffll || gk > 0x7ffffffll) return SB_BAD_ARGUMENT;
-  const int sq = dq ? sb_cluster_splits((const void*)xattn_dq_kernel<T, DP>, DQ_THREADS, DqSmem<DP>::BYTES, gq, (a.Tk + DqSmem<DP>::BN - 1) / DqSmem<DP>::BN, DQ_OWN_BLOCKS,
-                                        DQ_OWN_BLOCKS / 2) : 1;
-  SbClusterLaunch lq(gq, sq, DQ_THREADS, DqSmem<DP>::BYTES, stream);
-  rc = (int)cudaLaunchKernelEx(&lq.config, xattn_dq_kernel<T, DP>, k64, v64, a, b, (uint16_t*)dq, sq);      // also lays out the statistics
+  using DQ = DqSmem<DP>;
+  using DKV = DkvSmem<DP>;
+  SbTilePlan plan = {gq, 1};                                 // without dq only the statistics are laid out, by a block per tile
+  if (dq) plan = sb_plan_tiles((const void*)xattn_dq_kernel<T, DP>, DQ_THREADS, DQ::BYTES, gq, (a.Tk + DQ::BN - 1) / DQ::BN, DQ_OWN_BLOCKS, DQ_OWN_BLOCKS / 2);
+  rc = sb_run_tiles(plan, gq, DQ_THREADS, DQ::BYTES, stream, xattn_dq_kernel<T, DP>, k64, v64, a, b, (uint16_t*)dq);
   if (rc || !dk) return rc;
-  const long long steps = (long long)a.G * a.rep * (b.Tqp / DkvSmem<DP>::BQ);
-  const int sk = sb_cluster_splits((const void*)xattn_dkv_kernel<T, DP>, DKV_THREADS, DkvSmem<DP>::BYTES, gk, (int)(steps < 0x7fffff00 ? steps : 0x7fffff00),
-                                   DKV_OWN_STEPS, DKV_OWN_STEPS / 2);
-  SbClusterLaunch lk(gk, sk, DKV_THREADS, DkvSmem<DP>::BYTES, stream);
-  return (int)cudaLaunchKernelEx(&lk.config, xattn_dkv_kernel<T, DP>, k64, v64, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv, sk);
+  const long long steps = (long long)a.G * a.rep * (b.Tqp / DKV::BQ);
+  plan = sb_plan_tiles((const void*)xattn_dkv_kernel<T, DP>, DKV_THREADS, DKV::BYTES, gk, (int)(steps < 0x7fffff00 ? steps : 0x7fffff00), DKV_OWN_STEPS,
+                       DKV_OWN_STEPS / 2);
+  return sb_run_tiles(plan, gk, DKV_THREADS, DKV::BYTES, stream, xattn_dkv_kernel<T, DP>, k64, v64, q64, do64, a, b, (uint16_t*)dk, (uint16_t*)dv);
 }
 
 }  // namespace

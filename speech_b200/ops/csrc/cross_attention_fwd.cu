@@ -36,7 +36,7 @@ template <int DP> struct FwdSmem {
 template <typename T, int DP>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, uint16_t* __restrict__ out,
-                 uint16_t* __restrict__ rest, float* __restrict__ lse, const int splits) {
+                 uint16_t* __restrict__ rest, float* __restrict__ lse, const long long tile0, const int splits) {
   using S = FwdSmem<DP>;
   constexpr int HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -56,7 +56,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   const uint32_t q_ready = bars + 8u * 30, tmem_slot = bars + 8u * 31;
 
   const int pairs = (a.R + 255) / 256;                    // row-tile pairs of a (memory, key head): neighbours in the grid, for the L2
-  const int index = blockIdx.x / splits, rank = blockIdx.x - index * splits;      // block `rank` of a cluster takes its part of the keys
+  const int local = blockIdx.x / splits, rank = blockIdx.x - local * splits;      // block `rank` of a cluster takes its part of the keys
+  const int index = (int)tile0 + local;
   const int unit = index / pairs, m = unit / a.Hk, hk = unit % a.Hk;
   const int row0 = (index - unit * pairs) * 256;
   const int tiles = a.R - row0 > 128 ? 2 : 1;
@@ -355,9 +356,8 @@ int launch(const XAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, voi
   if (grid > 0x7ffffffll) return SB_BAD_ARGUMENT;
   const int rc = sb_allow_smem((const void*)xattn_fwd_kernel<T, DP>, FwdSmem<DP>::BYTES);
   if (rc) return rc;
-  const int splits = sb_cluster_splits((const void*)xattn_fwd_kernel<T, DP>, FWD_THREADS, FwdSmem<DP>::BYTES, grid, (a.Tk + BN - 1) / BN, OWN_BLOCKS, OWN_BLOCKS);
-  SbClusterLaunch l(grid, splits, FWD_THREADS, FwdSmem<DP>::BYTES, stream);
-  return (int)cudaLaunchKernelEx(&l.config, xattn_fwd_kernel<T, DP>, mk, mv, a, (uint16_t*)out, (uint16_t*)rest, lse, splits);
+  const SbTilePlan plan = sb_plan_tiles((const void*)xattn_fwd_kernel<T, DP>, FWD_THREADS, FwdSmem<DP>::BYTES, grid, (a.Tk + BN - 1) / BN, OWN_BLOCKS, OWN_BLOCKS);
+  return sb_run_tiles(plan, grid, FWD_THREADS, FwdSmem<DP>::BYTES, stream, xattn_fwd_kernel<T, DP>, mk, mv, a, (uint16_t*)out, (uint16_t*)rest, lse);
 }
 
 }  // namespace

@@ -78,20 +78,21 @@ int clusters_at_once(const void* kernel, int n, int threads, int smem) {
 }
 }  // namespace
 
-int sb_cluster_splits(const void* kernel, int threads, int smem, long long tiles, int steps, int own, int join) {
-  int best = 1;
-  const long long sms = sb_num_sms();
-  long long least = (tiles + sms - 1) / sms * (steps + own);
-  for (int n = 2; n <= 8 && steps >= 2 * n && tiles < sms; n *= 2) {
+SbTilePlan sb_plan_tiles(const void* kernel, int threads, int smem, long long tiles, int steps, int own, int join) {
+  SbTilePlan plan = {tiles, 1};
+  const long long sms = sb_num_sms(), left = tiles % sms;
+  if (left != tiles) join += 2;                              // a launch more
+  long long least = steps + own;
+  for (int n = 2; n <= 8 && steps >= 2 * n && left > 0; n *= 2) {
     const int at_once = clusters_at_once(kernel, n, threads, smem);
     if (at_once <= 0) break;
-    const long long cost = (tiles + at_once - 1) / at_once * ((steps + n - 1) / n + own + join);
+    const long long cost = (left + at_once - 1) / at_once * ((steps + n - 1) / n + own + join);
     if (cost < least) {
-      best = n;
+      plan = {tiles - left, n};
       least = cost;
     }
   }
-  return best;
+  return plan;
 }
 
 int sb_allow_smem(const void* kernel, int bytes) {
