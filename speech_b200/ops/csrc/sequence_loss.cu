@@ -342,8 +342,8 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 // NV = 0: rows of any length, read again for the gradient, from the L2 (148 rows of 300 KB in flight are a third of it).
 // lse: (m, log s) fp32 [rows]; logp / slope: fp32 [rows]; dlogits: contiguous [rows, V] or null (no gradient wanted now); partial:
 // fp64, per block the sum of its policy terms; ratio: fp64 [rows], preference only.
-// [rows = 110080, V = 2024, bf16, all directions: 199 us with the row read as it is needed and 64 KB less shared memory, 186 us one row ahead
-// without branches around its groups; 16 / 20 / 24 warps per SM: 186 / 246 / 281 us (spills).  Loss without a gradient: 47 and 43 us.]
+// [110080 rows of 2024, bf16, with the gradient: 199 us with the row read as it is needed, 186 us a row ahead and without branches around
+// its groups; 16 / 20 / 24 warps per SM: 186 / 246 / 281 us (spills).  27520 rows without a gradient: 16 / 20 / 24 warps 51 / 49 / 47 us.]
 template <int MODE, int TPR> constexpr int resident_warps() { return TPR == 32 && MODE == LOSS_POLICY ? 16 : TPR == 32 || TPR == 256 ? 24 : 32; }
 template <typename T, int MODE, int TPR, int NV, int THREADS, bool COUNT_HERE>
 __global__ void __launch_bounds__(THREADS, resident_warps<MODE, TPR>() * 32 / THREADS) rows_forward_kernel(const RowArgs a, int* __restrict__ count_p, float* __restrict__ logp_out, float2* __restrict__ lse_out,
