@@ -645,9 +645,10 @@ __global__ void __launch_bounds__(1024) count_kernel(const uint8_t* __restrict__
   if (threadIdx.x == 0) *count = n;
 }
 
-__global__ void policy_finish_kernel(const double* __restrict__ partial, int n, const int* __restrict__ count, float* __restrict__ loss) {
+__global__ void __launch_bounds__(1024) policy_finish_kernel(const double* __restrict__ partial, int n, const int* __restrict__ count, float* __restrict__ loss) {
   __shared__ double red[32];
   double t = 0.0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < n; i += blockDim.x) t += partial[i];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
@@ -818,7 +819,7 @@ SB_API int sb_policy_loss_fwd(const void* logits, int type, long long sn, long l
   else if (type == 2) rc = forward<float, LOSS_POLICY>(a, count, logp, lse, slope, dlogits, partial, nullptr, &blocks, stream);
   else return SB_BAD_ARGUMENT;
   if (rc) return rc;
-  policy_finish_kernel<<<1, 256, 0, stream>>>(partial, blocks, count, loss);
+  policy_finish_kernel<<<1, 1024, 0, stream>>>(partial, blocks, count, loss);
   return (int)cudaGetLastError();
 }
 
