@@ -299,35 +299,37 @@ template <int DP> __device__ __forceinline__ void add_part8(uint32_t base, int r
   }
 }
 
-// A warp zeroes the hidden rows (bits of w[0], w[1]) of a [64, DP] tile: a hidden infinity or NaN would turn its zero weight into NaN
-// inside a matrix product.  (A loop over the set bits would find them with the unit that the exponentials keep busy.)
+// A warp zeroes the hidden rows (bits of w[0], w[1]) of a [64, DP] tile, two a lane: a hidden infinity or NaN would turn its zero weight
+// into NaN inside a matrix product.
 template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, const uint32_t* w, int lane) {
-  constexpr int CH = DP / 8, RPI = 32 / CH;
-  const int sub = lane / CH, ch = lane % CH;
-#pragma unroll 4
-  for (int row = sub; row < 64; row += RPI)
-    if (((row < 32 ? w[0] : w[1]) >> (row & 31)) & 1u) st_shared_v4(tile_addr(tile, 64, row, ch), 0, 0, 0, 0);
-}
-
-// What is added to the scores of a block's 64 keys: 0, or -inf where hidden.  In shared memory, for all rows.
-__device__ __forceinline__ void store_score_mask(uint32_t addr, const uint32_t* w, int lane) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
-    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr + (uint32_t)(h * 32 + lane) * 4u), "f"((w[h] >> lane) & 1u ? -INFINITY : 0.f) : "memory");
-}
-__device__ __forceinline__ void add_score_mask(uint32_t addr, uint32_t* r) {
+    if ((w[h] >> lane) & 1u) {
 #pragma unroll
-  for (int k = 0; k < 64; k += 4) {
-    uint64_t lo, hi;
-    float x, y;
-    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(addr + k * 4));
-    split(add2(pair(r[k], r[k + 1]), lo), x, y);
-    r[k] = __float_as_uint(x);
-    r[k + 1] = __float_as_uint(y);
-    split(add2(pair(r[k + 2], r[k + 3]), hi), x, y);
-    r[k + 2] = __float_as_uint(x);
-    r[k + 3] = __float_as_uint(y);
-  }
+      for (int ch = 0; ch < DP / 8; ++ch) st_shared_v4(tile_addr(tile, 64, h * 32 + lane, ch), 0, 0, 0, 0);
+    }
+}
+
+// Hidden keys as one more step of the score product: 16 elements more per row and key, the rows' being (1, 0, ...) and the keys' (0 or -inf,
+// 0, ...), so that scores come out of the tensor core as they are or -inf (of 64 x 64 scores a warp, 32 packed additions and 16 loads
+// from shared memory less: forward / dq of 2 x 4 x 301 queries, 1111 keys, 16 heads of 64 with a mask 53 / 66 us before).  Tiles without
+// swizzle: 8 rows x 16 bytes side by side, the two halves of the 16 elements 128 bytes apart, groups of rows 256.
+constexpr int ONES_BYTES = 128 * 32, ADDEND_BYTES = 64 * 32;
+__device__ __forceinline__ uint64_t make_desc_plain(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(128 >> 4) << 16 | (uint64_t)(256 >> 4) << 32 | (uint64_t)1 << 46;
+}
+// The rows' tile, and `stages` keys' tiles as zeros behind it, by `threads` threads.
+template <typename T> __device__ __forceinline__ void init_addends(uint32_t addr, int stages, int thread, int threads) {
+  constexpr uint32_t ONE = Half2<T>::KIND == 0 ? 0x3c00u : 0x3f80u;
+  for (int i = thread; i < (ONES_BYTES + stages * ADDEND_BYTES) / 16; i += threads)
+    st_shared_v4(addr + i * 16, i < ONES_BYTES / 16 && !(i & 8) ? ONE : 0u, 0u, 0u, 0u);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// by a warp, from the block's hidden bits
+template <typename T> __device__ __forceinline__ void store_addends(uint32_t addr, const uint32_t* w, int lane) {
+  constexpr uint32_t HIDE = Half2<T>::KIND == 0 ? 0xfc00u : 0xff80u;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) st_shared_v4(addr + (uint32_t)((h * 4 + (lane >> 3)) * 256 + (lane & 7) * 16), (w[h] >> lane) & 1u ? HIDE : 0u, 0u, 0u, 0u);
 }
 
 }  // namespace

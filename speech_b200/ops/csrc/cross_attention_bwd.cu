@@ -113,7 +113,9 @@ template <int DP> struct DqSmem {
   static constexpr int STAGES = 5;
   static constexpr int ROWS = 128 * DP * 2, KEYS = BN * DP * 2;
   static constexpr int DO0 = ROWS, KV0 = 2 * ROWS, BAR = KV0 + STAGES * 2 * KEYS;
-  static constexpr int MASK0 = BAR + 768, BYTES = MASK0 + STAGES * BN * 4 + 1024;
+  static constexpr int ONES0 = 0, ADD0 = ONES0 + ONES_BYTES;        // where the queries were, once they are in tensor memory
+  static constexpr int BYTES = BAR + 768 + 1024;
+  static_assert(ADD0 + STAGES * ADDEND_BYTES <= ROWS, "");
   // tensor memory: dq, q, do, scores of even and odd blocks, dp, ds of even and odd blocks
   static constexpr int Q_COL = DP, DO_COL = DP + DP / 2, S_COL = 2 * DP, DP_COL = S_COL + 128, DS_COL = DP_COL + 64;
 };
@@ -191,6 +193,11 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     bool ok = true;
     for (; issued < nt && issued < S::STAGES - 2 && ok; ++issued) ok = load(issued);
     bool hid[2] = {hidden_key(a, m, len, first + lane), hidden_key(a, m, len, first + 32 + lane)};      // this lane's keys of block j, read a block ahead
+    if (nt > 0 && ok && (hide || first + nt * BN > len)) {
+      ok = warp_wait(rows_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (ok) init_addends<T>(base + S::ONES0, S::STAGES, lane, 32);
+      __syncwarp();
+    }
     for (int j = 0; j < nt && ok; ++j) {
       const int s = j % S::STAGES;
       const bool some = hide || first + (j + 1) * BN > len;
@@ -206,7 +213,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (some) {
         clear_rows<DP>(base + S::KV0 + s * 2 * S::KEYS, w, lane);
         clear_rows<DP>(base + S::KV0 + s * 2 * S::KEYS + S::KEYS, w, lane);
-        store_score_mask(base + S::MASK0 + s * BN * 4, w, lane);
+        store_addends<T>(base + S::ADD0 + s * ADDEND_BYTES, w, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -241,6 +248,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
 #pragma unroll
         for (int kk = 0; kk < DP / 16; ++kk)
           umma_ts(d, rows + kk * 8, kd + st + (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0);
+        if (!second && (hide || first + (j + 1) * BN > len))
+          umma_bf16(d, make_desc_plain(base + S::ONES0), make_desc_plain(base + S::ADD0 + s * ADDEND_BYTES), idesc_s, 1);
         umma_commit(second ? dp_full(j & 1) : s_full(j & 1));
       }
       __syncwarp();
@@ -337,11 +346,6 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         ok = warp_wait(ds_read(wg), ph ^ 1u, a.status, SB_TIMEOUT_TMEM_FULL);
         if (!ok) break;
         tc_fence_after();
-      }
-      if (hide || first + (j + 1) * BN > len) {
-        ok = warp_wait(kv_clean(j % S::STAGES), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
-        if (!ok) break;
-        add_score_mask(base + S::MASK0 + (j % S::STAGES) * BN * 4, r);
       }
 #pragma unroll
       for (int k = 0; k < 64; k += 2) {                    // p over s

@@ -30,7 +30,7 @@ template <int DP> struct FwdSmem {
   static constexpr int STAGES = 4;
   static constexpr int TILE = 128 * DP * 2, KEYS = BN * DP * 2;      // 128 query rows, a block of keys or values
   static constexpr int K0 = 2 * TILE, V0 = K0 + STAGES * KEYS, BAR = V0 + STAGES * KEYS;
-  static constexpr int MASK0 = BAR + 512, BYTES = MASK0 + STAGES * BN * 4 + 1024;
+  static constexpr int ONES0 = BAR + 512, ADD0 = ONES0 + ONES_BYTES, BYTES = ADD0 + STAGES * ADDEND_BYTES + 1024;
 };
 
 template <typename T, int DP>
@@ -66,6 +66,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   const int nt = min(share, max(0, blocks - rank * share));
   const bool hide = a.mask != nullptr;
 
+  init_addends<T>(base + S::ONES0, S::STAGES, threadIdx.x, FWD_THREADS);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(k_full(s), 1); mbar_init(k_clean(s), 1); mbar_init(k_empty(s), tiles);
@@ -134,6 +135,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           const uint64_t ro = (uint64_t)(((kk >> 2) * 16384 + (kk & 3) * 32) >> 4), ko = (uint64_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4);
           umma_bf16(tmem + t * 128 + (j & 1) * 64, qd + ro, kd + st + ko, idesc_s, kk > 0);
         }
+        if (hide || first + (j + 1) * BN > len)
+          umma_bf16(tmem + t * 128 + (j & 1) * 64, make_desc_plain(base + S::ONES0), make_desc_plain(base + S::ADD0 + (j % S::STAGES) * ADDEND_BYTES), idesc_s, 1);
         umma_commit(s_full(t, j & 1));
         umma_commit(k_empty(j % S::STAGES));
       }
@@ -184,6 +187,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (!warp_wait(k_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
       if (some) {
         clear_rows<DP>(base + S::K0 + s * S::KEYS, w, lane);
+        store_addends<T>(base + S::ADD0 + s * ADDEND_BYTES, w, lane);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -191,7 +195,6 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (!warp_wait(v_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
       if (some) {
         clear_rows<DP>(base + S::V0 + s * S::KEYS, w, lane);
-        store_score_mask(base + S::MASK0 + s * BN * 4, w, lane);      // lives as long as the values: until the block's second product
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -219,11 +222,6 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       tc_fence_after();
       uint32_t r[BN];
       tmem_load64(s_addr, r);
-      if (hide || first + (j + 1) * BN > len) {
-        ok = warp_wait(v_clean(j % S::STAGES), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
-        if (!ok) break;
-        add_score_mask(base + S::MASK0 + (j % S::STAGES) * BN * 4, r);
-      }
       float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
       for (int k = 0; k < BN; k += 8)
