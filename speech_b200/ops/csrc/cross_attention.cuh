@@ -312,7 +312,7 @@ template <int DP> __device__ __forceinline__ void clear_rows(uint32_t tile, cons
 
 // Hidden keys as one more step of the score product: 16 elements more per row and key, the rows' being (1, 0, ...) and the keys' (0 or -inf,
 // 0, ...), so that scores come out of the tensor core as they are or -inf (of 64 x 64 scores a warp, 32 packed additions and 16 loads
-// from shared memory less: forward / dq of 2 x 4 x 301 queries, 1111 keys, 16 heads of 64 with a mask 53 / 66 us before).  Tiles without
+// from shared memory less: forward / dq of 2 x 4 x 301 queries, 1111 keys, 16 heads of 64 on 4 with a mask 46 / 58 us for 53 / 66).  Tiles without
 // swizzle: 8 rows x 16 bytes side by side, the two halves of the 16 elements 128 bytes apart, groups of rows 256.
 constexpr int ONES_BYTES = 128 * 32, ADDEND_BYTES = 64 * 32;
 __device__ __forceinline__ uint64_t make_desc_plain(uint32_t addr) {
