@@ -123,8 +123,8 @@ constexpr int DQ_THREADS = 384;
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(DQ_THREADS, 1)
-xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b, uint16_t* __restrict__ dq, const long long tile0,
-                const int splits) {
+xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, const BwdArgs b,
+                uint16_t* __restrict__ dq, const long long tile0, const int splits) {
   using S = DqSmem<DP>;
   constexpr int BN = S::BN, HALVES = DP / 64;
   extern __shared__ uint8_t smem_raw[];
@@ -139,7 +139,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   auto ds_read = [&](int u) { return bars + 8u * (16 + u); };
   auto dp_full = [&](int u) { return bars + 8u * (18 + u); };     // one per warpgroup: each sees every other block only
   auto kv_clean = [&](int s) { return bars + 8u * (24 + s); };
-  const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23, stats = bars + 240u;      // stats: -delta of the tile's rows, largest |do| of four warps
+  const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23;
+  const uint32_t stats = bars + 240u;                      // -delta of the tile's rows, peaks of four warps
 
   const int tiles = b.tiles;
   const int local = blockIdx.x / splits, rank = blockIdx.x - local * splits;      // block `rank` of a cluster takes its part of the keys
@@ -504,7 +505,8 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     __syncwarp();
     const int seg = step0 / lines;
-    int s = 0, issued = 0, t0 = (step0 - seg * lines) * BQ, g = seg / a.rep, head = seg - g * a.rep;      // step step0 + i: rows t0 .. of head hk * rep + head of batch row m * G + g
+    // step step0 + i: rows t0 .. of head hk * rep + head of batch row m * G + g
+    int s = 0, issued = 0, t0 = (step0 - seg * lines) * BQ, g = seg / a.rep, head = seg - g * a.rep;
     uint32_t ph = 0;
     for (int i = 0; i < nq; ++i) {
       if (!warp_wait(q_empty(s), ph ^ 1u, a.status, SB_TIMEOUT_SMEM_EMPTY)) break;
@@ -724,8 +726,8 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
 // out, rest, dout: contiguous [B, Tq, H, D]; out, rest, lse: the forward pass's; ws: 2 * B * H * (Tq rounded up to 64) floats and
 // one per 128 packed rows of every (memory, key head); dq [B, Tq, H, D] or null; dk, dv
 // [M, Tk, Hk, D], both or neither.
-SB_API int sb_cross_attention_bwd(const SbCrossAttention* g, const void* out, const void* rest, const void* dout, const float* lse, float* ws, void* dq, void* dk, void* dv,
-                                  cudaStream_t stream) {
+SB_API int sb_cross_attention_bwd(const SbCrossAttention* g, const void* out, const void* rest, const void* dout, const float* lse, float* ws, void* dq,
+                                  void* dk, void* dv, cudaStream_t stream) {
   XAttnArgs a;
   const int rc = sb_xattn_args(g, &a);
   if (rc) return rc;

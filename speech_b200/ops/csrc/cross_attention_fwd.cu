@@ -7,8 +7,8 @@
 // A CTA takes two tiles of 128 packed rows and streams blocks of 64 keys of its memory and key head past both, so that keys and values
 // cross the L2 once per 256 rows.  Warp 0 loads keys and values by TMA, warps 1 and 3 issue the tcgen05.mma of a tile each, warp 2
 // clears the rows of hidden keys and lays out their addends (one more step of the score product), and one warpgroup per row tile does the
-// softmax: scores and output accumulate in tensor memory (per tile two buffers of 64 columns and DP columns), the probabilities go back there as 16-bit pairs over the scores they came from and are the A operand of
-// the second product.  The scores of the next block are there before the softmax of this one ends; with one buffer of 128 keys the
+// softmax: scores and output accumulate in tensor memory (per tile two buffers of 64 columns and DP columns), the probabilities go back
+// there as 16-bit pairs over the scores they came from and are the A operand of the second product.  The scores of the next block are there before the softmax of this one ends; with one buffer of 128 keys the
 // warpgroups waited for the tensor core and it for them (41 % of its cycles busy).  The output is rescaled only when a row's maximum
 // has grown by more than 2^8 since the last time; p then stays below 2^8, and the result does not depend on it beyond rounding.
 // Where there are fewer tile pairs than SMs, up to eight CTAs of a cluster share one, each with its part of the keys; unnormalised outputs
@@ -164,7 +164,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
       __syncwarp();
       if (j + 2 < nt) {
-        ok = warp_wait(hide || first + (j + 3) * BN > len ? k_clean((j + 2) % S::STAGES) : k_full((j + 2) % S::STAGES), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+        const int s2 = (j + 2) % S::STAGES;
+        ok = warp_wait(hide || first + (j + 3) * BN > len ? k_clean(s2) : k_full(s2), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
         if (!ok) break;
         tc_fence_after();
         scores(j + 2);

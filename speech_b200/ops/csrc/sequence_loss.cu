@@ -346,9 +346,9 @@ __device__ __forceinline__ void copy_async(void* to, const void* from) {
 // its groups; 16 / 20 / 24 warps per SM: 186 / 246 / 281 us (spills).  27520 rows without a gradient: 16 / 20 / 24 warps 51 / 49 / 47 us.]
 template <int MODE, int TPR> constexpr int resident_warps() { return TPR == 32 && MODE == LOSS_POLICY ? 16 : TPR == 32 || TPR == 256 ? 24 : 32; }
 template <typename T, int MODE, int TPR, int NV, int THREADS, bool COUNT_HERE>
-__global__ void __launch_bounds__(THREADS, resident_warps<MODE, TPR>() * 32 / THREADS) rows_forward_kernel(const RowArgs a, int* __restrict__ count_p, float* __restrict__ logp_out, float2* __restrict__ lse_out,
-                                                               float* __restrict__ slope_out, void* __restrict__ dlogits, double* __restrict__ partial,
-                                                               double* __restrict__ ratio) {
+__global__ void __launch_bounds__(THREADS, resident_warps<MODE, TPR>() * 32 / THREADS)
+rows_forward_kernel(const RowArgs a, int* __restrict__ count_p, float* __restrict__ logp_out, float2* __restrict__ lse_out, float* __restrict__ slope_out,
+                    void* __restrict__ dlogits, double* __restrict__ partial, double* __restrict__ ratio) {
   constexpr int E = Vec<T>::N, GROUPS = THREADS / TPR;
   __shared__ float redf[32];
   __shared__ double redd[32];
@@ -700,8 +700,9 @@ __device__ void ratio_sums(const double* __restrict__ ratio, long long per, int 
 }
 
 // Scalar losses of all pairs, their mean, rewards beta * ratio and the slope of every sequence's positions.  One block.
-__global__ void __launch_bounds__(1024) preference_finish_kernel(const double* __restrict__ ratio, long long per, double* total, int pairs, int kind, float beta_f, const float* __restrict__ gap,
-                                         float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ seq_slope) {
+__global__ void __launch_bounds__(1024)
+preference_finish_kernel(const double* __restrict__ ratio, long long per, double* total, int pairs, int kind, float beta_f, const float* __restrict__ gap,
+                         float* __restrict__ loss, float* __restrict__ rewards, float* __restrict__ seq_slope) {
   __shared__ double red[32];
   const double beta = (double)beta_f;
   double mine = 0.0;

@@ -184,7 +184,8 @@ __global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step
     uint4 v = make_uint4(0, 0, 0, 0);
     if (r < s.R && qc * 8 < a.D) {
       const int y = r / a.Tq, t = r - y * a.Tq, gr = y / a.rep;
-      v = *reinterpret_cast<const uint4*>(a.q + (long long)(mem * s.rows_per + gr) * a.q_sb + (long long)t * a.q_st + (long long)(hk * a.rep + y - gr * a.rep) * a.q_sh + qc * 8);
+      v = *reinterpret_cast<const uint4*>(a.q + (long long)(mem * s.rows_per + gr) * a.q_sb + (long long)t * a.q_st +
+                                          (long long)(hk * a.rep + y - gr * a.rep) * a.q_sh + qc * 8);
     }
     st_shared_v4(row_addr<DP>(qs, lr, qc), v.x, v.y, v.z, v.w);
   }
