@@ -3,7 +3,7 @@
 #include "cross_attention.cuh"
 #include <math.h>
 
-// Mirrored by a ctypes structure in native_cross_attention.py; strides in elements.
+// Packed field by field in native_cross_attention.py; strides in elements.
 struct SbCrossAttention {
   const void *q, *k, *v;
   long long q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh;

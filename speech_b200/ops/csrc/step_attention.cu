@@ -551,7 +551,7 @@ SB_API long long sb_cross_attention_workspace(const SbCrossAttention* g) {
   return sb_few_rows(g) ? workspace(a) : 0;
 }
 
-// Own caches of a shared-prefix call; mirrored in native_cross_attention.py.
+// Own caches of a shared-prefix call; packed field by field in native_cross_attention.py.
 struct SbOwnCache {
   const void *k, *v;
   long long k_sb, k_st, k_sh, v_sb, v_st, v_sh;

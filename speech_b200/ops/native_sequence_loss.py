@@ -100,7 +100,7 @@ def _policy_backward(ctx, dloss, _):
     out, ctx.grad = ctx.grad, None
     first = out is not None
     if not first:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = logits.new_empty(logits.shape)
     lse = ctx.kept.data_ptr() + 8 * _blocks() + 8
     return _gradient(dloss, logits, targets, mask, lse, lse + 8 * targets.numel(), 0, out, int(first)), None, None, None, None, None, None, None, None, None
 
@@ -111,13 +111,13 @@ class _PolicyLossFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, targets, mask, old, adv, ref, lo, hi, kl_beta, want_grad):
-        dev, rows = logits.device, targets.numel()
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        logp = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-        kept = torch.empty(2 * _blocks() + 2 + 3 * rows, dtype=torch.float32, device=dev)       # fp64 sums of the blocks and the count, lse (two parts), slopes
+        rows = targets.numel()
+        loss = logits.new_empty((), dtype=torch.float32)
+        logp = logits.new_empty(targets.shape, dtype=torch.float32)
+        kept = logits.new_empty(2 * _blocks() + 2 + 3 * rows, dtype=torch.float32)       # fp64 sums of the blocks and the count, lse (two parts), slopes
         ws = kept.data_ptr()
         lse = ws + 8 * _blocks() + 8
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
+        grad = logits.new_empty(logits.shape) if want_grad else None
         layout, sizes = _layout(logits)
         N._check(bind("sb_policy_loss_fwd")(logits.data_ptr(), *layout, targets.data_ptr(), address(mask), old.data_ptr(), address(ref), adv.data_ptr(), *sizes,
                                             lo, hi, kl_beta, ws + 8 * _blocks(), ws, loss.data_ptr(), logp.data_ptr(), lse, lse + 8 * rows, address(grad),
@@ -138,18 +138,18 @@ def _preference_backward(ctx, dloss, _):
     logits, targets, mask = ctx.saved_tensors
     rows = targets.numel()
     lse = ctx.kept.data_ptr() + 8 * (rows + logits.shape[0])
-    out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    out = logits.new_empty(logits.shape)
     return _gradient(dloss, logits, targets, mask, lse, 0, lse + 8 * rows, out, 0), None, None, None, None, None, None
 
 
 class _PreferenceLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, mask, ref, beta, kind, gap):
-        dev, rows, n = logits.device, targets.numel(), logits.shape[0]
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        rewards = torch.empty(n, dtype=torch.float32, device=dev)
+        rows, n = targets.numel(), logits.shape[0]
+        loss = logits.new_empty((), dtype=torch.float32)
+        rewards = logits.new_empty(n, dtype=torch.float32)
         # log ratios of the positions and of the sequences (fp64), lse (two parts) and the slopes of the sequences (fp32)
-        ctx.kept = torch.empty(4 * rows + 3 * n, dtype=torch.float32, device=dev)
+        ctx.kept = logits.new_empty(4 * rows + 3 * n, dtype=torch.float32)
         ws = ctx.kept.data_ptr()
         lse = ws + 8 * (rows + n)
         layout, sizes = _layout(logits)
