@@ -117,7 +117,8 @@ def test_backward(shape, hide, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("hide", ["none", "lengths", "both", "front"])
-@pytest.mark.parametrize("shape", [(1, 1, 100, 2500, 2, 1, 128), (2, 1, 70, 1100, 1, 2, 64), (1, 3, 500, 40, 1, 2, 72), (3, 1, 65, 600, 1, 1, 40)])
+@pytest.mark.parametrize("shape", [(1, 1, 100, 2500, 2, 1, 128), (2, 1, 70, 1100, 1, 2, 64), (1, 3, 500, 40, 1, 2, 72), (3, 1, 65, 600, 1, 1, 40),
+                                   (38, 1, 65, 2500, 4, 1, 40)])           # 152 tiles: 148 blocks and four clusters
 def test_few_tiles_of_long_axes(shape, hide, dtype):
     """Result tiles that several blocks share: parts of the keys that are hidden wholly, lengths that leave blocks without keys."""
     from speech_b200 import ops
