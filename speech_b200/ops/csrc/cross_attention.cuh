@@ -263,8 +263,8 @@ __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.a
 template <int DP> __device__ __forceinline__ uint32_t part_addr(uint32_t base, int row, int piece) {
   return base + (uint32_t)row * (uint32_t)(DP * 4) + (uint32_t)((piece & ~7) | ((piece ^ row) & 7)) * 16u;
 }
-// 64 accumulator columns of this lane's row (zeros unless `have`)
-template <int DP> __device__ __forceinline__ void keep_part64(uint32_t base, int row, int col, uint32_t taddr, bool have) {
+// 64 accumulator columns of this lane's row; zeros unless `have` (for the warp) and where `zero` (for the lane)
+template <int DP> __device__ __forceinline__ void keep_part64(uint32_t base, int row, int col, uint32_t taddr, bool have, bool zero = false) {
   uint32_t r[64];
   if (have) {
     tmem_load64(taddr, r);
@@ -272,6 +272,8 @@ template <int DP> __device__ __forceinline__ void keep_part64(uint32_t base, int
 #pragma unroll
     for (int k = 0; k < 64; ++k) r[k] = 0u;
   }
+#pragma unroll
+  for (int k = 0; k < 64; ++k) r[k] = zero ? 0u : r[k];
 #pragma unroll
   for (int k = 0; k < 16; ++k) st_shared_v4(part_addr<DP>(base, row, col / 4 + k), r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
 }

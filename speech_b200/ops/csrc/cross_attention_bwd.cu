@@ -92,9 +92,10 @@ template <typename T, int DP> __device__ __forceinline__ void join_parts8(uint32
                                               Half2<T>::pack(o[6] * f, o[7] * f));
 }
 
-// 64 accumulator columns of a warp's 32 rows, times f, rounded and written.
+// 64 accumulator columns of a warp's 32 rows, times f, rounded and written; zeros unless `have`, and in the lanes' rows with `zero`.
 template <typename T>
-__device__ __forceinline__ void store_acc64(uint32_t buf, uint32_t taddr, bool have, float f, uint16_t* dst, long long off, int col, int D, int lane) {
+__device__ __forceinline__ void store_acc64(uint32_t buf, uint32_t taddr, bool have, float f, uint16_t* dst, long long off, int col, int D, int lane,
+                                            bool zero = false) {
   uint32_t r[64], v[32];
   if (have) {
     tmem_load64(taddr, r);
@@ -103,7 +104,7 @@ __device__ __forceinline__ void store_acc64(uint32_t buf, uint32_t taddr, bool h
     for (int k = 0; k < 64; ++k) r[k] = 0u;
   }
 #pragma unroll
-  for (int k = 0; k < 32; ++k) v[k] = Half2<T>::pack(__uint_as_float(r[2 * k]) * f, __uint_as_float(r[2 * k + 1]) * f);
+  for (int k = 0; k < 32; ++k) v[k] = zero ? 0u : Half2<T>::pack(__uint_as_float(r[2 * k]) * f, __uint_as_float(r[2 * k + 1]) * f);
   store_rows64(buf, v, dst, off, col, D, lane);
 }
 
@@ -140,6 +141,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   auto dp_full = [&](int u) { return bars + 8u * (18 + u); };     // one per warpgroup: each sees every other block only
   auto kv_clean = [&](int s) { return bars + 8u * (24 + s); };
   const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23;
+  const uint32_t seen_slot = bars + 8u * 29;               // whether the mask leaves any of these keys
   const uint32_t stats = bars + 240u;                      // -delta of the tile's rows, peaks of four warps
 
   const int tiles = b.tiles;
@@ -199,6 +201,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (ok) init_addends<T>(base + S::ONES0, S::STAGES, lane, 32);
       __syncwarp();
     }
+    bool seen = false;
     for (int j = 0; j < nt && ok; ++j) {
       const int s = j % S::STAGES;
       const bool some = hide || first + (j + 1) * BN > len;
@@ -215,6 +218,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         clear_rows<DP>(base + S::KV0 + s * 2 * S::KEYS, w, lane);
         clear_rows<DP>(base + S::KV0 + s * 2 * S::KEYS + S::KEYS, w, lane);
         store_addends<T>(base + S::ADD0 + s * ADDEND_BYTES, w, lane);
+        seen |= (w[0] & w[1]) != 0xffffffffu;
+        if (j == nt - 1 && lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(seen_slot), "r"((uint32_t)seen) : "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -388,6 +393,12 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
     if (nt > 0 && ok) ok = warp_wait(dq_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
+    if (hide && nt > 0 && ok) {                              // zero where the mask leaves nothing, whatever the query holds
+      uint32_t seen = 1;
+      ok = warp_wait(kv_clean((nt - 1) % S::STAGES), (uint32_t)((nt - 1) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (ok) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(seen) : "r"(seen_slot) : "memory");
+      ok = ok && seen;
+    }
     if (splits > 1) {
       if (wg < DP / 64) keep_part64<DP>(base, quarter * 32 + lane, 64 * wg, lane_base + 64 * wg, nt > 0 && ok);
     } else if (dq && wg < DP / 64) {                       // 64 columns a warpgroup
@@ -670,11 +681,12 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     tc_fence_after();
     // dv by two warpgroups, dk by the others, 64 columns each (DP = 64: one of the two)
     if (splits > 1) {
-      if (half < DP / 64) keep_part64<DP>(base + u * 128 * DP * 4, quarter * 32 + lane, half * 64, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok);
+      if (half < DP / 64) keep_part64<DP>(base + u * 128 * DP * 4, quarter * 32 + lane, half * 64, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok,
+                                        hidden);
     } else if (half < DP / 64) {
       const long long off = key < a.Tk ? (((long long)m * a.Tk + key) * a.Hk + hk) * a.D : -1;
       store_acc64<T>(base + ((u * 2 + half) * 4 + quarter) * 4096, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok, u ? b.scale / dsf : ex2(-p_shift<T>()),
-                     u ? dk : dv, off, half * 64, a.D, lane);
+                     u ? dk : dv, off, half * 64, a.D, lane, hidden);      // its weights' zeros may have met infinite queries
     }
   }
   if (splits > 1) {

@@ -53,7 +53,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto p_full = [&](int t, int u) { return bars + 8u * (24 + 2 * t + u); };
   auto pv_done = [&](int t) { return bars + 8u * (28 + t); };   // every block's product: at most one is outstanding when it is waited for
   auto o_full = [&](int t) { return bars + 8u * (32 + t); };    // the last one
-  const uint32_t q_ready = bars + 8u * 30, tmem_slot = bars + 8u * 31;
+  const uint32_t q_ready = bars + 8u * 30, tmem_slot = bars + 8u * 31, seen_slot = bars + 8u * 40;      // seen: whether the mask leaves any of these keys
 
   const int pairs = (a.R + 255) / 256;                    // row-tile pairs of a (memory, key head): neighbours in the grid, for the L2
   const int local = blockIdx.x / splits, rank = blockIdx.x - local * splits;      // block `rank` of a cluster takes its part of the keys
@@ -176,6 +176,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     int s = 0;
     uint32_t ph = 0;
     bool hid[2] = {hidden_key(a, m, len, first + lane), hidden_key(a, m, len, first + 32 + lane)};      // this lane's keys of block j, read a block ahead
+    bool seen = false;
     for (int j = 0; j < nt; ++j) {
       const bool some = hide || first + (j + 1) * BN > len;
       uint32_t w[2] = {0, 0};
@@ -196,6 +197,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (!warp_wait(v_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
       if (some) {
         clear_rows<DP>(base + S::V0 + s * S::KEYS, w, lane);
+        seen |= (w[0] & w[1]) != 0xffffffffu;
+        if (j == nt - 1 && lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(seen_slot), "r"((uint32_t)seen) : "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
@@ -289,6 +292,17 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (nt > 0 && ok) ok = warp_wait(o_full(t), 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
+    if (hide && nt > 0 && ok) {
+      // a mask that leaves nothing: the output is zero whatever the query holds (its infinities met the cleared keys' zeros)
+      uint32_t seen = 1;
+      ok = warp_wait(v_clean((nt - 1) % S::STAGES), (uint32_t)((nt - 1) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+      if (ok) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(seen) : "r"(seen_slot) : "memory");
+      if (!seen) {
+        mx = -INFINITY;
+        l = 0.f;
+        ok = false;
+      }
+    }
     if (splits > 1) {
       asm volatile("bar.sync 2, %0;" ::"r"(tiles * 128) : "memory");     // no product of either tile reads shared memory any more
       const int r = t * 128 + quarter * 32 + lane;

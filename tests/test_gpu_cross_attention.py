@@ -145,6 +145,28 @@ def test_few_tiles_of_long_axes(shape, hide, dtype):
     ops.native.check_status()
 
 
+@pytest.mark.parametrize("tq", [1, 70, 300])
+@pytest.mark.parametrize("tk", [50, 1100])
+def test_queries_of_any_value_that_see_nothing(tq, tk):
+    """A query that sees no key gets zeros, and no gradient, also where it is infinite or NaN; the other memories' rows are as ever."""
+    from speech_b200 import ops
+
+    q, k, v, lengths, mask, hidden = make(3, 2, tq, tk, 2, 1, 64, torch.bfloat16, "both")       # memory 1 is masked wholly, memory 2 has no length
+    with torch.no_grad():
+        want = ops.cross_attention(q, k, v, key_lengths=lengths, key_mask=mask)
+    q = q.clone()
+    q[2:, :, 0] = float("inf")
+    q[2:, :, 1] = float("nan")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask)
+    with torch.no_grad():
+        again = ops.cross_attention(q, k, v, key_lengths=lengths, key_mask=mask)
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert torch.equal(out, want) and torch.equal(again, want) and bool((out[2:] == 0).all())
+    assert all(bool(torch.isfinite(g).all()) for g in grads) and bool((grads[0][2:] == 0).all())
+    assert bool((grads[1][1:] == 0).all()) and bool((grads[2][1:] == 0).all())
+
+
 @pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** 12])
 def test_fp16_gradients_of_any_size(size):
     """Upstream gradients far from one keep their precision in fp16 (score gradients are scaled)."""
