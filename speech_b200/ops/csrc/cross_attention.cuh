@@ -152,6 +152,24 @@ __device__ __forceinline__ bool hidden_key(const XAttnArgs& a, int m, int len, i
   return key >= len || (a.mask && a.mask[(long long)m * a.Tk + key] != 0);
 }
 
+// By a warp: whether the mask leaves exactly one of memory m's keys.  Its softmax is then constant, and dq and dk are zero; p (dp - delta) from
+// rounded p and delta would be their rounding.  Ends with the second visible key, so that only a memory that is hidden nearly wholly is read to
+// its end.
+__device__ __forceinline__ bool one_key_left(const XAttnArgs& a, int m, int len, int lane) {
+  const uint8_t* mask = a.mask + (long long)m * a.Tk;
+  int n = 0;
+  for (int k0 = 0; k0 < len && n < 2; k0 += 512) {
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int key = k0 + 32 * i + lane;
+      mine += key < len && mask[key] == 0;
+    }
+    n += __reduce_add_sync(0xffffffffu, mine);
+  }
+  return n == 1;
+}
+
 // Rows of a [rows, DP] operand tile in shared memory: 64-element halves of 128-byte rows, 16-byte chunks XORed with the row (the
 // 128-byte swizzle of TMA and of the matrix descriptors).
 __device__ __forceinline__ uint32_t tile_addr(uint32_t base, int rows, int row, int chunk) {

@@ -19,6 +19,9 @@
 // Where there are fewer tiles than SMs, up to eight CTAs of a cluster share one (keys of dq, query rows of dk / dv in parts) and add their
 // fp32 sums up through one another's shared memory, in a fixed order.
 //
+// A softmax over one key is constant: dq and dk of a memory with one visible key are multiplied by zero at the end (of its NaN and
+// infinities they keep the NaN).
+//
 // Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
 // matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do|, or a 64th of the largest
 // |delta| where the values are that large, to [8, 16), and the sums are scaled back, so that neither small weights nor small upstream
@@ -142,6 +145,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   auto kv_clean = [&](int s) { return bars + 8u * (24 + s); };
   const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23;
   const uint32_t seen_slot = bars + 8u * 29;               // whether the mask leaves any of these keys
+  const uint32_t one_slot = seen_slot + 4;                 // whether it leaves just one of the memory's
   const uint32_t stats = bars + 240u;                      // -delta of the tile's rows, peaks of four warps
 
   const int tiles = b.tiles;
@@ -263,6 +267,12 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     }
   } else if (warp == 2) {
     // dq += ds k
+    if (hide) {
+      const bool one = one_key_left(a, m, len, lane);
+      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(one_slot), "r"((uint32_t)one) : "memory");
+      __syncwarp();
+      asm volatile("bar.arrive 2, 288;" ::: "memory");
+    }
     constexpr uint32_t idesc_o = instr_desc<T>(DP, true);
     const uint64_t kn = make_desc(base + S::KV0, BN * 128, 1024);
     bool ok = true;
@@ -399,11 +409,18 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (ok) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(seen) : "r"(seen_slot) : "memory");
       ok = ok && seen;
     }
+    bool one = len == 1;
+    if (hide) {
+      asm volatile("bar.sync 2, 288;" ::: "memory");         // with warp 2
+      uint32_t v;
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(one_slot) : "memory");
+      one = v != 0;
+    }
     if (splits > 1) {
       if (wg < DP / 64) keep_part64<DP>(base, quarter * 32 + lane, 64 * wg, lane_base + 64 * wg, nt > 0 && ok);
     } else if (dq && wg < DP / 64) {                       // 64 columns a warpgroup
       const long long off = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
-      store_acc64<T>(base + (wg * 4 + quarter) * 4096, lane_base + 64 * wg, nt > 0 && ok, b.scale / dsf, dq, off, 64 * wg, a.D, lane);
+      store_acc64<T>(base + (wg * 4 + quarter) * 4096, lane_base + 64 * wg, nt > 0 && ok, one ? 0.f : b.scale / dsf, dq, off, 64 * wg, a.D, lane);
     }
   }
   if (splits > 1) {                                        // only with dq
@@ -416,7 +433,9 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       asm volatile("ld.shared.f32 %0, [%1];" : "=f"(p) : "r"(stats + (128 + i) * 4) : "memory");
       peak = fmaxf(peak, p);
     }
-    const float f = b.scale / ds_scale<T>(peak);
+    uint32_t one = len == 1;
+    if (hide) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(one) : "r"(one_slot) : "memory");
+    const float f = one ? 0.f : b.scale / ds_scale<T>(peak);
     constexpr int CH = DP / 8;
     for (int x = rank * DQ_THREADS + threadIdx.x; x < 128 * CH; x += splits * DQ_THREADS) {
       const int r = x / CH, c8 = x % CH;
@@ -462,6 +481,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto p_read = [&](int u) { return bars + 8u * (14 + u); };
   const uint32_t s_read = bars + 8u * 16, dp_read = bars + 8u * 17, kv_full = bars + 8u * 18, kv_tmem = bars + 8u * 19, d_full = bars + 8u * 20,
                  tmem_slot = bars + 8u * 21, scale_slot = tmem_slot + 4;
+  const uint32_t one_slot = bars + 8u * 22;                // whether the mask leaves just one of the memory's keys
 
   const int ktiles = (a.Tk + 127) / 128;
   const int local = blockIdx.x / splits, rank = blockIdx.x - local * splits;      // block `rank` of a cluster takes its part of the rows
@@ -575,6 +595,12 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
   } else if (warp == 3) {
     // ---------------------------------------------------------------- dv += p^T do, dk += ds^T q
+    if (a.mask) {
+      const bool one = one_key_left(a, m, len, lane);
+      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(one_slot), "r"((uint32_t)one) : "memory");
+      __syncwarp();
+      asm volatile("bar.arrive 1, 544;" ::: "memory");
+    }
     constexpr uint32_t idesc_o = instr_desc<T>(DP, true);
     const uint64_t qn = make_desc(base + S::Q0, BQ * 128, 1024);
     bool ok = true;
@@ -679,14 +705,22 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (nq > 0 && ok) ok = warp_wait(d_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
+    bool one = len == 1;
+    if (a.mask) {
+      asm volatile("bar.sync 1, 544;" ::: "memory");         // with warp 3
+      uint32_t v;
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(one_slot) : "memory");
+      one = v != 0;
+    }
     // dv by two warpgroups, dk by the others, 64 columns each (DP = 64: one of the two)
     if (splits > 1) {
       if (half < DP / 64) keep_part64<DP>(base + u * 128 * DP * 4, quarter * 32 + lane, half * 64, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok,
                                         hidden);
     } else if (half < DP / 64) {
       const long long off = key < a.Tk ? (((long long)m * a.Tk + key) * a.Hk + hk) * a.D : -1;
-      store_acc64<T>(base + ((u * 2 + half) * 4 + quarter) * 4096, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok, u ? b.scale / dsf : ex2(-p_shift<T>()),
-                     u ? dk : dv, off, half * 64, a.D, lane, hidden);      // its weights' zeros may have met infinite queries
+      store_acc64<T>(base + ((u * 2 + half) * 4 + quarter) * 4096, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok,
+                     u ? (one ? 0.f : b.scale / dsf) : ex2(-p_shift<T>()), u ? dk : dv, off, half * 64, a.D, lane,
+                     hidden);                               // its weights' zeros may have met infinite queries
     }
   }
   if (splits > 1) {
@@ -694,11 +728,13 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     cluster_sync();
     float dsf;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
+    uint32_t one = len == 1;
+    if (a.mask) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(one) : "r"(one_slot) : "memory");
     constexpr int CH = DP / 8;
     for (int x = rank * DKV_THREADS + threadIdx.x; x < 2 * 128 * CH; x += splits * DKV_THREADS) {
       const int u = x / (128 * CH), r = x / CH % 128, c8 = x % CH, key = key0 + r;
       if (key >= a.Tk || c8 * 8 >= a.D) continue;
-      join_parts8<T, DP>(base + u * 128 * DP * 4, r, c8, splits, u ? b.scale / dsf : ex2(-p_shift<T>()),
+      join_parts8<T, DP>(base + u * 128 * DP * 4, r, c8, splits, u ? (one ? 0.f : b.scale / dsf) : ex2(-p_shift<T>()),
                          (u ? dk : dv) + (((long long)m * a.Tk + key) * a.Hk + hk) * a.D + c8 * 8);
     }
     cluster_sync();                                          // the others may still read this block's part

@@ -167,6 +167,45 @@ def test_queries_of_any_value_that_see_nothing(tq, tk):
     assert bool((grads[1][1:] == 0).all()) and bool((grads[2][1:] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("how", ["size", "length", "mask", "both"])
+@pytest.mark.parametrize("shape", [(3, 1, 1, 2, 2, 64), (2, 1, 65, 2, 1, 128), (1, 1, 190, 1, 1, 40), (2, 1, 33, 1, 2, 96)])      # M, G, Tq, Hk, rep, D
+def test_one_visible_key_has_no_gradient_but_its_value(shape, how, dtype):
+    """A softmax over one key is constant: dq and dk are zero, exactly, and the output and dv are the value and the sum of the upstream
+    gradients.  Other memories of the same call are as ever."""
+    from speech_b200 import ops
+
+    M, G, Tq, Hk, rep, D = shape
+    Tk = 1 if how == "size" else 150
+    q, k, v, _, _, hidden = make(M, G, Tq, Tk, Hk, rep, D, dtype, "none")
+    lengths = mask = None
+    rest = slice(M - 1, M) if M > 1 else slice(0, 0)           # the last of several memories keeps all of its keys
+    if how in ("length", "both"):
+        lengths = torch.full((M,), 1 if how == "length" else 77, device="cuda")
+        lengths[rest] = Tk
+        hidden = hidden | (torch.arange(Tk, device="cuda")[None] >= lengths[:, None])
+    if how in ("mask", "both"):
+        mask = torch.arange(Tk, device="cuda")[None].repeat(M, 1) != (149 if how == "mask" else 70)
+        mask[rest] = False
+        hidden = hidden | mask
+    k.masked_fill_(hidden[:, :, None, None], float("nan"))
+    v.masked_fill_(hidden[:, :, None, None], float("inf"))
+    one = (~hidden).sum(1) == 1
+    assert bool(one[0]) and (how == "size" or M == 1 or not bool(one[-1]))
+    dout = torch.randn(q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)).to(dtype)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    out = ops.cross_attention(*leaves, key_lengths=lengths, key_mask=mask)
+    grads = torch.autograd.grad(out, leaves, dout.flatten(2))
+    want, err, dwant, derr = plain(q, k, v, hidden, 1 / math.sqrt(D), dout)
+    check(out.view(want.shape), want, err, "out")
+    for g, w, e, n in zip(grads, dwant, derr, ("dq", "dk", "dv")):
+        check(g, w, e, n)
+    assert bool((grads[0].view(M, -1)[one] == 0).all()) and bool((grads[1][one] == 0).all())
+    if int(one.sum()) < M:
+        assert bool((grads[0].view(M, -1)[~one] != 0).any()) and bool((grads[1][~one] != 0).any())
+    ops.native.check_status()
+
+
 @pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** 12])
 def test_fp16_gradients_of_any_size(size):
     """Upstream gradients far from one keep their precision in fp16 (score gradients are scaled)."""
