@@ -69,8 +69,10 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   init_addends<T>(base + S::ONES0, S::STAGES, threadIdx.x, FWD_THREADS);
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
-      mbar_init(k_full(s), 1); mbar_init(k_clean(s), 1); mbar_init(k_empty(s), tiles);
-      mbar_init(v_full(s), 1); mbar_init(v_clean(s), 1); mbar_init(v_empty(s), tiles);
+      // empty: the tiles' products and the warp that clears.  That warp looks at every block, also where no product waits for it; were it not
+      // counted, a stage could be filled twice under it, and the parity of its next wait, and of a wait for it, would be another phase's.
+      mbar_init(k_full(s), 1); mbar_init(k_clean(s), 1); mbar_init(k_empty(s), tiles + 1);
+      mbar_init(v_full(s), 1); mbar_init(v_clean(s), 1); mbar_init(v_empty(s), tiles + 1);
     }
     for (int t = 0; t < 2; ++t) {
       for (int u = 0; u < 2; ++u) { mbar_init(s_full(t, u), 1); mbar_init(p_full(t, u), 4); }
@@ -142,17 +144,23 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
       __syncwarp();
     };
+    // A block has landed, and where it has hidden keys they have been cleared: in this order, because only a block that has landed says that the
+    // clearing of its stage's last one is done.
+    auto landed = [&](int j, uint32_t full, uint32_t clean) {
+      const uint32_t ph = (uint32_t)(j / S::STAGES) & 1u;
+      return warp_wait(full, ph, a.status, SB_TIMEOUT_SMEM_FULL) &&
+             (!(hide || first + (j + 1) * BN > len) || warp_wait(clean, ph, a.status, SB_TIMEOUT_SMEM_FULL));
+    };
     bool ok = nt > 0 && warp_wait(q_ready, 0, a.status, SB_TIMEOUT_SMEM_FULL);
     for (int j = 0; j < 2 && j < nt && ok; ++j) {
-      ok = warp_wait(hide || first + (j + 1) * BN > len ? k_clean(j) : k_full(j), 0, a.status, SB_TIMEOUT_SMEM_FULL);
+      ok = landed(j, k_full(j), k_clean(j));
       if (!ok) break;
       tc_fence_after();
       scores(j);
     }
     for (int j = 0; j < nt && ok; ++j) {
       const int s = j % S::STAGES;
-      ok = warp_wait(hide || first + (j + 1) * BN > len ? v_clean(s) : v_full(s), (uint32_t)(j / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL) &&
-           warp_wait(p_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
+      ok = landed(j, v_full(s), v_clean(s)) && warp_wait(p_full(t, j & 1), (uint32_t)(j >> 1) & 1u, a.status, SB_TIMEOUT_TMEM_EMPTY);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -165,7 +173,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       __syncwarp();
       if (j + 2 < nt) {
         const int s2 = (j + 2) % S::STAGES;
-        ok = warp_wait(hide || first + (j + 3) * BN > len ? k_clean(s2) : k_full(s2), (uint32_t)((j + 2) / S::STAGES) & 1u, a.status, SB_TIMEOUT_SMEM_FULL);
+        ok = landed(j + 2, k_full(s2), k_clean(s2));
         if (!ok) break;
         tc_fence_after();
         scores(j + 2);
@@ -193,7 +201,10 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(k_clean(s));
+      if (lane == 0) {
+        mbar_arrive(k_clean(s));
+        mbar_arrive(k_empty(s));
+      }
       if (!warp_wait(v_full(s), ph, a.status, SB_TIMEOUT_SMEM_FULL)) break;
       if (some) {
         clear_rows<DP>(base + S::V0 + s * S::KEYS, w, lane);
@@ -202,7 +213,10 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(v_clean(s));
+      if (lane == 0) {
+        mbar_arrive(v_clean(s));
+        mbar_arrive(v_empty(s));
+      }
       if (++s == S::STAGES) { s = 0; ph ^= 1u; }
     }
   } else if (warp >= 4 && (warp - 4) / 4 < tiles) {

@@ -145,6 +145,26 @@ def test_few_tiles_of_long_axes(shape, hide, dtype):
     ops.native.check_status()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tq", [65, 130])                       # one and two row tiles
+def test_lengths_that_end_anywhere(tq, dtype):
+    """One tile pair per SM of up to 24 key blocks, of which only the last has hidden keys: the warp that clears them runs past all of the others,
+    and nothing waits for it until then."""
+    from speech_b200 import ops
+
+    M, Tk = 37, 1500
+    q, k, v, _, _, hidden = make(M, 1, tq, Tk, 4, 1, 64, dtype, "none", seed=6)
+    lengths = torch.tensor([1500 - i if i % 2 else 1 + 40 * i for i in range(M)], device="cuda")
+    hidden = torch.arange(Tk, device="cuda")[None] >= lengths[:, None]
+    k.masked_fill_(hidden[:, :, None, None], float("nan"))
+    v.masked_fill_(hidden[:, :, None, None], float("inf"))
+    want, err = plain(q, k, v, hidden, 1 / 8)
+    for _ in range(5):
+        out = ops.cross_attention(q, k, v, key_lengths=lengths)
+        check(out.view(want.shape), want, err, "out")
+    ops.native.check_status()
+
+
 @pytest.mark.parametrize("tq", [1, 70, 300])
 @pytest.mark.parametrize("tk", [50, 1100])
 def test_queries_of_any_value_that_see_nothing(tq, tk):
