@@ -243,7 +243,10 @@ __device__ __forceinline__ void store_rows64(uint32_t buf, const uint32_t* packe
 
 // Blocks of a cluster that share one tile of results, each over its part of the summed axis: fp32 rows of DP values stand in every
 // block's shared memory, 16-byte pieces XORed with the row, and block r of n adds up and writes every n-th eight columns.
-__device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+  __syncwarp();                                              // .aligned wants whole warps, and this often stands behind a loop that lanes leave apart
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 template <int DP> __device__ __forceinline__ uint32_t part_addr(uint32_t base, int row, int piece) {
   return base + (uint32_t)row * (uint32_t)(DP * 4) + (uint32_t)((piece & ~7) | ((piece ^ row) & 7)) * 16u;
 }

@@ -323,8 +323,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
           }
       }
     }
+    __syncwarp();                                            // lanes wrote statistics by themselves
     if (nt > 0) {
-      __syncwarp();
       row_to_tmem<DP>(tile, quarter * 32 + lane, lane_base + (wg ? S::DO_COL : S::Q_COL));
       tmem_store_wait();
       tc_fence_before();
@@ -379,6 +379,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
         split(add2(d2[0], d2[1]), x, y);
         ndelta = -(x + y);
         if (valid) b.ndelta[stat] = ndelta;
+        __syncwarp();
       }
       const uint64_t nd2 = pair(ndelta, ndelta);
 #pragma unroll

@@ -326,6 +326,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     } else {
       const long long at_row = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
       if (lse && row < a.R) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
+      __syncwarp();                                          // whole warps again for the loads below
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const uint32_t buf = base + t * S::TILE + quarter * 4096;      // the tile's queries have been read
 #pragma unroll

@@ -165,6 +165,28 @@ def test_lengths_that_end_anywhere(tq, dtype):
     ops.native.check_status()
 
 
+@pytest.mark.parametrize("tq,tk,dim", [(70, 1100, 40), (130, 2050, 72), (259, 700, 104), (2001, 90, 8)])
+def test_ragged_tiles_joined_by_clusters(tq, tk, dim):
+    """Rows, keys and columns that end inside a tile that several blocks share, where some of a warp's lanes have nothing to join: the same on every
+    run, with gradients and without."""
+    from speech_b200 import ops
+
+    q, k, v, lengths, mask, hidden = make(1, 1, tq, tk, 1, 1, dim, torch.bfloat16, "none", seed=8)
+    dout = torch.randn(q.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(9)).to(torch.bfloat16)
+    want, err, dwant, derr = plain(q, k, v, hidden, 1 / math.sqrt(dim), dout)
+    first = None
+    for _ in range(20):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = ops.cross_attention(*leaves)
+        got = (out.detach(),) + torch.autograd.grad(out, leaves, dout.flatten(2))
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+    check(first[0].view(want.shape), want, err, "out")
+    for g, w, e, n in zip(first[1:], dwant, derr, ("dq", "dk", "dv")):
+        check(g, w, e, n)
+    ops.native.check_status()
+
+
 @pytest.mark.parametrize("tq", [1, 70, 300])
 @pytest.mark.parametrize("tk", [50, 1100])
 def test_queries_of_any_value_that_see_nothing(tq, tk):
@@ -189,7 +211,7 @@ def test_queries_of_any_value_that_see_nothing(tq, tk):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("how", ["size", "length", "mask", "both"])
-@pytest.mark.parametrize("shape", [(3, 1, 1, 2, 2, 64), (2, 1, 65, 2, 1, 128), (1, 1, 190, 1, 1, 40), (2, 1, 33, 1, 2, 96)])      # M, G, Tq, Hk, rep, D
+@pytest.mark.parametrize("shape", [(3, 1, 1, 2, 2, 64), (2, 1, 65, 2, 1, 128), (1, 1, 190, 1, 1, 40), (2, 1, 33, 1, 2, 96), (1, 1, 700, 1, 1, 128), (2, 4, 301, 1, 2, 64)])      # M, G, Tq, Hk, rep, D
 def test_one_visible_key_has_no_gradient_but_its_value(shape, how, dtype):
     """A softmax over one key is constant: dq and dk are zero, exactly, and the output and dv are the value and the sum of the upstream
     gradients.  Other memories of the same call are as ever."""
