@@ -15,7 +15,7 @@
 // Rounding: exponentials are fp32 and so is a thread's share of a policy row's sum; shares are joined in fp64, and logp, the clip
 // decision and the sums over rows are fp64: a policy at its reference has log ratios near zero, and in fp32 the rounding of a logp of
 // -8 (5e-7) would be all that is left after a few thousand positions are summed.  For the same reason the preference loss has
-// exponentials of its own, off by 4e-10 in the mean (the library's moved every row's log sum the same way, by 1e-8, the approximate
+// exponentials of its own, off by 4e-10 in the mean of many arguments (the library's moved every row's log sum the same way, by 1e-8, the approximate
 // power of two by 7e-8, which a sum over a sequence multiplies and the mean of the policy loss does not), and rounds only the
 // sums of four of them.  log s = k ln 2 + log f with s = 2^k f, f in [0.71, 1.42): the fp32 logarithm
 // of f is off by less than 2^-24.  The gradient is rounded once.  Every sum has a fixed order (no floating-point atomics).
@@ -155,9 +155,10 @@ __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY
 constexpr float LOG2E = 1.44269504f;
 enum { LOSS_POLICY = 0, LOSS_PREFERENCE = 1 };
 
-// exp of two values t <= 0, off by less than 0.6 units in the last place and by 4e-10 in the mean: t log2 e = n + f with n the nearest
-// integer and f from the product with log2 e in two parts; 2^f = 1 + f q(f), q of degree 5 through (2^f - 1) / f at the six Chebyshev
-// nodes of [-1/2, 1/2]; times 2^n.  Below e^-88 the result is 0; NaN stays NaN.
+// exp of two values t <= 0 (above 88 the exponent's bits overflow), off by less than 0.6 units in the last place and, in the mean of many
+// arguments, by 4e-10 (of the few differences that bf16 logits have, by up to 4e-9: rewards of 2 x 512 rows of 40001, 3.4e-9 a row):
+// t log2 e = n + f with n the nearest integer and f from the product with log2 e in two parts; 2^f = 1 + f q(f), q of degree 5 through
+// (2^f - 1) / f at the six Chebyshev nodes of [-1/2, 1/2]; times 2^n.  Below e^-88 the result is 0; NaN stays NaN.
 __device__ __forceinline__ uint64_t exp_fine(uint64_t v) {
   float t, u;
   split(v, t, u);
@@ -181,6 +182,12 @@ __device__ __forceinline__ float exp_fine(float t) {
   float a, b;
   split(exp_fine(pair(t, t)), a, b);
   return a;
+}
+
+// A share of a row's sum, taken relative to m, relative to `base` >= m instead.  A share that has met no logit above -inf (m = -inf) stays as it
+// is, zero or NaN: its factor would be exp of 0 - base, which is infinite or worse where base is below -88.
+template <typename S> __device__ __forceinline__ S rebased(S share, float m, float base) {
+  return m == -INFINITY ? share : share * (S)exp_fine(m - base);
 }
 
 // Softmax weight of a logit, 2^((x - m) log2 e - log2 s), from the row's m and log s.  Kept apart: in a row of nothing but the type's
@@ -226,7 +233,7 @@ template <int MODE> using Sum = typename SumOf<MODE>::type;
 // Joins the (max, sum) shares of the TPR threads of a row: one warp (TPR = 32) or a whole block.
 template <int TPR, typename S> __device__ __forceinline__ void join(float& m, double& sum, S share, float* redf, double* redd) {
   const float wm = warp_max(m);
-  double v = (double)share * (double)exp_fine(finite_or_zero(m) - finite_or_zero(wm));
+  double v = rebased((double)share, m, wm);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (TPR == 32) {
@@ -246,7 +253,7 @@ template <int TPR, typename S> __device__ __forceinline__ void join(float& m, do
   m = finite_or_zero(bm);
   sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < TPR / 32; ++i) sum += redd[i] * (double)exp_fine(finite_or_zero(redf[i]) - m);
+  for (int i = 0; i < TPR / 32; ++i) sum += rebased(redd[i], redf[i], m);
 }
 
 __device__ __forceinline__ double log_of_sum(double s) {
@@ -495,7 +502,7 @@ rows_forward_kernel(const RowArgs a, int* __restrict__ count_p, float* __restric
         base = finite_or_zero(nm);
         if (nm > m) {                                    // rare after the first groups
           if (MODE == LOSS_PREFERENCE) share += fine.take();
-          share *= exp_fine(finite_or_zero(m) - base);
+          share = rebased(share, m, base);
           m = nm;
         }
         const uint64_t shift2 = pair(-base, -base);

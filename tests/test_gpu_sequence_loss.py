@@ -288,6 +288,106 @@ def test_infinite_and_nan_logits(v):
             assert bool(torch.isnan(rewards[1])) and int(torch.isnan(rewards).sum()) == 1
 
 
+def far_logits(how, v, dtype):
+    """Logits far below zero, [4, 134, v]: every row shifted by another amount in [-300, -60], the first ids or a whole row at the type's lowest value."""
+    logits, targets, mask, _, _, adv = make(4, 134, None, v, torch.float32, seed=v, whole=True)
+    low = torch.finfo(dtype).min
+    if how == "shifted":
+        logits = logits - torch.linspace(60.0, 300.0, 4 * 134, device="cuda").view(4, 134, 1)
+    elif how == "first ids lowest":
+        n = min(10000, v // 2)
+        logits[..., :n] = low
+        targets = n + targets % (v - n)
+    else:
+        logits[0] = low
+        logits[1] = -88.7
+        logits[2, :, ::2] = low
+        logits[2, :, 1::2] = -266.0
+        targets[2] = targets[2] // 2 * 2 + 1 - 2 * (targets[2] // 2 * 2 + 1 >= v).long()
+    logits = logits.to(dtype)
+    # relative to the maximum first: the lowest value plus the logarithm of the row's size is the lowest value, in 64 bits too
+    lp, m, w = plain_logp(logits.double() - logits.double().amax(-1, keepdim=True), targets, mask)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    # ratios 0.5 to 2 that are not on a border of the clip range
+    apart = torch.tensor([-0.7, -0.3, -0.1, 0.1, 0.25, 0.7], device="cuda")[torch.randint(0, 6, lp.shape, generator=g, device="cuda")]
+    old, ref = (lp - apart).float(), (lp + 0.2 * torch.randn(lp.shape, generator=g, device="cuda")).float()
+    return logits, targets, mask, old, ref, adv, lp, m, w
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("v", [130, 500, 2024, 9000, 40001])
+@pytest.mark.parametrize("how", ["shifted", "first ids lowest", "whole rows"])
+def test_logits_far_below_zero(how, v, dtype):
+    """A thread's share of a row that is still empty when it meets a maximum far below zero adds nothing, in both losses."""
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv, lp, m, w = far_logits(how, v, dtype)
+    tol, up = lp_tolerance(v), 512.0 if dtype == torch.float16 else 1.0
+    x = logits.clone().requires_grad_()
+    loss, logp = ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.04)
+    (g,) = torch.autograd.grad(loss, x, torch.tensor(up, device="cuda"))
+    assert bool(((logp.double() - lp).abs() <= tol + EPS[torch.float32] * lp.abs()).all())
+    a, r, d = adv.double().view(-1, 1), torch.exp(lp - old.double()), ref.double() - lp
+    plain, clipped = r * a, r.clamp(0.8, 1.2) * a
+    term, slope = -torch.minimum(plain, clipped) + 0.04 * (torch.exp(d) - d - 1), torch.where(plain <= clipped, -plain, 0.0) + 0.04 * (1 - torch.exp(d))
+    reach = ((r * a).abs() + 0.04 * (1 + torch.exp(d))).mean()                                    # how far the loss moves with the log-probabilities
+    assert abs(float(loss) - float(term.mean())) <= 2.0 ** -23 * abs(float(term.mean())) + float(reach) * tol
+    # as check_gradient, but the slope's two parts may cancel: each moves with the log-probability by its own size (d/dlp of r a and of
+    # 0.04 (1 - exp(d))), which is no longer within the log-probability's error of their sum
+    s = (slope / lp.numel() * up).unsqueeze(-1)
+    moves = (torch.where(plain <= clipped, plain.abs(), 0.0) + 0.04 * (1 + torch.exp(d))).unsqueeze(-1) / lp.numel() * up * (tol + 2.0 ** -22)
+    spread = w + torch.zeros_like(w).scatter_(-1, targets.unsqueeze(-1), 1.0)
+    want = -w * s
+    want.scatter_add_(-1, targets.unsqueeze(-1), s)
+    allow = EPS[dtype] * want.abs() + (s.abs() * 2 * (2 * tol + 2.0 ** -18) + moves) * spread + 2.0 ** -25 * (dtype == torch.float16) + 1e-38
+    bad = ((g.double() - want).abs() / allow).max()
+    assert float(bad) <= 1.0, float(bad)
+    x = logits.clone().requires_grad_()
+    loss, rewards = ops.preference_loss(x, targets, mask, ref)
+    (g,) = torch.autograd.grad(loss, x, torch.tensor(up, device="cuda"))
+    ratio = (lp - ref.double()).sum(1)
+    margin = 0.1 * (ratio[:2] - ratio[2:])
+    assert bool(((rewards.double() - 0.1 * ratio).abs() <= 13.4 * tol + 2.0 ** -23 * (0.1 * ratio).abs()).all())
+    each = -torch.nn.functional.logsigmoid(margin)
+    assert abs(float(loss) - float(each.mean())) <= 2 * 13.4 * tol + 2.0 ** -23 * float(each.mean())
+    # the slope moves with the margin: by at most 0.1 times the margin's error, relative to the slope's own bound of 0.1 / 2
+    s = (0.05 * torch.cat([-torch.sigmoid(-margin), torch.sigmoid(-margin)]) * up).view(-1, 1).expand(lp.shape)
+    want = -w * s.unsqueeze(-1)
+    want.scatter_add_(-1, targets.unsqueeze(-1), s.unsqueeze(-1))
+    allow = EPS[dtype] * want.abs() + (s.abs() * (2 * tol + 2.0 ** -17) + 0.05 * up * 2 * 13.4 * tol).unsqueeze(-1) * spread + 2.0 ** -25 * (dtype == torch.float16) + 1e-38
+    bad = ((g.double() - want).abs() / allow).max()
+    assert float(bad) <= 1.0, float(bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,v", [(4096, 2024), (512, 40001), (8192, 200)])
+def test_rewards_of_long_sequences_have_no_bias(t, v, dtype):
+    """Every row's log sum moves the reward of its sequence, so the exponentials may be off to both sides but not to one."""
+    from speech_b200 import ops
+
+    logits, targets, mask, _, _, _ = make(2, t, None, v, dtype, seed=4, whole=True)
+    lp, _, w = plain_logp(logits, targets, mask)
+    ref = lp.float()
+    _, rewards = ops.preference_loss(logits, targets, mask, ref, beta=1.0)
+    ratio = (lp - ref.double()).sum(1)
+    # an exponential is off by 0.6 units in the last place (2^-23) and its sum with three others by two half steps, at random: at most 1.9e-7
+    # of the term, a standard deviation below 1.1e-7; terms of a row weigh w, rows add up; six deviations, and 4e-10 a row to one side
+    deviation = 1.1e-7 * (w * w).sum((1, 2)).sqrt()
+    if dtype == torch.bfloat16:
+        # an exponential's error is a function of its argument, and of the differences of bf16 values there are few: equal ones have equal
+        # errors, at most 0.6 * 2^-23 of the term, a deviation of 0.6 * 2^-23 / sqrt(3) for each of them, weighted by all the terms that have it
+        x = logits.double()
+        same = []
+        for i in range(2):
+            _, at = torch.unique(x[i] - x[i].amax(-1, keepdim=True), return_inverse=True)
+            same.append((torch.zeros(int(at.max()) + 1, dtype=torch.float64, device="cuda").scatter_add_(0, at.flatten(), w[i].flatten()) ** 2).sum().sqrt())
+        deviation = deviation + 0.6 * 2.0 ** -23 / 3 ** 0.5 * torch.stack(same)
+    bound = t * 4e-10 + 6 * deviation
+    assert bool(((rewards.double() - ratio).abs() <= bound + 2.0 ** -24 * ratio.abs()).all()), ((rewards.double() - ratio) / t).tolist()
+    # what it tells apart: an exponential that is off by 7e-8 to one side, and from fp32 logits one by 1e-8
+    assert float(bound.max()) < t * (1e-8 if dtype == torch.float32 else 7e-8), float(bound.max()) / t
+
+
 def test_rows_beyond_32_bit_offsets():
     from speech_b200 import ops
 
