@@ -36,13 +36,14 @@ def _call(name):
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """The tensor itself if the kernels can address it (contiguous head rows on 16-byte boundaries), else a contiguous copy."""
+    """The tensor itself if the kernels can address it (contiguous head rows on 16-byte boundaries), else a dense copy of its own."""
     sb, st, sh, sd = t.stride()
     if sd == 1 and not (sb | st | sh) & 7 and not t.data_ptr() & 15:
         nb, nt, nh, _ = t.shape
         if (sb > 0 or nb == 1) and (st > 0 or nt == 1) and (sh > 0 or nh == 1):
             return t
-    return t.contiguous()
+    # not contiguous(): that is the same tensor for a dense view at an odd offset, or with odd strides of axes of size one
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _lengths(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:

@@ -323,6 +323,37 @@ def test_strides_and_unaligned_inputs():
                            ops.cross_attention(q, k, v, key_lengths=torch.tensor([150, 200], dtype=torch.int32, device="cuda"), key_mask=mask))
 
 
+@pytest.mark.parametrize("tq", [1, 3, 140])
+def test_dense_views_that_the_kernels_cannot_address(tq):
+    """Views that count as contiguous and still start off a 16-byte boundary, or have odd strides of axes of size one."""
+    from speech_b200 import ops
+
+    def at_one(t):                                             # the same values, dense, one element into their storage
+        flat = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")
+        flat[1:] = t.flatten()
+        return flat[1:].view(t.shape)
+
+    def odd(t):                                                # [1, 1, H, D] out of a projection of odd width
+        wide = torch.zeros((1, 1, t.shape[2] * t.shape[3] + 3), dtype=t.dtype, device="cuda")
+        wide[..., :-3] = t.flatten(2)
+        return wide.as_strided(t.shape, (wide.shape[2], wide.shape[2], t.shape[3], 1))
+
+    for M, tk, move in ((2, 200, at_one), (1, 1, odd)) if tq == 1 else ((2, 200, at_one),):
+        q, k, v, _, _, _ = make(M, 1, tq, tk, 2, 1, 64, torch.bfloat16, "none", fused=False)
+        moved = [move(t) for t in (q, k, v)]
+        assert all(t.is_contiguous() and torch.equal(t, u) for t, u in zip(moved, (q, k, v)))
+        results = []
+        for tensors in [(q, k, v)] + [tuple(m if i == j else t for j, (t, m) in enumerate(zip((q, k, v), moved))) for i in range(3)] + [moved]:
+            leaves = [t.detach().requires_grad_() for t in tensors]
+            out = ops.cross_attention(*leaves)
+            with torch.no_grad():
+                both = [ops.shared_prefix_attention(*tensors, *tensors[1:], torch.full((M,), tk, device="cuda"))] if tq <= 3 else []
+            results.append([out.detach(), ops.cross_attention(*tensors), *both, *torch.autograd.grad(out, leaves, torch.ones_like(out))])
+        for r in results[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(r, results[0]))
+    ops.native.check_status()
+
+
 def test_partial_gradients_and_determinism():
     from speech_b200 import ops
 
