@@ -274,6 +274,11 @@ __device__ __forceinline__ float2 load_remote2(uint32_t addr) {
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ float load_remote(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
 // sum[0 .. 7] += w * eight columns of a row in block `rank`
 template <int DP> __device__ __forceinline__ void add_part8(uint32_t base, int row, int c8, int rank, float w, float* sum) {
 #pragma unroll

@@ -1,8 +1,8 @@
 // Fused cross attention, forward, for many query rows:  o = softmax(scale q k^T) v  without the score matrix in memory.
 //
 // One pass over the keys with the running maximum m and sum l of every row; p = 2^(c s - c m) is held unnormalised:
-//   s = q k_j^T,  m' = max(m, max s),  o = o 2^(c (m - m')) + p v_j,  l = l 2^(c (m - m')) + sum p,  at the end o / l
-// and lse = c m + log2 l is kept for the backward pass (+inf for a row that sees nothing: its probabilities are then 2^-inf = 0).
+//   s = q k_j^T,  m' = max(m, max s),  o = o 2^(c (m - m')) + p v_j,  l = l 2^(c (m - m')) + sum p,  at the end o / w
+// with w the sum of p as it is rounded for the product with v (below), and lse = c m + log2 l is kept for the backward pass (+inf for a row that sees nothing: its probabilities are then 2^-inf = 0).
 //
 // A CTA takes two tiles of 128 packed rows and streams blocks of 64 keys of its memory and key head past both, so that keys and values
 // cross the L2 once per 256 rows.  Warp 0 loads keys and values by TMA, warps 1 and 3 issue the tcgen05.mma of a tile each, warp 2
@@ -15,7 +15,10 @@
 // and (m, l) meet in shared memory and are joined in a fixed order: w_i = 2^(c (m_i - max m)), o = sum w_i o_i / sum w_i l_i.
 //
 // Rounding: scores, maxima, sums and output are fp32; p is rounded to the operands' 16-bit type, which is what the tensor core
-// multiplies (relative 2^-9 per weight in bf16, random, as large as the one rounding of the result); l sums the unrounded p.
+// multiplies (relative 2^-9 per weight in bf16), and the output is divided by the sum w of the rounded weights.  Divided by l it would be off by the
+// rounding of the largest weight where one key leads (a weight up to 2^8, because of the maximum that stands still): a common factor, which the
+// backward pass's delta = sum do o takes on and subtracts from values of its own size.  [Rows that one of 512 keys leads by 3 / 4 / 5 nats, bf16: dq
+// off by 11 / 17 / 60 % of its norm; so by 1 %.]  lse is the unrounded p's.
 #include "cross_attention.cuh"
 #include "cross_attention_host.h"
 
@@ -33,7 +36,8 @@ template <int DP> struct FwdSmem {
   static constexpr int ONES0 = BAR + 512, ADD0 = ONES0 + ONES_BYTES, BYTES = ADD0 + STAGES * ADDEND_BYTES + 1024;
 };
 
-template <typename T, int DP>
+// KEEP: rest and lse are written for a backward pass.
+template <typename T, int DP, bool KEEP>
 __global__ void __launch_bounds__(FWD_THREADS, 1)
 xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const XAttnArgs a, uint16_t* __restrict__ out,
                  uint16_t* __restrict__ rest, float* __restrict__ lse, const long long tile0, const int splits) {
@@ -224,7 +228,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const int t = (warp - 4) >> 2, quarter = warp & 3;
     const int tile_row = row0 + t * 128, row = tile_row + quarter * 32 + lane;
     bool ok = true;
-    float mx = -INFINITY, l = 0.f;
+    float mx = -INFINITY, l = 0.f, w = 0.f;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t o_addr = lane_base + 256 + t * DP;
     if (nt > 0) {
@@ -253,6 +257,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const float f = mx == -INFINITY ? 1.f : ex2((mx - nm) * a.c);
         if (mx != -INFINITY) {
           l *= f;
+          w *= f;
           mx = nm;
         }
         if (j > 0) {
@@ -274,7 +279,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (mx == -INFINITY) mx = tile_max;                  // nothing seen so far: output and sum are zero at any scale
       const float mc = mx == -INFINITY ? 0.f : mx * a.c;
       const uint64_t c2 = pair(a.c, a.c), shift2 = pair(-mc, -mc);
-      uint64_t sum[2] = {0, 0};
+      uint64_t sum[2] = {0, 0}, rounded[2] = {0, 0};
 #pragma unroll
       for (int i = 0; i < BN / 32; ++i) {
         uint32_t p[16];
@@ -289,8 +294,10 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             x = ex2(x);
             y = ex2(y);
           }
-          sum[k & 1] = add2(sum[k & 1], pair(x, y));
+          if (KEEP) sum[k & 1] = add2(sum[k & 1], pair(x, y));
           p[k] = Half2<T>::pack(x, y);
+          const float2 back = Half2<T>::unpack(p[k]);
+          rounded[k & 1] = add2(rounded[k & 1], pair(back.x, back.y));
         }
         tmem_store16(s_addr + 16 * i, p);
       }
@@ -298,6 +305,8 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         float x, y;
         split(add2(sum[0], sum[1]), x, y);
         l += x + y;
+        split(add2(rounded[0], rounded[1]), x, y);
+        w += x + y;
       }
       tmem_store_wait();
       tc_fence_before();
@@ -313,7 +322,7 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (ok) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(seen) : "r"(seen_slot) : "memory");
       if (!seen) {
         mx = -INFINITY;
-        l = 0.f;
+        l = w = 0.f;
         ok = false;
       }
     }
@@ -322,16 +331,17 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const int r = t * 128 + quarter * 32 + lane;
 #pragma unroll
       for (int i = 0; i < DP / 64; ++i) keep_part64<DP>(base, r, 64 * i, o_addr + 64 * i, nt > 0 && ok);
-      asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(base + 256 * DP * 4 + r * 8), "f"(mx), "f"(l) : "memory");
+      asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(base + 256 * DP * 4 + r * 8), "f"(mx), "f"(w) : "memory");
+      if (KEEP) asm volatile("st.shared.f32 [%0], %1;" ::"r"(base + 256 * (DP * 4 + 8) + r * 4), "f"(l) : "memory");
     } else {
       const long long at_row = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row);
-      if (lse && row < a.R) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
+      if (KEEP && row < a.R) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(mx, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
       __syncwarp();                                          // whole warps again for the loads below
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = w == 0.f ? 0.f : 1.f / w;
       const uint32_t buf = base + t * S::TILE + quarter * 4096;      // the tile's queries have been read
 #pragma unroll
       for (int i = 0; i < DP / 64; ++i) {
-        uint32_t r[64], v[32], w[32];
+        uint32_t r[64], v[32], off[32];
         if (nt > 0 && ok) {
           tmem_load64(o_addr + 64 * i, r);
         } else {
@@ -339,9 +349,9 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           for (int k = 0; k < 64; ++k) r[k] = 0u;
         }
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = out_pair<T>(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv, w[k]);
+        for (int k = 0; k < 32; ++k) v[k] = out_pair<T>(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv, off[k]);
         store_rows64(buf, v, out, at_row, 64 * i, a.D, lane);
-        if (rest) store_rows64(buf, w, rest, at_row, 64 * i, a.D, lane);
+        if (KEEP) store_rows64(buf, off, rest, at_row, 64 * i, a.D, lane);
       }
     }
   }
@@ -353,23 +363,24 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const int r = x / CH, c8 = x % CH, row = row0 + r;
       if (row >= a.R || c8 * 8 >= a.D) continue;
       const uint32_t ml = base + 256 * DP * 4 + r * 8;
-      float top = -INFINITY, sum = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      float top = -INFINITY, sum = 0.f, l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (int i = 0; i < splits; ++i) top = fmaxf(top, load_remote2(in_block(ml, i)).x);
       for (int i = 0; i < splits; ++i) {
         const float2 v = load_remote2(in_block(ml, i));
         if (v.y == 0.f) continue;                            // saw nothing
-        const float w = ex2((v.x - top) * a.c);
-        sum = fmaf(w, v.y, sum);
-        add_part8<DP>(base, r, c8, i, w, o);
+        const float f = ex2((v.x - top) * a.c);
+        sum = fmaf(f, v.y, sum);
+        if (KEEP && c8 == 0) l = fmaf(f, load_remote(in_block(base + 256 * (DP * 4 + 8) + r * 4, i)), l);
+        add_part8<DP>(base, r, c8, i, f, o);
       }
-      if (lse && c8 == 0) lse[(long long)unit * a.R + row] = sum > 0.f ? fmaf(top, a.c, log2f(sum)) : (sum == 0.f ? INFINITY : sum);
+      if (KEEP && c8 == 0) lse[(long long)unit * a.R + row] = l > 0.f ? fmaf(top, a.c, log2f(l)) : (l == 0.f ? INFINITY : l);
       const float inv = sum == 0.f ? 0.f : 1.f / sum;
       const long long at = row_offset(a, (long long)a.Tq * a.H * a.D, (long long)a.H * a.D, a.D, m, hk, row) + c8 * 8;
-      uint32_t v[4], w[4];
+      uint32_t v[4], off[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = out_pair<T>(o[2 * k] * inv, o[2 * k + 1] * inv, w[k]);
+      for (int k = 0; k < 4; ++k) v[k] = out_pair<T>(o[2 * k] * inv, o[2 * k + 1] * inv, off[k]);
       *reinterpret_cast<uint4*>(out + at) = make_uint4(v[0], v[1], v[2], v[3]);
-      if (rest) *reinterpret_cast<uint4*>(rest + at) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (KEEP) *reinterpret_cast<uint4*>(rest + at) = make_uint4(off[0], off[1], off[2], off[3]);
     }
     cluster_sync();                                          // the others may still read this block's part
   }
@@ -378,14 +389,20 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool KEEP>
 int launch(const XAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, void* out, void* rest, float* lse, cudaStream_t stream) {
   const long long grid = (long long)((a.R + 255) / 256) * a.M * a.Hk;
   if (grid > 0x7ffffffll) return SB_BAD_ARGUMENT;
-  const int rc = sb_allow_smem((const void*)xattn_fwd_kernel<T, DP>, FwdSmem<DP>::BYTES);
+  const auto kernel = xattn_fwd_kernel<T, DP, KEEP>;
+  const int rc = sb_allow_smem((const void*)kernel, FwdSmem<DP>::BYTES);
   if (rc) return rc;
-  const SbTilePlan plan = sb_plan_tiles((const void*)xattn_fwd_kernel<T, DP>, FWD_THREADS, FwdSmem<DP>::BYTES, grid, (a.Tk + BN - 1) / BN, OWN_BLOCKS, OWN_BLOCKS);
-  return sb_run_tiles(plan, grid, FWD_THREADS, FwdSmem<DP>::BYTES, stream, xattn_fwd_kernel<T, DP>, mk, mv, a, (uint16_t*)out, (uint16_t*)rest, lse);
+  const SbTilePlan plan = sb_plan_tiles((const void*)kernel, FWD_THREADS, FwdSmem<DP>::BYTES, grid, (a.Tk + BN - 1) / BN, OWN_BLOCKS, OWN_BLOCKS);
+  return sb_run_tiles(plan, grid, FWD_THREADS, FwdSmem<DP>::BYTES, stream, kernel, mk, mv, a, (uint16_t*)out, (uint16_t*)rest, lse);
+}
+template <typename T>
+int launch(const XAttnArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, void* out, void* rest, float* lse, cudaStream_t stream) {
+  if (a.D <= 64) return lse ? launch<T, 64, true>(a, mk, mv, out, rest, lse, stream) : launch<T, 64, false>(a, mk, mv, out, rest, lse, stream);
+  return lse ? launch<T, 128, true>(a, mk, mv, out, rest, lse, stream) : launch<T, 128, false>(a, mk, mv, out, rest, lse, stream);
 }
 
 }  // namespace
@@ -402,6 +419,5 @@ SB_API int sb_cross_attention_fwd(const SbCrossAttention* g, void* out, void* re
   rc = sb_rows_map(&mk, g->k, g->type, a.D, a.Tk, a.Hk, a.M, g->k_st, g->k_sh, g->k_sb, BN);
   if (!rc) rc = sb_rows_map(&mv, g->v, g->type, a.D, a.Tk, a.Hk, a.M, g->v_st, g->v_sh, g->v_sb, BN);
   if (rc) return rc;
-  if (g->type == 0) return a.D <= 64 ? launch<__nv_bfloat16, 64>(a, mk, mv, out, rest, lse, stream) : launch<__nv_bfloat16, 128>(a, mk, mv, out, rest, lse, stream);
-  return a.D <= 64 ? launch<__half, 64>(a, mk, mv, out, rest, lse, stream) : launch<__half, 128>(a, mk, mv, out, rest, lse, stream);
+  return g->type == 0 ? launch<__nv_bfloat16>(a, mk, mv, out, rest, lse, stream) : launch<__half>(a, mk, mv, out, rest, lse, stream);
 }

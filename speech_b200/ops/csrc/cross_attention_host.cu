@@ -98,7 +98,7 @@ SbTilePlan sb_plan_tiles(const void* kernel, int threads, int smem, long long ti
 int sb_allow_smem(const void* kernel, int bytes) {
   // a handful of kernels: remembered per device, so that a launch costs no driver call
   struct Seen { const void* kernel; int device; };
-  static thread_local Seen seen[32];
+  static thread_local Seen seen[64];
   static thread_local int n = 0;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -107,6 +107,6 @@ int sb_allow_smem(const void* kernel, int bytes) {
     if (seen[i].kernel == kernel && seen[i].device == dev) return 0;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return (int)e;
-  if (n < 32) seen[n++] = {kernel, dev};
+  if (n < 64) seen[n++] = {kernel, dev};
   return 0;
 }

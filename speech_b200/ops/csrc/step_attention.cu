@@ -4,16 +4,17 @@
 // Keys and values are read once and little is computed on them, so bytes bound it, and what counts is how many loads are in flight.
 // The keys of a (memory, key head) are split over blocks and over the four warps of a block; every warp streams tiles of 16 keys through
 // a ring of its own in shared memory (cp.async, 16 or 24 KB per warp, 190 KB per SM; no barrier between warps), takes
-// its fragments of mma.m16n8k16 from there with ldmatrix, and keeps running maximum m, sum l and the unnormalised output in registers.
+// its fragments of mma.m16n8k16 from there with ldmatrix, and keeps running maximum m, sum l (of rounded weights: w) and the unnormalised output in
+// registers.
 // The parts are joined in the block; up to eight blocks of a (memory, key head) are a cluster and join theirs through one another's
 // shared memory, more blocks, and the two kinds of keys of a shared prompt, through memory and a second small kernel:
-//   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+//   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) w_i.
 // Loads straight into registers (16 keys ahead, 228 registers, or fewer and spills) reached a third of this.
 //
 // Packed rows (rows that read the same keys: group x heads of a key head x tokens, as in cross_attention.cuh) fill blocks of 16, one or
 // two per warp; more rows than 32 read the keys again, from the L2.
 //
-// Rounding: as in cross_attention_fwd.cu (weights rounded to 16 bits for the second product, all else fp32).
+// Rounding: as in cross_attention_fwd.cu (weights rounded to 16 bits for the second product and for the sum that divides it, all else fp32).
 #include "cross_attention_host.h"
 
 namespace {
@@ -43,7 +44,8 @@ struct StepArgs {
   uint16_t *out, *rest;     // [B, Tq, H, D]; rest: what rounding took from out, or null
   float* lse;               // packed rows of segment 0, or null
   float* part_o;            // [slots, B * Tq * H, D]
-  float2* part_ml;          // [slots, B * Tq * H]
+  float2* part_mw;          // [slots, B * Tq * H]: maximum, sum of rounded weights
+  float* part_l;            // the same: sum of the weights, where lse is wanted
 };
 
 template <typename T> __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1);
@@ -85,31 +87,25 @@ __device__ __forceinline__ long long query_row(const StepArgs& a, const Segment&
   return ((long long)(mem * s.rows_per + gr) * a.Tq + t) * a.H + hk * a.rep + y - gr * a.rep;
 }
 template <typename T>
-__device__ __forceinline__ void write_row(const StepArgs& a, const Segment& s, int mem, int hk, int r, int d, float big, float sum, const float* v) {
+__device__ __forceinline__ void write_row(const StepArgs& a, const Segment& s, int mem, int hk, int r, int d, float big, float l, float w, const float* v) {
   const long long qrow = query_row(a, s, mem, hk, r);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = w == 0.f ? 0.f : 1.f / w;
   uint32_t o4[4], r4[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) o4[k] = out_pair<T>(v[2 * k] * inv, v[2 * k + 1] * inv, r4[k]);
   *reinterpret_cast<uint4*>(a.out + qrow * a.D + d) = make_uint4(o4[0], o4[1], o4[2], o4[3]);
   if (a.rest) *reinterpret_cast<uint4*>(a.rest + qrow * a.D + d) = make_uint4(r4[0], r4[1], r4[2], r4[3]);
-  if (a.lse && d == 0) a.lse[((long long)mem * a.Hk + hk) * s.R + r] = sum > 0.f ? big + log2f(sum) : (sum == 0.f ? INFINITY : sum);
+  if (a.lse && d == 0) a.lse[((long long)mem * a.Hk + hk) * s.R + r] = l > 0.f ? big + log2f(l) : (l == 0.f ? INFINITY : l);
 }
 // two floats at a shared-memory address of block `rank` of the cluster
-__device__ __forceinline__ float2 remote_float2(uint32_t addr, int rank) {
-  uint32_t there;
-  float2 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(there) : "memory");
-  return v;
-}
+__device__ __forceinline__ float2 remote_float2(uint32_t addr, int rank) { return load_remote2(in_block(addr, rank)); }
 
-// MT: row blocks of 16 per warp
-template <typename T, int DP, int MT>
+// MT: row blocks of 16 per warp; KEEP: lse is written for a backward pass, which takes the sum of the unrounded weights too
+template <typename T, int DP, int MT, bool KEEP>
 __global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step_kernel(const __grid_constant__ StepArgs a) {
   using S = StepSmem<DP, MT>;
   constexpr int CH = DP / 8, NT = DP / 8, KS = DP / 16;
-  __shared__ float s_m[4][16 * MT], s_l[4][16 * MT];
+  __shared__ float s_m[4][16 * MT], s_l[4][16 * MT], s_w[4][16 * MT], s_join_l[16 * MT];
   __shared__ float2 s_join[16 * MT];
   extern __shared__ __align__(16) uint8_t smem_raw[];
   const uint32_t base = smem_u32(smem_raw), qs = base + S::Q0;
@@ -205,11 +201,11 @@ __global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step
 #pragma unroll
     for (int k = 0; k < KS; ++k) ldmatrix4(row_addr<DP>(qs, mrow, 2 * k + mch), qf[MT == 1 ? k : 0]);
   }
-  float m[MT][2], l[MT][2], o[MT][NT][4];
+  float m[MT][2], l[MT][2], w[MT][2], o[MT][NT][4];
 #pragma unroll
   for (int t = 0; t < MT; ++t) {
     m[t][0] = m[t][1] = -INFINITY;
-    l[t][0] = l[t][1] = 0.f;
+    l[t][0] = l[t][1] = w[t][0] = w[t][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
   }
@@ -274,7 +270,8 @@ __global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step
           const float nm = m[t][u] == -INFINITY ? m[t][u] : fmaxf(m[t][u], mx);
           const float f = m[t][u] == -INFINITY ? 1.f : ex2(m[t][u] - nm);
           m[t][u] = nm;
-          l[t][u] *= f;
+          if (KEEP) l[t][u] *= f;
+          w[t][u] *= f;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             o[t][n][2 * u] *= f;
@@ -285,9 +282,11 @@ __global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step
         const float from = m[t][u] == -INFINITY ? 0.f : m[t][u];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = ex2(fmaf(v[e], a.c, -from));
-        l[t][u] += (v[0] + v[1]) + (v[2] + v[3]);
+        if (KEEP) l[t][u] += (v[0] + v[1]) + (v[2] + v[3]);
         p[t][u] = Half2<T>::pack(v[0], v[1]);
         p[t][2 + u] = Half2<T>::pack(v[2], v[3]);
+        const float2 r0 = Half2<T>::unpack(p[t][u]), r1 = Half2<T>::unpack(p[t][2 + u]);
+        w[t][u] += (r0.x + r0.y) + (r1.x + r1.y);
       }
 #pragma unroll
     for (int n = 0; n < NT; n += 2) {
@@ -311,12 +310,17 @@ __global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], 1);
-      l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], 2);
+      if (KEEP) {
+        l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], 1);
+        l[t][u] += __shfl_xor_sync(0xffffffffu, l[t][u], 2);
+      }
+      w[t][u] += __shfl_xor_sync(0xffffffffu, w[t][u], 1);
+      w[t][u] += __shfl_xor_sync(0xffffffffu, w[t][u], 2);
       const int lr = 16 * t + g + 8 * u;
       if (c == 0) {
         s_m[warp][lr] = m[t][u];
-        s_l[warp][lr] = l[t][u];
+        if (KEEP) s_l[warp][lr] = l[t][u];
+        s_w[warp][lr] = w[t][u];
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) *reinterpret_cast<float2*>(mine + lr * LD + 8 * n + 2 * c) = make_float2(o[t][n][2 * u], o[t][n][2 * u + 1]);
@@ -329,55 +333,61 @@ __global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step
     const int lr = i / per_row, d = (i - lr * per_row) * 8, r = row0 + lr;
     float big = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) big = fmaxf(big, s_m[w][lr]);
+    for (int i = 0; i < 4; ++i) big = fmaxf(big, s_m[i][lr]);
     const float from = big == -INFINITY ? 0.f : big;
-    float sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float sum = 0.f, weights = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = ex2(s_m[w][lr] - from);
-      sum += f * s_l[w][lr];
-      const float* po = s_o + (w * 16 * MT + lr) * LD + d;
+    for (int i = 0; i < 4; ++i) {
+      const float f = ex2(s_m[i][lr] - from);
+      if (KEEP) sum += f * s_l[i][lr];
+      weights += f * s_w[i][lr];
+      const float* po = s_o + (i * 16 * MT + lr) * LD + d;
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] += f * po[k];
     }
     if (a.slots == 1) {
-      write_row<T>(a, s, mem, hk, r, d, big, sum, v);
+      write_row<T>(a, s, mem, hk, r, d, big, sum, weights, v);
     } else if (a.cluster) {
       // over the first warp's share, which only this thread still reads
       float* po = s_o + lr * LD + d;
 #pragma unroll
       for (int k = 0; k < 8; ++k) po[k] = v[k];
       if (d == 0) {
-        s_join[lr] = make_float2(big, sum);
+        s_join[lr] = make_float2(big, weights);
+        if (KEEP) s_join_l[lr] = sum;
       }
     } else {
       const long long qrow = query_row(a, s, mem, hk, r);
       float* po = a.part_o + ((long long)slot_out * qrows + qrow) * a.D + d;
       *reinterpret_cast<float4*>(po) = make_float4(v[0], v[1], v[2], v[3]);
       *reinterpret_cast<float4*>(po + 4) = make_float4(v[4], v[5], v[6], v[7]);
-      if (d == 0) a.part_ml[slot_out * qrows + qrow] = make_float2(big, sum);
+      if (d == 0) {
+        a.part_mw[slot_out * qrows + qrow] = make_float2(big, weights);
+        if (KEEP) a.part_l[slot_out * qrows + qrow] = sum;
+      }
     }
   }
   if (a.cluster && a.slots > 1) {
     __syncwarp();
     // every block of the cluster has its part in shared memory; block b of n takes every n-th 8-column piece of the rows
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    const uint32_t o_at = smem_u32(s_o), j_at = smem_u32(s_join);
+    const uint32_t o_at = smem_u32(s_o), j_at = smem_u32(s_join), l_at = smem_u32(s_join_l);
     for (int i = split * STEP_THREADS + threadIdx.x; i < rows_here * per_row; i += a.slots * STEP_THREADS) {
       const int lr = i / per_row, d = (i - lr * per_row) * 8;
-      float big = -INFINITY, sum = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      float2 ml[8];
+      float big = -INFINITY, sum = 0.f, weights = 0.f, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      float2 mw[8];
 #pragma unroll
       for (int b = 0; b < 8; ++b) {
-        ml[b] = b < a.slots ? remote_float2(j_at + lr * 8, b) : make_float2(-INFINITY, 0.f);
-        big = fmaxf(big, ml[b].x);
+        mw[b] = b < a.slots ? remote_float2(j_at + lr * 8, b) : make_float2(-INFINITY, 0.f);
+        big = fmaxf(big, mw[b].x);
       }
       const float from = big == -INFINITY ? 0.f : big;
 #pragma unroll
       for (int b = 0; b < 8; ++b)
         if (b < a.slots) {
-          const float f = ex2(ml[b].x - from);
-          sum += f * ml[b].y;
+          const float f = ex2(mw[b].x - from);
+          weights += f * mw[b].y;
+          if (KEEP && d == 0) sum += f * load_remote(in_block(l_at + lr * 4, b));
 #pragma unroll
           for (int k = 0; k < 8; k += 2) {
             const float2 x = remote_float2(o_at + (lr * LD + d + k) * 4, b);
@@ -385,7 +395,7 @@ __global__ void __launch_bounds__(STEP_THREADS, (StepSmem<DP, MT>::BLOCKS)) step
             v[k + 1] += f * x.y;
           }
         }
-      write_row<T>(a, s, mem, hk, row0 + lr, d, big, sum, v);
+      write_row<T>(a, s, mem, hk, row0 + lr, d, big, sum, weights, v);
     }
     __syncwarp();
     // no block leaves while another may still read its shared memory
@@ -399,21 +409,24 @@ template <typename T> __global__ void __launch_bounds__(128) step_join_kernel(co
   if (qrow >= qrows) return;
   const int lane = threadIdx.x & 31;
   float big = -INFINITY;
-  for (int i = lane; i < a.slots; i += 32) big = fmaxf(big, a.part_ml[i * qrows + qrow].x);
+  for (int i = lane; i < a.slots; i += 32) big = fmaxf(big, a.part_mw[i * qrows + qrow].x);
   big = warp_max(big);
   const float base = big == -INFINITY ? 0.f : big;
-  float sum = 0.f;
+  float sum = 0.f, weights = 0.f;
   for (int i = lane; i < a.slots; i += 32) {
-    const float2 ml = a.part_ml[i * qrows + qrow];
-    sum += ex2(ml.x - base) * ml.y;
+    const float2 mw = a.part_mw[i * qrows + qrow];
+    const float f = ex2(mw.x - base);
+    weights += f * mw.y;
+    if (a.lse) sum += f * a.part_l[i * qrows + qrow];
   }
+  weights = warp_sum(weights);
   sum = warp_sum(sum);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = weights == 0.f ? 0.f : 1.f / weights;
   if (4 * lane < a.D) {
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int i = 0; i < a.slots; ++i) {
-      const float f = ex2(a.part_ml[i * qrows + qrow].x - base);
+      const float f = ex2(a.part_mw[i * qrows + qrow].x - base);
       const float4 p = *reinterpret_cast<const float4*>(a.part_o + (i * qrows + qrow) * a.D + 4 * lane);
       v.x += f * p.x; v.y += f * p.y; v.z += f * p.z; v.w += f * p.w;
     }
@@ -464,11 +477,12 @@ int plan(StepArgs& a, int memories0, int memories1) {
 }
 
 long long workspace(const StepArgs& a) {
-  return a.slots <= 1 || a.cluster ? 0 : (long long)a.slots * a.B * a.Tq * a.H * (a.D + 2) * 4;
+  return a.slots <= 1 || a.cluster ? 0 : (long long)a.slots * a.B * a.Tq * a.H * (a.D + 3) * 4;
 }
 
 template <typename T, int DP, int MT> int launch_rows(const StepArgs& a, cudaStream_t stream) {
-  const int rc = sb_allow_smem((const void*)step_kernel<T, DP, MT>, StepSmem<DP, MT>::BYTES);
+  const auto kernel = a.lse ? step_kernel<T, DP, MT, true> : step_kernel<T, DP, MT, false>;
+  const int rc = sb_allow_smem((const void*)kernel, StepSmem<DP, MT>::BYTES);
   if (rc) return rc;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3((unsigned)(a.seg[0].blocks + a.seg[1].blocks));
@@ -481,7 +495,7 @@ template <typename T, int DP, int MT> int launch_rows(const StepArgs& a, cudaStr
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = a.cluster && a.slots > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&config, step_kernel<T, DP, MT>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
   return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
 }
 template <typename T, int DP> int launch_step(const StepArgs& a, cudaStream_t stream) {
@@ -496,7 +510,9 @@ int run(StepArgs& a, int type, void* ws, cudaStream_t stream) {
   if (a.slots > 1 && !a.cluster) {
     if (!ws) return SB_BAD_ARGUMENT;
     a.part_o = (float*)ws;
-    a.part_ml = (float2*)(a.part_o + (long long)a.slots * a.B * a.Tq * a.H * a.D);
+    const long long rows = (long long)a.slots * a.B * a.Tq * a.H;
+    a.part_mw = (float2*)(a.part_o + rows * a.D);
+    a.part_l = (float*)(a.part_mw + rows);
   }
   if (type == 0) return a.D <= 64 ? launch_step<__nv_bfloat16, 64>(a, stream) : launch_step<__nv_bfloat16, 128>(a, stream);
   return a.D <= 64 ? launch_step<__half, 64>(a, stream) : launch_step<__half, 128>(a, stream);

@@ -248,6 +248,42 @@ def test_one_visible_key_has_no_gradient_but_its_value(shape, how, dtype):
     ops.native.check_status()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lead", [3, 4, 5])                    # nats by which a later key leads an early one: less than the maximum may lag
+@pytest.mark.parametrize("shape", [(2, 1, 8, 1, 1, 64), (64, 1, 2, 8, 2, 64), (1, 1, 130, 1, 2, 128), (37, 1, 70, 4, 1, 64)])  # M, G, Tq, Hk, rep, D
+def test_gradients_of_peaked_rows(shape, lead, dtype):
+    """Rows that one key leads: score gradients are differences of nearly equal values, and the output's error, which delta takes on, has to be
+    that of a softmax of slightly other weights and not a common factor."""
+    from speech_b200 import ops
+
+    M, G, Tq, Hk, rep, D = shape
+    q, k, v, _, _, hidden = make(M, G, Tq, 512, Hk, rep, D, dtype, "none", seed=11, fused=False)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    axis = torch.nn.functional.normalize(torch.randn(D, generator=g, device="cuda"), dim=0) * (8 * D ** 0.5) ** 0.5
+    q.copy_(axis + 0.05 * torch.randn(q.shape, generator=g, device="cuda"))
+    k.mul_(0.1)
+    k[:, 3], k[:, 388] = (axis * 10 / 8).to(dtype), (axis * (10 + lead) / 8).to(dtype)              # scores of 10 and 10 + lead nats, the others' about 0
+    dout = torch.randn(q.shape, generator=g, device="cuda").to(dtype)
+    e, scale = EPS[dtype], 1 / math.sqrt(D)
+    out, _, dwant, _ = plain(q, k, v, hidden, scale, dout)
+    qd, kd, vd, do = q.double().view(M, G, Tq, Hk, rep, D), k.double(), v.double(), dout.double().view(M, G, Tq, Hk, rep, D)
+    p = torch.softmax(torch.einsum("mgthrd,mshd->mghrts", qd, kd) * scale, -1)
+    dp = torch.einsum("mgthrd,mshd->mghrts", do, vd)
+    line = torch.einsum("mgthrd,mgthrd->mghrt", do.abs(), out.abs().view(do.shape)).unsqueeze(-1)
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    # weights that are rounded by e each and divided by their own sum add up to one, so that delta is off by sum (p' - p) (dp - delta), of
+    # |p' - p| <= 2 e p; the output's rounding is made good by its remainder (e^2); fp32 everywhere else
+    ds_err = (e + 2 * FAST) * ds.abs() + p * (2 * e * ds.abs().sum(-1, keepdim=True) + (e * e + FAST) * line + FAST * dp.abs())
+    ds_err = ds_err + (2.0 ** -28 * float(dout.abs().max()) if dtype == torch.float16 else 0.0)
+    dq_err = torch.einsum("mghrts,mshd->mgthrd", ds_err + FAST * ds.abs(), kd.abs()).reshape(q.shape) * scale + e * dwant[0].abs() + 2.0 ** -25
+    dk_err = torch.einsum("mghrts,mgthrd->mshd", ds_err + FAST * ds.abs(), qd.abs()) * scale + e * dwant[1].abs() + 2.0 ** -25
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.cross_attention(*leaves), leaves, dout.flatten(2))
+    check(grads[0], dwant[0], dq_err, "dq")
+    check(grads[1], dwant[1], dk_err, "dk")
+    ops.native.check_status()
+
+
 @pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** 12])
 def test_fp16_gradients_of_any_size(size):
     """Upstream gradients far from one keep their precision in fp16 (score gradients are scaled)."""
