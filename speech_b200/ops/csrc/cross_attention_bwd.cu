@@ -145,7 +145,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
   auto kv_clean = [&](int s) { return bars + 8u * (24 + s); };
   const uint32_t dp_read = bars + 8u * 20, dq_full = bars + 8u * 21, rows_ready = bars + 8u * 22, tmem_slot = bars + 8u * 23;
   const uint32_t seen_slot = bars + 8u * 29;               // whether the mask leaves any of these keys
-  const uint32_t one_slot = seen_slot + 4;                 // whether it leaves just one of the memory's
+  const uint32_t one_slot = seen_slot + 4;                 // whether just one of the memory's is visible
   const uint32_t stats = bars + 240u;                      // -delta of the tile's rows, peaks of four warps
 
   const int tiles = b.tiles;
@@ -165,6 +165,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
     mbar_init(dp_read, 4);
     mbar_init(dq_full, 1);
     mbar_init(rows_ready, 8);
+    if (!hide) asm volatile("st.shared.u32 [%0], %1;" ::"r"(one_slot), "r"((uint32_t)(len == 1)) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -410,13 +411,9 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       if (ok) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(seen) : "r"(seen_slot) : "memory");
       ok = ok && seen;
     }
-    bool one = len == 1;
-    if (hide) {
-      asm volatile("bar.sync 2, 288;" ::: "memory");         // with warp 2
-      uint32_t v;
-      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(one_slot) : "memory");
-      one = v != 0;
-    }
+    if (hide) asm volatile("bar.sync 2, 288;" ::: "memory");      // with warp 2
+    uint32_t one;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(one) : "r"(one_slot) : "memory");
     if (splits > 1) {
       if (wg < DP / 64) keep_part64<DP>(base, quarter * 32 + lane, 64 * wg, lane_base + 64 * wg, nt > 0 && ok);
     } else if (dq && wg < DP / 64) {                       // 64 columns a warpgroup
@@ -434,8 +431,8 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       asm volatile("ld.shared.f32 %0, [%1];" : "=f"(p) : "r"(stats + (128 + i) * 4) : "memory");
       peak = fmaxf(peak, p);
     }
-    uint32_t one = len == 1;
-    if (hide) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(one) : "r"(one_slot) : "memory");
+    uint32_t one;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(one) : "r"(one_slot) : "memory");
     const float f = one ? 0.f : b.scale / ds_scale<T>(peak);
     constexpr int CH = DP / 8;
     for (int x = rank * DQ_THREADS + threadIdx.x; x < 128 * CH; x += splits * DQ_THREADS) {
@@ -482,7 +479,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto p_read = [&](int u) { return bars + 8u * (14 + u); };
   const uint32_t s_read = bars + 8u * 16, dp_read = bars + 8u * 17, kv_full = bars + 8u * 18, kv_tmem = bars + 8u * 19, d_full = bars + 8u * 20,
                  tmem_slot = bars + 8u * 21, scale_slot = tmem_slot + 4;
-  const uint32_t one_slot = bars + 8u * 22;                // whether the mask leaves just one of the memory's keys
+  const uint32_t one_slot = bars + 8u * 22;                // whether just one of the memory's keys is visible
 
   const int ktiles = (a.Tk + 127) / 128;
   const int local = blockIdx.x / splits, rank = blockIdx.x - local * splits;      // block `rank` of a cluster takes its part of the rows
@@ -502,6 +499,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     mbar_init(kv_full, 1);
     mbar_init(kv_tmem, S::V_TMEM ? 8 : 4);
     mbar_init(d_full, 1);
+    if (!a.mask) asm volatile("st.shared.u32 [%0], %1;" ::"r"(one_slot), "r"((uint32_t)(len == 1)) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -706,13 +704,10 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (nq > 0 && ok) ok = warp_wait(d_full, 0, a.status, SB_TIMEOUT_TMEM_FULL);
     tc_fence_after();
-    bool one = len == 1;
-    if (a.mask) {
-      asm volatile("bar.sync 1, 544;" ::: "memory");         // with warp 3
-      uint32_t v;
-      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(one_slot) : "memory");
-      one = v != 0;
-    }
+    if (a.mask) asm volatile("bar.sync 1, 544;" ::: "memory");     // with warp 3
+    uint32_t one;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(one) : "r"(one_slot) : "memory");
+    const float f = !u ? ex2(-p_shift<T>()) : one ? 0.f : Half2<T>::KIND == 0 ? b.scale / dsf : b.scale;
     // dv by two warpgroups, dk by the others, 64 columns each (DP = 64: one of the two)
     if (splits > 1) {
       if (half < DP / 64) keep_part64<DP>(base + u * 128 * DP * 4, quarter * 32 + lane, half * 64, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok,
@@ -720,8 +715,7 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     } else if (half < DP / 64) {
       const long long off = key < a.Tk ? (((long long)m * a.Tk + key) * a.Hk + hk) * a.D : -1;
       store_acc64<T>(base + ((u * 2 + half) * 4 + quarter) * 4096, lane_base + (u ? S::DK_COL : 0) + half * 64, nq > 0 && ok,
-                     u ? (one ? 0.f : b.scale / dsf) : ex2(-p_shift<T>()), u ? dk : dv, off, half * 64, a.D, lane,
-                     hidden);                               // its weights' zeros may have met infinite queries
+                     f, u ? dk : dv, off, half * 64, a.D, lane, hidden);      // its weights' zeros may have met infinite queries
     }
   }
   if (splits > 1) {
@@ -729,8 +723,8 @@ xattn_dkv_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     cluster_sync();
     float dsf;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(dsf) : "r"(scale_slot) : "memory");
-    uint32_t one = len == 1;
-    if (a.mask) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(one) : "r"(one_slot) : "memory");
+    uint32_t one;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(one) : "r"(one_slot) : "memory");
     constexpr int CH = DP / 8;
     for (int x = rank * DKV_THREADS + threadIdx.x; x < 2 * 128 * CH; x += splits * DKV_THREADS) {
       const int u = x / (128 * CH), r = x / CH % 128, c8 = x % CH, key = key0 + r;
