@@ -25,7 +25,11 @@
 // Rounding: p and ds are rounded to the operands' 16-bit type for the products that sum them, all else is fp32.  In fp16 their range
 // matters: p is multiplied by 2^12 (it is at most 1), ds by a power of two that brings the largest |do|, or a 64th of the largest
 // |delta| where the values are that large, to [8, 16), and the sums are scaled back, so that neither small weights nor small upstream
-// gradients fall below the type's normal range and ds stays below its end (behind which it is infinite).
+// gradients fall below the type's normal range.  ds stays below its end whatever the values are: |dp| <= |do| |v| (norms), and
+// |ds| = p |dp - sum p dp| <= p (1 - p) 2 max |dp| <= max |do| |v| / 2.  A kernel ahead takes the largest norm of a visible value, and where
+// sqrt(D) max|v| exceeds 4096 the peak of do counts that many times as much: ds then ends below 16 * 2048.  (Not needed for bf16; in fp16 it
+// reads the values once more: 6 us of 199 for forward and backward of 12 x 301 queries, 3 x 1111 keys, 16 heads on 4 of 64, 8 of 575 for 4 x 1024
+// queries, 7500 keys, 8 heads of 128.)
 #include "cross_attention.cuh"
 #include "cross_attention_host.h"
 
@@ -44,20 +48,68 @@ struct BwdArgs {
   float *nlse, *ndelta;               // [M * Hk, G * rep, Tqp]: -lse (-inf behind the last row, too) and -delta (0 there)
   int Tqp;                            // Tq rounded up to 64
   float* peak;                        // fp16: what ds_scale() takes, of every block of the dq kernel
+  float* norms;                       // fp16: the largest norm of a visible value, of every NORM_KEYS keys of a (memory, key head)
   int tiles;                          // its blocks of a (memory, key head)
   float scale;
 };
 
 // Power of two that brings the peak of a (memory, key head) to [8, 16); 1 for bf16, whose range needs none.  The peak is the largest
-// |do|, or |delta| / 64: ds is large only where p is, and there dp is of delta's size.
+// |do| (times sqrt(D) max|v| / 4096 where that is above one), or |delta| / 64.
 template <typename T> __device__ __forceinline__ float ds_scale(float peak) {
   if (Half2<T>::KIND != 0 || !(peak > 0.f) || !(peak < 3e38f)) return 1.f;
   return __int_as_float((127 + 3 - ((__float_as_int(fmaxf(peak, 1e-8f)) >> 23) - 127)) << 23);      // |do| of fp16 is at least 2^-24
 }
 
+constexpr int NORM_KEYS = 256;
+__host__ __device__ inline int norm_parts(int Tk) { return (Tk + NORM_KEYS - 1) / NORM_KEYS; }
+template <int DP>
+__global__ void __launch_bounds__(256) xattn_norms_kernel(const XAttnArgs a, const __half* __restrict__ v, const long long sb, const long long st,
+                                                          const long long sh, float* __restrict__ norms, const int parts) {
+  constexpr int CH = DP / 8;
+  const int unit = blockIdx.x / parts, key0 = (blockIdx.x - unit * parts) * NORM_KEYS, m = unit / a.Hk, hk = unit % a.Hk;
+  const int len = visible_keys(a, m), sub = threadIdx.x / CH, ch = threadIdx.x % CH;
+  const __half* at = v + m * sb + hk * sh + ch * 8;
+  float top = 0.f;
+#pragma unroll 4
+  for (int r = sub; r < NORM_KEYS; r += 256 / CH) {
+    const int key = key0 + r;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (ch * 8 < a.D && !hidden_key(a, m, len, key)) x = *reinterpret_cast<const uint4*>(at + key * st);
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = Half2<__half>::unpack(xs[k]);
+      sum += f.x * f.x + f.y * f.y;
+    }
+#pragma unroll
+    for (int s = CH / 2; s > 0; s >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, s);
+    top = fmaxf(top, sum);
+  }
+  __shared__ float red[8];
+  top = warp_max(top);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, red[i]);
+    norms[blockIdx.x] = sqrtf(top);
+  }
+}
+
+// By a warp: what the largest |do| counts for the values' sake.
+template <typename T> __device__ __forceinline__ float value_factor(const XAttnArgs& a, const BwdArgs& b, int unit, int lane) {
+  if (Half2<T>::KIND != 0) return 1.f;
+  const int parts = norm_parts(a.Tk);
+  float top = 0.f;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, b.norms[(long long)unit * parts + i]);
+  return fmaxf(1.f, warp_max(top) * sqrtf((float)a.D) * (1.f / 4096.f));
+}
+
 // A warp's 32 rows of do into a swizzled tile (as load_rows), with sum(do * (out + rest)) of this lane's row and the peak of all.
 template <typename T, int DP>
-__device__ __forceinline__ void load_do_rows(const BwdArgs& b, long long off, int D, uint32_t tile, int quarter, int lane, float& delta, float& peak) {
+__device__ __forceinline__ void load_do_rows(const BwdArgs& b, long long off, int D, uint32_t tile, int quarter, int lane, float& delta, float& peak,
+                                             float factor) {
   constexpr int CH = DP / 8, RPI = 32 / CH;
   const int sub = lane / CH, ch = lane % CH;
   delta = peak = 0.f;
@@ -84,7 +136,7 @@ __device__ __forceinline__ void load_do_rows(const BwdArgs& b, long long off, in
     const float mine = __shfl_sync(0xffffffffu, d, ((lane - i) & (RPI - 1)) * CH);
     if (lane >= i && lane < i + RPI) delta = mine;
   }
-  if (Half2<T>::KIND == 0) peak = warp_max(fmaxf(peak, fabsf(delta) * (1.f / 64.f)));
+  if (Half2<T>::KIND == 0) peak = warp_max(fmaxf(peak * factor, fabsf(delta) * (1.f / 64.f)));
 }
 
 // Eight columns of a row from all blocks of the cluster, in turn, times f, rounded and written.
@@ -311,7 +363,7 @@ xattn_dq_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant
       load_rows<DP>(a.q, row_offset(a, a.q_sb, a.q_st, a.q_sh, m, hk, row), a.D, tile, quarter, lane);
     } else {
       float delta, peak;
-      load_do_rows<T, DP>(b, row_offset(a, st * a.Tq, st, a.D, m, hk, row), a.D, tile, quarter, lane, delta, peak);
+      load_do_rows<T, DP>(b, row_offset(a, st * a.Tq, st, a.D, m, hk, row), a.D, tile, quarter, lane, delta, peak, value_factor<T>(a, b, unit, lane));
       asm volatile("st.shared.f32 [%0], %1;" ::"r"(stat_row), "f"(-delta) : "memory");
       if (lane == 0) asm volatile("st.shared.f32 [%0], %1;" ::"r"(stats + (128 + quarter) * 4), "f"(peak) : "memory");
       if (valid && rank == 0) {
@@ -752,6 +804,13 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   b.tiles = (a.R + 127) / 128;
   const long long units = (long long)a.M * a.Hk, gq = units * b.tiles, gk = units * ((a.Tk + 127) / 128);
   if (gq > 0x7ffffffll || gk > 0x7ffffffll) return SB_BAD_ARGUMENT;
+  if (Half2<T>::KIND == 0) {
+    b.norms = b.peak + gq;
+    const int parts = norm_parts(a.Tk);                      // units * parts is within a grid's limit: gk, of twice as many tiles a key, is
+    xattn_norms_kernel<DP><<<(unsigned)(units * parts), 256, 0, stream>>>(a, (const __half*)g->v, g->v_sb, g->v_st, g->v_sh, b.norms, parts);
+    rc = (int)cudaGetLastError();
+    if (rc) return rc;
+  }
   using DQ = DqSmem<DP>;
   using DKV = DkvSmem<DP>;
   SbTilePlan plan = {gq, 1};                                 // without dq only the statistics are laid out, by a block per tile
@@ -766,8 +825,8 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
 
 }  // namespace
 
-// out, rest, dout: contiguous [B, Tq, H, D]; out, rest, lse: the forward pass's; ws: 2 * B * H * (Tq rounded up to 64) floats and
-// one per 128 packed rows of every (memory, key head); dq [B, Tq, H, D] or null; dk, dv
+// out, rest, dout: contiguous [B, Tq, H, D]; out, rest, lse: the forward pass's; ws: 2 * B * H * (Tq rounded up to 64) floats, one per 128 packed
+// rows and, in fp16, one per 256 keys of every (memory, key head); dq [B, Tq, H, D] or null; dk, dv
 // [M, Tk, Hk, D], both or neither.
 SB_API int sb_cross_attention_bwd(const SbCrossAttention* g, const void* out, const void* rest, const void* dout, const float* lse, float* ws, void* dq,
                                   void* dk, void* dv, cudaStream_t stream) {

@@ -314,6 +314,37 @@ def test_fp16_gradients_of_large_values(size):
         check(g, w, e, n)
 
 
+@pytest.mark.parametrize("tq,tk", [(5, 2), (70, 200), (130, 700)])
+@pytest.mark.parametrize("size", [200.0, 4000.0, 60000.0])
+def test_fp16_gradients_of_values_that_cancel(size, tq, tk):
+    """Values of both signs whose weighted mean is small: delta cancels and dp does not, and score gradients still stay within fp16 (their bound is
+    that of |do| |v|, whatever the sum)."""
+    from speech_b200 import ops
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q = (0.01 * torch.randn(1, tq, 2, 128, generator=g, device="cuda")).half()
+    k = (0.01 * torch.randn(1, tk, 2, 128, generator=g, device="cuda")).half()
+    sign = 1.0 - 2.0 * (torch.arange(tk, device="cuda") % 2)
+    v = (size * sign).view(1, tk, 1, 1).expand(1, tk, 2, 128).half()
+    mask = torch.zeros((1, tk + 1), dtype=torch.bool, device="cuda")
+    mask[:, tk] = True                                        # a hidden infinity has no part in the bound
+    k, v = torch.cat([k, k[:, :1]], 1), torch.cat([v, torch.full_like(v[:, :1], float("inf"))], 1)
+    dout = (torch.ones(q.shape, device="cuda") / max(1.0, size / 200)).half()
+    hidden = mask
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    grads = torch.autograd.grad(ops.cross_attention(*leaves, key_mask=mask), leaves, dout.flatten(2))
+    _, _, dwant, derr = plain(q, k, v, hidden, 1 / 128 ** 0.5, dout)
+    # besides plain()'s bounds: ds has an absolute step where the values' size sets its scale: the factor is at least 2^3 / (|do| sqrt(D) |v| / 2^12)
+    # for a power of two, the step 2^-25 over that
+    step = 2.0 ** -25 * float(dout.abs().max()) * 128 ** 0.5 * size * 128 ** 0.5 / 2.0 ** 12 / 2.0 ** 3
+    dq_more = step * k.double().abs().sum(1, keepdim=True) / 128 ** 0.5
+    dk_more = step * q.double().abs().sum(1, keepdim=True) / 128 ** 0.5
+    check(grads[0], dwant[0], derr[0] + dq_more, "dq")
+    check(grads[1], dwant[1], derr[1] + dk_more, "dk")
+    check(grads[2], dwant[2], derr[2], "dv")
+    ops.native.check_status()
+
+
 def test_gradients_against_differences():
     from speech_b200 import ops
 
