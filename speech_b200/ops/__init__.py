@@ -173,7 +173,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: Optional[fl
     no key gets zeros.  ``scale`` defaults to ``1 / sqrt(D)``.  No dropout on the weights: :func:`mha_attention` has it.
 
     On GPUs bf16 and fp16 with ``D`` a multiple of 8 up to 128 run as fused kernels, one for a few query rows per key head (decoding
-    steps) and one for many; anything else runs the plain form.  First derivatives only."""
+    steps) and one for many; anything else runs the plain form, forward-mode differentiation too.  First derivatives only."""
     reference.check_cross_attention(q, k, v, key_lengths, key_mask)
     if _use_native(q) and q.dtype in (torch.bfloat16, torch.float16):
         return _nat().cross_attention(q, k, v, key_lengths, key_mask, scale)
@@ -190,7 +190,7 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths
     one that sees nothing gets zeros.  Lengths beyond a cache count as its size.  The prompt's keys and values are read once for the
     whole group.  Caches may have any strides (``[B, Hk, Smax, D]`` caches are passed as ``cache.transpose(1, 2)``).
 
-    For inference: on GPUs there is no backward pass, and inputs that need gradients are refused."""
+    For inference: on GPUs there is no backward pass, and inputs that need gradients, of either mode, are refused."""
     reference.check_shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths)
     if _use_native(q) and q.dtype in (torch.bfloat16, torch.float16):
         return _nat().shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths, scale)

@@ -8,6 +8,7 @@ import struct
 from typing import Optional
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import native as N
 from .native_sequence_loss import address, bind, current_stream, first_derivative, on_device
@@ -106,6 +107,11 @@ def _backward(ctx, dout):
     return dq, dk if want_k else None, dv if want_v else None, None, None, None
 
 
+def _has_tangent(*tensors) -> bool:
+    """Whether forward-mode differentiation is on for one of them; such a tensor need not require a gradient."""
+    return forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask, scale):
@@ -122,7 +128,7 @@ class _CrossAttentionFn(torch.autograd.Function):
 def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
     D, Tk = q.shape[3], k.shape[1]
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if D % 8 or D > 128 or Tk == 0 or q.numel() == 0 or not 0.0 < scale < 1e30:
+    if D % 8 or D > 128 or Tk == 0 or q.numel() == 0 or not 0.0 < scale < 1e30 or _has_tangent(q, k, v):
         from . import reference
 
         return reference.cross_attention(q, k, v, key_lengths, key_mask, scale)
@@ -137,6 +143,8 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale=None):
 def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths=None, scale=None):
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k_prefix, v_prefix, k, v)):
         raise RuntimeError("shared_prefix_attention has no backward pass on GPUs: call it under torch.no_grad() or on detached tensors")
+    if _has_tangent(q, k_prefix, v_prefix, k, v):
+        raise RuntimeError("shared_prefix_attention has no forward-mode derivative on GPUs")
     B, Tq, H, D = q.shape
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if D % 8 or D > 128 or q.numel() == 0 or k_prefix.shape[1] == 0 or k.shape[1] == 0 or not 0.0 < scale < 1e30:

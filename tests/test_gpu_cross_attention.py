@@ -455,6 +455,37 @@ def test_double_backward_is_refused():
         g.float().sum().backward()
 
 
+def test_forward_mode_derivatives_are_there_or_refused():
+    """A dual tensor has no requires_grad; its tangent must not be lost."""
+    import torch.autograd.forward_ad as forward_ad
+
+    from speech_b200 import ops
+
+    q, k, v, lengths, _, hidden = make(2, 1, 5, 40, 2, 1, 64, torch.bfloat16, "lengths")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    tangents = [torch.randn(t.shape, generator=g, device="cuda").to(torch.bfloat16) for t in (q, k, v)]
+    # 64-bit: derivative along the tangents from three gradients
+    dout = torch.randn(q.shape, generator=g, device="cuda").to(torch.bfloat16)
+    _, _, (dq, dk, dv), _ = plain(q, k, v, hidden, 1 / 8, dout)
+    want = sum(float((d * t.double()).sum()) for d, t in zip((dq, dk, dv), tangents))
+    size = sum(float((d * t.double()).norm()) for d, t in zip((dq, dk, dv), tangents))
+    with forward_ad.dual_level():
+        duals = [forward_ad.make_dual(t, d) for t, d in zip((q, k, v), tangents)]
+        out = forward_ad.unpack_dual(ops.cross_attention(*duals, key_lengths=lengths))
+        assert out.tangent is not None
+        # the result's tangent is rounded to bf16: by at most 2^-8 of itself at random signs, as many as there are elements (factor 6)
+        got = float((out.tangent.double() * dout.flatten(2).double()).sum())
+        assert abs(got - want) <= 6 * 2.0 ** -8 * (float((out.tangent.double() * dout.flatten(2).double()).norm()) + size)
+        for i in range(3):
+            args = [duals[j] if i == j else t for j, t in enumerate((q, k, v))]
+            assert forward_ad.unpack_dual(ops.cross_attention(*args, key_lengths=lengths)).tangent is not None
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                ops.shared_prefix_attention(*args, k, v, torch.tensor([3, 9], device="cuda"))
+        assert forward_ad.unpack_dual(ops.cross_attention(q, k, v, key_lengths=lengths)).tangent is None
+    _, tangent = torch.func.jvp(lambda x: ops.cross_attention(x, k, v, key_lengths=lengths), (q,), (tangents[0],))
+    assert float(tangent.float().abs().max()) > 0
+
+
 def test_other_stream_and_captured_graphs():
     """Two captured graphs and an eager call in between, on inputs that change between replays."""
     from speech_b200 import ops

@@ -219,6 +219,20 @@ def test_extreme_logits():
     assert bool(torch.isfinite(torch.autograd.grad(p, x)[0]).all())
 
 
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as forward_ad
+
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(2, 3, None, 64, torch.bfloat16)
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(logits, torch.ones_like(logits))
+        with pytest.raises(NotImplementedError):
+            ops.policy_loss(x, targets, mask, old, adv)
+        with pytest.raises(NotImplementedError):
+            ops.preference_loss(x, targets, mask, ref)
+
+
 def test_captured_and_replayed():
     from speech_b200 import ops
 
