@@ -50,8 +50,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _lengths(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     if t is None or (t.dtype == torch.int32 and t.is_contiguous()):
         return t
-    # clamped before the narrowing, so that a 64-bit length cannot wrap
-    return t.clamp(0, 2 ** 31 - 1).to(torch.int32).contiguous()
+    # clamped in 64 bits before the narrowing, so that a 64-bit length cannot wrap and a type without the bound need not hold it
+    return t.long().clamp(0, 2 ** 31 - 1).to(torch.int32).contiguous()
 
 
 def _block(q, k, v, lengths, mask, scale) -> bytes:

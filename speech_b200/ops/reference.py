@@ -429,7 +429,7 @@ def cross_attention(q, k, v, key_lengths=None, key_mask=None, scale: Optional[fl
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     hidden = torch.zeros((M, Tk), dtype=torch.bool, device=q.device) if key_mask is None else key_mask
     if key_lengths is not None:
-        hidden = hidden | (torch.arange(Tk, device=q.device)[None, :] >= key_lengths[:, None])
+        hidden = hidden | (torch.arange(Tk, device=q.device)[None, :] >= key_lengths.long()[:, None])
     kf = k.float().masked_fill(hidden[:, :, None, None], 0.0)          # whatever stands in a hidden place (NaN, too) has no influence
     vf = v.float().masked_fill(hidden[:, :, None, None], 0.0)
     qf = q.float().reshape(M, G, Tq, Hk, rep, D)
@@ -462,8 +462,8 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     hide_p = torch.zeros((P, S), dtype=torch.bool, device=dev)
     if prefix_lengths is not None:
-        hide_p = torch.arange(S, device=dev)[None, :] >= prefix_lengths[:, None]
-    last = lengths.clamp(max=Smax)[:, None] - Tq + torch.arange(Tq, device=dev)[None, :]
+        hide_p = torch.arange(S, device=dev)[None, :] >= prefix_lengths.long()[:, None]
+    last = lengths.long().clamp(max=Smax)[:, None] - Tq + torch.arange(Tq, device=dev)[None, :]
     hide_o = torch.arange(Smax, device=dev)[None, None, :] > last[:, :, None]                       # [B, Tq, Smax]
     kp, vp = (x.float().masked_fill(hide_p[:, :, None, None], 0.0) for x in (k_prefix, v_prefix))
     unused = hide_o.all(dim=1) if Tq else torch.ones((B, Smax), dtype=torch.bool, device=dev)

@@ -95,6 +95,17 @@ def test_shared_prefix_attention_against_single_queries(heads, kv_heads, group, 
                 assert torch.allclose(out[b, t, h * D:(h + 1) * D].double(), want, rtol=0, atol=64 * 2.0 ** -24)
 
 
+@pytest.mark.parametrize("kind", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.uint16, torch.uint32])
+def test_lengths_of_any_integer_type(kind):
+    """Types that do not hold a cache's size, or no negative number: a new token before the first position sees nothing."""
+    g = torch.Generator().manual_seed(5)
+    q, kp, k = torch.randn(2, 3, 2, 8, generator=g), torch.randn(1, 9, 2, 8, generator=g), torch.randn(2, 300, 2, 8, generator=g)
+    lengths, prefix = torch.tensor([1, 7]), torch.tensor([4])
+    want = ops.shared_prefix_attention(q, kp, kp, k, k, lengths, prefix_lengths=prefix)
+    assert torch.equal(ops.shared_prefix_attention(q, kp, kp, k, k, lengths.to(kind), prefix_lengths=prefix.to(kind)), want)
+    assert torch.equal(ops.cross_attention(q, k, k, key_lengths=lengths.to(kind)), ops.cross_attention(q, k, k, key_lengths=lengths))
+
+
 def test_empty_sizes():
     q, k = torch.randn(2, 3, 2, 8), torch.randn(2, 0, 2, 8)
     assert bool((ops.cross_attention(q, k, k) == 0).all())

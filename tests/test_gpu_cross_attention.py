@@ -421,6 +421,21 @@ def test_dense_views_that_the_kernels_cannot_address(tq):
     ops.native.check_status()
 
 
+@pytest.mark.parametrize("kind", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.uint16, torch.uint32])
+def test_lengths_of_any_integer_type(kind):
+    from speech_b200 import ops
+
+    for tq in (3, 70):
+        q, k, v, _, _, _ = make(2, 1, tq, 300, 2, 1, 64, torch.bfloat16, "none")
+        lengths = torch.tensor([1, 100], device="cuda")
+        assert torch.equal(ops.cross_attention(q, k, v, key_lengths=lengths.to(kind)), ops.cross_attention(q, k, v, key_lengths=lengths))
+        want = ops.shared_prefix_attention(q, k, v, k, v, lengths, prefix_lengths=lengths)
+        assert torch.equal(ops.shared_prefix_attention(q, k, v, k, v, lengths.to(kind), prefix_lengths=lengths.to(kind)), want)
+        if kind in (torch.int8, torch.int16, torch.int32):
+            none = torch.tensor([-1, -100], device="cuda")
+            assert bool((ops.cross_attention(q, k, v, key_lengths=none.to(kind)) == 0).all())
+
+
 def test_partial_gradients_and_determinism():
     from speech_b200 import ops
 
