@@ -64,9 +64,12 @@ def _layout(logits: torch.Tensor):
 
 
 def _plain(t: Optional[torch.Tensor], dtype: torch.dtype) -> Optional[torch.Tensor]:
-    if t is None or (t.dtype == dtype and t.is_contiguous()):
-        return t
-    return t.detach().to(dtype).contiguous()
+    """A tensor that takes no gradient, dense and of the kernels' type."""
+    if t is None:
+        return None
+    if t.requires_grad:
+        t = t.detach()
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
 
 
 def _mask8(mask: Optional[torch.Tensor]) -> Optional[torch.Tensor]:

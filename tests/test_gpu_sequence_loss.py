@@ -233,6 +233,24 @@ def test_forward_mode_derivatives_are_refused():
             ops.preference_loss(x, targets, mask, ref)
 
 
+def test_gradients_go_to_the_logits_only():
+    """Log-probabilities, advantages and gaps that require gradients: the loss does not on their account, and they get none."""
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(4, 3, None, 64, torch.bfloat16)
+    gap = torch.rand(2, device="cuda").requires_grad_()
+    for t in (old, ref, adv):
+        t.requires_grad_()
+    losses = (lambda x: ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.1)[0],
+              lambda x: ops.preference_loss(x, targets, mask, ref, loss_type="rpo_sq", reward_gap=gap)[0])
+    for f in losses:
+        assert not f(logits.detach()).requires_grad
+        x = logits.detach().clone().requires_grad_()
+        f(x).backward()
+        assert x.grad is not None and float(x.grad.abs().max()) > 0
+    assert all(t.grad is None for t in (old, ref, adv, gap))
+
+
 def test_captured_and_replayed():
     from speech_b200 import ops
 

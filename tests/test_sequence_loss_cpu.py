@@ -112,6 +112,22 @@ def test_hidden_positions_have_no_influence_and_empty_batches_give_zero():
     assert float(loss) == 0.0 and logp.shape == (4, 0)
 
 
+def test_gradients_go_to_the_logits_only():
+    """Log-probabilities, advantages and gaps that require gradients: the loss does not on their account, and they get none."""
+    logits, targets, mask, old, ref, adv = batch()
+    gap = torch.rand(2).requires_grad_()
+    for t in (old, ref, adv):
+        t.requires_grad_()
+    losses = (lambda x: ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.1)[0],
+              lambda x: ops.preference_loss(x, targets, mask, ref, loss_type="rpo_sq", reward_gap=gap)[0])
+    for f in losses:
+        assert not f(logits.detach()).requires_grad
+        x = logits.detach().clone().requires_grad_()
+        f(x).backward()
+        assert x.grad is not None and float(x.grad.abs().max()) > 0
+    assert all(t.grad is None for t in (old, ref, adv, gap))
+
+
 def test_refusals():
     logits, targets, mask, old, ref, adv = batch()
     with pytest.raises(ValueError, match="ref_logp"):
