@@ -14,11 +14,12 @@
 //
 // Rounding: exponentials are fp32 and so is a thread's share of a policy row's sum; shares are joined in fp64, and logp, the clip
 // decision and the sums over rows are fp64: a policy at its reference has log ratios near zero, and in fp32 the rounding of a logp of
-// -8 (5e-7) would be all that is left after a few thousand positions are summed.  For the same reason the preference loss has
-// exponentials of its own, off by 4e-10 in the mean of many arguments (the library's moved every row's log sum the same way, by 1e-8, the approximate
-// power of two by 7e-8, which a sum over a sequence multiplies and the mean of the policy loss does not), and rounds only the
-// sums of four of them.  log s = k ln 2 + log f with s = 2^k f, f in [0.71, 1.42): the fp32 logarithm
-// of f is off by less than 2^-24.  The gradient is rounded once.  Every sum has a fixed order (no floating-point atomics).
+// -8 (5e-7) would be all that is left after a few thousand positions are summed.  A position's term and slope come from its fp64 log
+// ratios in fp32, each a few units in its last place off.  For the same reason the preference loss has exponentials of its own, off by 4e-10 in
+// the mean of many arguments (the library's moved every row's log sum the same way, by 1e-8, the approximate power of two by 7e-8, which a sum
+// over a sequence multiplies and the mean of the policy loss does not), and rounds only the sums of four of them.  Its logarithm of the row's sum is
+// the library's in fp64; the policy loss's is log s = k ln 2 + log f with s = 2^k f, f in [0.71, 1.42): the fp32 logarithm of f is off by less
+// than 2^-24.  The gradient is rounded once.  Every sum has a fixed order (no floating-point atomics).
 #include "packed_math.cuh"
 #include <cuda_fp16.h>
 #include <math.h>
@@ -254,6 +255,21 @@ template <int TPR, typename S> __device__ __forceinline__ void join(float& m, do
   sum = 0.0;
 #pragma unroll
   for (int i = 0; i < TPR / 32; ++i) sum += rebased(redd[i], redf[i], m);
+}
+
+// exp(d) - 1 - d, to a few units in the last place: near zero by its Taylor series d^2 (1/2! + d/3! + ... + d^7/9!), because the difference
+// of two numbers near d has their rounding (1e-4 of the term at d = 1e-3).  The series' rest is below 2^-24 of it for |d| <= 1/2.
+__device__ __forceinline__ float expm1_beyond(float d) {
+  if (fabsf(d) > 0.5f) return expm1f(d) - d;
+  float p = 1.f / 362880.f;
+  p = fmaf(p, d, 1.f / 40320.f);
+  p = fmaf(p, d, 1.f / 5040.f);
+  p = fmaf(p, d, 1.f / 720.f);
+  p = fmaf(p, d, 1.f / 120.f);
+  p = fmaf(p, d, 1.f / 24.f);
+  p = fmaf(p, d, 1.f / 6.f);
+  p = fmaf(p, d, 0.5f);
+  return p * d * d;
 }
 
 __device__ __forceinline__ double log_of_sum(double s) {
@@ -535,9 +551,9 @@ rows_forward_kernel(const RowArgs a, int* __restrict__ count_p, float* __restric
       float each = above ? -(1.f + a.clip_hi) * A : below ? -(1.f - a.clip_lo) * A : -plain;
       slope = above || below ? 0.f : -plain;
       if (a.ref && a.kl_beta != 0.f) {
-        const float kd = (float)((double)ref - logp), em = expm1f(kd);
-        each += a.kl_beta * (em - kd);
-        slope -= a.kl_beta * em;
+        const float kd = (float)((double)ref - logp);
+        slope -= a.kl_beta * expm1f(kd);
+        each += a.kl_beta * expm1_beyond(kd);
       }
       mine += (double)each;
       slope *= inv_count;

@@ -251,6 +251,34 @@ def test_gradients_go_to_the_logits_only():
     assert all(t.grad is None for t in (old, ref, adv, gap))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_kl_term_near_the_reference(dtype):
+    """exp(d) - d - 1 of log ratios down to 1e-5.  Rows of equal logits, 2^k of them: their log-probability is -k ln 2 to the last of 64 bits, so
+    that the term's own error shows."""
+    import math
+
+    from speech_b200 import ops
+
+    for k in (1, 7, 11, 16):
+        logits = torch.full((1, 40, 2 ** k), -3.0, device="cuda").to(dtype)
+        targets, none = torch.zeros((1, 40), dtype=torch.long, device="cuda"), torch.zeros(1, device="cuda")
+        lp = -k * math.log(2.0)
+        for size in (1e-5, 1e-4, 1e-3, 0.01, 0.1, 0.499, 0.501, 2.0):
+            for sign in (-1.0, 1.0):
+                ref = torch.linspace(size / 2, size, 40, dtype=torch.float64, device="cuda").mul(sign).add(lp).float().view(1, 40)
+                d = ref.double() - lp
+                # 64-bit term by the series where the difference would cancel there, too (the rest of six terms is below 1e-13 of it)
+                want = torch.where(d.abs() < 0.02, d * d * (1 / 2 + d * (1 / 6 + d * (1 / 24 + d * (1 / 120 + d * (1 / 720 + d / 5040))))), torch.expm1(d) - d)
+                loss, logp = ops.policy_loss(logits, targets, None, logp_of(lp, ref), none, ref_logp=ref, kl_beta=1.0)
+                # d to half a step, twice in d^2; nine operations; above 1/2 the library's expm1 and d, two units at most, in a difference of at
+                # least a seventh of them (expm1(d) / (expm1(d) - d) = 4.4 at 1/2, 3.7 at -1/2)
+                assert abs(float(loss) / float(want.mean()) - 1) <= 16 * 2.0 ** -24 * (1 if size < 0.5 else 3), (k, size, sign)
+
+
+def logp_of(lp, like):
+    return torch.full_like(like, lp)
+
+
 def test_captured_and_replayed():
     from speech_b200 import ops
 
