@@ -85,8 +85,7 @@ def _forward(q, k, v, lengths, mask, scale, for_backward):
 
 
 def _backward(ctx, dout):
-    q, k, v, out, lengths, mask = ctx.saved_tensors
-    kept = ctx.kept
+    q, k, v, out, lengths, mask, kept = ctx.saved_tensors
     if not dout.is_contiguous() or dout.data_ptr() & 15:
         dout = dout.clone(memory_format=torch.contiguous_format)
     want_q, want_k, want_v = ctx.needs_input_grad[:3]
@@ -115,8 +114,8 @@ def _has_tangent(*tensors) -> bool:
 class _CrossAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, lengths, mask, scale):
-        out, ctx.kept = _forward(q, k, v, lengths, mask, scale, True)
-        ctx.save_for_backward(q, k, v, out, lengths, mask)
+        out, kept = _forward(q, k, v, lengths, mask, scale, True)
+        ctx.save_for_backward(q, k, v, out, lengths, mask, kept)
         ctx.scale = scale
         return out
 

@@ -99,12 +99,11 @@ def _gradient(upstream, logits, targets, mask, lse, slope, seq_slope, out, unles
 
 
 def _policy_backward(ctx, dloss, _):
-    logits, targets, mask = ctx.saved_tensors
-    out, ctx.grad = ctx.grad, None
-    first = out is not None
-    if not first:
-        out = logits.new_empty(logits.shape)
-    lse = ctx.kept.data_ptr() + 8 * _blocks() + 8
+    logits, targets, mask, kept, grad = ctx.saved_tensors
+    first, ctx.first = ctx.first, False
+    # handed out with a version counter of its own: what its owner does to it is nothing to a further backward pass, which does not read it
+    out = grad.data if first else logits.new_empty(logits.shape)
+    lse = kept.data_ptr() + 8 * _blocks() + 8
     return _gradient(dloss, logits, targets, mask, lse, lse + 8 * targets.numel(), 0, out, int(first)), None, None, None, None, None, None, None, None, None
 
 
@@ -126,9 +125,8 @@ class _PolicyLossFn(torch.autograd.Function):
                                             lo, hi, kl_beta, ws + 8 * _blocks(), ws, loss.data_ptr(), logp.data_ptr(), lse, lse + 8 * rows, address(grad),
                                             current_stream()), "sb_policy_loss_fwd")
         if want_grad:
-            ctx.save_for_backward(logits, targets, mask)
-            ctx.kept = kept
-            ctx.grad = grad
+            ctx.save_for_backward(logits, targets, mask, kept, grad)
+            ctx.first = True
         ctx.mark_non_differentiable(logp)
         return loss, logp
 
@@ -138,9 +136,9 @@ class _PolicyLossFn(torch.autograd.Function):
 
 
 def _preference_backward(ctx, dloss, _):
-    logits, targets, mask = ctx.saved_tensors
+    logits, targets, mask, kept = ctx.saved_tensors
     rows = targets.numel()
-    lse = ctx.kept.data_ptr() + 8 * (rows + logits.shape[0])
+    lse = kept.data_ptr() + 8 * (rows + logits.shape[0])
     out = logits.new_empty(logits.shape)
     return _gradient(dloss, logits, targets, mask, lse, 0, lse + 8 * rows, out, 0), None, None, None, None, None, None
 
@@ -152,14 +150,14 @@ class _PreferenceLossFn(torch.autograd.Function):
         loss = logits.new_empty((), dtype=torch.float32)
         rewards = logits.new_empty(n, dtype=torch.float32)
         # log ratios of the positions and of the sequences (fp64), lse (two parts) and the slopes of the sequences (fp32)
-        ctx.kept = logits.new_empty(4 * rows + 3 * n, dtype=torch.float32)
-        ws = ctx.kept.data_ptr()
+        kept = logits.new_empty(4 * rows + 3 * n, dtype=torch.float32)
+        ws = kept.data_ptr()
         lse = ws + 8 * (rows + n)
         layout, sizes = _layout(logits)
         N._check(bind("sb_preference_loss_fwd")(logits.data_ptr(), *layout, targets.data_ptr(), address(mask), ref.data_ptr(), *sizes, kind, beta, address(gap),
                                                 ws, ws + 8 * rows, loss.data_ptr(), rewards.data_ptr(), lse + 8 * rows, lse, current_stream()),
                  "sb_preference_loss_fwd")
-        ctx.save_for_backward(logits, targets, mask)
+        ctx.save_for_backward(logits, targets, mask, kept)
         ctx.mark_non_differentiable(rewards)
         return loss, rewards
 

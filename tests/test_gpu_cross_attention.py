@@ -501,6 +501,36 @@ def test_forward_mode_derivatives_are_there_or_refused():
     assert float(tangent.float().abs().max()) > 0
 
 
+def test_what_backward_needs_is_seen_by_autograd():
+    """Everything kept for the backward pass goes through saved variables: hooks move it, and it is freed with the graph though the output lives."""
+    from speech_b200 import ops
+
+    q, k, v, lengths, _, _ = make(4, 2, 500, 300, 4, 1, 64, torch.bfloat16, "lengths")
+    dout = torch.randn(q.shape, device="cuda").to(torch.bfloat16).flatten(2)
+    size = q.numel() * q.element_size()
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        before = torch.cuda.memory_allocated()
+        out = ops.cross_attention(*leaves, key_lengths=lengths)
+        after = torch.cuda.memory_allocated() - before
+        grads = torch.autograd.grad(out, leaves, dout)
+        return out, grads, after, torch.cuda.memory_allocated() - before - sum(g.numel() * g.element_size() for g in grads)
+
+    out, grads, _, left = run()
+    assert left < 1.25 * size                               # the output alone
+    with torch.autograd.graph.save_on_cpu():
+        again, moved, held, _ = run()
+    assert held < 1.25 * size
+    assert torch.equal(again, out) and all(torch.equal(a, b) for a, b in zip(moved, grads))
+
+    from torch.utils.checkpoint import checkpoint
+
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    once = checkpoint(lambda *t: ops.cross_attention(*t, key_lengths=lengths), *leaves, use_reentrant=False)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(once, leaves, dout), grads))
+
+
 def test_other_stream_and_captured_graphs():
     """Two captured graphs and an eager call in between, on inputs that change between replays."""
     from speech_b200 import ops

@@ -279,6 +279,34 @@ def logp_of(lp, like):
     return torch.full_like(like, lp)
 
 
+def test_what_backward_needs_is_seen_by_autograd():
+    """The gradient that the forward pass writes, and the rows' statistics, go through saved variables."""
+    from torch.utils.checkpoint import checkpoint
+
+    from speech_b200 import ops
+
+    logits, targets, mask, old, ref, adv = make(8, 64, None, 2024, torch.bfloat16)
+    size = logits.numel() * logits.element_size()
+    for f in (lambda x: ops.policy_loss(x, targets, mask, old, adv, ref_logp=ref, kl_beta=0.04)[0], lambda x: ops.preference_loss(x, targets, mask, ref)[0]):
+        x = logits.detach().clone().requires_grad_()
+        loss = f(x)
+        (want,) = torch.autograd.grad(loss, x)
+        with torch.autograd.graph.save_on_cpu():
+            before = torch.cuda.memory_allocated()
+            loss = f(x)
+            assert torch.cuda.memory_allocated() - before < size // 8
+        assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+        loss = checkpoint(f, x, use_reentrant=False)
+        assert torch.equal(torch.autograd.grad(loss, x)[0], want)
+        # a gradient that its owner changes does not reach a further backward pass
+        loss = f(x)
+        (g,) = torch.autograd.grad(loss, x, retain_graph=True)
+        g.zero_()
+        (h,) = torch.autograd.grad(loss, x)
+        # computed from memory: another exponential, a step of the type apart at most
+        assert bool(((h.double() - want.double()).abs() <= 2.0 ** -7 * want.double().abs() + 1e-12).all())
+
+
 def test_captured_and_replayed():
     from speech_b200 import ops
 
