@@ -259,7 +259,7 @@ def policy_loss(logits, targets, mask, old_logp, advantages, ref_logp=None, clip
     go to ``logits`` only.  Masked positions are not read, whatever they hold.  On GPUs a counted target outside the vocabulary makes
     the loss NaN (the CPU raises), and a forward pass that needs gradients holds the logits' gradient until backward."""
     reference.check_sequence_loss("policy_loss", logits, targets, mask, (("old_logp", old_logp), ("ref_logp", ref_logp)),
-                                  (("advantages", advantages, logits.shape[0]),))
+                                  (("advantages", advantages, logits.shape[0] if logits.dim() > 0 else 0),))
     if kl_beta != 0.0 and ref_logp is None:
         raise ValueError("a KL term (kl_beta != 0) needs ref_logp")
     if clip < 0 or (clip_high is not None and clip_high < 0):
@@ -285,6 +285,8 @@ def preference_loss(logits, targets, mask, ref_logp, beta: float = 0.1, loss_typ
         raise NotImplementedError(f"loss type {loss_type} is not implemented")
     if loss_type == "rpo_sq" and reward_gap is None:
         raise ValueError("rpo_sq needs the reward gap of every pair")
+    if loss_type == "ipo" and beta == 0.0:
+        raise ValueError("ipo aims at a margin of 1 / (2 beta): beta must not be zero")
     if _use_native(logits) and logits.dtype in (torch.bfloat16, torch.float16, torch.float32) and targets.numel() > 0:
         return _nat().preference_loss(logits, targets, mask, ref_logp, beta, loss_type, reward_gap)
     return reference.preference_loss(logits, targets, mask, ref_logp, beta, loss_type, reward_gap)

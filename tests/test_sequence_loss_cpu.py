@@ -154,3 +154,15 @@ def test_refusals():
         ops.preference_loss(logits, targets, mask, ref, loss_type="rpo_sq", reward_gap=torch.zeros(4))
     with pytest.raises(NotImplementedError):
         ops.preference_loss(logits, targets, mask, ref, loss_type="hinge")
+
+
+def test_refusals_of_scalars():
+    _, targets, mask, old, ref, adv = batch()
+    none = torch.zeros(())
+    with pytest.raises(ValueError, match="logits"):
+        ops.policy_loss(none, targets, mask, old, adv)
+    with pytest.raises(ValueError, match="logits"):
+        ops.preference_loss(none, targets, mask, ref)
+    logits = batch()[0]
+    with pytest.raises(ValueError, match="beta"):
+        ops.preference_loss(logits, targets, mask, ref, beta=0.0, loss_type="ipo")
