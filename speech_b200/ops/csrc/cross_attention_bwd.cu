@@ -28,7 +28,7 @@
 // gradients fall below the type's normal range.  ds stays below its end whatever the values are: |dp| <= |do| |v| (norms), and
 // |ds| = p |dp - sum p dp| <= p (1 - p) 2 max |dp| <= max |do| |v| / 2.  A kernel ahead takes the largest norm of a visible value, and where
 // sqrt(D) max|v| exceeds 4096 the peak of do counts that many times as much: ds then ends below 16 * 2048.  (Not needed for bf16; in fp16 it
-// reads the values once more: 6 us of 199 for forward and backward of 12 x 301 queries, 3 x 1111 keys, 16 heads on 4 of 64, 8 of 575 for 4 x 1024
+// reads the values once more: 4 us of 197 for forward and backward of 12 x 301 queries, 3 x 1111 keys, 16 heads on 4 of 64, 8 of 575 for 4 x 1024
 // queries, 7500 keys, 8 heads of 128.)
 #include "cross_attention.cuh"
 #include "cross_attention_host.h"
@@ -60,7 +60,8 @@ template <typename T> __device__ __forceinline__ float ds_scale(float peak) {
   return __int_as_float((127 + 3 - ((__float_as_int(fmaxf(peak, 1e-8f)) >> 23) - 127)) << 23);      // |do| of fp16 is at least 2^-24
 }
 
-constexpr int NORM_KEYS = 256;
+// Few keys a block: it is the latency of its loads that counts (256 keys: 9 us for 64 at 3 x 1111 keys, 4 heads of 64).
+constexpr int NORM_KEYS = 64;
 __host__ __device__ inline int norm_parts(int Tk) { return (Tk + NORM_KEYS - 1) / NORM_KEYS; }
 template <int DP>
 __global__ void __launch_bounds__(256) xattn_norms_kernel(const XAttnArgs a, const __half* __restrict__ v, const long long sb, const long long st,
@@ -70,11 +71,13 @@ __global__ void __launch_bounds__(256) xattn_norms_kernel(const XAttnArgs a, con
   const int len = visible_keys(a, m), sub = threadIdx.x / CH, ch = threadIdx.x % CH;
   const __half* at = v + m * sb + hk * sh + ch * 8;
   float top = 0.f;
-#pragma unroll 4
+#pragma unroll
   for (int r = sub; r < NORM_KEYS; r += 256 / CH) {
     const int key = key0 + r;
+    const bool in = ch * 8 < a.D && key < len;
     uint4 x = make_uint4(0, 0, 0, 0);
-    if (ch * 8 < a.D && !hidden_key(a, m, len, key)) x = *reinterpret_cast<const uint4*>(at + key * st);
+    if (in) x = *reinterpret_cast<const uint4*>(at + key * st);
+    if (a.mask && in && a.mask[(long long)m * a.Tk + key]) x = make_uint4(0, 0, 0, 0);      // read beside its value, not before
     const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
     float sum = 0.f;
 #pragma unroll
@@ -806,7 +809,7 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
   if (gq > 0x7ffffffll || gk > 0x7ffffffll) return SB_BAD_ARGUMENT;
   if (Half2<T>::KIND == 0) {
     b.norms = b.peak + gq;
-    const int parts = norm_parts(a.Tk);                      // units * parts is within a grid's limit: gk, of twice as many tiles a key, is
+    const int parts = norm_parts(a.Tk);                      // units * parts <= 2 gk is within a grid's limit
     xattn_norms_kernel<DP><<<(unsigned)(units * parts), 256, 0, stream>>>(a, (const __half*)g->v, g->v_sb, g->v_st, g->v_sh, b.norms, parts);
     rc = (int)cudaGetLastError();
     if (rc) return rc;
@@ -826,7 +829,7 @@ int launch(const SbCrossAttention* g, const XAttnArgs& a, BwdArgs b, void* dq, v
 }  // namespace
 
 // out, rest, dout: contiguous [B, Tq, H, D]; out, rest, lse: the forward pass's; ws: 2 * B * H * (Tq rounded up to 64) floats, one per 128 packed
-// rows and, in fp16, one per 256 keys of every (memory, key head); dq [B, Tq, H, D] or null; dk, dv
+// rows and, in fp16, one per 64 keys of every (memory, key head); dq [B, Tq, H, D] or null; dk, dv
 // [M, Tk, Hk, D], both or neither.
 SB_API int sb_cross_attention_bwd(const SbCrossAttention* g, const void* out, const void* rest, const void* dout, const float* lse, float* ws, void* dq,
                                   void* dk, void* dv, cudaStream_t stream) {

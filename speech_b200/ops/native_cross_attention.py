@@ -93,8 +93,8 @@ def _backward(ctx, dout):
     with on_device(q):
         M, Hk = k.shape[0], k.shape[2]
         units = M * Hk
-        # statistics in lines of a multiple of 64, a maximum per 128 rows that read the same keys, in fp16 one per 256 keys
-        norms = (k.shape[1] + 255) // 256 if q.dtype == torch.float16 else 0
+        # statistics in lines of a multiple of 64, a maximum per 128 rows that read the same keys, in fp16 one per 64 keys
+        norms = (k.shape[1] + 63) // 64 if q.dtype == torch.float16 else 0
         ws = q.new_empty(2 * B * H * ((Tq + 63) // 64 * 64) + units * ((B * H * Tq // units + 127) // 128 + norms), dtype=torch.float32)
         dq = q.new_empty(q.shape) if want_q else None
         dk = k.new_empty(k.shape) if want_k or want_v else None
