@@ -110,26 +110,6 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t* r) 
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-constexpr float EX2_C0 = 1.f, EX2_C1 = 0.693121045f, EX2_C2 = 0.24022349f, EX2_C3 = 0.0559219758f, EX2_C4 = 0.00966636852f;
-// 2^x for two values without the special-function unit: x = n + f with n the nearest integer, 2^f by a polynomial, times 2^n.
-// Coefficients: 2^f interpolated at the five Chebyshev nodes of [-1/2, 1/2], off by less than 2^-18 there.  For x < 128; below -126.5
-// the result is 0, and NaN stays NaN.
-__device__ __forceinline__ void ex2_poly(uint64_t v, float& lo, float& hi) {
-  split(v, lo, hi);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-127.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-127.f));
-  const uint64_t x = pair(lo, hi);
-  constexpr float ROUND = 12582912.f;                      // 1.5 * 2^23: adding it rounds to an integer, which the low bits then hold
-  const uint64_t r = add2(x, pair(ROUND, ROUND));
-  const uint64_t f = add2(x, fma2(r, pair(-1.f, -1.f), pair(ROUND, ROUND)));      // x - n
-  uint64_t p = fma2(f, pair(EX2_C4, EX2_C4), pair(EX2_C3, EX2_C3));
-  p = fma2(p, f, pair(EX2_C2, EX2_C2));
-  p = fma2(p, f, pair(EX2_C1, EX2_C1));
-  p = fma2(p, f, pair(EX2_C0, EX2_C0));
-  split(r, lo, hi);
-  split(mul2(p, pair(__int_as_float((__float_as_int(lo) << 23) + 0x3f800000), __int_as_float((__float_as_int(hi) << 23) + 0x3f800000))), lo, hi);
-}
-
 // whole-warp bounded wait: the same answer in every lane, so that the .aligned instructions that follow stay converged
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, int* status, int code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, code) ? 1 : 0) != 0;

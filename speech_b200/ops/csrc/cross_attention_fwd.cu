@@ -286,14 +286,9 @@ xattn_fwd_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
           float x, y;
-          const uint64_t e = fma2(pair(r[32 * i + 2 * k], r[32 * i + 2 * k + 1]), c2, shift2);
-          if (k % 8 >= 6) {                                 // a quarter: 120 us, none 129, half 130 (1024 queries, 7500 keys, 32 heads)
-            ex2_poly(e, x, y);
-          } else {
-            split(e, x, y);
-            x = ex2(x);
-            y = ex2(y);
-          }
+          split(fma2(pair(r[32 * i + 2 * k], r[32 * i + 2 * k + 1]), c2, shift2), x, y);
+          x = ex2(x);
+          y = ex2(y);
           if (KEEP) sum[k & 1] = add2(sum[k & 1], pair(x, y));
           p[k] = Half2<T>::pack(x, y);
           const float2 back = Half2<T>::unpack(p[k]);
