@@ -187,8 +187,9 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths
     ``v_prefix [P, S, Hk, D]`` the prompts, row ``b`` continuing prompt ``b // (B / P)``, of which the first ``prefix_lengths [P]``
     positions count (default: all); ``k``, ``v [B, Smax, Hk, D]`` the rows' own caches, in which row ``b`` holds ``lengths[b]``
     positions, the new tokens included.  Token ``t`` sees its prompt and its row's positions up to its own, ``lengths[b] - Tq + t``;
-    one that sees nothing gets zeros.  Lengths beyond a cache count as its size.  The prompt's keys and values are read once for the
-    whole group.  Caches may have any strides (``[B, Hk, Smax, D]`` caches are passed as ``cache.transpose(1, 2)``).
+    one that sees nothing gets zeros.  Lengths beyond a cache count as its size.  What stands behind the lengths has no influence;
+    the new tokens' own keys and values are taken to be finite (an infinite value of a later one makes NaN of the earlier ones that share a
+    call with it).  The prompt's keys and values are read once for the whole group.  Caches may have any strides (``[B, Hk, Smax, D]`` caches are passed as ``cache.transpose(1, 2)``).
 
     For inference: on GPUs there is no backward pass, and inputs that need gradients, of either mode, are refused."""
     reference.check_shared_prefix_attention(q, k_prefix, v_prefix, k, v, lengths, prefix_lengths)

@@ -37,7 +37,7 @@ namespace {
 
 constexpr int DKV_THREADS = 640;       // 20 warps of 96 registers
 // What a CTA takes besides its blocks or steps, in those; a join takes half of it.  [dq, 100 queries, 8 heads of 128, 1 / 2 / 4 / 8 CTAs a
-// tile: 73 / 47 / 30 / 24 us for 7500 keys, 24 / 22 / 20 / 18 for 1500; dk / dv, 5 x 1500 queries against 100 keys: 102 / 57 / 36 / 28 us]
+// tile: 74 / 47 / 33 / 27 us for 7500 keys, 25 / 23 / 18 / 18 for 1500; dk / dv, 5 x 1500 queries against 100 keys: 102 / 59 / 37 / 29 us]
 constexpr int DQ_OWN_BLOCKS = 10, DKV_OWN_STEPS = 8;
 template <typename T> constexpr float p_shift() { return Half2<T>::KIND == 0 ? 12.f : 0.f; }
 

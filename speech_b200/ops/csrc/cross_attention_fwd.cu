@@ -15,7 +15,7 @@
 // and (m, l) meet in shared memory and are joined in a fixed order: w_i = 2^(c (m_i - max m)), o = sum w_i o_i / sum w_i l_i.
 //
 // Rounding: scores, maxima, sums and output are fp32; p is rounded to the operands' 16-bit type, which is what the tensor core
-// multiplies (relative 2^-9 per weight in bf16), and the output is divided by the sum w of the rounded weights.  Divided by l it would be off by the
+// multiplies (up to 2^-8 of a weight in bf16), and the output is divided by the sum w of the rounded weights.  Divided by l it would be off by the
 // rounding of the largest weight where one key leads (a weight up to 2^8, because of the maximum that stands still): a common factor, which the
 // backward pass's delta = sum do o takes on and subtracts from values of its own size.  [Rows that one of 512 keys leads by 3 / 4 / 5 nats, bf16: dq
 // off by 11 / 17 / 60 % of its norm; so by 1 %.]  lse is the unrounded p's.
@@ -27,7 +27,7 @@ namespace {
 constexpr int FWD_THREADS = 384;
 constexpr int BN = 64;
 // What a CTA takes besides its blocks, and what a join takes, in blocks.  [1 x 100 queries, 8 heads of 128, 1 / 2 / 4 / 8 CTAs a tile:
-// 104 / 63 / 42 / 34 us for 7500 keys, 34 / 28 / 24 / 24 for 1500, 22 / 22 / 20 / 22 for 500]
+// 102 / 63 / 43 / 33 us for 7500 keys, 33 / 29 / 25 / 25 for 1500, 20 / 23 / 23 / 21 for 500]
 constexpr int OWN_BLOCKS = 9;
 template <int DP> struct FwdSmem {
   static constexpr int STAGES = 4;

@@ -158,7 +158,8 @@ enum { LOSS_POLICY = 0, LOSS_PREFERENCE = 1 };
 
 // exp of two values t <= 0 (above 88 the exponent's bits overflow), off by less than 0.6 units in the last place and, in the mean of many
 // arguments, by 4e-10 (of the few differences that bf16 logits have, by up to 4e-9: rewards of 2 x 512 rows of 40001, 3.4e-9 a row):
-// t log2 e = n + f with n the nearest integer and f from the product with log2 e in two parts; 2^f = 1 + f q(f), q of degree 5 through
+// t log2 e = n + f with n the nearest integer (what adding 1.5 * 2^23 leaves) and f from the product with log2 e in two parts, after Cody and Waite
+// (Software Manual for the Elementary Functions, 1980); 2^f = 1 + f q(f), q of degree 5 through
 // (2^f - 1) / f at the six Chebyshev nodes of [-1/2, 1/2]; times 2^n.  Below e^-88 the result is 0; NaN stays NaN.
 __device__ __forceinline__ uint64_t exp_fine(uint64_t v) {
   float t, u;

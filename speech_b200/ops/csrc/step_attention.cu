@@ -544,8 +544,8 @@ int fill(StepArgs& a, const SbCrossAttention* g) {
 
 }  // namespace
 
-// Up to 32 packed rows.  [This kernel / the one for many rows, 8 heads of 128, us.  1 memory of 7500 keys: 1 row 22 / 22, 16 rows 24 / 28, 32
-// rows 28 / 30, 64 rows 36 / 30; 16 of 500: 16 / 18, 22 / 22, 28 / 24, 38 / 24; 64 of 500: 38 / 57, 43 / 69, 49 / 77]
+// Up to 32 packed rows.  [This kernel / the one for many rows, 8 heads of 128, us.  1 memory of 7500 keys: 1 row 23 / 25, 16 rows 27 / 29, 32
+// rows 29 / 33, 64 rows 39 / 33; 16 of 500: 18 / 18, 23 / 23, 29 / 25, 41 / 25; 64 of 500: 41 / 55, 43 / 68, 49 / 78]
 bool sb_few_rows(const SbCrossAttention* g) { return (long long)g->G * g->rep * g->Tq <= 32; }
 
 int sb_step_cross_attention(const SbCrossAttention* g, void* out, void* rest, float* lse, void* ws, cudaStream_t stream) {
