@@ -2,7 +2,8 @@
 //
 // One pass over the keys with the running maximum m and sum l of every row; p = 2^(c s - c m) is held unnormalised:
 //   s = q k_j^T,  m' = max(m, max s),  o = o 2^(c (m - m')) + p v_j,  l = l 2^(c (m - m')) + sum p,  at the end o / w
-// with w the sum of p as it is rounded for the product with v (below), and lse = c m + log2 l is kept for the backward pass (+inf for a row that sees nothing: its probabilities are then 2^-inf = 0).
+// with w the sum of p as it is rounded for the product with v (below), and lse = c m + log2 l is kept for the backward pass (+inf for a row
+// that sees nothing: its probabilities are then 2^-inf = 0).
 //
 // A CTA takes two tiles of 128 packed rows and streams blocks of 64 keys of its memory and key head past both, so that keys and values
 // cross the L2 once per 256 rows.  Warp 0 loads keys and values by TMA, warps 1 and 3 issue the tcgen05.mma of a tile each, warp 2
