@@ -9,11 +9,11 @@
 // cross the L2 once per 256 rows.  Warp 0 loads keys and values by TMA, warps 1 and 3 issue the tcgen05.mma of a tile each, warp 2
 // clears the rows of hidden keys and lays out their addends (one more step of the score product), and one warpgroup per row tile does the
 // softmax: scores and output accumulate in tensor memory (per tile two buffers of 64 columns and DP columns), the probabilities go back
-// there as 16-bit pairs over the scores they came from and are the A operand of the second product.  The scores of the next block are there before the softmax of this one ends; with one buffer of 128 keys the
-// warpgroups waited for the tensor core and it for them (41 % of its cycles busy).  The output is rescaled only when a row's maximum
+// there as 16-bit pairs over the scores they came from and are the A operand of the second product.  The scores of the next block are there before the softmax of this
+// one ends; with one buffer of 128 keys the warpgroups waited for the tensor core and it for them (41 % of its cycles busy).  The output is rescaled only when a row's maximum
 // has grown by more than 2^8 since the last time; p then stays below 2^8, and the result does not depend on it beyond rounding.
 // Where there are fewer tile pairs than SMs, up to eight CTAs of a cluster share one, each with its part of the keys; unnormalised outputs
-// and (m, l) meet in shared memory and are joined in a fixed order: w_i = 2^(c (m_i - max m)), o = sum w_i o_i / sum w_i l_i.
+// and (m, w, l) meet in shared memory and are joined in a fixed order: f_i = 2^(c (m_i - max m)), o = sum f_i o_i / sum f_i w_i.
 //
 // Rounding: scores, maxima, sums and output are fp32; p is rounded to the operands' 16-bit type, which is what the tensor core
 // multiplies (up to 2^-8 of a weight in bf16), and the output is divided by the sum w of the rounded weights.  Divided by l it would be off by the
